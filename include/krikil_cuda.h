@@ -5,7 +5,8 @@
  * The reference is a Rust library whose public surface is src/lib.rs:1-6; its
  * model API (src/model.rs) is what a Rust `build.rs` + `extern "C"` binding of
  * this header replaces.  Each entry point below names the reference interface
- * it stands in for.  All computation is fp32, on the GPU; there is no CPU
+ * it stands in for.  All computation is fp32, on the GPU (the paged cache's
+ * operators also take 16-bit elements); there is no CPU
  * fallback -- if the device or the kernels are unusable, calls fail with
  * KRK_CUDA and krk_last_error() says why.
  *
@@ -401,6 +402,110 @@ KRK_API int krk_k_rope_kv_attn_decode_noalloc(const float* q, const float* k, co
  * the attention kernels.  The kernel returns either way and the context stays
  * usable. */
 KRK_API int krk_k_wait_probe(const float* src16, int polls, int copy, int32_t* status, void* stream);
+
+/* ------------------------------------------------------ paged key-value cache
+ * Serving many requests of different lengths from one pool (no counterpart in
+ * the reference, whose caches are one contiguous array a sequence).  The pool
+ * is num_pages pages of page_size tokens (a power of two, at most 65536;
+ * num_pages * page_size < 2^31).  Element (page, t, head, d) of the key cache
+ * is kc[page*c_sp + t*c_st + head*c_sh + d], of the value cache the same in vc,
+ * so both [page][t][head][d] and [page][head][t][d] layouts are covered.
+ * Request b's token j lives in page table[b*table_ld + j / page_size], at t =
+ * j % page_size; its slot is page * page_size + t.  One table serves every
+ * attention layer, each layer having its own kc and vc.
+ *
+ * A serving step is: krk_k_kv_page_release for finished requests,
+ * krk_k_kv_page_plan for the step's tokens, then per layer
+ * krk_k_rope_kv_append_paged and krk_k_attn_decode_paged.  Nothing is read
+ * back to the host, so the step can be captured into a CUDA graph.
+ *
+ * q, k, v, out are all of `type`, the caches of `cache_type` (KRK_TYPE_*):
+ * equal, or a 16-bit cache under float32 activations.  Computation is in 32
+ * bits or more throughout, and rounded once when written.  dh is a multiple of
+ * 4 of at most 256; pointers are aligned to four elements and strides are
+ * multiples of four; the last dimension is dense.  The calls run on the current
+ * device, to which `stream` and all pointers belong. */
+#define KRK_TYPE_F32 0
+#define KRK_TYPE_F16 1
+#define KRK_TYPE_BF16 2
+
+/* Bits of the device status word of the next two calls. */
+#define KRK_PAGES_EXHAUSTED 1  /* the free list holds fewer pages than the step needs */
+#define KRK_PAGES_ROW_FULL 2   /* a request would need more than `width` pages */
+#define KRK_PAGES_ROWS 4       /* the step has more than `rows` new tokens */
+#define KRK_PAGES_BAD_LENGTH 8 /* a negative length or count, or one past its array */
+#define KRK_PAGES_OVERFLOW 16  /* a release would put more than num_pages pages on the list */
+
+/* Plans a step in which request b (of B) adds new_tokens[b] >= 0 tokens to the
+ * lens[b] that it holds.  free_pages [num_pages] is a stack of free page ids
+ * with *free_count of them, the top last: requests take the pages that they
+ * lack from its top, in request order, into table[b*table_ld + i].  Writes
+ * lens_out[b] = lens[b] + new_tokens[b], *free_count_out, the packed offsets
+ * cu_new [B+1] of each request's new tokens, and for token i of request b,
+ * packed row r = cu_new[b] + i: positions[r] = lens[b] + i and slots[r].  Rows
+ * from cu_new[B] to `rows` get slot -1 (skipped by the append) and position 0.
+ * lens_out may be lens and free_count_out may be free_count; no other outputs
+ * overlap.  *status is 0, or the KRK_PAGES_* bits of what does not fit: then
+ * nothing is taken (table untouched, lens_out = lens, free_count_out =
+ * free_count), cu_new is 0 and every slot -1.  Page ids on the list are copied
+ * as they are. */
+KRK_API int krk_k_kv_page_plan(const int32_t* new_tokens, const int32_t* lens, int32_t* table, int64_t table_ld,
+                               int B, int width, const int32_t* free_pages, const int32_t* free_count, int num_pages,
+                               int page_size, int32_t* lens_out, int32_t* free_count_out, int32_t* cu_new,
+                               int32_t* positions, int32_t* slots, int rows, int32_t* status, void* stream);
+
+/* Puts the pages of every request with done_mask[b] != 0 back on the stack, in
+ * request order and each request's pages in table order, and sets lens_out[b]
+ * to 0 (lens[b] for the others); the table is left as it is.  Aliasing and
+ * *status as above: with a bit set nothing changes. */
+KRK_API int krk_k_kv_page_release(const uint8_t* done_mask, const int32_t* lens, const int32_t* table,
+                                  int64_t table_ld, int B, int width, int32_t* free_pages,
+                                  const int32_t* free_count, int num_pages, int page_size, int32_t* lens_out,
+                                  int32_t* free_count_out, int32_t* status, void* stream);
+
+/* RoPE (the rotate-half convention of src/math.rs:234-260 on the first rot_dim
+ * elements of each head, pairs (i, i + rot_dim/2); the rest passes through) of
+ * T packed rows' queries and keys, and the append of the rotated keys and the
+ * values to the caches.  Element (t, head, d) of q is q[t*q_st + head*q_sh + d];
+ * k, v and q_out likewise (q_out may be q with its strides).  Row t goes to
+ * slots[t]; a row with a negative slot is padding: neither the caches nor its
+ * q_out are written, and its other inputs do not matter.  A slot past the pool
+ * is skipped the same way (reported by checked builds); two rows with the same
+ * slot leave either one's key and value.  Angles are positions[t] *
+ * theta^(-2i/rot_dim) reduced in 64 bits, so they hold at any int32 position
+ * (krk_k_rope_kv_attn_decode keeps the reference's 32-bit product).  Hq may be
+ * 0 (q and q_out unused).  q, k, v are only read. */
+KRK_API int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void* k, int64_t k_st, int64_t k_sh,
+                                       void* v, int64_t v_st, int64_t v_sh, int type, void* q_out, int64_t qo_st,
+                                       int64_t qo_sh, void* kc, void* vc, int64_t c_sp, int64_t c_st, int64_t c_sh,
+                                       int cache_type, const int32_t* slots, const int32_t* positions, int T, int Hq,
+                                       int Hkv, int dh, int rot_dim, int num_pages, int page_size, float theta,
+                                       void* stream);
+
+/* Softmax attention of one query token a request over its pages
+ * (src/model.rs:736-760 on a paged cache, with Hq / Hkv query heads sharing
+ * each cache head): with n = lens[b],
+ *   out[b*o_sb + h*o_sh + :] = sum_j p_j v_j,
+ *   p = softmax over j in [max(0, n - window), n) of scale * q_h . k_j
+ * (window 0: every key) and, when lse is not NULL, lse[b*Hq + h] = log of the
+ * softmax's denominator (natural logarithm of the sum of e^(scale * q . k)),
+ * with which partial attentions can be joined.  n counts the query's own
+ * token, so lens is what krk_k_kv_page_plan left.  A request of length 0 gets
+ * zeros and lse -inf.  Lengths past width * page_size are cut there and
+ * negative ones read as 0; keys on pages outside the pool are left out (both
+ * reported by checked builds).  Cache cells past a request's length or before
+ * its window are never used, whatever they hold.
+ * max_len: a bound of the lengths by which the launch is sized, 0 = width *
+ * page_size; it moves the result by rounding at most.  work: krk_attn_paged_work_floats
+ * floats of 16-byte aligned device scratch, with no initial contents, for calls
+ * that do not run at the same time. */
+KRK_API size_t krk_attn_paged_work_floats(int Hq, int Hkv, int dh);
+KRK_API int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void* kc, void* vc, int64_t c_sp,
+                                    int64_t c_st, int64_t c_sh, int cache_type, const int32_t* table,
+                                    int64_t table_ld, int width, int num_pages, int page_size, const int32_t* lens,
+                                    int B, int Hq, int Hkv, int dh, float scale, int window, int max_len, void* out,
+                                    int64_t o_sb, int64_t o_sh, float* lse, float* work, size_t work_floats,
+                                    void* stream);
 
 /* Greedy pick (src/sampler.rs:50-80) per row of logits [B][ld]: repetition
  * penalty on tokens whose bit is set in seen [B][vocab/32] (seen may be NULL;

@@ -75,6 +75,15 @@ _SIGS = {
                                    + [_f32, _vp] + [_i32] * 3 + [_fp, _i64, _i64, _vp]),
     "krk_k_rope_kv_attn_decode_noalloc": (_i32, [_fp] * 7 + [_i32] * 5 + [_f32, _vp]),
     "krk_k_wait_probe": (_i32, [_fp, _i32, _i32, _vp, _vp]),
+    "krk_k_kv_page_plan": (_i32, [_vp] * 3 + [_i64, _i32, _i32, _vp, _vp, _i32, _i32] + [_vp] * 5
+                           + [_i32, _vp, _vp]),
+    "krk_k_kv_page_release": (_i32, [_vp] * 3 + [_i64, _i32, _i32, _vp, _vp, _i32, _i32] + [_vp] * 4),
+    "krk_k_rope_kv_append_paged": (_i32, [_vp, _i64, _i64] * 3 + [_i32, _vp, _i64, _i64, _vp, _vp] + [_i64] * 3
+                                   + [_i32, _vp, _vp] + [_i32] * 7 + [_f32, _vp]),
+    "krk_attn_paged_work_floats": (C.c_size_t, [_i32] * 3),
+    "krk_k_attn_decode_paged": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp] + [_i64] * 3 + [_i32, _vp, _i64]
+                                + [_i32] * 3 + [_vp] + [_i32] * 4 + [_f32, _i32, _i32, _vp, _i64, _i64, _vp, _vp,
+                                                                    C.c_size_t, _vp]),
     # include/krikil_text.h
     "krk_tokenizer_load": (_i32, [C.c_char_p, C.POINTER(_vp)]),
     "krk_tokenizer_free": (_i32, [_vp]),
@@ -97,6 +106,9 @@ for _name, (_res, _args) in _SIGS.items():
 EXPORTED = tuple(_SIGS)
 
 OK, BAD_TOKEN, CONTEXT_OVERFLOW, EMPTY, IO, NOT_FOUND, INVALID, CUDA, CHECK_FAILED = range(9)
+TYPE_F32, TYPE_F16, TYPE_BF16 = range(3)  # KRK_TYPE_*
+# status word of the page planner and the release
+PAGES_EXHAUSTED, PAGES_ROW_FULL, PAGES_ROWS, PAGES_BAD_LENGTH, PAGES_OVERFLOW = 1, 2, 4, 8, 16
 CHECK_TOKEN, CHECK_POSITION, CHECK_TABLE, CHECK_COLUMN = 1, 2, 4, 8  # krk_check_status bits
 
 # krk_state_profile_read classes

@@ -6,11 +6,12 @@ of this library's sm_100a kernels (krk_k_* in include/krikil_cuda.h).
 from __future__ import annotations
 
 import itertools
+import math
 from typing import Optional
 
 import torch
 
-from ._lib import check, lib
+from ._lib import TYPE_BF16, TYPE_F16, TYPE_F32, check, lib
 
 
 def _stream() -> int:
@@ -187,3 +188,181 @@ def greedy(logits: torch.Tensor, seen: Optional[torch.Tensor] = None, penalty: f
     check(lib.krk_k_greedy(logits.data_ptr(), v, v, b, seen.data_ptr() if seen is not None else None, penalty,
                            tok.data_ptr(), _stream()))
     return tok
+
+
+# ------------------------------------------------------ paged key-value cache
+_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+
+
+def _i32_on(dev, **named):
+    for name, t in named.items():
+        if t is not None and not (t.dtype == torch.int32 and t.device == dev and t.is_contiguous()):
+            raise ValueError(f"{name}: expected a contiguous int32 tensor on {dev}")
+
+
+def _elems_on(dev, dims, **named):
+    for name, t in named.items():
+        if t is not None and not (t.device == dev and t.dim() == dims and t.dtype in _TYPES and t.stride(-1) == 1):
+            raise ValueError(f"{name}: expected a float32, float16 or bfloat16 tensor of {dims} dimensions on {dev} "
+                             "whose last dimension is dense")
+
+
+def _cuda_device(t):
+    if not t.is_cuda:
+        raise ValueError("expected CUDA tensors")
+    return t.device
+
+
+def _strides(t, n):
+    """The first n strides, 0 for a dimension of one element (torch leaves any number there)."""
+    return [st if size > 1 else 0 for size, st in zip(t.shape[:n], t.stride())]
+
+
+def _call_on(dev, fn, *args) -> None:
+    """fn(*args, stream) on dev's current stream, with dev current."""
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+        return
+    with torch.cuda.device(dev):
+        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _table_shape(table, dev):
+    if not (table.dtype == torch.int32 and table.device == dev and table.dim() == 2 and table.stride(1) == 1):
+        raise ValueError(f"table: expected an int32 [requests, pages] tensor on {dev} with dense rows")
+    return table.shape
+
+
+def _cache_dims(kc, vc, dev):
+    _elems_on(dev, 4, kc=kc, vc=vc)
+    if kc.dtype != vc.dtype or kc.shape != vc.shape or _strides(kc, 3) != _strides(vc, 3):
+        raise ValueError("kc and vc: expected the same type, shape and strides")
+    return kc.shape
+
+
+def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int, rows: int, lens_out=None,
+                 free_count_out=None):
+    """Plans a step of new_tokens[b] tokens on top of lens[b] (int32 [B]): takes
+    the pages that requests lack from the top of the stack free_pages
+    [num_pages] (free_count int32 [1]) into table [B, width], in place.  Returns
+    (lens_out, free_count_out, cu [B+1], positions [rows], slots [rows], status
+    [1]): the lengths after the step, what is left on the stack, the packed
+    offsets of each request's tokens, and each packed token's position and cache
+    slot (-1 behind the last one).  status is 0, or PAGES_* bits of what does
+    not fit, in which case nothing was taken.  lens_out and free_count_out may be
+    the inputs; they and the others are new tensors when not given."""
+    dev = _cuda_device(table)
+    b, width = _table_shape(table, dev)
+    _i32_on(dev, new_tokens=new_tokens, lens=lens, free_pages=free_pages, free_count=free_count, lens_out=lens_out,
+            free_count_out=free_count_out)
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    if new_tokens.numel() != b or lens.numel() != b or lens_out.numel() != b:
+        raise ValueError(f"new_tokens, lens, lens_out: expected {b} values, one a row of the table")
+    if free_count.numel() != 1 or free_count_out.numel() != 1:
+        raise ValueError("free_count: expected one value")
+    cu = torch.empty(b + 1, device=dev, dtype=torch.int32)
+    positions = torch.empty(rows, device=dev, dtype=torch.int32)
+    slots = torch.empty(rows, device=dev, dtype=torch.int32)
+    status = torch.empty(1, device=dev, dtype=torch.int32)
+    _call_on(dev, lib.krk_k_kv_page_plan, new_tokens.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0),
+             b, width, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size,
+             lens_out.data_ptr(), free_count_out.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+             rows, status.data_ptr())
+    return lens_out, free_count_out, cu, positions, slots, status
+
+
+def kv_page_release(done, lens, table, free_pages, free_count, page_size: int, lens_out=None, free_count_out=None):
+    """Puts the pages of the requests whose done flag (bool or uint8 [B]) is set
+    back on the stack free_pages, in place, and their lengths to 0.  Returns
+    (lens_out, free_count_out, status)."""
+    dev = _cuda_device(table)
+    b, width = _table_shape(table, dev)
+    _i32_on(dev, lens=lens, free_pages=free_pages, free_count=free_count, lens_out=lens_out,
+            free_count_out=free_count_out)
+    if not (done.dtype in (torch.bool, torch.uint8) and done.device == dev and done.is_contiguous()):
+        raise ValueError(f"done: expected a contiguous bool or uint8 tensor on {dev}")
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    if done.numel() != b or lens.numel() != b or lens_out.numel() != b:
+        raise ValueError(f"done, lens, lens_out: expected {b} values, one a row of the table")
+    if free_count.numel() != 1 or free_count_out.numel() != 1:
+        raise ValueError("free_count: expected one value")
+    status = torch.empty(1, device=dev, dtype=torch.int32)
+    _call_on(dev, lib.krk_k_kv_page_release, done.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0), b,
+             width, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size, lens_out.data_ptr(),
+             free_count_out.data_ptr(), status.data_ptr())
+    return lens_out, free_count_out, status
+
+
+def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000.0, rot_dim: Optional[int] = None,
+                         q_out=None):
+    """Rotates q [T, Hq, dh] and k [T, Hkv, dh] by their positions (int32 [T];
+    rotate-half on the first rot_dim elements, all by default) and writes k and
+    v to the slots (int32 [T], -1: padding) of the pages kc, vc [pages,
+    page_size, Hkv, dh].  Strided views are fine as long as dh is dense.
+    Returns the rotated q (q_out, which may be q; padding rows of a given q_out
+    are left as they were).  q may be None."""
+    dev = _cuda_device(k)
+    pages, page_size, hkv, dh = _cache_dims(kc, vc, dev)
+    _elems_on(dev, 3, q=q, k=k, v=v, q_out=q_out)
+    _i32_on(dev, slots=slots, positions=positions)
+    t = k.shape[0]
+    if k.shape != (t, hkv, dh) or v.shape != k.shape or slots.numel() != t or positions.numel() != t:
+        raise ValueError(f"expected k and v of [T, {hkv}, {dh}], slots and positions of [T]")
+    if v.dtype != k.dtype or (q is not None and (q.dtype != k.dtype or q.shape[0] != t or q.shape[2] != dh)):
+        raise ValueError(f"expected q of [T, heads, {dh}] and q, k and v of one type")
+    if q is None:
+        hq, q_args, qo_args = 0, (None, 0, 0), (None, 0, 0)
+    else:
+        if q_out is None:
+            q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise ValueError("q_out: expected q's shape and type")
+        hq = q.shape[1]
+        q_args, qo_args = (q.data_ptr(), *_strides(q, 2)), (q_out.data_ptr(), *_strides(q_out, 2))
+    _call_on(dev, lib.krk_k_rope_kv_append_paged, *q_args, k.data_ptr(), *_strides(k, 2), v.data_ptr(),
+             *_strides(v, 2), _TYPES[k.dtype], *qo_args, kc.data_ptr(), vc.data_ptr(), *_strides(kc, 3),
+             _TYPES[kc.dtype], slots.data_ptr(), positions.data_ptr(), t, hq, hkv, dh,
+             dh if rot_dim is None else rot_dim, pages, page_size, theta)
+    return q_out
+
+
+def attn_paged_work_floats(hq: int, hkv: int, dh: int) -> int:
+    return int(lib.krk_attn_paged_work_floats(hq, hkv, dh))
+
+
+def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, window: int = 0, max_len: int = 0,
+                      out=None, work=None, return_lse: bool = False):
+    """Attention of one token a request, q [B, Hq, dh], over the lens[b] (int32
+    [B]) tokens in its pages table[b] of kc, vc [pages, page_size, Hkv, dh], the
+    last `window` of them if that is not 0.  scale defaults to 1/sqrt(dh);
+    max_len, a bound of the lengths, only sizes the launch.  `work` is scratch
+    (allocated here when not given).  Returns out [B, Hq, dh], or (out, lse)."""
+    dev = _cuda_device(q)
+    pages, page_size, hkv, dh = _cache_dims(kc, vc, dev)
+    _elems_on(dev, 3, q=q, out=out)
+    _i32_on(dev, lens=lens)
+    b, hq = q.shape[:2]
+    rows, width = _table_shape(table, dev)
+    if q.shape[2] != dh or rows != b or lens.numel() != b:
+        raise ValueError(f"expected q of [B, heads, {dh}], a table of B rows and lens of [B]")
+    if out is None:
+        out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("out: expected q's shape and type")
+    lse = torch.empty((b, hq), device=dev, dtype=torch.float32) if return_lse else None
+    if work is None:
+        work = torch.empty(attn_paged_work_floats(hq, hkv, dh), device=dev, dtype=torch.float32)
+    elif not (work.dtype == torch.float32 and work.device == dev and work.is_contiguous()):
+        raise ValueError(f"work: expected a contiguous float32 tensor on {dev}")
+    _call_on(dev, lib.krk_k_attn_decode_paged, q.data_ptr(), *_strides(q, 2), _TYPES[q.dtype],
+             kc.data_ptr(), vc.data_ptr(), *_strides(kc, 3), _TYPES[kc.dtype], table.data_ptr(), table.stride(0),
+             width, pages, page_size, lens.data_ptr(), b, hq, hkv, dh,
+             1.0 / math.sqrt(dh) if scale is None else scale, window, max_len, out.data_ptr(),
+             *_strides(out, 2), lse.data_ptr() if return_lse else None, work.data_ptr(), work.numel())
+    return (out, lse) if return_lse else out

@@ -56,6 +56,18 @@ pub const KRK_CHECK_POSITION: u32 = 2;
 pub const KRK_CHECK_TABLE: u32 = 4;
 pub const KRK_CHECK_COLUMN: u32 = 8;
 
+// element types of the paged key-value cache
+pub const KRK_TYPE_F32: c_int = 0;
+pub const KRK_TYPE_F16: c_int = 1;
+pub const KRK_TYPE_BF16: c_int = 2;
+
+// status bits of krk_k_kv_page_plan and krk_k_kv_page_release
+pub const KRK_PAGES_EXHAUSTED: i32 = 1;
+pub const KRK_PAGES_ROW_FULL: i32 = 2;
+pub const KRK_PAGES_ROWS: i32 = 4;
+pub const KRK_PAGES_BAD_LENGTH: i32 = 8;
+pub const KRK_PAGES_OVERFLOW: i32 = 16;
+
 #[repr(C)]
 pub struct krk_model {
     _private: [u8; 0],
@@ -150,6 +162,31 @@ extern "C" {
                                              kc: *mut c_float, vc: *mut c_float, pos: *const i32,
                                              out: *mut c_float, b: c_int, h: c_int, dh: c_int, ctx: c_int,
                                              split: c_int, theta: c_float, stream: *mut c_void) -> c_int;
+    pub fn krk_k_kv_page_plan(new_tokens: *const i32, lens: *const i32, table: *mut i32, table_ld: i64, b: c_int,
+                              width: c_int, free_pages: *const i32, free_count: *const i32, num_pages: c_int,
+                              page_size: c_int, lens_out: *mut i32, free_count_out: *mut i32, cu_new: *mut i32,
+                              positions: *mut i32, slots: *mut i32, rows: c_int, status: *mut i32,
+                              stream: *mut c_void) -> c_int;
+    pub fn krk_k_kv_page_release(done_mask: *const u8, lens: *const i32, table: *const i32, table_ld: i64,
+                                 b: c_int, width: c_int, free_pages: *mut i32, free_count: *const i32,
+                                 num_pages: c_int, page_size: c_int, lens_out: *mut i32, free_count_out: *mut i32,
+                                 status: *mut i32, stream: *mut c_void) -> c_int;
+    pub fn krk_k_rope_kv_append_paged(q: *mut c_void, q_st: i64, q_sh: i64, k: *mut c_void, k_st: i64, k_sh: i64,
+                                      v: *mut c_void, v_st: i64, v_sh: i64, dtype: c_int, q_out: *mut c_void,
+                                      qo_st: i64, qo_sh: i64, kc: *mut c_void, vc: *mut c_void, c_sp: i64,
+                                      c_st: i64, c_sh: i64, cache_type: c_int, slots: *const i32,
+                                      positions: *const i32, t: c_int, hq: c_int, hkv: c_int, dh: c_int,
+                                      rot_dim: c_int, num_pages: c_int, page_size: c_int, theta: c_float,
+                                      stream: *mut c_void) -> c_int;
+    /// Returns a size, not a status.
+    pub fn krk_attn_paged_work_floats(hq: c_int, hkv: c_int, dh: c_int) -> usize;
+    pub fn krk_k_attn_decode_paged(q: *mut c_void, q_sb: i64, q_sh: i64, dtype: c_int, kc: *mut c_void,
+                                   vc: *mut c_void, c_sp: i64, c_st: i64, c_sh: i64, cache_type: c_int,
+                                   table: *const i32, table_ld: i64, width: c_int, num_pages: c_int,
+                                   page_size: c_int, lens: *const i32, b: c_int, hq: c_int, hkv: c_int, dh: c_int,
+                                   scale: c_float, window: c_int, max_len: c_int, out: *mut c_void, o_sb: i64,
+                                   o_sh: i64, lse: *mut c_float, work: *mut c_float, work_floats: usize,
+                                   stream: *mut c_void) -> c_int;
     pub fn krk_k_wait_probe(src16: *const c_float, polls: c_int, copy: c_int, status: *mut i32,
                             stream: *mut c_void) -> c_int;
     pub fn krk_k_greedy(logits: *const c_float, ld: i64, vocab: c_int, b: c_int, seen: *mut u32, penalty: c_float,

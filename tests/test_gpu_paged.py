@@ -1,0 +1,740 @@
+"""The paged key-value cache on the GPU, against plain 64-bit implementations.
+
+Tolerances count roundings.  With u = 2^-24 (half a step of float32) and h the
+output type's half step (finfo.eps / 2):
+
+append: cos and sin of a reduced angle are off by at most 3u (the fraction of a
+turn rounded to 32 bits, times 2 pi) + 4u (two units in the last place) + 8u
+(two roundings to 64 bits of 2^31 / (2 pi) turns) + 6u (the same in the reference
+here); each product and the sum round once more: 24u (|a| + |b|), and h |result|
+when it is stored.
+
+attention: a score, a sum of dh products, is off by at most s = 2 (dh + 8) u
+scale sum_d |q_d k_d| (2 for accumulators that may round towards zero); every
+weight by 2 s + 16u relative, the two sums of n weights by 2 n u each; so the
+result by (2 s + 2 (n + 32) u) max |v| and h |result|, and the logarithm by s +
+2 (n + 32) u + 2u |lse|.  Exact tests (whole-number values under equal weights)
+hold the long sums."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover
+    pytest.skip("no CUDA device", allow_module_level=True)
+
+from krikil_rs_b200 import kernels as K, launch_count  # noqa: E402
+from krikil_rs_b200._lib import (PAGES_BAD_LENGTH, PAGES_EXHAUSTED, PAGES_OVERFLOW, PAGES_ROW_FULL,  # noqa: E402
+                                 PAGES_ROWS)
+
+DEV = torch.device("cuda:0")
+U = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
+IDS = ["f32", "f32-f16", "f32-bf16", "f16", "bf16"]
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def i32(values):
+    return torch.tensor(values, device=DEV, dtype=torch.int32)
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+class Pool:
+    """Requests of the given lengths on random pages; every cell that no request holds is NaN, unused
+    table entries are far outside the pool."""
+
+    def __init__(self, lens, hkv, dh, page, cache, seed, spare=3, layout="pthd", pad=0, fill=None):
+        g = gen(seed)
+        self.lens_h, self.page = list(lens), page
+        need = [-(-n // page) for n in lens]
+        self.pages = sum(need) + spare
+        width = max(1, max(need))
+        order = torch.randperm(self.pages, generator=g, device=DEV).tolist()
+        rows, at = [], 0
+        for n in need:
+            rows.append(order[at:at + n] + [2 ** 30] * (width - n))
+            at += n
+        self.table, self.lens = i32(rows), i32(lens)
+        full = torch.full((2, self.pages, page, hkv, dh + pad), float("nan"), device=DEV, dtype=cache)
+        if layout == "phtd":
+            full = torch.full((2, self.pages, hkv, page, dh + pad), float("nan"), device=DEV, dtype=cache)
+            full = full.transpose(2, 3)
+        self.kc, self.vc = full[0][..., :dh], full[1][..., :dh]
+        self.k, self.v = [], []  # per request [n, hkv, dh], as stored
+        for b, n in enumerate(lens):
+            if fill is None:
+                k = torch.randn(n, hkv, dh, generator=g, device=DEV).to(cache)
+                v = torch.randn(n, hkv, dh, generator=g, device=DEV).to(cache)
+            else:
+                k, v = fill(n, hkv, dh, g)
+                k, v = k.to(cache), v.to(cache)
+            self.k.append(k)
+            self.v.append(v)
+            if n:
+                j = torch.arange(n, device=DEV)
+                where = self.table[b, j // page].long(), j % page
+                self.kc[where], self.vc[where] = k, v
+
+
+def attn_reference(pool, q, scale, window=0, keep=None):
+    """out, lse and their tolerances in 64 bits, request by request."""
+    b, hq, dh = q.shape
+    out = torch.zeros(b, hq, dh, device=DEV, dtype=torch.float64)
+    lse = torch.full((b, hq), -math.inf, device=DEV, dtype=torch.float64)
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    for i, n in enumerate(pool.lens_h):
+        first = max(0, n - window) if window else 0
+        js = [j for j in range(first, n) if keep is None or keep(i, j)]
+        if not js:
+            continue
+        k, v = pool.k[i][js].double(), pool.v[i][js].double()
+        hkv = k.shape[1]
+        share = hq // hkv
+        qi = q[i].double().reshape(hkv, share, dh)
+        x = torch.einsum("hgd,jhd->hgj", qi, k) * scale
+        size = torch.einsum("hgd,jhd->hgj", qi.abs(), k.abs()).amax(-1) * abs(scale)
+        p = torch.softmax(x, -1)
+        out[i] = torch.einsum("hgj,jhd->hgd", p, v).reshape(hq, dh)
+        lse[i] = torch.logsumexp(x, -1).reshape(hq)
+        s = 2 * (dh + 8) * U * size
+        n = len(js)
+        top = v.abs().amax((0, 2))[:, None]
+        tol[i] = (((2 * s + 2 * (n + 32) * U) * top).reshape(hq, 1) + half_step(q.dtype) * out[i].abs()
+                  + torch.finfo(q.dtype).tiny)
+        ltol[i] = (s + 2 * (n + 32) * U).reshape(hq) + 2 * U * lse[i].abs()
+    return out, lse, tol, ltol
+
+
+def check_attn(pool, q, window=0, scale=None, keep=None, **kw):
+    sc = 1 / math.sqrt(q.shape[2]) if scale is None else scale
+    out, lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, scale=scale, window=window,
+                                   return_lse=True, **kw)
+    ref, rl, tol, ltol = attn_reference(pool, q, sc, window, keep)
+    empty = rl == -math.inf
+    assert torch.equal(lse[empty], torch.full_like(lse[empty], -math.inf))
+    assert torch.equal(out[empty], torch.zeros_like(out[empty]))
+    bad = (out.double() - ref).abs() > tol
+    assert not bad.any() and not out.isnan().any(), ((out.double() - ref).abs() / tol).nan_to_num(math.inf).max().item()
+    off = (lse.double() - rl).abs()[~empty]
+    assert (off <= ltol[~empty]).all(), (off / ltol[~empty]).max().item()
+    return out, lse
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page", [(8, 8, 76, 16), (8, 8, 64, 8), (32, 8, 128, 64), (4, 4, 4, 1),
+                                            (7, 1, 80, 32), (12, 4, 96, 4), (16, 2, 256, 16), (33, 1, 192, 2),
+                                            (40, 2, 36, 128), (9, 1, 200, 16), (3, 3, 252, 2)])
+def test_attention_types_heads_and_lengths(act, cache, hq, hkv, dh, page):
+    lens = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 100, 127, 129, 255, 300]
+    pool = Pool(lens, hkv, dh, page, cache, seed=dh + page)
+    q = torch.randn(len(lens), hq, dh, generator=gen(5), device=DEV).to(act)
+    check_attn(pool, q)
+    check_attn(pool, q, window=40)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page,lens", [
+    (8, 8, 64, 16, [5000, 1, 0, 777]), (32, 8, 128, 16, [4097]), (4, 1, 76, 32, [1] * 300 + [9000]),
+    (16, 2, 256, 1, [2500, 3]), (2, 2, 128, 4096, [10000]), (64, 1, 64, 8, [3001, 2999])])
+@pytest.mark.parametrize("window", [0, 1, 1029])
+def test_equal_weights_of_whole_numbers_are_exact(act, cache, hq, hkv, dh, page, lens, window):
+    """With q = 0 every weight is 1 and the values' sums, whole numbers below 2^24, are exact in any
+    order: a key that is left out, read twice or read from another page shows.  The quotient is off by
+    the reciprocal's and the product's rounding (2u each, with room for an approximate reciprocal of
+    one unit more) and by the store."""
+    def fill(n, h, d, g):
+        return (torch.randn(n, h, d, generator=g, device=DEV),
+                torch.randint(-8, 9, (n, h, d), generator=g, device=DEV).float())
+    pool = Pool(lens, hkv, dh, page, cache, seed=len(lens) + dh, fill=fill)
+    q = torch.zeros(len(lens), hq, dh, device=DEV, dtype=act)
+    out, lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, window=window, return_lse=True)
+    for i, n in enumerate(lens):
+        first = max(0, n - window) if window else 0
+        seen = pool.v[i][first:].double().sum(0).repeat_interleave(hq // hkv, 0) / max(1, n - first)
+        tol = (8 * U + half_step(act)) * seen.abs() + torch.finfo(act).tiny
+        assert ((out[i].double() - seen).abs() <= tol).all(), (i, n)
+        want = math.log(n - first) if n else -math.inf
+        assert torch.allclose(lse[i].double(), torch.full_like(lse[i].double(), want), rtol=8 * U, atol=8 * U)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("layout,pad,hq,hkv,dh", [("pthd", 0, 8, 4, 76), ("phtd", 0, 8, 4, 76), ("pthd", 4, 8, 4, 76),
+                                                  ("phtd", 4, 6, 2, 64), ("phtd", 0, 32, 8, 128),
+                                                  ("pthd", 52, 4, 1, 12), ("phtd", 8, 16, 2, 128)])
+def test_attention_layouts_and_strides(act, cache, layout, pad, hq, hkv, dh):
+    lens = [37, 0, 200, 129, 64]
+    pool = Pool(lens, hkv, dh, 16, cache, seed=3, layout=layout, pad=pad)
+    packed = torch.randn(len(lens), (hq + 2 * hkv) * dh + 4, generator=gen(6), device=DEV).to(act)
+    q = packed[:, 4:4 + hq * dh].unflatten(1, (hq, dh))
+    whole = torch.full((len(lens) + 2, hq + 3, dh + 12), 7.0, device=DEV, dtype=act)
+    out = whole[1:-1, 1:hq + 1, 4:4 + dh]
+    got, lse = check_attn(pool, q, out=out)
+    assert got.data_ptr() == out.data_ptr()
+    inside = torch.zeros_like(whole, dtype=torch.bool)
+    inside[1:-1, 1:hq + 1, 4:4 + dh] = True
+    assert (whole[~inside] == 7.0).all()  # nothing around the rows is written
+    same, _ = check_attn(pool, q.contiguous())
+    assert torch.equal(same, out)  # where rows lie does not change them
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_table_rows_may_be_strided(act, cache):
+    pool = Pool([50, 3, 90], 2, 64, 8, cache, seed=9)
+    q = torch.randn(3, 4, 64, generator=gen(1), device=DEV).to(act)
+    a = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens)
+    wide = torch.full((3, pool.table.shape[1] + 5), -9, device=DEV, dtype=torch.int32)
+    wide[:, :pool.table.shape[1]] = pool.table
+    assert torch.equal(a, K.attn_decode_paged(q, pool.kc, pool.vc, wide[:, :pool.table.shape[1]], pool.lens))
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_large_scores_and_scales(act, cache):
+    """Scores in the thousands (one key takes all the weight), a negative scale, a scale of 0."""
+    pool = Pool([1, 70, 400], 2, 64, 16, cache, seed=4)
+    q = (100 * torch.randn(3, 6, 64, generator=gen(2), device=DEV)).to(act)
+    for scale in (1.0, -1.0, 1e-3, 0.0):
+        check_attn(pool, q, scale=scale)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_small_and_uneven_queries(act, cache):
+    """Queries whose elements differ a thousandfold, large ones and tiny ones, under a scale that brings the scores
+    back to one: parts of q that a shorter type would drop count."""
+    pool = Pool([130, 17], 2, 64, 16, cache, seed=14)
+    q = torch.randn(2, 4, 64, generator=gen(3), device=DEV)
+    q[:, :, 1::2] *= 1e-3
+    for size, scale in ((1.0, None), (2.0 ** -12, 512.0), (2.0 ** 10, 2.0 ** -13)):
+        check_attn(pool, (q * size).to(act), scale=scale)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_one_dominant_key_and_a_long_faint_tail(act, cache):
+    """One key of weight 1 and thousands near 2^-20: together they matter, each is faint."""
+    n, dh = 6000, 64
+    def fill(n, h, d, g):
+        k = torch.zeros(n, h, d, device=DEV)
+        k[:, :, 0] = -14.0
+        k[n // 3, :, 0] = 0.0
+        return k, torch.randn(n, h, d, generator=g, device=DEV)
+    pool = Pool([n, 40], 1, dh, 16, cache, seed=8, fill=fill)
+    q = torch.zeros(2, 8, dh, device=DEV, dtype=act)
+    q[:, :, 0] = 1.0
+    check_attn(pool, q, scale=1.0)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_infinities_and_nan_stay_where_they_are(act, cache):
+    """A NaN key reaches its own request and cache head alone; a key of score -inf gets weight 0, and a row
+    of nothing but -inf scores gives zeros; an infinite value of a visible key leaves its own column not finite
+    (infinite or, where the product of a weight's parts is undefined, NaN) and nothing else."""
+    def make(seed):
+        return Pool([64, 90, 33, 5], 2, 64, 16, cache, seed=seed)
+    pool = make(7)
+    q = torch.rand(4, 4, 64, generator=gen(4), device=DEV).to(act) + 0.5
+    clean, _ = check_attn(pool, q)
+    def at(b, j):
+        return int(pool.table[b, j // 16]), j % 16
+    pool.kc[at(1, 40)][0] = float("nan")
+    out = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens)
+    assert out[1, :2].isnan().all()
+    others = torch.ones(4, 4, dtype=torch.bool, device=DEV)
+    others[1, :2] = False
+    assert torch.equal(out[others], clean[others])
+    pool = make(7)
+    pool.kc[at(2, 10)][1] = -float("inf")
+    out, lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, return_lse=True)
+    pool.k[2][10, 1] = -1e4  # a weight of 0 in 32 bits
+    ref, rl, tol, ltol = attn_reference(pool, q, 1 / 8)
+    # sum |q k| of the key that was moved away has no part in the others' rounding
+    assert ((out.double() - ref).abs() <= tol).all() and not lse.isnan().any()
+    pool = make(7)
+    for j in range(5):
+        pool.kc[at(3, j)][:] = -float("inf")
+    out, lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, return_lse=True)
+    assert (out[3] == 0).all() and (lse[3] == -math.inf).all()
+    assert torch.equal(out[:3], clean[:3])
+    pool = make(7)
+    pool.vc[at(0, 3)][0, 5] = float("inf")
+    out = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens)
+    assert not out[0, :2, 5].isfinite().any()
+    out[0, :2, 5] = clean[0, :2, 5]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("page", [4, 16, 64])
+def test_pages_outside_the_pool_are_left_out(act, cache, page):
+    lens = [130, 64, 200]
+    pool = Pool(lens, 2, 64, page, cache, seed=2)
+    q = torch.randn(3, 4, 64, generator=gen(8), device=DEV).to(act)
+    lost = {(0, 1): -1, (0, 64 // page): pool.pages, (1, 0): 2 ** 31 - 1, (2, 128 // page): -2 ** 31}
+    for (b, i), bad in lost.items():
+        pool.table[b, i] = bad
+    check_attn(pool, q, keep=lambda b, j: (b, j // page) not in lost)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_lengths_outside_the_table(act, cache):
+    """Longer than width * page_size: cut there; negative: empty."""
+    pool = Pool([64, 64, 64], 2, 64, 16, cache, seed=2)
+    q = torch.randn(3, 4, 64, generator=gen(8), device=DEV).to(act)
+    want = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens)
+    got = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, i32([65, 2 ** 31 - 1, -5]))
+    assert torch.equal(got[:2], want[:2]) and (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_attention_is_repeatable_and_the_bound_only_sizes_it(act, cache):
+    pool = Pool([900, 0, 3000, 12], 2, 128, 16, cache, seed=12)
+    q = torch.randn(4, 8, 128, generator=gen(3), device=DEV).to(act)
+    first, _ = check_attn(pool, q)
+    work = torch.full((K.attn_paged_work_floats(8, 2, 128) + 8,), float("nan"), device=DEV)
+    for _ in range(3):
+        again = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=work)
+        assert torch.equal(first, again)
+    for bound in (1, 100, 3000, 2 ** 31 - 1):  # even a bound that is too small
+        check_attn(pool, q, max_len=bound, work=work)
+
+
+def test_scratch_that_is_too_small_is_refused():
+    pool = Pool([64], 2, 64, 16, F32, seed=2)
+    q = torch.randn(1, 4, 64, device=DEV)
+    need = K.attn_paged_work_floats(4, 2, 64)
+    if need:
+        with pytest.raises(Exception, match="work"):
+            K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=torch.empty(need - 1, device=DEV))
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F32), (F32, BF16), (BF16, BF16), (F16, F16)])
+def test_attention_replayed_from_a_graph_on_another_stream(act, cache):
+    """A captured call follows the lengths, table and queries that it finds at replay, beside eager calls of the
+    same tensors with their own scratch."""
+    lens = [10, 0, 700, 64]
+    pool = Pool([800] * 4, 2, 64, 16, cache, seed=21)
+    q = torch.randn(4, 8, 64, generator=gen(3), device=DEV).to(act)
+    now = i32(lens)
+    s = torch.cuda.Stream()
+    out, work = torch.empty_like(q), torch.empty(K.attn_paged_work_floats(8, 2, 64), device=DEV)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now, out=out, work=work, max_len=800)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now, out=out, work=work, max_len=800)
+    for step, lens in enumerate(([10, 0, 700, 64], [0, 0, 0, 0], [800, 800, 800, 800], [1, 2, 3, 799])):
+        now.copy_(i32(lens))
+        q.copy_(torch.randn(4, 8, 64, generator=gen(step), device=DEV).to(act))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+        eager = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now, max_len=800)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        pool.lens_h = lens
+        ref, _, tol, _ = attn_reference(pool, q, 1 / 8)
+        assert ((out.double() - ref).abs() <= tol).all()
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^31 elements a cache, of which the last and first pages are used."""
+    hkv, dh, page = 8, 128, 16
+    pages = 2 ** 31 // (hkv * dh * page) + 40
+    if torch.cuda.mem_get_info()[0] < 5 * pages * page * hkv * dh:
+        pytest.skip("not enough memory")
+    kc = torch.empty(pages, page, hkv, dh, device=DEV, dtype=BF16)
+    vc = torch.empty_like(kc)
+    n = 100
+    rows = [[pages - 1 - i for i in range(7)], [0, pages - 9, 1, pages - 10, 2, pages - 11, 3]]
+    table, lens = i32(rows), i32([0, 0])
+    k = torch.randn(2 * n, hkv, dh, generator=gen(1), device=DEV).to(BF16)
+    v = torch.randn(2 * n, hkv, dh, generator=gen(2), device=DEV).to(BF16)
+    slots = i32([rows[b][j // page] * page + j % page for b in range(2) for j in range(n)])
+    K.rope_kv_append_paged(None, k, v, kc, vc, slots, torch.zeros_like(slots))  # position 0 turns nothing
+    q = torch.randn(2, 32, dh, generator=gen(3), device=DEV).to(BF16)
+    pool = Pool.__new__(Pool)
+    pool.kc, pool.vc, pool.table, pool.lens_h, pool.lens = kc, vc, table, [n, n], i32([n, n])
+    pool.k, pool.v = [k[:n], k[n:]], [v[:n], v[n:]]
+    check_attn(pool, q)
+
+
+# ------------------------------------------------------------------ RoPE + append
+def rotated(x, positions, rot, theta=10000.0):
+    """The rotation in 64 bits, and its tolerance before the store."""
+    x = x.double()
+    half = rot // 2
+    if half == 0:
+        return x, torch.zeros_like(x)
+    rate = theta ** (-2.0 * torch.arange(half, device=DEV, dtype=torch.float64) / rot)
+    turn = positions.double()[:, None] * rate
+    c, s = torch.cos(turn)[:, None], torch.sin(turn)[:, None]
+    a, b = x[..., :half], x[..., half:rot]
+    t = 24 * U * (a.abs() + b.abs())
+    return (torch.cat([a * c - b * s, b * c + a * s, x[..., rot:]], -1),
+            torch.cat([t, t, torch.zeros_like(x[..., rot:])], -1))
+
+
+def close(got, ref, tol):
+    off = (got.double() - ref).abs()
+    lim = tol + half_step(got.dtype) * (ref.abs() + tol) + torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps
+    assert (off <= lim).all(), (off - lim).max().item()
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("t,hq,hkv,dh,rot,page,far", [
+    (1, 8, 8, 76, 76, 16, 2048), (37, 32, 8, 128, 128, 16, 10 ** 6), (300, 4, 1, 64, 32, 1, 2 ** 31 - 1),
+    (65, 7, 7, 80, 40, 8, 32768), (5, 2, 2, 256, 256, 256, 10 ** 6), (129, 1, 1, 4, 2, 4, 100),
+    (40, 6, 2, 96, 0, 16, 1000), (1111, 12, 4, 192, 190, 32, 5000)])
+def test_append_types_heads_and_positions(act, cache, t, hq, hkv, dh, rot, page, far):
+    g = gen(t + dh)
+    pages = -(-t // page) + 2
+    packed = torch.randn(t, (hq + 2 * hkv) * dh, generator=g, device=DEV).to(act)
+    q, k, v = (x.unflatten(1, (-1, dh)) for x in packed.split([hq * dh, hkv * dh, hkv * dh], 1))
+    before = packed.clone()
+    slots = torch.randperm(pages * page, generator=g, device=DEV)[:t].int()
+    positions = torch.randint(0, far, (t,), generator=g, device=DEV, dtype=torch.int64).int()
+    kc = torch.full((pages, page, hkv, dh), 9.0, device=DEV, dtype=cache)
+    vc = torch.full_like(kc, -9.0)
+    got = K.rope_kv_append_paged(q, k, v, kc, vc, slots, positions, rot_dim=rot)
+    assert torch.equal(packed, before)
+    close(got, *rotated(q, positions, rot))
+    ref, tol = rotated(k, positions, rot)
+    close(kc.view(-1, hkv, dh)[slots.long()], ref, tol)
+    assert torch.equal(vc.view(-1, hkv, dh)[slots.long()], v.to(cache))
+    rest = torch.ones(pages * page, dtype=torch.bool, device=DEV)
+    rest[slots.long()] = False
+    assert (kc.view(-1, hkv, dh)[rest] == 9.0).all() and (vc.view(-1, hkv, dh)[rest] == -9.0).all()
+    # in place: the same values
+    K.rope_kv_append_paged(q, k, v, kc, vc, slots, positions, rot_dim=rot, q_out=q)
+    assert torch.equal(q, got) and torch.equal(packed[:, hq * dh:], before[:, hq * dh:])
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("pad,dh,layout", [(0, 76, "phtd"), (4, 76, "pthd"), (12, 64, "phtd"), (8, 128, "phtd")])
+def test_append_layouts_padding_and_bad_slots(act, cache, pad, dh, layout):
+    """Rows behind the last sequence (slot -1) and slots outside the pool write nothing, NaN in them included;
+    cells between the heads of a padded layout are left alone."""
+    t, hq, hkv, page, pages = 23, 6, 3, 8, 5
+    shape = (pages, page, hkv, dh + pad) if layout == "pthd" else (pages, hkv, page, dh + pad)
+    raw = torch.full((2,) + shape, 5.0, device=DEV, dtype=cache)
+    view = raw if layout == "pthd" else raw.transpose(2, 3)
+    kc, vc = view[0][..., :dh], view[1][..., :dh]
+    g = gen(77)
+    q = torch.randn(t, hq, dh + 4, generator=g, device=DEV).to(act)[..., :dh]
+    k = torch.randn(hkv, t, dh, generator=g, device=DEV).to(act).transpose(0, 1)
+    v = torch.randn(t, hkv, dh + 8, generator=g, device=DEV).to(act)[..., 8:]
+    slots = torch.randperm(pages * page, generator=g, device=DEV)[:t].int()
+    skip = [3, 4, 11, 20, 21, 22]
+    for i, s in zip(skip, (-1, pages * page, 2 ** 31 - 1, -1, -2 ** 31, -1)):
+        slots[i] = s
+    q[skip[-1]] = float("nan")
+    k[skip[-1]] = float("nan")
+    positions = torch.randint(0, 999, (t,), generator=g, device=DEV, dtype=torch.int32)
+    positions[skip[0]] = -7
+    q_out = torch.full((t, hq, dh), 3.0, device=DEV, dtype=act)
+    K.rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta=500000.0, q_out=q_out)
+    keep = [i for i in range(t) if i not in skip]
+    assert (q_out[skip] == 3.0).all()
+    close(q_out[keep], *rotated(q[keep], positions[keep], dh, 500000.0))
+    p, o = slots[keep].long() // page, slots[keep].long() % page
+    close(kc[p, o], *rotated(k[keep], positions[keep], dh, 500000.0))
+    assert torch.equal(vc[p, o], v[keep].to(cache))
+    kc[p, o], vc[p, o] = 5.0, 5.0
+    assert (raw == 5.0).all()
+
+
+def test_append_stores_the_nearest_values():
+    """float32 values into 16-bit caches: the values' own rounding (to even at ties, overflow to infinity), the
+    last of what fits; NaN and infinities stay."""
+    x = torch.tensor([1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8, 65504.0, 65519.9, 65520.0, 3.4e38, float("inf"),
+                      -float("inf"), float("nan"), 2.0 ** -24, 2.0 ** -25, 2.0 ** -26, -0.0, 2.0 ** -140, 1e-8, 3.0],
+                     device=DEV)
+    for cache in (F16, BF16):
+        k = x.reshape(1, 1, 16)
+        kc, vc = (torch.zeros(1, 1, 1, 16, device=DEV, dtype=cache) for _ in range(2))
+        K.rope_kv_append_paged(None, k, k, kc, vc, i32([0]), i32([5]), rot_dim=0)
+        for c in (kc, vc):
+            assert torch.equal(c.view(-1).view(torch.int16)[x == x], x.to(cache).view(torch.int16)[x == x])
+            assert c.view(-1)[8].isnan()
+
+
+# ------------------------------------------------------------------ pages
+class Books:
+    """The same bookkeeping in plain Python."""
+
+    def __init__(self, batch, width, num_pages, page, seed):
+        rng = np.random.default_rng(seed)
+        self.page, self.width = page, width
+        self.free = [int(x) for x in rng.permutation(num_pages)]
+        self.num_pages = num_pages
+        self.lens = [0] * batch
+        self.rows = [[] for _ in range(batch)]
+
+    def fits(self, new, rows):
+        need, st = 0, 0
+        for b, n in enumerate(new):
+            want = -(-(self.lens[b] + n) // self.page)
+            st |= PAGES_ROW_FULL if want > self.width else 0
+            need += want - len(self.rows[b])
+        return st | (PAGES_EXHAUSTED if need > len(self.free) else 0) | (PAGES_ROWS if sum(new) > rows else 0)
+
+    def plan(self, new):
+        positions, slots = [], []
+        for b, n in enumerate(new):
+            while len(self.rows[b]) < -(-(self.lens[b] + n) // self.page):
+                self.rows[b].append(self.free.pop())
+            for i in range(self.lens[b], self.lens[b] + n):
+                positions.append(i)
+                slots.append(self.rows[b][i // self.page] * self.page + i % self.page)
+            self.lens[b] += n
+        return positions, slots
+
+    def release(self, done):
+        for b, d in enumerate(done):
+            if d:
+                self.free += self.rows[b]
+                self.rows[b], self.lens[b] = [], 0
+
+
+def device_books(books, batch):
+    free = torch.full((books.num_pages,), -1, device=DEV, dtype=torch.int32)
+    free[:len(books.free)] = i32(books.free)
+    return {"lens": torch.zeros(batch, device=DEV, dtype=torch.int32), "free": free,
+            "count": i32([len(books.free)]),
+            "table": torch.full((batch, books.width), -1, device=DEV, dtype=torch.int32)}
+
+
+def same_books(d, books):
+    assert d["lens"].tolist() == books.lens and d["count"].item() == len(books.free)
+    assert d["free"][:len(books.free)].tolist() == books.free
+    table = d["table"].tolist()
+    for b, row in enumerate(books.rows):
+        assert table[b][:len(row)] == row
+
+
+@pytest.mark.parametrize("batch,width,num_pages,page,most,rows", [
+    (1, 4, 4, 16, 30, 64), (3, 8, 20, 1, 5, 20), (61, 33, 900, 64, 300, 20000), (1024, 5, 3000, 16, 3, 2048),
+    (2500, 3, 7000, 8, 2, 6000), (5, 600, 2500, 16, 6000, 40000), (70, 20, 1000, 4, 40, 4096)])
+def test_planned_steps_match_plain_books(batch, width, num_pages, page, most, rows):
+    """Steps of random new tokens and releases, in place: pages, slots, positions and lengths as in plain Python,
+    and steps that do not fit leave everything as it was."""
+    rng = np.random.default_rng(batch)
+    books = Books(batch, width, num_pages, page, seed=batch)
+    d = device_books(books, batch)
+    refusals = 0
+    for step in range(14):
+        if step % 3 == 2:
+            done = rng.random(batch) < 0.4
+            K.kv_page_release(torch.tensor(done, device=DEV), d["lens"], d["table"], d["free"], d["count"], page,
+                              lens_out=d["lens"], free_count_out=d["count"])
+            books.release(done)
+            same_books(d, books)
+        new = rng.integers(0, most + 1, batch)
+        if step % 4 == 0:
+            new[rng.random(batch) < 0.7] = 0
+        new = [int(x) for x in new]
+        want = books.fits(new, rows)
+        before = d["table"].clone()
+        _, _, cu, positions, slots, status = K.kv_page_plan(i32(new), d["lens"], d["table"], d["free"], d["count"],
+                                                            page, rows, lens_out=d["lens"],
+                                                            free_count_out=d["count"])
+        assert status.item() == want
+        if want:
+            refusals += 1
+            assert torch.equal(d["table"], before) and not cu.any() and (slots == -1).all() and not positions.any()
+        else:
+            p, s = books.plan(new)
+            assert cu.tolist() == [0] + np.cumsum(new).tolist()
+            assert positions[:len(p)].tolist() == p and not positions[len(p):].any()
+            assert slots[:len(s)].tolist() == s and (slots[len(s):] == -1).all()
+        same_books(d, books)
+    assert refusals < 14
+
+
+def test_page_requests_that_do_not_fit():
+    d = dict(lens=i32([3, 0]), table=i32([[4, 5], [6, 7]]), free=i32([0, 1, 2, 3]), count=i32([2]))
+
+    def plan(new, rows=64, **kw):
+        a = dict(d, **kw)
+        out = K.kv_page_plan(i32(new), a["lens"], a["table"], a["free"], a["count"], 4, rows)
+        return out[5].item(), out
+
+    assert plan([1, 4])[0] == 0
+    st, out = plan([2, 8])
+    assert st == PAGES_EXHAUSTED and out[0].tolist() == [3, 0] and out[1].item() == 2
+    assert plan([6, 0])[0] == PAGES_ROW_FULL
+    assert plan([1, 4], rows=4)[0] == PAGES_ROWS and plan([1, 4], rows=5)[0] == 0
+    assert plan([0, 0], rows=0)[0] == 0
+    assert plan([-1, 1])[0] == PAGES_BAD_LENGTH and plan([1, 1], lens=i32([-3, 0]))[0] & PAGES_BAD_LENGTH
+    assert plan([0, 0], count=i32([5]))[0] == PAGES_BAD_LENGTH and plan([0, 0], count=i32([-1]))[0] & PAGES_BAD_LENGTH
+    big = 2 ** 31 - 1
+    assert plan([big, big])[0] == PAGES_ROW_FULL | PAGES_ROWS | PAGES_EXHAUSTED
+    assert d["table"].tolist() == [[4, 1], [0, 7]] or d["table"].tolist() == [[4, 5], [1, 7]]
+
+    def release(done, lens, count):
+        free = d["free"].clone()
+        out = K.kv_page_release(torch.tensor(done, device=DEV), i32(lens), d["table"], free, i32([count]), 4)
+        return out[2].item(), out[0].tolist(), out[1].item(), free.tolist()
+
+    assert release([True, False], [3, 8], 2) == (0, [0, 8], 3, [0, 1, 4, 3])
+    assert release([True, True], [3, 8], 2) == (PAGES_OVERFLOW, [3, 8], 2, [0, 1, 2, 3])
+    assert release([True, False], [9, 8], 0)[0] == PAGES_BAD_LENGTH  # more than its row holds
+    assert release([True, False], [-1, 8], 0)[0] == PAGES_BAD_LENGTH
+    assert release([False, False], [-1, 99], 0) == (0, [-1, 99], 0, [0, 1, 2, 3])
+    assert release([False, False], [1, 1], 5)[0] & PAGES_BAD_LENGTH
+
+
+# ------------------------------------------------------------------ together
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page", [(8, 8, 76, 16), (8, 2, 128, 8)])
+def test_serving_steps_of_requests_that_come_and_go(act, cache, hq, hkv, dh, page):
+    """A small server: two layers, six request rows, prompts admitted and finished at different times, one token
+    a step for the rest, padded token rows.  Every decode step's attention is that of plain attention over each
+    request's own keys and values, kept outside; the steps of single tokens run from one captured graph."""
+    batch, width, rows, layers = 6, 12, 96, 2
+    g = gen(100 + dh)
+    rng = np.random.default_rng(dh)
+    books = Books(batch, width, 50, page, seed=1)
+    d = device_books(books, batch)
+    pools = [[torch.full((50, page, hkv, dh), float("nan"), device=DEV, dtype=cache) for _ in range(2)]
+             for _ in range(layers)]
+    kept = [[[[], []] for _ in range(batch)] for _ in range(layers)]
+    packed = torch.zeros(layers, rows, (hq + 2 * hkv) * dh, device=DEV, dtype=act)
+    new_d, done_d = torch.zeros(batch, device=DEV, dtype=torch.int32), torch.zeros(batch, device=DEV, dtype=torch.bool)
+    last = torch.zeros(batch, hq, dh, device=DEV, dtype=act)
+    outs = [torch.zeros(batch, hq, dh, device=DEV, dtype=act) for _ in range(layers)]
+    q_outs = [torch.zeros(rows, hq, dh, device=DEV, dtype=act) for _ in range(layers)]
+    got = {}
+
+    def step():
+        K.kv_page_release(done_d, d["lens"], d["table"], d["free"], d["count"], page, lens_out=d["lens"],
+                          free_count_out=d["count"])
+        _, _, cu, positions, slots, status = K.kv_page_plan(new_d, d["lens"], d["table"], d["free"], d["count"],
+                                                            page, rows, lens_out=d["lens"],
+                                                            free_count_out=d["count"])
+        for l in range(layers):
+            q, k, v = (x.unflatten(1, (-1, dh)) for x in packed[l].split([hq * dh, hkv * dh, hkv * dh], 1))
+            K.rope_kv_append_paged(q, k, v, *pools[l], slots, positions, q_out=q_outs[l])
+            torch.index_select(q_outs[l], 0, (cu[1:] - 1).clamp_min(0), out=last)
+            K.attn_decode_paged(last, *pools[l], d["table"], d["lens"], out=outs[l], max_len=width * page)
+        got.update(status=status, cu=cu, positions=positions)
+
+    graph = None
+    for n in range(14):
+        done = [books.lens[b] > 0 and rng.random() < 0.15 for b in range(batch)]
+        books.release(done)
+        new = [1 if books.lens[b] else (int(rng.integers(1, 30)) if n % 4 == 0 and rng.random() < 0.6 else 0)
+               for b in range(batch)]
+        if n > 8:
+            new = [min(x, 1) for x in new]
+        assert books.fits(new, rows) == 0
+        positions, _ = books.plan(new)
+        x = torch.randn(packed.shape, generator=g, device=DEV).to(act)
+        packed.copy_(x)
+        new_d.copy_(i32(new))
+        done_d.copy_(torch.tensor(done, device=DEV))
+        if n == 8:  # the rest runs from a graph
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            saved = {k: v.clone() for k, v in d.items()}
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                step()
+            for k, v in saved.items():
+                d[k].copy_(v)
+        step() if graph is None else graph.replay()
+        torch.cuda.synchronize()
+        assert got["status"].item() == 0 and got["cu"].tolist() == [0] + np.cumsum(new).tolist()
+        assert got["positions"][:len(positions)].tolist() == positions
+        same_books(d, books)
+        at = torch.tensor(positions, device=DEV)
+        owner = [b for b in range(batch) for _ in range(new[b])]
+        for l in range(layers):
+            q, k, v = (y[:len(owner)].unflatten(1, (-1, dh)) for y in x[l].split([hq * dh, hkv * dh, hkv * dh], 1))
+            if owner:
+                kr, kt = rotated(k, at, dh)
+                close(q_outs[l][:len(owner)], *rotated(q, at, dh))
+            for b in range(batch):
+                if done[b]:
+                    kept[l][b] = [[], []]
+            for r, b in enumerate(owner):  # what the cache holds, checked against the rotation as it is taken over
+                j = len(kept[l][b][0])
+                cell = (d["table"][b, j // page].long(), j % page)
+                close(pools[l][0][cell], kr[r], kt[r])
+                kept[l][b][0].append(pools[l][0][cell].clone())
+                kept[l][b][1].append(v[r].to(cache))
+            view = Pool.__new__(Pool)
+            view.lens_h = books.lens
+            view.k = [torch.stack(kept[l][b][0]) if kept[l][b][0] else None for b in range(batch)]
+            view.v = [torch.stack(kept[l][b][1]) if kept[l][b][1] else None for b in range(batch)]
+            queries = torch.stack([q_outs[l][max(0, int(c) - 1)] for c in np.cumsum(new)])
+            ref, _, tol, _ = attn_reference(view, queries, 1 / math.sqrt(dh))
+            assert ((outs[l].double() - ref).abs() <= tol).all()
+
+
+def test_every_call_launches_its_own_kernels():
+    n0 = launch_count()
+    pool = Pool([40], 2, 64, 16, F32, seed=2)
+    q = torch.randn(1, 4, 64, device=DEV)
+    K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens)
+    n1 = launch_count()
+    K.rope_kv_append_paged(q, q[:, :2], q[:, :2], pool.kc, pool.vc, i32([0]), i32([0]))
+    n2 = launch_count()
+    K.kv_page_plan(i32([1]), pool.lens, pool.table, torch.arange(pool.pages, device=DEV, dtype=torch.int32), i32([1]),
+                   16, 1)
+    n3 = launch_count()
+    assert n1 > n0 and n2 > n1 and n3 > n2
+    K.rope_kv_append_paged(None, q[:0, :2], q[:0, :2], pool.kc, pool.vc, i32([]), i32([]))
+    K.attn_decode_paged(q[:0], pool.kc, pool.vc, pool.table[:0], pool.lens[:0])
+    assert launch_count() == n3  # empty steps launch nothing
+
+
+def test_wrappers_refuse_what_does_not_belong_together():
+    pool = Pool([40, 3], 2, 64, 16, F32, seed=2)
+    q = torch.randn(2, 4, 64, device=DEV)
+    kv = torch.randn(2, 2, 64, device=DEV)
+    two = i32([0, 1])
+
+    def attn(q=q, kc=pool.kc, vc=pool.vc, table=pool.table, lens=pool.lens, **kw):
+        return K.attn_decode_paged(q, kc, vc, table, lens, **kw)
+
+    for bad in (dict(q=q.double()), dict(q=q[0]), dict(q=q.transpose(1, 2)), dict(q=q.cpu()), dict(kc=pool.kc.half()),
+                dict(vc=pool.vc[1:]), dict(table=pool.table.long()), dict(table=pool.table[:1]),
+                dict(table=pool.table.t().contiguous().t()), dict(lens=pool.lens.long()), dict(lens=pool.lens[:1]),
+                dict(lens=pool.lens.cpu()), dict(out=q[:1]), dict(out=q.half()), dict(work=q.half()),
+                dict(q=q[..., :60])):
+        with pytest.raises(ValueError):
+            attn(**bad)
+    with pytest.raises(Exception, match="16-bit q"):
+        attn(q=q.half())
+    with pytest.raises(Exception, match="multiple"):
+        attn(q=q[:, :3])
+
+    def append(q=q, k=kv, v=kv, kc=pool.kc, vc=pool.vc, slots=two, positions=two, **kw):
+        return K.rope_kv_append_paged(q, k, v, kc, vc, slots, positions, **kw)
+
+    for bad in (dict(k=kv[:, :1]), dict(v=kv[:1]), dict(slots=two[:1]), dict(positions=two.long()),
+                dict(q=q.half()), dict(q_out=q.half()), dict(q=q[:1]), dict(v=kv.half()), dict(k=kv.cpu())):
+        with pytest.raises(ValueError):
+            append(**bad)
+    with pytest.raises(Exception, match="rot_dim"):
+        append(rot_dim=63)
+    free, one = i32([0, 1]), i32([1])
+    for bad in ((two.long(), pool.lens, pool.table, free, one), (two[:1], pool.lens, pool.table, free, one),
+                (two, pool.lens, pool.table, free, two), (two, pool.lens[:1], pool.table, free, one),
+                (two, pool.lens, pool.table[0], free, one), (two, pool.lens.cpu(), pool.table, free, one)):
+        with pytest.raises(ValueError):
+            K.kv_page_plan(*bad, 16, 4)
+    with pytest.raises(ValueError):
+        K.kv_page_release(two, *(pool.lens, pool.table, free, one), 16)
