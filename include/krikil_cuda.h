@@ -407,7 +407,7 @@ KRK_API int krk_k_wait_probe(const float* src16, int polls, int copy, int32_t* s
  * Serving many requests of different lengths from one pool (no counterpart in
  * the reference, whose caches are one contiguous array a sequence).  The pool
  * is num_pages pages of page_size tokens (a power of two, at most 65536;
- * num_pages * page_size < 2^31).  Element (page, t, head, d) of the key cache
+ * num_pages * page_size < 2^31; a table row holds at most 2^30 tokens).  Element (page, t, head, d) of the key cache
  * is kc[page*c_sp + t*c_st + head*c_sh + d], of the value cache the same in vc,
  * so both [page][t][head][d] and [page][head][t][d] layouts are covered.
  * Request b's token j lives in page table[b*table_ld + j / page_size], at t =

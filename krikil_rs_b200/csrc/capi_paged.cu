@@ -57,8 +57,8 @@ std::string pool_fault(int num_pages, int page_size, int width) {
     if (shift < 0 || page_size > 65536) return "page_size must be a power of two of at most 65536";
     if (num_pages <= 0 || ((int64_t)num_pages << shift) > INT32_MAX)
         return "num_pages must be positive and num_pages * page_size below 2^31";
-    if (width <= 0 || ((int64_t)width << shift) > INT32_MAX)
-        return "the table's width must be positive and width * page_size below 2^31";
+    if (width <= 0 || ((int64_t)width << shift) > (1 << 30))
+        return "the table's width must be positive and width * page_size at most 2^30";
     return "";
 }
 
@@ -149,8 +149,8 @@ int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void*
     const std::string f = pool_fault(num_pages, page_size, width), g = types_fault(type, cache_type);
     if (!f.empty()) return invalid(who, f);
     if (!g.empty()) return invalid(who, g);
-    if (B < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 65535)
-        return invalid(who, "B must not be negative, Hq a positive multiple of Hkv of at most 65535");
+    if (B < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 65535 || (int64_t)B * Hq > INT32_MAX)
+        return invalid(who, "B must not be negative, Hq a positive multiple of Hkv of at most 65535, B * Hq below 2^31");
     if (dh < 4 || dh > 256 || dh % 4) return invalid(who, "dh must be a multiple of 4 of at most 256");
     if (!std::isfinite(scale)) return invalid(who, "scale must be finite");
     if (window < 0 || max_len < 0) return invalid(who, "window and max_len must not be negative");

@@ -1,0 +1,226 @@
+// Decode attention over float32 pages: the engine on float32 fused
+// multiply-adds (as the framework's other float32 paths, no tensor cores: their
+// 10-bit operands would change results).
+//
+// A warp's tile is eight 16-byte loads a lane of keys and eight of values: LPK
+// lanes hold a key's elements four at a time, 32 / LPK keys side by side.  A
+// lane multiplies its elements of eight (four) keys with its elements of a
+// query; the eight partial sums are added over the LPK lanes by exchanging
+// halves -- four, two, one, so that each lane ends with one key's score after
+// 8 or 9 shuffles instead of 8 x 5 -- and one exponential a lane weighs the
+// tile.
+#include "paged_attn.cuh"
+
+namespace krk {
+namespace {
+
+template <int DC_, int GW>
+struct F32Engine {
+    using Act = float;
+    using Cache = float;
+    static constexpr int DC = DC_, HW = GW;
+    static constexpr int LPK = DC >= 128 ? 32 : 16;    // lanes of a key
+    static constexpr int NL = DC / (LPK * 4);          // 16-byte loads of a lane for a key
+    static constexpr int J = 8 / NL;                   // key steps of a tile
+    static constexpr int KPL = 32 / LPK;               // keys side by side
+    static constexpr int KT = J * KPL;                 // 16, 8 or 4 keys
+    static constexpr int Q_BYTES = 0;
+    static constexpr int BLOCKS = GW <= 2 && DC <= 128 ? 4 : 3;
+    static constexpr float SCALE = 1.f;
+
+    float4 k[8], v[8], q[GW][NL], acc[GW][NL];
+    float s[GW], m[GW], l[GW], fade[GW], c;
+
+    KRK_DEV void init(const PagedAttnArgs& a, const float* qp, int heads, unsigned char*, int lane, int, int) {
+        c = a.scale * 1.44269504088896341f;
+#pragma unroll
+        for (int h = 0; h < GW; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int d = ((lane & (LPK - 1)) + i * LPK) * 4;
+                acc[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                q[h][i] = h < heads && d < a.dh ? load4(qp + h * a.q_sh + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        }
+    }
+    KRK_DEV void load(const PagedAttnArgs& a, const float* base, long long off, int lane, float4 (&x)[8]) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const long long o = __shfl_sync(0xffffffffu, off, j * KPL + lane / LPK);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int d = ((lane & (LPK - 1)) + i * LPK) * 4;
+                x[j * NL + i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (o >= 0 && d < a.dh) x[j * NL + i] = __ldg(reinterpret_cast<const float4*>(base + o + d));
+            }
+        }
+    }
+    KRK_DEV void load_k(const PagedAttnArgs& a, const float* base, long long off, int lane) {
+        load(a, base, off, lane, k);
+    }
+    KRK_DEV void load_v(const PagedAttnArgs& a, const float* base, long long off, int lane) {
+        load(a, base, off, lane, v);
+    }
+
+    // The key step whose score this lane holds after `fold`, and the lane (of its half) that holds step j's.
+    static KRK_DEV int step_of(int lane) {
+        int j = 0;
+#pragma unroll
+        for (int o = LPK / 2, n = J / 2; n >= 1; o >>= 1, n >>= 1) j += (lane & o) ? n : 0;
+        return j;
+    }
+    static KRK_DEV constexpr int lane_of(int j) {
+        int lane = 0;
+        for (int o = LPK / 2, n = J / 2; n >= 1; o >>= 1, n >>= 1) lane += (j & n) ? o : 0;
+        return lane;
+    }
+    static KRK_DEV float fold(float (&x)[J], int lane) {
+        int o = LPK / 2;
+#pragma unroll
+        for (int n = J / 2; n >= 1; n >>= 1, o >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const float give = up ? x[i] : x[i + n], keep = up ? x[i + n] : x[i];
+                x[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        }
+        float r = x[0];
+#pragma unroll
+        for (int p = LPK / 2 / J; p >= 1; p >>= 1) r += __shfl_xor_sync(0xffffffffu, r, p);
+        return r;
+    }
+
+    KRK_DEV void scores(const unsigned char*, int lane) {
+#pragma unroll
+        for (int h = 0; h < GW; ++h) {
+            float x[J];
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                x[j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const float4 y = k[j * NL + i];
+                    x[j] = fmaf(y.x, q[h][i].x, x[j]);
+                    x[j] = fmaf(y.y, q[h][i].y, x[j]);
+                    x[j] = fmaf(y.z, q[h][i].z, x[j]);
+                    x[j] = fmaf(y.w, q[h][i].w, x[j]);
+                }
+            }
+            s[h] = fold(x, lane);
+        }
+    }
+    KRK_DEV void weigh(unsigned mask, int lane) {
+        const bool seen = mask >> (step_of(lane) * KPL + lane / LPK) & 1u;
+#pragma unroll
+        for (int h = 0; h < GW; ++h) {
+            const float x = seen ? s[h] * c : -INFINITY;
+            float top = x;
+#pragma unroll
+            for (int o = LPK / 2, n = J / 2; n >= 1; o >>= 1, n >>= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (LPK == 16) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            top = fmaxf(top, m[h]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            fade[h] = exp2f(m[h] - ref);
+            m[h] = top;
+            s[h] = exp2f(x - ref);
+            l[h] = l[h] * fade[h] + s[h];
+        }
+    }
+    KRK_DEV void values(int lane) {
+        const int side = lane & ~(LPK - 1);
+#pragma unroll
+        for (int h = 0; h < GW; ++h) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                acc[h][i].x *= fade[h];
+                acc[h][i].y *= fade[h];
+                acc[h][i].z *= fade[h];
+                acc[h][i].w *= fade[h];
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float p = __shfl_sync(0xffffffffu, s[h], side + lane_of(j));
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const float4 y = v[j * NL + i];
+                    acc[h][i].x = fmaf(p, y.x, acc[h][i].x);
+                    acc[h][i].y = fmaf(p, y.y, acc[h][i].y);
+                    acc[h][i].z = fmaf(p, y.z, acc[h][i].z);
+                    acc[h][i].w = fmaf(p, y.w, acc[h][i].w);
+                }
+            }
+        }
+    }
+    KRK_DEV void finish(float* obuf, float* sm, float* sl, int lane) {
+#pragma unroll
+        for (int h = 0; h < GW; ++h) {
+            float sum = l[h];
+#pragma unroll
+            for (int o = LPK / 2, n = J / 2; n >= 1; o >>= 1, n >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (LPK == 16) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+            if (lane == 0) {
+                sm[h] = m[h];
+                sl[h] = sum;
+            }
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                float4 o = acc[h][i];
+                if (LPK == 16) {
+                    o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
+                    o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+                    o.z += __shfl_xor_sync(0xffffffffu, o.z, 16);
+                    o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+                }
+                if (lane < LPK) *reinterpret_cast<float4*>(obuf + h * (DC + 4) + (lane + i * LPK) * 4) = o;
+            }
+        }
+    }
+};
+
+template <int GW>
+cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
+    if (a.dh <= 64) return launch_paged_attn<F32Engine<64, GW>>(a, s);
+    if (a.dh <= 128) return launch_paged_attn<F32Engine<128, GW>>(a, s);
+    return launch_paged_attn<F32Engine<256, GW>>(a, s);
+}
+
+}  // namespace
+
+int paged_sm_count() {
+    static int known[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int n = __atomic_load_n(&known[dev], __ATOMIC_RELAXED);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        __atomic_store_n(&known[dev], n, __ATOMIC_RELAXED);
+    }
+    return n;
+}
+
+size_t attn_paged_work_floats(int Hq, int Hkv, int dh) {
+    // as many heads a block as any engine takes
+    int heads = 8;
+    while (heads < PA_MAX_HEADS && heads < Hq / Hkv) heads *= 2;
+    return (size_t)PA_MAX_BLOCKS * (2 * (size_t)heads * (dh + 2) + 2);
+}
+
+cudaError_t attn_decode_paged_f32(const PagedAttnArgs& a, cudaStream_t s) {
+    const int G = a.Hq / a.Hkv;
+    if (G == 1) return by_width<1>(a, s);
+    if (G == 2) return by_width<2>(a, s);
+    return by_width<4>(a, s);
+}
+
+cudaError_t attn_decode_paged_half(const PagedAttnArgs& a, int act, int cache, cudaStream_t s);
+
+cudaError_t attn_decode_paged(const PagedAttnArgs& a, int act, int cache, cudaStream_t s) {
+    if (act == ELEM_F32 && cache == ELEM_F32) return attn_decode_paged_f32(a, s);
+    return attn_decode_paged_half(a, act, cache, s);
+}
+
+}  // namespace krk

@@ -1,0 +1,297 @@
+// Decode attention over half and bfloat16 pages: the engine on m16n8k16 matrix
+// instructions, operands straight from global memory.
+//
+// A warp's tile is 16 keys and 8 query heads that share them.  The contraction
+// index of a matrix instruction may be permuted as long as both operands agree,
+// and so may its rows and columns, so the lanes' 16-byte loads are the operands
+// as they come:
+//   S = Q K^T (heads x keys, contracted over dh): lane 4n + t of a load holds
+//     elements 8t .. 8t+7 of a 32-element block of key n (and n + 8): two
+//     k = 16 steps, whose Q operand holds the same elements.
+//   O^T = V^T P^T (dh x heads, contracted over keys): lane 4r + t loads elements
+//     8r .. 8r+7 of a 64-element block of keys 2t, 2t+1, 2t+8, 2t+9; pairs of
+//     keys are put side by side with byte permutes, and P^T is S's own layout.
+// No key or value passes through shared memory and no warp waits for another
+// before a piece ends.
+//
+// Precision: the products are exact and added in 32 bits, and a tile's sum is
+// folded into the float32 accumulators once a tile.  A float32 weight is the
+// sum of two 16-bit parts (three when float32 results are wanted from bfloat16
+// pages: 24 bits), and a float32 query of two half parts after scaling its row
+// by a power of two (22 bits and a sign) or three bfloat16 parts (24 bits).
+// Half weights are scaled by 2^14, so that a key 2^-24 as likely as the
+// strongest still has 14 bits.
+#include "paged_attn.cuh"
+
+namespace krk {
+namespace {
+
+KRK_DEV void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+KRK_DEV void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                 __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two floats rounded into one register (x in the low half), and what is left of them.
+KRK_DEV uint32_t pack_rest(float& x, float& y, __half) {
+    const __half2 h = __floats2half2_rn(x, y);
+    x -= __low2float(h);
+    y -= __high2float(h);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+KRK_DEV uint32_t pack_rest(float& x, float& y, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
+    x -= __uint_as_float(u << 16);
+    y -= __uint_as_float(u & 0xffff0000u);
+    return u;
+}
+
+// Elements 8 * chunk .. + 7 of a row (zeros past dh); wide: rows are 16-byte aligned and dh a multiple of 8.
+template <bool WIDE, typename C>
+KRK_DEV uint4 load_chunk(const C* base, long long off, int chunk, int dh) {
+    uint4 r = make_uint4(0u, 0u, 0u, 0u);
+    const C* p = base + off + chunk * 8;
+    if (WIDE) {
+        if (off >= 0 && chunk * 8 < dh) r = __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+        if (off >= 0 && chunk * 8 < dh) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+            r.x = x.x;
+            r.y = x.y;
+        }
+        if (off >= 0 && chunk * 8 + 4 < dh) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+            r.z = x.x;
+            r.w = x.y;
+        }
+    }
+    return r;
+}
+KRK_DEV uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+template <typename T, typename C, int DC_, bool WIDE>
+struct HalfEngine {
+    using Act = T;
+    using Cache = C;
+    static constexpr bool kSame = sizeof(T) == 2, kHalf = sizeof(__half) == 2 && std::is_same<C, __half>::value;
+    static constexpr int DC = DC_, KT = 16, HW = 8;
+    static constexpr int NB = DC / 32, NV = DC / 64;
+    static constexpr int QP = kSame ? 1 : kHalf ? 2 : 3;  // parts of a query
+    static constexpr int PP = !kSame && !kHalf ? 3 : 2;   // parts of a weight
+    static constexpr int Q_BYTES = QP * NB * 32 * 16;
+    static constexpr int BLOCKS = DC == 64 ? 4 : DC == 128 ? 3 : 2;
+    static constexpr float SCALE = kHalf ? 16384.f : 1.f;
+
+    uint4 k[NB][2], v[NV][4];
+    float acc[NV][4][4];
+    float s[4], m, l, c;
+
+    // Lays the parts of the group's queries out as the first operand's registers.  Each warp of a group prepares
+    // every kwarps-th head.
+    KRK_DEV void init(const PagedAttnArgs& a, const T* q, int heads, unsigned char* qs, int lane, int kwarp,
+                      int kwarps) {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[i][j][x] = 0.f;
+        c = a.scale * 1.44269504088896341f;
+        for (int h = kwarp; h < HW; h += kwarps) {
+            float4 x[DC / 128 ? DC / 128 : 1];
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < (DC + 127) / 128; ++i) {
+                const int d = (i * 32 + lane) * 4;
+                x[i] = h < heads && d < a.dh ? load4(q + h * a.q_sh + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+            }
+            float up = 1.f;
+            if (QP == 2) up = row_scale(warp_max(most));
+#pragma unroll
+            for (int i = 0; i < (DC + 127) / 128; ++i) {
+                const int d = (i * 32 + lane) * 4;
+                if (d >= DC) continue;
+                float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
+#pragma unroll
+                for (int p = 0; p < QP; ++p) {
+                    uint2 u;
+                    u.x = pack_rest(y.x, y.y, C());
+                    u.y = pack_rest(y.z, y.w, C());
+                    *reinterpret_cast<uint2*>(qs + ((p * NB + d / 32) * 32 + h * 4 + d % 32 / 8) * 16 + d % 8 * 2) = u;
+                }
+            }
+            if (QP == 2 && lane / 4 == h) c *= 1.0f / up;
+        }
+        if (QP == 2) {  // the other warps' heads: the same scales again
+            for (int h = 0; h < HW; ++h) {
+                if (h % kwarps == kwarp) continue;
+                float most = 0.f;
+                for (int d = lane * 4; h < heads && d < a.dh; d += 128) {
+                    const float4 x = load4(q + h * a.q_sh + d);
+                    most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+                }
+                const float up = row_scale(warp_max(most));
+                if (lane / 4 == h) c *= 1.0f / up;
+            }
+        }
+    }
+    // The power of two that brings the row's largest element to 2^14 .. 2^15 (at most 2^+-100; 1 for zeros,
+    // infinities and NaN).
+    static KRK_DEV float row_scale(float most) {
+        if (!(most > 0.f) || most == INFINITY) return 1.f;
+        return exp2f((float)min(100, max(-100, 14 - ilogbf(most))));
+    }
+
+    KRK_DEV void load_k(const PagedAttnArgs& a, const C* base, long long off, int lane) {
+        const long long o0 = __shfl_sync(0xffffffffu, off, lane >> 2), o1 = __shfl_sync(0xffffffffu, off, (lane >> 2) + 8);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            k[i][0] = load_chunk<WIDE>(base, o0, i * 4 + (lane & 3), a.dh);
+            k[i][1] = load_chunk<WIDE>(base, o1, i * 4 + (lane & 3), a.dh);
+        }
+    }
+    KRK_DEV void load_v(const PagedAttnArgs& a, const C* base, long long off, int lane) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long o = __shfl_sync(0xffffffffu, off, 2 * (lane & 3) + (j & 1) + (j >> 1) * 8);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i][j] = load_chunk<WIDE>(base, o, i * 8 + (lane >> 2), a.dh);
+        }
+    }
+
+    KRK_DEV void scores(const unsigned char* qs, int lane) {
+        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+        float e0[4] = {0.f, 0.f, 0.f, 0.f}, e1[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint4* qf = reinterpret_cast<const uint4*>(qs) + lane;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint4 h = qf[i * 32];
+            const uint4 r = QP > 1 ? qf[(NB + i) * 32] : make_uint4(0u, 0u, 0u, 0u);
+            mma(d0, h.x, r.x, h.y, r.y, k[i][0].x, k[i][0].y, C());
+            mma(d1, h.x, r.x, h.y, r.y, k[i][1].x, k[i][1].y, C());
+            mma(d0, h.z, r.z, h.w, r.w, k[i][0].z, k[i][0].w, C());
+            mma(d1, h.z, r.z, h.w, r.w, k[i][1].z, k[i][1].w, C());
+            if (QP > 2) {
+                const uint4 t = qf[(2 * NB + i) * 32];
+                mma(e0, t.x, 0u, t.y, 0u, k[i][0].x, k[i][0].y, C());
+                mma(e1, t.x, 0u, t.y, 0u, k[i][1].x, k[i][1].y, C());
+                mma(e0, t.z, 0u, t.w, 0u, k[i][0].z, k[i][0].w, C());
+                mma(e1, t.z, 0u, t.w, 0u, k[i][1].z, k[i][1].w, C());
+            }
+        }
+        s[0] = joined(d0[0], d0[2], e0[0]);
+        s[1] = joined(d0[1], d0[3], e0[1]);
+        s[2] = joined(d1[0], d1[2], e1[0]);
+        s[3] = joined(d1[1], d1[3], e1[1]);
+    }
+    // The parts' products; an infinite key's first part decides (the others may be infinite the other way, or NaN).
+    static KRK_DEV float joined(float first, float second, float third) {
+        if (QP == 1) return first;
+        const float sum = QP > 2 ? first + (second + third) : first + second;
+        return fabsf(first) == INFINITY ? first : sum;
+    }
+
+    KRK_DEV void weigh(unsigned mask, int lane) {
+        const int t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] *= c;
+        if ((mask & 0xffffu) != 0xffffu) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!(mask >> (2 * t + (i & 1) + (i >> 1) * 8) & 1u)) s[i] = -INFINITY;
+        }
+        float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = fmaxf(top, m);
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float fade = exp2f(m - ref);
+        m = top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = exp2f(s[i] - ref) * SCALE;
+        l = l * fade + ((s[0] + s[1]) + (s[2] + s[3]));
+        c_fade = fade;
+    }
+    float c_fade;
+
+    KRK_DEV void values(int lane) {
+        const float f0 = __shfl_sync(0xffffffffu, c_fade, (lane & 3) * 8);
+        const float f1 = __shfl_sync(0xffffffffu, c_fade, (lane & 3) * 8 + 4);
+        uint32_t p[PP][2];
+#pragma unroll
+        for (int i = 0; i < PP; ++i) {
+            p[i][0] = pack_rest(s[0], s[1], C());
+            p[i][1] = pack_rest(s[2], s[3], C());
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w0 = word(v[i][0], j), w1 = word(v[i][1], j), w2 = word(v[i][2], j),
+                               w3 = word(v[i][3], j);
+                const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+                const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = PP - 1; x >= 0; --x) mma(d, a0, a1, a2, a3, p[x][0], p[x][1], C());
+                acc[i][j][0] = fmaf(acc[i][j][0], f0, d[0]);
+                acc[i][j][1] = fmaf(acc[i][j][1], f1, d[1]);
+                acc[i][j][2] = fmaf(acc[i][j][2], f0, d[2]);
+                acc[i][j][3] = fmaf(acc[i][j][3], f1, d[3]);
+            }
+    }
+
+    KRK_DEV void finish(float* obuf, float* sm, float* sl, int lane) {
+        const int r = lane >> 2, t = lane & 3;
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t == 0) {
+            sm[r] = m;
+            sl[r] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float* o = obuf + 2 * t * (DC + 4) + i * 64 + r * 8 + j * 2;
+                *reinterpret_cast<float2*>(o) = make_float2(acc[i][j][0], acc[i][j][2]);
+                *reinterpret_cast<float2*>(o + DC + 4) = make_float2(acc[i][j][1], acc[i][j][3]);
+            }
+    }
+};
+
+template <typename T, typename C, bool WIDE>
+cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
+    if (a.dh <= 64) return launch_paged_attn<HalfEngine<T, C, 64, WIDE>>(a, s);
+    if (a.dh <= 128) return launch_paged_attn<HalfEngine<T, C, 128, WIDE>>(a, s);
+    return launch_paged_attn<HalfEngine<T, C, 256, WIDE>>(a, s);
+}
+
+template <typename T, typename C>
+cudaError_t by_alignment(const PagedAttnArgs& a, cudaStream_t s) {
+    const bool wide = a.dh % 8 == 0 && a.c_sp % 8 == 0 && a.c_st % 8 == 0 && a.c_sh % 8 == 0 &&
+                      (reinterpret_cast<uintptr_t>(a.kc) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.vc) & 15) == 0;
+    return wide ? by_width<T, C, true>(a, s) : by_width<T, C, false>(a, s);
+}
+
+}  // namespace
+
+cudaError_t attn_decode_paged_half(const PagedAttnArgs& a, int act, int cache, cudaStream_t s) {
+    if (act == ELEM_F32 && cache == ELEM_F16) return by_alignment<float, __half>(a, s);
+    if (act == ELEM_F32 && cache == ELEM_BF16) return by_alignment<float, __nv_bfloat16>(a, s);
+    if (act == ELEM_F16 && cache == ELEM_F16) return by_alignment<__half, __half>(a, s);
+    if (act == ELEM_BF16 && cache == ELEM_BF16) return by_alignment<__nv_bfloat16, __nv_bfloat16>(a, s);
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace krk
