@@ -25,10 +25,11 @@ struct F32Engine {
     static constexpr int KPL = 32 / LPK;               // keys side by side
     static constexpr int KT = J * KPL;                 // 16, 8 or 4 keys
     static constexpr int Q_BYTES = 0;
-    static constexpr int BLOCKS = GW <= 2 && DC <= 128 ? 4 : 3;
+    static constexpr int TILE_BYTES = 16 * 512;
+    static constexpr int BLOCKS = 3;
     static constexpr float SCALE = 1.f;
 
-    float4 k[8], v[8], q[GW][NL], acc[GW][NL];
+    float4 q[GW][NL], acc[GW][NL];
     float s[GW], m[GW], l[GW], fade[GW], c;
 
     KRK_DEV void init(const PagedAttnArgs& a, const float* qp, int heads, unsigned char*, int lane, int, int) {
@@ -45,23 +46,20 @@ struct F32Engine {
             }
         }
     }
-    KRK_DEV void load(const PagedAttnArgs& a, const float* base, long long off, int lane, float4 (&x)[8]) {
+    KRK_DEV void issue(const PagedAttnArgs& a, const float* kc, const float* vc, long long off, uint32_t to,
+                       int lane) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const long long o = __shfl_sync(0xffffffffu, off, j * KPL + lane / LPK);
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int d = ((lane & (LPK - 1)) + i * LPK) * 4;
-                x[j * NL + i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (o >= 0 && d < a.dh) x[j * NL + i] = __ldg(reinterpret_cast<const float4*>(base + o + d));
+                const bool take = o >= 0 && d < a.dh;
+                const long long at = take ? o + d : 0;
+                pa_copy<16>(to + (j * NL + i) * 512, kc + at, take);
+                pa_copy<16>(to + (8 + j * NL + i) * 512, vc + at, take);
             }
         }
-    }
-    KRK_DEV void load_k(const PagedAttnArgs& a, const float* base, long long off, int lane) {
-        load(a, base, off, lane, k);
-    }
-    KRK_DEV void load_v(const PagedAttnArgs& a, const float* base, long long off, int lane) {
-        load(a, base, off, lane, v);
     }
 
     // The key step whose score this lane holds after `fold`, and the lane (of its half) that holds step j's.
@@ -93,7 +91,10 @@ struct F32Engine {
         return r;
     }
 
-    KRK_DEV void scores(const unsigned char*, int lane) {
+    KRK_DEV void scores(const unsigned char*, const unsigned char* from, int lane) {
+        float4 k[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const float4*>(from + j * 512);
 #pragma unroll
         for (int h = 0; h < GW; ++h) {
             float x[J];
@@ -130,7 +131,10 @@ struct F32Engine {
             l[h] = l[h] * fade[h] + s[h];
         }
     }
-    KRK_DEV void values(int lane) {
+    KRK_DEV void values(const unsigned char* from, int lane) {
+        float4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float4*>(from + (8 + j) * 512);
         const int side = lane & ~(LPK - 1);
 #pragma unroll
         for (int h = 0; h < GW; ++h) {

@@ -1,18 +1,18 @@
 // Decode attention over half and bfloat16 pages: the engine on m16n8k16 matrix
-// instructions, operands straight from global memory.
+// instructions.
 //
 // A warp's tile is 16 keys and 8 query heads that share them.  The contraction
 // index of a matrix instruction may be permuted as long as both operands agree,
-// and so may its rows and columns, so the lanes' 16-byte loads are the operands
-// as they come:
+// and so may its rows and columns, so the 16 bytes that a lane copies are its
+// operands as they come:
 //   S = Q K^T (heads x keys, contracted over dh): lane 4n + t of a load holds
 //     elements 8t .. 8t+7 of a 32-element block of key n (and n + 8): two
 //     k = 16 steps, whose Q operand holds the same elements.
 //   O^T = V^T P^T (dh x heads, contracted over keys): lane 4r + t loads elements
 //     8r .. 8r+7 of a 64-element block of keys 2t, 2t+1, 2t+8, 2t+9; pairs of
 //     keys are put side by side with byte permutes, and P^T is S's own layout.
-// No key or value passes through shared memory and no warp waits for another
-// before a piece ends.
+// No lane reads what another one copied, and no warp waits for another before a
+// piece ends.
 //
 // Precision: the products are exact and added in 32 bits, and a tile's sum is
 // folded into the float32 accumulators once a tile.  A float32 weight is the
@@ -53,26 +53,19 @@ KRK_DEV uint32_t pack_rest(float& x, float& y, __nv_bfloat16) {
     return u;
 }
 
-// Elements 8 * chunk .. + 7 of a row (zeros past dh); wide: rows are 16-byte aligned and dh a multiple of 8.
+// Starts the copy of elements 8 * chunk .. + 7 of a row (zeros past dh, and for off < 0); wide: rows are 16-byte
+// aligned and dh a multiple of 8.
 template <bool WIDE, typename C>
-KRK_DEV uint4 load_chunk(const C* base, long long off, int chunk, int dh) {
-    uint4 r = make_uint4(0u, 0u, 0u, 0u);
-    const C* p = base + off + chunk * 8;
+KRK_DEV void copy_chunk(uint32_t to, const C* base, long long off, int chunk, int dh) {
+    const bool take = off >= 0 && chunk * 8 < dh;
+    const C* p = take ? base + off + chunk * 8 : base;
     if (WIDE) {
-        if (off >= 0 && chunk * 8 < dh) r = __ldg(reinterpret_cast<const uint4*>(p));
+        pa_copy<16>(to, p, take);
     } else {
-        if (off >= 0 && chunk * 8 < dh) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-            r.x = x.x;
-            r.y = x.y;
-        }
-        if (off >= 0 && chunk * 8 + 4 < dh) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-            r.z = x.x;
-            r.w = x.y;
-        }
+        const bool more = take && chunk * 8 + 4 < dh;
+        pa_copy<8>(to, p, take);
+        pa_copy<8>(to + 8, more ? p + 4 : base, more);
     }
-    return r;
 }
 KRK_DEV uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -86,10 +79,11 @@ struct HalfEngine {
     static constexpr int QP = kSame ? 1 : kHalf ? 2 : 3;  // parts of a query
     static constexpr int PP = !kSame && !kHalf ? 3 : 2;   // parts of a weight
     static constexpr int Q_BYTES = QP * NB * 32 * 16;
-    static constexpr int BLOCKS = DC == 64 ? 4 : DC == 128 ? 3 : 2;
+    static constexpr int K_LOADS = NB * 2, V_LOADS = NV * 4;  // of a lane, for a tile
+    static constexpr int TILE_BYTES = (K_LOADS + V_LOADS) * 512;
+    static constexpr int BLOCKS = DC == 64 ? 4 : DC == 128 ? 3 : 1;
     static constexpr float SCALE = kHalf ? 16384.f : 1.f;
 
-    uint4 k[NB][2], v[NV][4];
     float acc[NV][4][4];
     float s[4], m, l, c;
 
@@ -152,41 +146,42 @@ struct HalfEngine {
         return exp2f((float)min(100, max(-100, 14 - ilogbf(most))));
     }
 
-    KRK_DEV void load_k(const PagedAttnArgs& a, const C* base, long long off, int lane) {
-        const long long o0 = __shfl_sync(0xffffffffu, off, lane >> 2), o1 = __shfl_sync(0xffffffffu, off, (lane >> 2) + 8);
+    KRK_DEV void issue(const PagedAttnArgs& a, const C* kc, const C* vc, long long off, uint32_t to, int lane) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            k[i][0] = load_chunk<WIDE>(base, o0, i * 4 + (lane & 3), a.dh);
-            k[i][1] = load_chunk<WIDE>(base, o1, i * 4 + (lane & 3), a.dh);
+        for (int j = 0; j < 2; ++j) {
+            const long long o = __shfl_sync(0xffffffffu, off, (lane >> 2) + 8 * j);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) copy_chunk<WIDE>(to + (i * 2 + j) * 512, kc, o, i * 4 + (lane & 3), a.dh);
         }
-    }
-    KRK_DEV void load_v(const PagedAttnArgs& a, const C* base, long long off, int lane) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const long long o = __shfl_sync(0xffffffffu, off, 2 * (lane & 3) + (j & 1) + (j >> 1) * 8);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i][j] = load_chunk<WIDE>(base, o, i * 8 + (lane >> 2), a.dh);
+            for (int i = 0; i < NV; ++i)
+                copy_chunk<WIDE>(to + (K_LOADS + i * 4 + j) * 512, vc, o, i * 8 + (lane >> 2), a.dh);
         }
     }
 
-    KRK_DEV void scores(const unsigned char* qs, int lane) {
+    KRK_DEV void scores(const unsigned char* qs, const unsigned char* from, int lane) {
         float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
         float e0[4] = {0.f, 0.f, 0.f, 0.f}, e1[4] = {0.f, 0.f, 0.f, 0.f};
         const uint4* qf = reinterpret_cast<const uint4*>(qs) + lane;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
+            const uint4 k0 = *reinterpret_cast<const uint4*>(from + (i * 2) * 512);
+            const uint4 k1 = *reinterpret_cast<const uint4*>(from + (i * 2 + 1) * 512);
             const uint4 h = qf[i * 32];
             const uint4 r = QP > 1 ? qf[(NB + i) * 32] : make_uint4(0u, 0u, 0u, 0u);
-            mma(d0, h.x, r.x, h.y, r.y, k[i][0].x, k[i][0].y, C());
-            mma(d1, h.x, r.x, h.y, r.y, k[i][1].x, k[i][1].y, C());
-            mma(d0, h.z, r.z, h.w, r.w, k[i][0].z, k[i][0].w, C());
-            mma(d1, h.z, r.z, h.w, r.w, k[i][1].z, k[i][1].w, C());
+            mma(d0, h.x, r.x, h.y, r.y, k0.x, k0.y, C());
+            mma(d1, h.x, r.x, h.y, r.y, k1.x, k1.y, C());
+            mma(d0, h.z, r.z, h.w, r.w, k0.z, k0.w, C());
+            mma(d1, h.z, r.z, h.w, r.w, k1.z, k1.w, C());
             if (QP > 2) {
                 const uint4 t = qf[(2 * NB + i) * 32];
-                mma(e0, t.x, 0u, t.y, 0u, k[i][0].x, k[i][0].y, C());
-                mma(e1, t.x, 0u, t.y, 0u, k[i][1].x, k[i][1].y, C());
-                mma(e0, t.z, 0u, t.w, 0u, k[i][0].z, k[i][0].w, C());
-                mma(e1, t.z, 0u, t.w, 0u, k[i][1].z, k[i][1].w, C());
+                mma(e0, t.x, 0u, t.y, 0u, k0.x, k0.y, C());
+                mma(e1, t.x, 0u, t.y, 0u, k1.x, k1.y, C());
+                mma(e0, t.z, 0u, t.w, 0u, k0.z, k0.w, C());
+                mma(e1, t.z, 0u, t.w, 0u, k1.z, k1.w, C());
             }
         }
         s[0] = joined(d0[0], d0[2], e0[0]);
@@ -224,7 +219,7 @@ struct HalfEngine {
     }
     float c_fade;
 
-    KRK_DEV void values(int lane) {
+    KRK_DEV void values(const unsigned char* from, int lane) {
         const float f0 = __shfl_sync(0xffffffffu, c_fade, (lane & 3) * 8);
         const float f1 = __shfl_sync(0xffffffffu, c_fade, (lane & 3) * 8 + 4);
         uint32_t p[PP][2];
@@ -234,11 +229,13 @@ struct HalfEngine {
             p[i][1] = pack_rest(s[2], s[3], C());
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(from + (K_LOADS + i * 4 + j) * 512);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint32_t w0 = word(v[i][0], j), w1 = word(v[i][1], j), w2 = word(v[i][2], j),
-                               w3 = word(v[i][3], j);
+                const uint32_t w0 = word(v[0], j), w1 = word(v[1], j), w2 = word(v[2], j), w3 = word(v[3], j);
                 const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
                 const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
@@ -249,6 +246,7 @@ struct HalfEngine {
                 acc[i][j][2] = fmaf(acc[i][j][2], f0, d[2]);
                 acc[i][j][3] = fmaf(acc[i][j][3], f1, d[3]);
             }
+        }
     }
 
     KRK_DEV void finish(float* obuf, float* sm, float* sl, int lane) {

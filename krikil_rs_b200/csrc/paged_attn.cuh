@@ -27,6 +27,7 @@ constexpr int PA_UNIT = 64;          // keys of one unit of work
 constexpr int PA_WHOLE_UNITS = 4;    // up to this many units a block takes a whole (request, head)
 constexpr int PA_MAX_BLOCKS = 592;   // blocks of a wave: four on each of 148 SMs
 constexpr int PA_MAX_HEADS = 32;     // query heads of a block, at most
+constexpr int PA_SLOTS = 2;          // tiles of a warp's ring
 constexpr int PA_ALIGN = 16;         // a piece's first key is aligned down to the largest tile
 
 // Scratch of a launch: two partial results a block -- slot 0 for a piece that
@@ -122,13 +123,34 @@ KRK_DEV long long pa_offset(const PagedAttnArgs& a, int page, int key0, int firs
     return page * a.c_sp + (key & ((1 << a.page_shift) - 1)) * a.c_st;
 }
 
+// Barrier of the warps that share a group's queries.
+KRK_DEV void pa_group_sync(int group, int warps) {
+    if (warps > 1)
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
+    else
+        __syncwarp();
+}
+
+// Asynchronous copy of BYTES (16 or 8) to shared memory; zeros, and no access, when !take.
+template <int BYTES>
+KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
+    const int n = take ? BYTES : 0;
+    if (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
+}
+
 // E: an engine.  Its warp holds KT keys of a tile and HW query heads:
-//   init(a, q, heads, qs, lane)     loads a warp's queries (or prepares them in shared memory)
-//   load_k / load_v (base, off)     issue the loads of a tile from the lanes' row offsets
-//   scores(qs)                      q . k of the tile's keys
-//   weigh(mask)                     softmax step over the visible keys of the tile
-//   values()                        weighted values into the accumulators
-//   finish(obuf, m, l)              accumulators, maxima and sums of the warp to shared memory
+//   init(a, q, heads, qs)     loads a warp's queries (or prepares them in shared memory)
+//   issue(k, v, off, to)      starts the copies of a tile, from the lanes' row offsets to its ring slot
+//   scores(qs, from)          q . k of the slot's keys
+//   weigh(mask)               softmax step over the visible keys of the tile
+//   values(from)              weighted values into the accumulators
+//   finish(obuf, m, l)        accumulators, maxima and sums of the warp to shared memory
+// A lane copies exactly the 16-byte pieces that it reads itself, each load of a
+// tile in 512 consecutive bytes of the warp's ring: no bank conflicts, no
+// barrier, and two tiles a warp in flight without holding registers.
 template <class E>
 __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a,
                                                                            const PagedShape sh,
@@ -143,7 +165,9 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int G = a.Hq / a.Hkv, pieces = a.Hkv * sh.per_kv;
     const int kwarps = PA_WARPS / sh.groups, group = warp % sh.groups, kwarp = warp / sh.groups;
-    float* obuf = reinterpret_cast<float*>(smem);
+    unsigned char* ring = smem + (size_t)warp * PA_SLOTS * E::TILE_BYTES;
+    unsigned char* qs = smem + PA_WARPS * PA_SLOTS * E::TILE_BYTES + (size_t)group * E::Q_BYTES;
+    const uint32_t ring_at = smem_addr(ring) + lane * 16;
 
     PagedShare share;
     if (sh.whole) {
@@ -173,38 +197,43 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
         E e;
         const int mine = min(HW, G - head0 - group * HW);  // this warp's heads, maybe none
         const long long h0 = (long long)hk * G + head0 + group * HW;
-        unsigned char* qs = smem + (size_t)group * E::Q_BYTES;
         // the first tiles' pages, then the queries while they are on their way
         int key = k0 + kwarp * KT;
         const int step = kwarps * KT;
-        int page = pa_page<KT>(a, row, key, k1);
-        int next = pa_page<KT>(a, row, key + step, k1);
+        const int page0 = pa_page<KT>(a, row, key, k1), page1 = pa_page<KT>(a, row, key + step, k1);
+        int page = pa_page<KT>(a, row, key + 2 * step, k1);
         e.init(a, (const T*)a.q + b * a.q_sb + h0 * a.q_sh, mine, qs, lane, kwarp, kwarps);
-        if (E::Q_BYTES) __syncthreads();
         if (key < k1) {
-            long long off = pa_offset<KT>(a, page, key, first, k1);
+            long long off = pa_offset<KT>(a, page0, key, first, k1);
             unsigned mask = __ballot_sync(0xffffffffu, off >= 0);
-            e.load_k(a, kc, off, lane);
-            e.load_v(a, vc, off, lane);
-            for (;;) {
-                const int nkey = key + step;
-                e.scores(qs, lane);
-                const unsigned now = mask;
-                if (nkey < k1) {
-                    off = pa_offset<KT>(a, next, nkey, first, k1);
-                    mask = __ballot_sync(0xffffffffu, off >= 0);
-                    next = pa_page<KT>(a, row, nkey + step, k1);
-                    e.load_k(a, kc, off, lane);
-                }
-                e.weigh(now, lane);
-                e.values(lane);
-                if (nkey >= k1) break;
-                e.load_v(a, vc, off, lane);
-                key = nkey;
+            e.issue(a, kc, vc, off, ring_at, lane);
+            cp_async_commit();
+            off = pa_offset<KT>(a, page1, key + step, first, k1);
+            unsigned mask_next = __ballot_sync(0xffffffffu, off >= 0);
+            if (key + step < k1) e.issue(a, kc, vc, off, ring_at + E::TILE_BYTES, lane);
+            cp_async_commit();
+            if (E::Q_BYTES) pa_group_sync(group, kwarps);
+            for (int slot = 0;; slot ^= 1) {
+                cp_async_wait<1>();
+                unsigned char* from = ring + slot * E::TILE_BYTES + lane * 16;
+                e.scores(qs, from, lane);
+                e.weigh(mask, lane);
+                e.values(from, lane);
+                key += step;
+                if (key >= k1) break;
+                mask = mask_next;
+                off = pa_offset<KT>(a, page, key + step, first, k1);
+                mask_next = __ballot_sync(0xffffffffu, off >= 0);
+                if (key + step < k1) e.issue(a, kc, vc, off, ring_at + slot * E::TILE_BYTES, lane);
+                cp_async_commit();
+                page = pa_page<KT>(a, row, key + 2 * step, k1);
             }
+            cp_async_wait<0>();
+        } else if (E::Q_BYTES) {
+            pa_group_sync(group, kwarps);
         }
-        if (E::Q_BYTES) __syncthreads();  // obuf lies over the queries
-        e.finish(obuf + (size_t)warp * HW * LD, sm[warp], sl[warp], lane);
+        __syncwarp();  // the warp's sums go where its tiles were
+        e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
         __syncthreads();
         // each head's factors for its warps' sums
         if (tid < sh.groups * HW) {
@@ -237,7 +266,7 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int w = g; w < PA_WARPS; w += sh.groups) {
                 const float f = sf[w][h];
-                const float4 x = *reinterpret_cast<const float4*>(obuf + ((size_t)w * HW + h) * LD + d);
+                const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * PA_SLOTS * E::TILE_BYTES + (h * LD + d) * 4);
                 o.x = fmaf(f, x.x, o.x);
                 o.y = fmaf(f, x.y, o.y);
                 o.z = fmaf(f, x.z, o.z);
@@ -345,17 +374,15 @@ int paged_sm_count();  // of the current device, 0 if it cannot be read
 template <class E>
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     static DeviceOnce once;
-    constexpr size_t kBuf = (size_t)PA_WARPS * E::HW * (E::DC + 4) * 4;
+    constexpr size_t kRing = (size_t)PA_WARPS * PA_SLOTS * E::TILE_BYTES;
+    static_assert(E::HW * (E::DC + 4) * 4 <= PA_SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
     const int G = a.Hq / a.Hkv;
     PagedShape sh{1, 1, 0};
     while (sh.groups < PA_WARPS && sh.groups * E::HW < G) sh.groups *= 2;
     sh.per_kv = (G + sh.groups * E::HW - 1) / (sh.groups * E::HW);
-    const size_t q_bytes = (size_t)sh.groups * E::Q_BYTES, smem = q_bytes > kBuf ? q_bytes : kBuf;
-    if (smem > 40 * 1024) {
-        const size_t most = PA_WARPS * (size_t)E::Q_BYTES > kBuf ? PA_WARPS * (size_t)E::Q_BYTES : kBuf;
-        const cudaError_t e = once.set_smem((const void*)paged_attn_kernel<E>, most);
-        if (e != cudaSuccess) return e;
-    }
+    const size_t smem = kRing + (size_t)sh.groups * E::Q_BYTES;
+    cudaError_t e = once.set_smem((const void*)paged_attn_kernel<E>, kRing + PA_WARPS * E::Q_BYTES);
+    if (e != cudaSuccess) return e;
     const long long items = (long long)a.B * a.Hkv * sh.per_kv;
     const int bound = a.window > 0 && a.window < a.max_len ? a.window + PA_ALIGN : a.max_len;
     const long long units = (bound + PA_UNIT - 1) / PA_UNIT;
@@ -375,7 +402,7 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     parts.ml = reinterpret_cast<float2*>(a.work + (size_t)PA_MAX_BLOCKS * 2 * parts.heads * a.dh);
     parts.rec = reinterpret_cast<int2*>(parts.ml + (size_t)PA_MAX_BLOCKS * 2 * parts.heads);
     paged_attn_kernel<E><<<blocks, PA_THREADS, smem, s>>>(a, sh, parts);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     add_launches(1);
     PdlScope pdl(true);
