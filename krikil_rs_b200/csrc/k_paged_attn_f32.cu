@@ -25,8 +25,8 @@ struct F32Engine {
     static constexpr int KPL = 32 / LPK;               // keys side by side
     static constexpr int KT = J * KPL;                 // 16, 8 or 4 keys
     static constexpr int Q_BYTES = 0;
-    static constexpr int TILE_BYTES = 16 * 512;
-    static constexpr int BLOCKS = 3;
+    static constexpr int TILE_BYTES = 8 * 512, SLOTS = 1;
+    static constexpr int BLOCKS = 4;
     static constexpr float SCALE = 1.f;
 
     float4 q[GW][NL], acc[GW][NL];
@@ -46,19 +46,19 @@ struct F32Engine {
             }
         }
     }
-    KRK_DEV void issue(const PagedAttnArgs& a, const float* kc, const float* vc, long long off, uint32_t to,
-                       int lane) {
+    // A lane copies what it reads itself: load i of a tile fills 512 consecutive bytes.
+    KRK_DEV void issue(const PagedAttnArgs& a, const float* base, const PagedTile& t, uint32_t to, int lane) {
+        constexpr unsigned kAll = (1u << KT) - 1;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const long long o = __shfl_sync(0xffffffffu, off, j * KPL + lane / LPK);
+            const int key = j * KPL + lane / LPK;
+            const bool seen = t.mask == kAll || (t.mask >> key & 1u);
+            const long long off = pa_key(a, t, key);
+            const float* p = seen ? base + off + (lane & (LPK - 1)) * 4 : base;
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                const int d = ((lane & (LPK - 1)) + i * LPK) * 4;
-                const bool take = o >= 0 && d < a.dh;
-                const long long at = take ? o + d : 0;
-                pa_copy<16>(to + (j * NL + i) * 512, kc + at, take);
-                pa_copy<16>(to + (8 + j * NL + i) * 512, vc + at, take);
-            }
+            for (int i = 0; i < NL; ++i)
+                pa_copy<16>(to + lane * 16 + (j * NL + i) * 512, p + (seen ? i * LPK * 4 : 0),
+                            seen && ((lane & (LPK - 1)) + i * LPK) * 4 < a.dh);
         }
     }
 
@@ -94,7 +94,7 @@ struct F32Engine {
     KRK_DEV void scores(const unsigned char*, const unsigned char* from, int lane) {
         float4 k[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const float4*>(from + j * 512);
+        for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const float4*>(from + lane * 16 + j * 512);
 #pragma unroll
         for (int h = 0; h < GW; ++h) {
             float x[J];
@@ -134,7 +134,7 @@ struct F32Engine {
     KRK_DEV void values(const unsigned char* from, int lane) {
         float4 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float4*>(from + (8 + j) * 512);
+        for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float4*>(from + lane * 16 + j * 512);
         const int side = lane & ~(LPK - 1);
 #pragma unroll
         for (int h = 0; h < GW; ++h) {
@@ -207,10 +207,8 @@ int paged_sm_count() {
 }
 
 size_t attn_paged_work_floats(int Hq, int Hkv, int dh) {
-    // as many heads a block as any engine takes
-    int heads = 8;
-    while (heads < PA_MAX_HEADS && heads < Hq / Hkv) heads *= 2;
-    return (size_t)PA_MAX_BLOCKS * (2 * (size_t)heads * (dh + 2) + 2);
+    const int share = Hq / Hkv, rows = 4 * share < PA_MAX_ROWS ? 4 * share : PA_MAX_ROWS;
+    return (size_t)PA_MAX_BLOCKS * (2 * (size_t)rows * (dh + 2) + 2);
 }
 
 cudaError_t attn_decode_paged_f32(const PagedAttnArgs& a, cudaStream_t s) {

@@ -1,18 +1,14 @@
 // Decode attention over half and bfloat16 pages: the engine on m16n8k16 matrix
 // instructions.
 //
-// A warp's tile is 16 keys and 8 query heads that share them.  The contraction
-// index of a matrix instruction may be permuted as long as both operands agree,
-// and so may its rows and columns, so the 16 bytes that a lane copies are its
-// operands as they come:
-//   S = Q K^T (heads x keys, contracted over dh): lane 4n + t of a load holds
-//     elements 8t .. 8t+7 of a 32-element block of key n (and n + 8): two
-//     k = 16 steps, whose Q operand holds the same elements.
-//   O^T = V^T P^T (dh x heads, contracted over keys): lane 4r + t loads elements
-//     8r .. 8r+7 of a 64-element block of keys 2t, 2t+1, 2t+8, 2t+9; pairs of
-//     keys are put side by side with byte permutes, and P^T is S's own layout.
-// No lane reads what another one copied, and no warp waits for another before a
-// piece ends.
+// A warp's tile is 16 keys and 8 query heads that share them:
+//   S = Q K^T        16 x 8 over k = 16: heads (two parts of each, or eight empty rows) x keys over dh
+//   O^T = V^T P^T    16 x 8 over k = 16: elements of dh x heads over keys
+// Rows of K are the second operand as they lie, rows of V the first one
+// transposed by the load (ldmatrix), and P^T's operand layout is the one that S
+// comes out in, so weights never leave their lane's registers.  The 16-byte
+// pieces of a row are permuted by its number so that neither the copies nor the
+// matrix loads meet in a bank.
 //
 // Precision: the products are exact and added in 32 bits, and a tile's sum is
 // folded into the float32 accumulators once a tile.  A float32 weight is the
@@ -53,21 +49,32 @@ KRK_DEV uint32_t pack_rest(float& x, float& y, __nv_bfloat16) {
     return u;
 }
 
-// Starts the copy of elements 8 * chunk .. + 7 of a row (zeros past dh, and for off < 0); wide: rows are 16-byte
-// aligned and dh a multiple of 8.
-template <bool WIDE, typename C>
-KRK_DEV void copy_chunk(uint32_t to, const C* base, long long off, int chunk, int dh) {
-    const bool take = off >= 0 && chunk * 8 < dh;
-    const C* p = take ? base + off + chunk * 8 : base;
-    if (WIDE) {
-        pa_copy<16>(to, p, take);
-    } else {
-        const bool more = take && chunk * 8 + 4 < dh;
-        pa_copy<8>(to, p, take);
-        pa_copy<8>(to + 8, more ? p + 4 : base, more);
-    }
+// The same onto zero.
+KRK_DEV void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                       __half) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-KRK_DEV uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+KRK_DEV void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                       __nv_bfloat16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Four 8 x 8 matrices of 16-bit elements, lane l giving row l % 8 of matrix l / 8.
+KRK_DEV void load_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+KRK_DEV void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
 
 template <typename T, typename C, int DC_, bool WIDE>
 struct HalfEngine {
@@ -75,17 +82,18 @@ struct HalfEngine {
     using Cache = C;
     static constexpr bool kSame = sizeof(T) == 2, kHalf = sizeof(__half) == 2 && std::is_same<C, __half>::value;
     static constexpr int DC = DC_, KT = 16, HW = 8;
-    static constexpr int NB = DC / 32, NV = DC / 64;
+    static constexpr int NB = DC / 32, NV = DC / 16;     // steps of the two products
+    static constexpr int ROW = DC * 2, CPR = DC / 8;      // bytes and 16-byte pieces of a row
+    static constexpr int RPC = 32 / CPR;                  // rows of one copy
     static constexpr int QP = kSame ? 1 : kHalf ? 2 : 3;  // parts of a query
     static constexpr int PP = !kSame && !kHalf ? 3 : 2;   // parts of a weight
     static constexpr int Q_BYTES = QP * NB * 32 * 16;
-    static constexpr int K_LOADS = NB * 2, V_LOADS = NV * 4;  // of a lane, for a tile
-    static constexpr int TILE_BYTES = (K_LOADS + V_LOADS) * 512;
-    static constexpr int BLOCKS = DC == 64 ? 4 : DC == 128 ? 3 : 1;
+    static constexpr int TILE_BYTES = KT * ROW, SLOTS = 1;
+    static constexpr int BLOCKS = DC <= 128 ? 4 : 2;
     static constexpr float SCALE = kHalf ? 16384.f : 1.f;
 
-    float acc[NV][4][4];
-    float s[4], m, l, c;
+    float acc[NV][4];
+    float s[4], m, l, c, fade;
 
     // Lays the parts of the group's queries out as the first operand's registers.  Each warp of a group prepares
     // every kwarps-th head.
@@ -96,9 +104,7 @@ struct HalfEngine {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) acc[i][j][x] = 0.f;
+            for (int x = 0; x < 4; ++x) acc[i][x] = 0.f;
         c = a.scale * 1.44269504088896341f;
         for (int h = kwarp; h < HW; h += kwarps) {
             float4 x[DC / 128 ? DC / 128 : 1];
@@ -118,10 +124,10 @@ struct HalfEngine {
                 float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
 #pragma unroll
                 for (int p = 0; p < QP; ++p) {
-                    uint2 u;
-                    u.x = pack_rest(y.x, y.y, C());
-                    u.y = pack_rest(y.z, y.w, C());
-                    *reinterpret_cast<uint2*>(qs + ((p * NB + d / 32) * 32 + h * 4 + d % 32 / 8) * 16 + d % 8 * 2) = u;
+                    uint32_t* to = reinterpret_cast<uint32_t*>(qs) +
+                                   ((p * NB + d / 32) * 32 + h * 4 + d % 8 / 2) * 4 + d % 32 / 8;
+                    to[0] = pack_rest(y.x, y.y, C());
+                    to[4] = pack_rest(y.z, y.w, C());
                 }
             }
             if (QP == 2 && lane / 4 == h) c *= 1.0f / up;
@@ -146,43 +152,62 @@ struct HalfEngine {
         return exp2f((float)min(100, max(-100, 14 - ilogbf(most))));
     }
 
-    KRK_DEV void issue(const PagedAttnArgs& a, const C* kc, const C* vc, long long off, uint32_t to, int lane) {
+    KRK_DEV void issue(const PagedAttnArgs& a, const C* base, const PagedTile& t, uint32_t to, int lane) {
+        const int chunk = lane & (CPR - 1), row0 = lane / CPR;
+        const bool in = chunk * 8 < a.dh, more = chunk * 8 + 4 < a.dh;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const long long o = __shfl_sync(0xffffffffu, off, (lane >> 2) + 8 * j);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) copy_chunk<WIDE>(to + (i * 2 + j) * 512, kc, o, i * 4 + (lane & 3), a.dh);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long long o = __shfl_sync(0xffffffffu, off, 2 * (lane & 3) + (j & 1) + (j >> 1) * 8);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                copy_chunk<WIDE>(to + (K_LOADS + i * 4 + j) * 512, vc, o, i * 8 + (lane >> 2), a.dh);
+        for (int j = 0; j < KT / RPC; ++j) {
+            const int row = j * RPC + row0;
+            const bool seen = t.mask == 0xffffu || (t.mask >> row & 1u);
+            const long long off = pa_key(a, t, row);
+            const C* p = seen ? base + off + chunk * 8 : base;
+            const uint32_t at = to + row * ROW + ((chunk ^ (row & 7)) << 4);
+            if (WIDE) {
+                pa_copy<16>(at, p, seen && in);
+            } else {
+                pa_copy<8>(at, p, seen && in);
+                pa_copy<8>(at + 8, p + (seen ? 4 : 0), seen && more);
+            }
         }
     }
 
     KRK_DEV void scores(const unsigned char* qs, const unsigned char* from, int lane) {
-        float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-        float e0[4] = {0.f, 0.f, 0.f, 0.f}, e1[4] = {0.f, 0.f, 0.f, 0.f};
+        float d0[4], d1[4], e0[4], e1[4];
         const uint4* qf = reinterpret_cast<const uint4*>(qs) + lane;
+        const uint32_t at = smem_addr(from) + (lane & 7) * ROW;
+        const int piece = lane >> 3, turn = lane & 7;
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            const uint4 k0 = *reinterpret_cast<const uint4*>(from + (i * 2) * 512);
-            const uint4 k1 = *reinterpret_cast<const uint4*>(from + (i * 2 + 1) * 512);
+            uint32_t k0[4], k1[4];
+            load_matrices(k0, at + (((i * 4 + piece) ^ turn) << 4));
+            load_matrices(k1, at + 8 * ROW + (((i * 4 + piece) ^ turn) << 4));
             const uint4 h = qf[i * 32];
             const uint4 r = QP > 1 ? qf[(NB + i) * 32] : make_uint4(0u, 0u, 0u, 0u);
-            mma(d0, h.x, r.x, h.y, r.y, k0.x, k0.y, C());
-            mma(d1, h.x, r.x, h.y, r.y, k1.x, k1.y, C());
-            mma(d0, h.z, r.z, h.w, r.w, k0.z, k0.w, C());
-            mma(d1, h.z, r.z, h.w, r.w, k1.z, k1.w, C());
+            if (i == 0) {
+                mma_first(d0, h.x, r.x, h.y, r.y, k0[0], k0[1], C());
+                mma_first(d1, h.x, r.x, h.y, r.y, k1[0], k1[1], C());
+            } else {
+                mma(d0, h.x, r.x, h.y, r.y, k0[0], k0[1], C());
+                mma(d1, h.x, r.x, h.y, r.y, k1[0], k1[1], C());
+            }
+            mma(d0, h.z, r.z, h.w, r.w, k0[2], k0[3], C());
+            mma(d1, h.z, r.z, h.w, r.w, k1[2], k1[3], C());
             if (QP > 2) {
                 const uint4 t = qf[(2 * NB + i) * 32];
-                mma(e0, t.x, 0u, t.y, 0u, k0.x, k0.y, C());
-                mma(e1, t.x, 0u, t.y, 0u, k1.x, k1.y, C());
-                mma(e0, t.z, 0u, t.w, 0u, k0.z, k0.w, C());
-                mma(e1, t.z, 0u, t.w, 0u, k1.z, k1.w, C());
+                if (i == 0) {
+                    mma_first(e0, t.x, 0u, t.y, 0u, k0[0], k0[1], C());
+                    mma_first(e1, t.x, 0u, t.y, 0u, k1[0], k1[1], C());
+                } else {
+                    mma(e0, t.x, 0u, t.y, 0u, k0[0], k0[1], C());
+                    mma(e1, t.x, 0u, t.y, 0u, k1[0], k1[1], C());
+                }
+                mma(e0, t.z, 0u, t.w, 0u, k0[2], k0[3], C());
+                mma(e1, t.z, 0u, t.w, 0u, k1[2], k1[3], C());
             }
+        }
+        if (QP <= 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e0[i] = e1[i] = 0.f;
         }
         s[0] = joined(d0[0], d0[2], e0[0]);
         s[1] = joined(d0[1], d0[3], e0[1]);
@@ -210,42 +235,37 @@ struct HalfEngine {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         top = fmaxf(top, m);
         const float ref = top == -INFINITY ? 0.f : top;
-        const float fade = exp2f(m - ref);
+        fade = exp2f(m - ref);
         m = top;
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[i] = exp2f(s[i] - ref) * SCALE;
         l = l * fade + ((s[0] + s[1]) + (s[2] + s[3]));
-        c_fade = fade;
     }
-    float c_fade;
 
     KRK_DEV void values(const unsigned char* from, int lane) {
-        const float f0 = __shfl_sync(0xffffffffu, c_fade, (lane & 3) * 8);
-        const float f1 = __shfl_sync(0xffffffffu, c_fade, (lane & 3) * 8 + 4);
+        const float f0 = __shfl_sync(0xffffffffu, fade, (lane & 3) * 8);
+        const float f1 = __shfl_sync(0xffffffffu, fade, (lane & 3) * 8 + 4);
         uint32_t p[PP][2];
 #pragma unroll
         for (int i = 0; i < PP; ++i) {
             p[i][0] = pack_rest(s[0], s[1], C());
             p[i][1] = pack_rest(s[2], s[3], C());
         }
+        // matrices: keys 0-7 and 8-15 of the pieces 2i and 2i + 1
+        const int key = (lane >> 4) * 8 + (lane & 7), piece = lane >> 3 & 1, turn = lane & 7;
+        const uint32_t at = smem_addr(from) + key * ROW;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            uint4 v[4];
+            uint32_t v[4];
+            load_matrices_t(v, at + (((i * 2 + piece) ^ turn) << 4));
+            float d[4];
+            mma_first(d, v[0], v[1], v[2], v[3], p[PP - 1][0], p[PP - 1][1], C());
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(from + (K_LOADS + i * 4 + j) * 512);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w0 = word(v[0], j), w1 = word(v[1], j), w2 = word(v[2], j), w3 = word(v[3], j);
-                const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
-                const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int x = PP - 1; x >= 0; --x) mma(d, a0, a1, a2, a3, p[x][0], p[x][1], C());
-                acc[i][j][0] = fmaf(acc[i][j][0], f0, d[0]);
-                acc[i][j][1] = fmaf(acc[i][j][1], f1, d[1]);
-                acc[i][j][2] = fmaf(acc[i][j][2], f0, d[2]);
-                acc[i][j][3] = fmaf(acc[i][j][3], f1, d[3]);
-            }
+            for (int x = PP - 2; x >= 0; --x) mma(d, v[0], v[1], v[2], v[3], p[x][0], p[x][1], C());
+            acc[i][0] = fmaf(acc[i][0], f0, d[0]);
+            acc[i][1] = fmaf(acc[i][1], f1, d[1]);
+            acc[i][2] = fmaf(acc[i][2], f0, d[2]);
+            acc[i][3] = fmaf(acc[i][3], f1, d[3]);
         }
     }
 
@@ -258,13 +278,13 @@ struct HalfEngine {
             sl[r] = l;
         }
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float* o = obuf + 2 * t * (DC + 4) + i * 64 + r * 8 + j * 2;
-                *reinterpret_cast<float2*>(o) = make_float2(acc[i][j][0], acc[i][j][2]);
-                *reinterpret_cast<float2*>(o + DC + 4) = make_float2(acc[i][j][1], acc[i][j][3]);
-            }
+        for (int i = 0; i < NV; ++i) {
+            float* o = obuf + 2 * t * (DC + 4) + i * 16 + r;
+            o[0] = acc[i][0];
+            o[DC + 4] = acc[i][1];
+            o[8] = acc[i][2];
+            o[DC + 12] = acc[i][3];
+        }
     }
 };
 

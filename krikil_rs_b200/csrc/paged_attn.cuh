@@ -8,8 +8,9 @@
 // units of 64, and the units of the whole batch -- whatever the requests'
 // lengths -- are dealt to one resident wave of blocks in equal contiguous
 // shares.  A block works off its share piece by piece (a piece lies within one
-// request and head); its warps take tiles of keys in turn, each with a running
-// maximum and sum, and are merged in shared memory at the piece's end.  A piece
+// request and one cache head, or up to four neighbours of it); its warps take
+// tiles of keys in turn, each with a running maximum and sum, and are merged in
+// shared memory at the piece's end.  A piece
 // that covers all of its keys is written as the result; otherwise its sums go
 // to the scratch, where attn_paged_join adds them up in the order of the
 // blocks, so that results do not depend on timing.
@@ -26,23 +27,25 @@ constexpr int PA_THREADS = 128, PA_WARPS = 4;
 constexpr int PA_UNIT = 64;          // keys of one unit of work
 constexpr int PA_WHOLE_UNITS = 4;    // up to this many units a block takes a whole (request, head)
 constexpr int PA_MAX_BLOCKS = 592;   // blocks of a wave: four on each of 148 SMs
-constexpr int PA_MAX_HEADS = 32;     // query heads of a block, at most
-constexpr int PA_SLOTS = 2;          // tiles of a warp's ring
+constexpr int PA_MAX_ROWS = 32;      // query heads of a piece, at most
+constexpr int PA_SIDE_UNITS = 8;     // units a block from which on its warps take different cache heads
 constexpr int PA_ALIGN = 16;         // a piece's first key is aligned down to the largest tile
 
 // Scratch of a launch: two partial results a block -- slot 0 for a piece that
 // does not start its keys, slot 1 for one that does -- and their owners.
 struct PagedParts {
-    float* acc;  // [blocks][2][heads][dh]
-    float2* ml;  // [blocks][2][heads] running maximum (base 2) and sum
-    int2* rec;   // [blocks] (request, head) of slots 0 and 1, -1: none
-    int heads;
+    float* acc;  // [blocks][2][rows][dh]
+    float2* ml;  // [blocks][2][rows] running maximum (base 2) and sum
+    int2* rec;   // [blocks] (request, heads) of slots 0 and 1, -1: none
 };
 
+// How a block's warps divide a piece: `side` neighbouring cache heads, `groups`
+// sets of query heads of each, and the keys among the warps that are left.
 struct PagedShape {
-    int groups;   // warps that share a tile, each with its own query heads
-    int per_kv;   // pieces side by side for the query heads of one cache head
-    int whole;    // blocks take whole (request, head)s
+    int side, groups;
+    int per_kv;   // pieces for the query heads of one cache head
+    int rows;     // query heads of a piece
+    int whole;    // blocks take whole (request, heads)
 };
 
 KRK_DEV int pa_len(const PagedAttnArgs& a, int b) {
@@ -105,22 +108,41 @@ KRK_DEV PagedShare pa_share(const PagedAttnArgs& a, int pieces, PagedShare* out,
     return *out;
 }
 
-// The row offset of this lane's key (key0 + lane % KT) of a tile, -1 when the
-// key is not visible or its page is outside the pool.
+// Where a tile's keys lie.  Tiles are aligned, so pages of 16 tokens or more
+// hold a tile in one piece: off is its first key's offset and the others follow
+// by c_st.  On smaller pages lane i holds the offset of key i (mod KT).
+struct PagedTile {
+    long long off;
+    unsigned mask;  // the visible keys
+};
 template <int KT>
 KRK_DEV int pa_page(const PagedAttnArgs& a, const int32_t* row, int key0, int k1) {
-    const int key = key0 + (threadIdx.x & (KT - 1));
-    return key < k1 ? row[key >> a.page_shift] : 0;
+    const int key = a.page_shift >= 4 ? key0 : key0 + (threadIdx.x & (KT - 1));
+    return key < k1 ? row[key >> a.page_shift] : -1;
 }
 template <int KT>
-KRK_DEV long long pa_offset(const PagedAttnArgs& a, int page, int key0, int first, int k1) {
-    const int key = key0 + (threadIdx.x & (KT - 1));
-    if (key < first || key >= k1) return -1;
-    if ((unsigned)page >= (unsigned)a.num_pages) {
-        check_fail(CHK_TABLE);
-        return -1;
+KRK_DEV PagedTile pa_tile(const PagedAttnArgs& a, int page, int key0, int first, int k1) {
+    constexpr unsigned kAll = KT == 32 ? ~0u : (1u << KT) - 1;
+    const int low = (1 << a.page_shift) - 1;
+    const bool in = (unsigned)page < (unsigned)a.num_pages;
+    PagedTile t;
+    if (a.page_shift >= 4) {
+        if (!in && key0 < k1) check_fail(CHK_TABLE);
+        t.mask = in ? kAll : 0u;
+        if (key0 < first) t.mask &= ~0u << min(first - key0, 31);
+        if (key0 + KT > k1) t.mask &= key0 < k1 ? kAll >> (key0 + KT - k1) : 0u;
+        t.off = page * a.c_sp + (key0 & low) * a.c_st;
+    } else {
+        const int key = key0 + (threadIdx.x & (KT - 1));
+        if (!in && key >= first && key < k1) check_fail(CHK_TABLE);
+        t.mask = __ballot_sync(0xffffffffu, in && key >= first && key < k1) & kAll;
+        t.off = page * a.c_sp + (key & low) * a.c_st;
     }
-    return page * a.c_sp + (key & ((1 << a.page_shift) - 1)) * a.c_st;
+    return t;
+}
+// The element offset of key `key` of the tile (a fixed key for each lane).
+KRK_DEV long long pa_key(const PagedAttnArgs& a, const PagedTile& t, int key) {
+    return a.page_shift >= 4 ? t.off + key * a.c_st : __shfl_sync(0xffffffffu, t.off, key);
 }
 
 // Barrier of the warps that share a group's queries.
@@ -142,32 +164,32 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 }
 
 // E: an engine.  Its warp holds KT keys of a tile and HW query heads:
-//   init(a, q, heads, qs)     loads a warp's queries (or prepares them in shared memory)
-//   issue(k, v, off, to)      starts the copies of a tile, from the lanes' row offsets to its ring slot
-//   scores(qs, from)          q . k of the slot's keys
-//   weigh(mask)               softmax step over the visible keys of the tile
-//   values(from)              weighted values into the accumulators
-//   finish(obuf, m, l)        accumulators, maxima and sums of the warp to shared memory
-// A lane copies exactly the 16-byte pieces that it reads itself, each load of a
-// tile in 512 consecutive bytes of the warp's ring: no bank conflicts, no
-// barrier, and two tiles a warp in flight without holding registers.
+//   init(a, q, heads, qs)       loads a warp's queries (or prepares them in shared memory)
+//   issue(base, tile, to)       starts the copies of a tile's keys or values to a ring slot
+//   scores(qs, from)            q . k of the slot's keys
+//   weigh(mask)                 softmax step over the visible keys of the tile
+//   values(from)                weighted values into the accumulators
+//   finish(obuf, m, l)          accumulators, maxima and sums of the warp to shared memory
+// A warp's ring has SLOTS slots for keys and as many for values; a slot is
+// filled again as soon as the warp has read it, with no barrier beyond the warp.
 template <class E>
 __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a,
                                                                            const PagedShape sh,
                                                                            const PagedParts parts) {
     using T = typename E::Act;
     using C = typename E::Cache;
-    constexpr int KT = E::KT, HW = E::HW, LD = E::DC + 4;
-    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int KT = E::KT, HW = E::HW, LD = E::DC + 4, S = E::SLOTS, HALF = E::TILE_BYTES;
+    extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sm[PA_WARPS][HW], sl[PA_WARPS][HW], sf[PA_WARPS][HW];
     __shared__ long long warp_sums[PA_WARPS];
     __shared__ PagedShare share_out;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int G = a.Hq / a.Hkv, pieces = a.Hkv * sh.per_kv;
-    const int kwarps = PA_WARPS / sh.groups, group = warp % sh.groups, kwarp = warp / sh.groups;
-    unsigned char* ring = smem + (size_t)warp * PA_SLOTS * E::TILE_BYTES;
-    unsigned char* qs = smem + PA_WARPS * PA_SLOTS * E::TILE_BYTES + (size_t)group * E::Q_BYTES;
-    const uint32_t ring_at = smem_addr(ring) + lane * 16;
+    const int G = a.Hq / a.Hkv, pieces = a.Hkv / sh.side * sh.per_kv;
+    // warp -> (keys, cache head, query heads)
+    const int sets = sh.side * sh.groups, kwarps = PA_WARPS / sets, kwarp = warp / sets, set = warp % sets;
+    unsigned char* ring = smem + (size_t)warp * 2 * S * HALF;
+    unsigned char* qs = smem + (size_t)PA_WARPS * 2 * S * HALF + (size_t)set * E::Q_BYTES;
+    const uint32_t ring_at = smem_addr(ring);
 
     PagedShare share;
     if (sh.whole) {
@@ -187,7 +209,8 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
 
     while (left > 0) {
         const int take = (int)min((long long)(units - unit), left);
-        const int hk = piece / sh.per_kv, head0 = (piece % sh.per_kv) * sh.groups * HW;  // within the cache head's G
+        const int hk0 = piece / sh.per_kv * sh.side, head0 = piece % sh.per_kv * sh.rows;  // head0: within G
+        const int hk = hk0 + set / sh.groups, head = head0 + set % sh.groups * HW;
         const int base = first & ~(PA_ALIGN - 1);
         const int k0 = base + unit * PA_UNIT, k1 = min(n, base + (unit + take) * PA_UNIT);
         const int32_t* row = a.table + b * a.table_ld;
@@ -195,88 +218,98 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
         const C* vc = (const C*)a.vc + hk * a.c_sh;
 
         E e;
-        const int mine = min(HW, G - head0 - group * HW);  // this warp's heads, maybe none
-        const long long h0 = (long long)hk * G + head0 + group * HW;
-        // the first tiles' pages, then the queries while they are on their way
         int key = k0 + kwarp * KT;
         const int step = kwarps * KT;
-        const int page0 = pa_page<KT>(a, row, key, k1), page1 = pa_page<KT>(a, row, key + step, k1);
-        int page = pa_page<KT>(a, row, key + 2 * step, k1);
-        e.init(a, (const T*)a.q + b * a.q_sb + h0 * a.q_sh, mine, qs, lane, kwarp, kwarps);
+        // the first tiles' pages, then the queries while they are on their way
+        int pages[S + 1];
+#pragma unroll
+        for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step, k1);
+        e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, min(HW, G - head), qs, lane, kwarp,
+               kwarps);
+        if (E::Q_BYTES) pa_group_sync(set, kwarps);
         if (key < k1) {
-            long long off = pa_offset<KT>(a, page0, key, first, k1);
-            unsigned mask = __ballot_sync(0xffffffffu, off >= 0);
-            e.issue(a, kc, vc, off, ring_at, lane);
-            cp_async_commit();
-            off = pa_offset<KT>(a, page1, key + step, first, k1);
-            unsigned mask_next = __ballot_sync(0xffffffffu, off >= 0);
-            if (key + step < k1) e.issue(a, kc, vc, off, ring_at + E::TILE_BYTES, lane);
-            cp_async_commit();
-            if (E::Q_BYTES) pa_group_sync(group, kwarps);
-            for (int slot = 0;; slot ^= 1) {
-                cp_async_wait<1>();
-                unsigned char* from = ring + slot * E::TILE_BYTES + lane * 16;
-                e.scores(qs, from, lane);
-                e.weigh(mask, lane);
-                e.values(from, lane);
+            unsigned mask[S + 1];
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
+                mask[i] = t.mask;
+                if (key + i * step < k1) e.issue(a, kc, t, ring_at + i * HALF, lane);
+                cp_async_commit();
+                if (key + i * step < k1) e.issue(a, vc, t, ring_at + (S + i) * HALF, lane);
+                cp_async_commit();
+            }
+            int page = pages[S];
+            for (int slot = 0;; slot = slot + 1 == S ? 0 : slot + 1) {
+                const int ahead = key + S * step;
+                cp_async_wait<2 * S - 1>();
+                __syncwarp();
+                e.scores(qs, ring + slot * HALF, lane);
+                __syncwarp();
+                const PagedTile t = pa_tile<KT>(a, page, ahead, first, k1);
+                mask[S] = t.mask;
+                if (ahead < k1) e.issue(a, kc, t, ring_at + slot * HALF, lane);
+                cp_async_commit();
+                page = pa_page<KT>(a, row, ahead + step, k1);
+                e.weigh(mask[0], lane);
+                cp_async_wait<2 * S - 1>();
+                __syncwarp();
+                e.values(ring + (S + slot) * HALF, lane);
                 key += step;
                 if (key >= k1) break;
-                mask = mask_next;
-                off = pa_offset<KT>(a, page, key + step, first, k1);
-                mask_next = __ballot_sync(0xffffffffu, off >= 0);
-                if (key + step < k1) e.issue(a, kc, vc, off, ring_at + slot * E::TILE_BYTES, lane);
+                __syncwarp();
+                if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * HALF, lane);
                 cp_async_commit();
-                page = pa_page<KT>(a, row, key + 2 * step, k1);
+#pragma unroll
+                for (int i = 0; i < S; ++i) mask[i] = mask[i + 1];
             }
-            cp_async_wait<0>();
-        } else if (E::Q_BYTES) {
-            pa_group_sync(group, kwarps);
         }
         __syncwarp();  // the warp's sums go where its tiles were
         e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
         __syncthreads();
-        // each head's factors for its warps' sums
-        if (tid < sh.groups * HW) {
-            const int g = tid / HW, h = tid % HW;
+        // each query head's factors for its warps' sums
+        const int rows = sh.side * sh.rows;
+        if (tid < sets * HW) {
+            const int w0 = tid / HW, h = tid % HW, in_g = w0 % sh.groups * HW + h;
             float top = -INFINITY, total = 0.f;
-            for (int w = g; w < PA_WARPS; w += sh.groups) top = fmaxf(top, sm[w][h]);
-            for (int w = g; w < PA_WARPS; w += sh.groups) {
+            for (int w = w0; w < PA_WARPS; w += sets) top = fmaxf(top, sm[w][h]);
+            for (int w = w0; w < PA_WARPS; w += sets) {
                 const float f = top == -INFINITY ? (sl[w][h] == 0.f ? 0.f : sl[w][h]) : exp2f(sm[w][h] - top);
                 sf[w][h] = f;
                 total = fmaf(f, sl[w][h], total);
             }
-            const int head = head0 + tid;
-            if (head < G) {
+            if (in_g < sh.rows && head0 + in_g < G) {
                 if (take == units) {
                     const float inv = total == 0.f ? 0.f : 1.0f / total;
-                    for (int w = g; w < PA_WARPS; w += sh.groups) sf[w][h] *= inv;
+                    for (int w = w0; w < PA_WARPS; w += sets) sf[w][h] *= inv;
                     if (a.lse)
-                        a.lse[(long long)b * a.Hq + hk * G + head] =
+                        a.lse[(long long)b * a.Hq + (long long)(hk0 + w0 / sh.groups) * G + head0 + in_g] =
                             (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
                 } else {
-                    parts.ml[((long long)blockIdx.x * 2 + (unit == 0)) * parts.heads + tid] = make_float2(top, total);
+                    parts.ml[((long long)blockIdx.x * 2 + (unit == 0)) * rows + w0 / sh.groups * sh.rows + in_g] =
+                        make_float2(top, total);
                 }
             }
         }
         __syncthreads();
         const int n4 = a.dh / 4;
-        for (int i = tid; i < sh.groups * HW * n4; i += PA_THREADS) {
-            const int gh = i / n4, d = (i % n4) * 4, g = gh / HW, h = gh % HW;
-            if (head0 + gh >= G) continue;
+        for (int i = tid; i < rows * n4; i += PA_THREADS) {
+            const int r = i / n4, d = (i - r * n4) * 4, s = r / sh.rows, in_g = r - s * sh.rows;
+            if (head0 + in_g >= G) continue;
+            const int w0 = s * sh.groups + in_g / HW, h = in_g % HW;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = g; w < PA_WARPS; w += sh.groups) {
+            for (int w = w0; w < PA_WARPS; w += sets) {
                 const float f = sf[w][h];
-                const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * PA_SLOTS * E::TILE_BYTES + (h * LD + d) * 4);
+                const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * HALF + (h * LD + d) * 4);
                 o.x = fmaf(f, x.x, o.x);
                 o.y = fmaf(f, x.y, o.y);
                 o.z = fmaf(f, x.z, o.z);
                 o.w = fmaf(f, x.w, o.w);
             }
             if (take == units)
-                store4((T*)a.out + b * a.o_sb + ((long long)hk * G + head0 + gh) * a.o_sh + d, o);
+                store4((T*)a.out + b * a.o_sb + ((long long)(hk0 + s) * G + head0 + in_g) * a.o_sh + d, o);
             else
                 *reinterpret_cast<float4*>(
-                    parts.acc + (((long long)blockIdx.x * 2 + (unit == 0)) * parts.heads + gh) * a.dh + d) = o;
+                    parts.acc + (((long long)blockIdx.x * 2 + (unit == 0)) * rows + r) * a.dh + d) = o;
         }
         if (take != units) (unit == 0 ? rec.y : rec.x) = b * pieces + piece;
         left -= take;
@@ -289,35 +322,34 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             first = pa_first(a, n);
             units = pa_units(n, first);
         }
-        __syncthreads();  // the next piece's queries go where this one's sums were
+        __syncthreads();  // the next piece's tiles go where this one's sums were
     }
     if (!sh.whole && tid == 0) parts.rec[blockIdx.x] = rec;
 }
 
-// Joins the partial results: block (c, h) looks whether block c of the
-// attention began a (request, head) that it did not finish, and if so adds up
-// query head h of it over the blocks c, c + 1, ... that worked on it.
+// Joins the partial results: block (c, r) looks whether block c of the
+// attention began a piece's keys without finishing them, and if so adds up query
+// head r of the piece over the blocks c, c + 1, ... that worked on it.
 template <typename T>
 __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnArgs a, const PagedShape sh,
-                                                               const PagedParts parts, int blocks, int hw,
-                                                               float scale) {
+                                                               const PagedParts parts, int blocks, float scale) {
     __shared__ float weight[PA_MAX_BLOCKS + 1];
     __shared__ float red[2][PA_WARPS];
     __shared__ float4 sums[PA_THREADS];
-    const int c = blockIdx.x, gh = blockIdx.y, tid = threadIdx.x;
+    const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
     pdl_wait();
     const int item = parts.rec[c].y;
     if (item < 0) return;
-    const int G = a.Hq / a.Hkv, pieces = a.Hkv * sh.per_kv;
-    const int b = item / pieces, piece = item % pieces, hk = piece / sh.per_kv;
-    const int head = (piece % sh.per_kv) * sh.groups * hw + gh;
-    if (head >= G) return;
+    const int G = a.Hq / a.Hkv, pieces = a.Hkv / sh.side * sh.per_kv, rows = sh.side * sh.rows;
+    const int b = item / pieces, piece = item % pieces, in_g = piece % sh.per_kv * sh.rows + r % sh.rows;
+    if (in_g >= G) return;
+    const long long head = (long long)(piece / sh.per_kv * sh.side + r / sh.rows) * G + in_g;
     int count = 1;  // the blocks of an item are neighbours
     for (int i = c + 1; i < blocks; i += PA_THREADS)
         count += __syncthreads_count(i + tid < blocks && parts.rec[min(i + tid, blocks - 1)].x == item);
     // weights 2^(m - top) and the sum
     float top = -INFINITY, total = 0.f;
-    auto ml = [&](int i) { return parts.ml[((long long)(c + i) * 2 + (i == 0)) * parts.heads + gh]; };
+    auto ml = [&](int i) { return parts.ml[((long long)(c + i) * 2 + (i == 0)) * rows + r]; };
     for (int i = tid; i < count; i += PA_THREADS) top = fmaxf(top, ml(i).x);
     top = warp_max(top);
     if ((tid & 31) == 0) red[0][tid >> 5] = top;
@@ -341,7 +373,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnA
 #pragma unroll 8
         for (int i = s0; i < count; i += side) {
             const float4 x = *reinterpret_cast<const float4*>(
-                parts.acc + (((long long)(c + i) * 2 + (i == 0)) * parts.heads + gh) * a.dh + d);
+                parts.acc + (((long long)(c + i) * 2 + (i == 0)) * rows + r) * a.dh + d);
             const float f = weight[i];
             o.x = fmaf(f, x.x, o.x);
             o.y = fmaf(f, x.y, o.y);
@@ -363,10 +395,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnA
         o.y *= inv;
         o.z *= inv;
         o.w *= inv;
-        store4((T*)a.out + b * a.o_sb + ((long long)hk * G + head) * a.o_sh + d, o);
+        store4((T*)a.out + b * a.o_sb + head * a.o_sh + d, o);
     }
     if (tid == 0 && a.lse)
-        a.lse[(long long)b * a.Hq + hk * G + head] = (top + log2f(total * (1.0f / scale))) * 0.693147180559945309f;
+        a.lse[(long long)b * a.Hq + head] = (top + log2f(total * (1.0f / scale))) * 0.693147180559945309f;
 }
 
 int paged_sm_count();  // of the current device, 0 if it cannot be read
@@ -374,40 +406,43 @@ int paged_sm_count();  // of the current device, 0 if it cannot be read
 template <class E>
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     static DeviceOnce once;
-    constexpr size_t kRing = (size_t)PA_WARPS * PA_SLOTS * E::TILE_BYTES;
-    static_assert(E::HW * (E::DC + 4) * 4 <= PA_SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
-    const int G = a.Hq / a.Hkv;
-    PagedShape sh{1, 1, 0};
-    while (sh.groups < PA_WARPS && sh.groups * E::HW < G) sh.groups *= 2;
-    sh.per_kv = (G + sh.groups * E::HW - 1) / (sh.groups * E::HW);
-    const size_t smem = kRing + (size_t)sh.groups * E::Q_BYTES;
+    constexpr size_t kRing = (size_t)PA_WARPS * 2 * E::SLOTS * E::TILE_BYTES;
+    static_assert(E::HW * (E::DC + 4) * 4 <= 2 * E::SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
+    const int G = a.Hq / a.Hkv, sms = paged_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
     cudaError_t e = once.set_smem((const void*)paged_attn_kernel<E>, kRing + PA_WARPS * E::Q_BYTES);
     if (e != cudaSuccess) return e;
-    const long long items = (long long)a.B * a.Hkv * sh.per_kv;
+    const int slots = sms * E::BLOCKS < PA_MAX_BLOCKS ? sms * E::BLOCKS : PA_MAX_BLOCKS;
     const int bound = a.window > 0 && a.window < a.max_len ? a.window + PA_ALIGN : a.max_len;
     const long long units = (bound + PA_UNIT - 1) / PA_UNIT;
+    PagedShape sh{1, 1, 1, 0, 0};
+    while (sh.groups < PA_WARPS && sh.groups * E::HW < G) sh.groups *= 2;
+    sh.per_kv = (G + sh.groups * E::HW - 1) / (sh.groups * E::HW);
+    sh.rows = G < sh.groups * E::HW ? G : sh.groups * E::HW;
+    // With work for every block, warps take neighbouring cache heads of the same keys.
+    while (sh.side * sh.groups < PA_WARPS && a.Hkv % (2 * sh.side) == 0 &&
+           (long long)a.B * (a.Hkv / sh.side / 2) * sh.per_kv * units >= PA_SIDE_UNITS * (long long)slots)
+        sh.side *= 2;
+    const size_t smem = kRing + (size_t)sh.side * sh.groups * E::Q_BYTES;
+    const long long items = (long long)a.B * (a.Hkv / sh.side) * sh.per_kv;
     if (units <= PA_WHOLE_UNITS) {
         sh.whole = 1;
         paged_attn_kernel<E><<<(unsigned)items, PA_THREADS, smem, s>>>(a, sh, PagedParts{});
         add_launches(1);
         return cudaGetLastError();
     }
-    const int sms = paged_sm_count();
-    if (sms <= 0) return cudaErrorInvalidDevice;
-    int blocks = sms * E::BLOCKS < PA_MAX_BLOCKS ? sms * E::BLOCKS : PA_MAX_BLOCKS;
-    if (items * units < blocks) blocks = (int)(items * units);
+    const int blocks = items * units < slots ? (int)(items * units) : slots, rows = sh.side * sh.rows;
     PagedParts parts;
-    parts.heads = sh.groups * E::HW;
     parts.acc = a.work;
-    parts.ml = reinterpret_cast<float2*>(a.work + (size_t)PA_MAX_BLOCKS * 2 * parts.heads * a.dh);
-    parts.rec = reinterpret_cast<int2*>(parts.ml + (size_t)PA_MAX_BLOCKS * 2 * parts.heads);
+    parts.ml = reinterpret_cast<float2*>(a.work + (size_t)PA_MAX_BLOCKS * 2 * rows * a.dh);
+    parts.rec = reinterpret_cast<int2*>(parts.ml + (size_t)PA_MAX_BLOCKS * 2 * rows);
     paged_attn_kernel<E><<<blocks, PA_THREADS, smem, s>>>(a, sh, parts);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     add_launches(1);
     PdlScope pdl(true);
-    e = launch_pdl(paged_join_kernel<typename E::Act>, dim3(blocks, G < parts.heads ? G : parts.heads),
-                   dim3(PA_THREADS), 0, s, a, sh, parts, blocks, E::HW, E::SCALE);
+    e = launch_pdl(paged_join_kernel<typename E::Act>, dim3(blocks, rows), dim3(PA_THREADS), 0, s, a, sh, parts, blocks,
+                   E::SCALE);
     if (e == cudaSuccess) add_launches(1);
     return e;
 }
