@@ -5,7 +5,6 @@
 
 #include <cmath>
 #include <string>
-#include <utility>
 
 #include "../../include/krikil_cuda.h"
 #include "paged.h"
@@ -36,18 +35,22 @@ int elem_size(int type) { return type == KRK_TYPE_F32 ? 4 : type == KRK_TYPE_F16
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+struct Dim {
+    int64_t size, stride;  // the stride of a dimension of one element does not matter
+};
+
 // Four elements at a time: the pointer and every stride.
-bool vec4(const void* p, int size, std::initializer_list<int64_t> strides) {
+bool vec4(const void* p, int size, std::initializer_list<Dim> dims) {
     if (!p || !aligned(p, 4 * size)) return false;
-    for (int64_t s : strides)
-        if (s < 0 || s % 4) return false;
+    for (const Dim& d : dims)
+        if (d.size > 1 && (d.stride < 0 || d.stride % 4)) return false;
     return true;
 }
 
 // Written memory: a dimension of more than one element steps over whole heads.
-bool distinct(int dh, std::initializer_list<std::pair<int64_t, int64_t>> size_stride) {
-    for (const auto& x : size_stride)
-        if (x.first > 1 && x.second < dh) return false;
+bool distinct(int dh, std::initializer_list<Dim> dims) {
+    for (const Dim& d : dims)
+        if (d.size > 1 && d.stride < dh) return false;
     return true;
 }
 
@@ -120,9 +123,10 @@ int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void* k, int
     if (!(theta > 0.f) || !std::isfinite(theta)) return invalid(who, "theta must be positive and finite");
     if (T == 0) return KRK_OK;
     const int es = elem_size(type), cs = elem_size(cache_type);
-    if (!vec4(k, es, {k_st, k_sh}) || !vec4(v, es, {v_st, v_sh}) || !vec4(kc, cs, {c_sp, c_st, c_sh}) ||
-        !vec4(vc, cs, {c_sp, c_st, c_sh}) ||
-        (Hq > 0 && (!vec4(q, es, {q_st, q_sh}) || !vec4(q_out, es, {qo_st, qo_sh}))))
+    if (!vec4(k, es, {{T, k_st}, {Hkv, k_sh}}) || !vec4(v, es, {{T, v_st}, {Hkv, v_sh}}) ||
+        !vec4(kc, cs, {{num_pages, c_sp}, {page_size, c_st}, {Hkv, c_sh}}) ||
+        !vec4(vc, cs, {{num_pages, c_sp}, {page_size, c_st}, {Hkv, c_sh}}) ||
+        (Hq > 0 && (!vec4(q, es, {{T, q_st}, {Hq, q_sh}}) || !vec4(q_out, es, {{T, qo_st}, {Hq, qo_sh}}))))
         return invalid(who, "pointers must be set and aligned to four elements, strides multiples of four");
     if (!distinct(dh, {{num_pages, c_sp}, {page_size, c_st}, {Hkv, c_sh}}) ||
         (Hq > 0 && !distinct(dh, {{T, qo_st}, {Hq, qo_sh}})))
@@ -135,9 +139,9 @@ int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void* k, int
     return done(who, krk::rope_kv_append_paged(a, type, cache_type, (cudaStream_t)stream));
 }
 
-size_t krk_attn_paged_work_floats(int Hq, int Hkv, int dh) {
-    if (Hkv <= 0 || Hq < Hkv || Hq % Hkv || dh < 4 || dh > 256 || dh % 4) return 0;
-    return krk::attn_paged_work_floats(Hq, Hkv, dh);
+size_t krk_attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len) {
+    if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || dh < 4 || dh > 256 || dh % 4 || max_len < 0) return 0;
+    return krk::attn_paged_work_floats(B, Hq, Hkv, dh, max_len);
 }
 
 int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void* kc, void* vc, int64_t c_sp,
@@ -157,19 +161,21 @@ int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void*
     if (table_ld < width) return invalid(who, "table_ld is shorter than the table's width");
     if (B == 0) return KRK_OK;
     const int es = elem_size(type), cs = elem_size(cache_type);
-    if (!vec4(q, es, {q_sb, q_sh}) || !vec4(out, es, {o_sb, o_sh}) || !vec4(kc, cs, {c_sp, c_st, c_sh}) ||
-        !vec4(vc, cs, {c_sp, c_st, c_sh}))
+    if (!vec4(q, es, {{B, q_sb}, {Hq, q_sh}}) || !vec4(out, es, {{B, o_sb}, {Hq, o_sh}}) ||
+        !vec4(kc, cs, {{num_pages, c_sp}, {page_size, c_st}, {Hkv, c_sh}}) ||
+        !vec4(vc, cs, {{num_pages, c_sp}, {page_size, c_st}, {Hkv, c_sh}}))
         return invalid(who, "pointers must be set and aligned to four elements, strides multiples of four");
     if (!distinct(dh, {{B, o_sb}, {Hq, o_sh}})) return invalid(who, "strides of out must not be shorter than dh");
     if (!table || !lens) return invalid(who, "null pointer");
-    const size_t need = krk::attn_paged_work_floats(Hq, Hkv, dh);
-    if (need > 0 && (!work || work_floats < need || !aligned(work, 16)))
-        return invalid(who, "work must be 16-byte aligned and hold " + std::to_string(need) + " floats");
     const int shift = log2_exact(page_size);
     const int64_t cap = (int64_t)width << shift;
+    const int bound = (int)(max_len > 0 && max_len < cap ? max_len : cap);
+    const size_t need = krk::attn_paged_work_floats(B, Hq, Hkv, dh, bound);
+    if (need > 0 && (!work || work_floats < need || !aligned(work, 16)))
+        return invalid(who, "work must be 16-byte aligned and hold " + std::to_string(need) + " floats");
     const krk::PagedAttnArgs a{q, q_sb, q_sh, kc, vc, c_sp, c_st, c_sh, table, table_ld, width, num_pages, shift,
                                lens, B, Hq, Hkv, dh, scale, window,
-                               (int)(max_len > 0 && max_len < cap ? max_len : cap), out, o_sb, o_sh, lse, work};
+                               bound, out, o_sb, o_sh, lse, work};
     return done(who, krk::attn_decode_paged(a, type, cache_type, (cudaStream_t)stream));
 }
 

@@ -206,7 +206,8 @@ int paged_sm_count() {
     return n;
 }
 
-size_t attn_paged_work_floats(int Hq, int Hkv, int dh) {
+size_t attn_paged_work_floats(int, int Hq, int Hkv, int dh, int max_len) {
+    if (pa_whole(max_len)) return 0;
     const int share = Hq / Hkv, rows = 4 * share < PA_MAX_ROWS ? 4 * share : PA_MAX_ROWS;
     return (size_t)PA_MAX_BLOCKS * (2 * (size_t)rows * (dh + 2) + 2);
 }

@@ -73,7 +73,7 @@ struct PagedAttnArgs {
     float* lse;                                      // [B][Hq] or nullptr
     float* work;
 };
-size_t attn_paged_work_floats(int Hq, int Hkv, int dh);
+size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len);
 cudaError_t attn_decode_paged(const PagedAttnArgs& a, int act, int cache, cudaStream_t s);
 
 }  // namespace krk

@@ -401,6 +401,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnA
         a.lse[(long long)b * a.Hq + head] = (top + log2f(total * (1.0f / scale))) * 0.693147180559945309f;
 }
 
+// Whether blocks take whole (request, heads): lengths up to `bound` are not worth a second kernel.
+inline bool pa_whole(int bound) { return bound <= PA_WHOLE_UNITS * PA_UNIT; }
+
 int paged_sm_count();  // of the current device, 0 if it cannot be read
 
 template <class E>
@@ -425,7 +428,7 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
         sh.side *= 2;
     const size_t smem = kRing + (size_t)sh.side * sh.groups * E::Q_BYTES;
     const long long items = (long long)a.B * (a.Hkv / sh.side) * sh.per_kv;
-    if (units <= PA_WHOLE_UNITS) {
+    if (pa_whole(a.max_len)) {
         sh.whole = 1;
         paged_attn_kernel<E><<<(unsigned)items, PA_THREADS, smem, s>>>(a, sh, PagedParts{});
         add_launches(1);

@@ -6,7 +6,6 @@ of this library's sm_100a kernels (krk_k_* in include/krikil_cuda.h).
 from __future__ import annotations
 
 import itertools
-import math
 from typing import Optional
 
 import torch
@@ -191,20 +190,24 @@ def greedy(logits: torch.Tensor, seen: Optional[torch.Tensor] = None, penalty: f
 
 
 # ------------------------------------------------------ paged key-value cache
+# The wrappers' checks are a large part of a small call's time: each tensor's
+# type, device, shape and strides are read once, and scratch and small outputs
+# come from one allocation.
 _TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _i32_on(dev, **named):
-    for name, t in named.items():
-        if t is not None and not (t.dtype == torch.int32 and t.device == dev and t.is_contiguous()):
-            raise ValueError(f"{name}: expected a contiguous int32 tensor on {dev}")
-
-
-def _elems_on(dev, dims, **named):
-    for name, t in named.items():
-        if t is not None and not (t.device == dev and t.dim() == dims and t.dtype in _TYPES and t.stride(-1) == 1):
-            raise ValueError(f"{name}: expected a float32, float16 or bfloat16 tensor of {dims} dimensions on {dev} "
-                             "whose last dimension is dense")
+def _call_on(dev, fn, *args) -> None:
+    """fn(*args, stream) on dev's current stream, with dev current."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)
 
 
 def _cuda_device(t):
@@ -213,31 +216,34 @@ def _cuda_device(t):
     return t.device
 
 
-def _strides(t, n):
-    """The first n strides, 0 for a dimension of one element (torch leaves any number there)."""
-    return [st if size > 1 else 0 for size, st in zip(t.shape[:n], t.stride())]
+def _elems(t, dims, dev, name):
+    """(type, shape, strides) of a float tensor whose last dimension is dense."""
+    kind, shape, strides = _TYPES.get(t.dtype), t.shape, t.stride()
+    if kind is None or len(shape) != dims or (strides[-1] != 1 and shape[-1] > 1) or t.device != dev:
+        raise ValueError(f"{name}: expected a float32, float16 or bfloat16 tensor of {dims} dimensions on {dev} "
+                         "whose last dimension is dense")
+    return kind, shape, strides
 
 
-def _call_on(dev, fn, *args) -> None:
-    """fn(*args, stream) on dev's current stream, with dev current."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
-        return
-    with torch.cuda.device(dev):
-        check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+def _ints(t, n, dev, name) -> int:
+    """The address of a dense int32 tensor of n elements."""
+    if t.dtype != torch.int32 or t.numel() != n or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of {n} elements on {dev}")
+    return t.data_ptr()
 
 
-def _table_shape(table, dev):
-    if not (table.dtype == torch.int32 and table.device == dev and table.dim() == 2 and table.stride(1) == 1):
+def _table(t, dev):
+    shape, strides = t.shape, t.stride()
+    if t.dtype != torch.int32 or len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or t.device != dev:
         raise ValueError(f"table: expected an int32 [requests, pages] tensor on {dev} with dense rows")
-    return table.shape
+    return shape, max(strides[0], shape[1])
 
 
-def _cache_dims(kc, vc, dev):
-    _elems_on(dev, 4, kc=kc, vc=vc)
-    if kc.dtype != vc.dtype or kc.shape != vc.shape or _strides(kc, 3) != _strides(vc, 3):
-        raise ValueError("kc and vc: expected the same type, shape and strides")
-    return kc.shape
+def _pool(kc, vc, dev):
+    kind, shape, strides = _elems(kc, 4, dev, "kc")
+    if vc.dtype != kc.dtype or vc.shape != shape or vc.stride() != strides or vc.device != dev:
+        raise ValueError("kc and vc: expected the same type, device, shape and strides")
+    return kind, shape, strides
 
 
 def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int, rows: int, lens_out=None,
@@ -252,25 +258,21 @@ def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int
     not fit, in which case nothing was taken.  lens_out and free_count_out may be
     the inputs; they and the others are new tensors when not given."""
     dev = _cuda_device(table)
-    b, width = _table_shape(table, dev)
-    _i32_on(dev, new_tokens=new_tokens, lens=lens, free_pages=free_pages, free_count=free_count, lens_out=lens_out,
-            free_count_out=free_count_out)
+    (b, width), ld = _table(table, dev)
+    new_at, lens_at = _ints(new_tokens, b, dev, "new_tokens"), _ints(lens, b, dev, "lens")
+    pages = free_pages.numel()
+    free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
+    padded = -rows % 4 + rows
+    buf = torch.empty(2 * padded + 2 * b + 3, device=dev, dtype=torch.int32)
+    positions, _, slots, _, cu, lens_new, count_new, status = buf.split(
+        [rows, padded - rows, rows, padded - rows, b + 1, b, 1, 1])
     if lens_out is None:
-        lens_out = torch.empty_like(lens)
+        lens_out = lens_new
     if free_count_out is None:
-        free_count_out = torch.empty_like(free_count)
-    if new_tokens.numel() != b or lens.numel() != b or lens_out.numel() != b:
-        raise ValueError(f"new_tokens, lens, lens_out: expected {b} values, one a row of the table")
-    if free_count.numel() != 1 or free_count_out.numel() != 1:
-        raise ValueError("free_count: expected one value")
-    cu = torch.empty(b + 1, device=dev, dtype=torch.int32)
-    positions = torch.empty(rows, device=dev, dtype=torch.int32)
-    slots = torch.empty(rows, device=dev, dtype=torch.int32)
-    status = torch.empty(1, device=dev, dtype=torch.int32)
-    _call_on(dev, lib.krk_k_kv_page_plan, new_tokens.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0),
-             b, width, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size,
-             lens_out.data_ptr(), free_count_out.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-             rows, status.data_ptr())
+        free_count_out = count_new
+    _call_on(dev, lib.krk_k_kv_page_plan, new_at, lens_at, table.data_ptr(), ld, b, width, free_at, count_at, pages,
+             page_size, _ints(lens_out, b, dev, "lens_out"), _ints(free_count_out, 1, dev, "free_count_out"),
+             cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), rows, status.data_ptr())
     return lens_out, free_count_out, cu, positions, slots, status
 
 
@@ -279,23 +281,19 @@ def kv_page_release(done, lens, table, free_pages, free_count, page_size: int, l
     back on the stack free_pages, in place, and their lengths to 0.  Returns
     (lens_out, free_count_out, status)."""
     dev = _cuda_device(table)
-    b, width = _table_shape(table, dev)
-    _i32_on(dev, lens=lens, free_pages=free_pages, free_count=free_count, lens_out=lens_out,
-            free_count_out=free_count_out)
-    if not (done.dtype in (torch.bool, torch.uint8) and done.device == dev and done.is_contiguous()):
-        raise ValueError(f"done: expected a contiguous bool or uint8 tensor on {dev}")
+    (b, width), ld = _table(table, dev)
+    if done.dtype not in (torch.bool, torch.uint8) or done.numel() != b or done.device != dev or not done.is_contiguous():
+        raise ValueError(f"done: expected a contiguous bool or uint8 tensor of {b} elements on {dev}")
+    lens_at, pages = _ints(lens, b, dev, "lens"), free_pages.numel()
+    free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
+    lens_new, count_new, status = torch.empty(b + 2, device=dev, dtype=torch.int32).split([b, 1, 1])
     if lens_out is None:
-        lens_out = torch.empty_like(lens)
+        lens_out = lens_new
     if free_count_out is None:
-        free_count_out = torch.empty_like(free_count)
-    if done.numel() != b or lens.numel() != b or lens_out.numel() != b:
-        raise ValueError(f"done, lens, lens_out: expected {b} values, one a row of the table")
-    if free_count.numel() != 1 or free_count_out.numel() != 1:
-        raise ValueError("free_count: expected one value")
-    status = torch.empty(1, device=dev, dtype=torch.int32)
-    _call_on(dev, lib.krk_k_kv_page_release, done.data_ptr(), lens.data_ptr(), table.data_ptr(), table.stride(0), b,
-             width, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size, lens_out.data_ptr(),
-             free_count_out.data_ptr(), status.data_ptr())
+        free_count_out = count_new
+    _call_on(dev, lib.krk_k_kv_page_release, done.data_ptr(), lens_at, table.data_ptr(), ld, b, width, free_at,
+             count_at, pages, page_size, _ints(lens_out, b, dev, "lens_out"),
+             _ints(free_count_out, 1, dev, "free_count_out"), status.data_ptr())
     return lens_out, free_count_out, status
 
 
@@ -308,32 +306,33 @@ def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000
     Returns the rotated q (q_out, which may be q; padding rows of a given q_out
     are left as they were).  q may be None."""
     dev = _cuda_device(k)
-    pages, page_size, hkv, dh = _cache_dims(kc, vc, dev)
-    _elems_on(dev, 3, q=q, k=k, v=v, q_out=q_out)
-    _i32_on(dev, slots=slots, positions=positions)
-    t = k.shape[0]
-    if k.shape != (t, hkv, dh) or v.shape != k.shape or slots.numel() != t or positions.numel() != t:
-        raise ValueError(f"expected k and v of [T, {hkv}, {dh}], slots and positions of [T]")
-    if v.dtype != k.dtype or (q is not None and (q.dtype != k.dtype or q.shape[0] != t or q.shape[2] != dh)):
-        raise ValueError(f"expected q of [T, heads, {dh}] and q, k and v of one type")
-    if q is None:
-        hq, q_args, qo_args = 0, (None, 0, 0), (None, 0, 0)
-    else:
+    ctype, (pages, page_size, hkv, dh), (c_sp, c_st, c_sh, _) = _pool(kc, vc, dev)
+    type_, shape, (k_st, k_sh, _) = _elems(k, 3, dev, "k")
+    vtype, vshape, (v_st, v_sh, _) = _elems(v, 3, dev, "v")
+    t = shape[0]
+    if shape[1] != hkv or shape[2] != dh or vshape != shape or vtype != type_:
+        raise ValueError(f"expected k and v of [T, {hkv}, {dh}] and one type")
+    slots_at, positions_at = _ints(slots, t, dev, "slots"), _ints(positions, t, dev, "positions")
+    hq = q_at = q_st = q_sh = o_at = o_st = o_sh = 0
+    if q is not None:
+        qtype, qshape, (q_st, q_sh, _) = _elems(q, 3, dev, "q")
+        hq = qshape[1]
+        if qshape[0] != t or qshape[2] != dh or qtype != type_:
+            raise ValueError(f"expected q of [T, heads, {dh}] and k's type")
         if q_out is None:
-            q_out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype:
+            q_out = q.new_empty(qshape)
+        otype, oshape, (o_st, o_sh, _) = _elems(q_out, 3, dev, "q_out")
+        if oshape != qshape or otype != qtype:
             raise ValueError("q_out: expected q's shape and type")
-        hq = q.shape[1]
-        q_args, qo_args = (q.data_ptr(), *_strides(q, 2)), (q_out.data_ptr(), *_strides(q_out, 2))
-    _call_on(dev, lib.krk_k_rope_kv_append_paged, *q_args, k.data_ptr(), *_strides(k, 2), v.data_ptr(),
-             *_strides(v, 2), _TYPES[k.dtype], *qo_args, kc.data_ptr(), vc.data_ptr(), *_strides(kc, 3),
-             _TYPES[kc.dtype], slots.data_ptr(), positions.data_ptr(), t, hq, hkv, dh,
-             dh if rot_dim is None else rot_dim, pages, page_size, theta)
+        q_at, o_at = q.data_ptr(), q_out.data_ptr()
+    _call_on(dev, lib.krk_k_rope_kv_append_paged, q_at, q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st,
+             v_sh, type_, o_at, o_st, o_sh, kc.data_ptr(), vc.data_ptr(), c_sp, c_st, c_sh, ctype, slots_at,
+             positions_at, t, hq, hkv, dh, dh if rot_dim is None else rot_dim, pages, page_size, theta)
     return q_out
 
 
-def attn_paged_work_floats(hq: int, hkv: int, dh: int) -> int:
-    return int(lib.krk_attn_paged_work_floats(hq, hkv, dh))
+def attn_paged_work_floats(b: int, hq: int, hkv: int, dh: int, max_len: int) -> int:
+    return int(lib.krk_attn_paged_work_floats(b, hq, hkv, dh, max_len))
 
 
 def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, window: int = 0, max_len: int = 0,
@@ -341,28 +340,37 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
     """Attention of one token a request, q [B, Hq, dh], over the lens[b] (int32
     [B]) tokens in its pages table[b] of kc, vc [pages, page_size, Hkv, dh], the
     last `window` of them if that is not 0.  scale defaults to 1/sqrt(dh);
-    max_len, a bound of the lengths, only sizes the launch.  `work` is scratch
-    (allocated here when not given).  Returns out [B, Hq, dh], or (out, lse)."""
+    max_len, a bound of the lengths, only sizes the launch (0: what a table row
+    holds).  `work` is scratch of attn_paged_work_floats floats (allocated here
+    when not given).  Returns out [B, Hq, dh], or (out, lse)."""
     dev = _cuda_device(q)
-    pages, page_size, hkv, dh = _cache_dims(kc, vc, dev)
-    _elems_on(dev, 3, q=q, out=out)
-    _i32_on(dev, lens=lens)
-    b, hq = q.shape[:2]
-    rows, width = _table_shape(table, dev)
-    if q.shape[2] != dh or rows != b or lens.numel() != b:
-        raise ValueError(f"expected q of [B, heads, {dh}], a table of B rows and lens of [B]")
+    ctype, (pages, page_size, hkv, dh), (c_sp, c_st, c_sh, _) = _pool(kc, vc, dev)
+    type_, shape, (q_sb, q_sh, _) = _elems(q, 3, dev, "q")
+    b, hq, _ = shape
+    (trows, width), ld = _table(table, dev)
+    if shape[2] != dh or trows != b:
+        raise ValueError(f"expected q of [B, heads, {dh}] and a table of B rows")
+    lens_at = _ints(lens, b, dev, "lens")
     if out is None:
-        out = torch.empty(q.shape, device=dev, dtype=q.dtype)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = q.new_empty(shape)
+    otype, oshape, (o_sb, o_sh, _) = _elems(out, 3, dev, "out")
+    if oshape != shape or otype != type_:
         raise ValueError("out: expected q's shape and type")
     lse = torch.empty((b, hq), device=dev, dtype=torch.float32) if return_lse else None
+    cap = width * page_size
+    bound = max_len if 0 < max_len < cap else cap
     if work is None:
-        work = torch.empty(attn_paged_work_floats(hq, hkv, dh), device=dev, dtype=torch.float32)
-    elif not (work.dtype == torch.float32 and work.device == dev and work.is_contiguous()):
-        raise ValueError(f"work: expected a contiguous float32 tensor on {dev}")
-    _call_on(dev, lib.krk_k_attn_decode_paged, q.data_ptr(), *_strides(q, 2), _TYPES[q.dtype],
-             kc.data_ptr(), vc.data_ptr(), *_strides(kc, 3), _TYPES[kc.dtype], table.data_ptr(), table.stride(0),
-             width, pages, page_size, lens.data_ptr(), b, hq, hkv, dh,
-             1.0 / math.sqrt(dh) if scale is None else scale, window, max_len, out.data_ptr(),
-             *_strides(out, 2), lse.data_ptr() if return_lse else None, work.data_ptr(), work.numel())
+        need = lib.krk_attn_paged_work_floats(b, hq, hkv, dh, bound)
+        work_at = 0
+        if need:
+            work = torch.empty(need, device=dev, dtype=torch.float32)
+            work_at = work.data_ptr()
+    else:
+        if work.dtype != torch.float32 or work.device != dev or not work.is_contiguous():
+            raise ValueError(f"work: expected a contiguous float32 tensor on {dev}")
+        need, work_at = work.numel(), work.data_ptr()
+    _call_on(dev, lib.krk_k_attn_decode_paged, q.data_ptr(), q_sb, q_sh, type_, kc.data_ptr(), vc.data_ptr(), c_sp,
+             c_st, c_sh, ctype, table.data_ptr(), ld, width, pages, page_size, lens_at, b, hq, hkv, dh,
+             dh ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), o_sb, o_sh,
+             lse.data_ptr() if return_lse else None, work_at, need)
     return (out, lse) if return_lse else out

@@ -26,7 +26,7 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover
     pytest.skip("no CUDA device", allow_module_level=True)
 
-from krikil_rs_b200 import kernels as K, launch_count  # noqa: E402
+from krikil_rs_b200 import KrikilError, kernels as K, launch_count  # noqa: E402
 from krikil_rs_b200._lib import (PAGES_BAD_LENGTH, PAGES_EXHAUSTED, PAGES_OVERFLOW, PAGES_ROW_FULL,  # noqa: E402
                                  PAGES_ROWS)
 
@@ -299,7 +299,7 @@ def test_attention_is_repeatable_and_the_bound_only_sizes_it(act, cache):
     pool = Pool([900, 0, 3000, 12], 2, 128, 16, cache, seed=12)
     q = torch.randn(4, 8, 128, generator=gen(3), device=DEV).to(act)
     first, _ = check_attn(pool, q)
-    work = torch.full((K.attn_paged_work_floats(8, 2, 128) + 8,), float("nan"), device=DEV)
+    work = torch.full((K.attn_paged_work_floats(4, 8, 2, 128, 3008) + 8,), float("nan"), device=DEV)
     for _ in range(3):
         again = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=work)
         assert torch.equal(first, again)
@@ -308,12 +308,13 @@ def test_attention_is_repeatable_and_the_bound_only_sizes_it(act, cache):
 
 
 def test_scratch_that_is_too_small_is_refused():
-    pool = Pool([64], 2, 64, 16, F32, seed=2)
+    pool = Pool([6400], 2, 64, 16, F32, seed=2)
     q = torch.randn(1, 4, 64, device=DEV)
-    need = K.attn_paged_work_floats(4, 2, 64)
-    if need:
-        with pytest.raises(Exception, match="work"):
-            K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=torch.empty(need - 1, device=DEV))
+    need = K.attn_paged_work_floats(1, 4, 2, 64, 6400)
+    for work in (torch.empty(need - 1, device=DEV), torch.empty(need + 1, device=DEV)[1:]):
+        with pytest.raises(KrikilError, match="work"):
+            K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=work)
+    K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=torch.empty(need, device=DEV))
 
 
 @pytest.mark.parametrize("act,cache", [(F32, F32), (F32, BF16), (BF16, BF16), (F16, F16)])
@@ -325,7 +326,7 @@ def test_attention_replayed_from_a_graph_on_another_stream(act, cache):
     q = torch.randn(4, 8, 64, generator=gen(3), device=DEV).to(act)
     now = i32(lens)
     s = torch.cuda.Stream()
-    out, work = torch.empty_like(q), torch.empty(K.attn_paged_work_floats(8, 2, 64), device=DEV)
+    out, work = torch.empty_like(q), torch.empty(K.attn_paged_work_floats(4, 8, 2, 64, 800), device=DEV)
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
         K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now, out=out, work=work, max_len=800)
@@ -716,9 +717,9 @@ def test_wrappers_refuse_what_does_not_belong_together():
                 dict(q=q[..., :60])):
         with pytest.raises(ValueError):
             attn(**bad)
-    with pytest.raises(Exception, match="16-bit q"):
+    with pytest.raises(KrikilError, match="16-bit q"):
         attn(q=q.half())
-    with pytest.raises(Exception, match="multiple"):
+    with pytest.raises(KrikilError, match="multiple"):
         attn(q=q[:, :3])
 
     def append(q=q, k=kv, v=kv, kc=pool.kc, vc=pool.vc, slots=two, positions=two, **kw):
@@ -728,7 +729,7 @@ def test_wrappers_refuse_what_does_not_belong_together():
                 dict(q=q.half()), dict(q_out=q.half()), dict(q=q[:1]), dict(v=kv.half()), dict(k=kv.cpu())):
         with pytest.raises(ValueError):
             append(**bad)
-    with pytest.raises(Exception, match="rot_dim"):
+    with pytest.raises(KrikilError, match="rot_dim"):
         append(rot_dim=63)
     free, one = i32([0, 1]), i32([1])
     for bad in ((two.long(), pool.lens, pool.table, free, one), (two[:1], pool.lens, pool.table, free, one),

@@ -96,8 +96,11 @@ def test_empty_steps_are_done_at_once():
 
 
 def test_sizes_of_the_attention_scratch():
-    assert lib.krk_attn_paged_work_floats(8, 3, 64) == 0 and lib.krk_attn_paged_work_floats(8, 8, 62) == 0
-    assert lib.krk_attn_paged_work_floats(0, 1, 64) == 0 and lib.krk_attn_paged_work_floats(8, 0, 64) == 0
+    f = lib.krk_attn_paged_work_floats
+    assert f(4, 8, 8, 64, 100000) > 0 and f(4, 8, 8, 64, 1) == 0  # a short bound needs none
+    for bad in ((0, 8, 8, 64, 9999), (4, 8, 3, 64, 9999), (4, 8, 8, 62, 9999), (4, 0, 1, 64, 9999),
+                (4, 8, 0, 64, 9999), (4, 8, 8, 64, -1)):
+        assert f(*bad) == 0
 
 
 def test_wrappers_refuse_cpu_tensors():
