@@ -9,237 +9,449 @@
 namespace krk {
 namespace {
 
-constexpr int PLAN_THREADS = 1024;
+// ---------------------------------------------------------------- the pages
+// Planning is two prefix sums over the requests -- of their new tokens and of
+// the pages that they lack -- and then independent writes: one entry a page and
+// a position and a slot a token.  A launch is one cluster of 1 or 8 blocks, one
+// kernel for every size: each block scans all requests itself (a few KB from
+// L2), so the blocks need nothing of each other but one barrier between the
+// last read of a chunk of requests and the first write, which lets the lengths
+// be updated in place.  Small steps are bound by latency; the writes of a large
+// one are dealt evenly to the cluster's threads, which find a token's or a
+// page's request by bisecting the chunk's prefix sums.
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_CLUSTER = 8;
+constexpr int PLAN_ONE_BLOCK = 8192;  // writes up to which one block does it
 
-// Exclusive prefix sums of one value pair a thread over the block, and the
-// totals.  scratch: 2 * 33 values.
-KRK_DEV void block_scan2(long long a, long long b, long long& ea, long long& eb, long long& ta, long long& tb,
-                         long long* scratch) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    long long ia = a, ib = b;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long xa = __shfl_up_sync(0xffffffffu, ia, o), xb = __shfl_up_sync(0xffffffffu, ib, o);
-        if (lane >= o) {
-            ia += xa;
-            ib += xb;
-        }
-    }
-    __syncthreads();
-    if (lane == 31) {
-        scratch[warp] = ia;
-        scratch[33 + warp] = ib;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        long long sa = 0, sb = 0;
-        for (int w = 0; w < nw; ++w) {
-            const long long xa = scratch[w], xb = scratch[33 + w];
-            scratch[w] = sa;
-            scratch[33 + w] = sb;
-            sa += xa;
-            sb += xb;
-        }
-        scratch[32] = sa;
-        scratch[65] = sb;
-    }
-    __syncthreads();
-    ea = scratch[warp] + ia - a;
-    eb = scratch[33 + warp] + ib - b;
-    ta = scratch[32];
-    tb = scratch[65];
+struct PlanScratch {
+    long long warp[2][PLAN_WARPS + 1];
+    int bad;
+    // of a chunk's requests: tokens and pages before them, what they hold, their pages so far
+    int tokens[PLAN_THREADS + 1], pages[PLAN_THREADS + 1], len[PLAN_THREADS], have[PLAN_THREADS];
+};
+
+KRK_DEV unsigned cluster_blocks() {
+    unsigned n;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    return n;
+}
+KRK_DEV unsigned cluster_rank() {
+    unsigned n;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+    return n;
+}
+KRK_DEV void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// One block.  Two passes over the requests: the first adds up what they need
-// and decides whether the step fits, the second writes it.
-__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PagePlanArgs a) {
-    __shared__ long long scratch[66];
-    __shared__ int bad;
-    const int tid = threadIdx.x, P = 1 << a.page_shift;
-    if (tid == 0) bad = 0;
+// Sums of two values a thread over the block.
+KRK_DEV void block_sum2(long long& x, long long& y, PlanScratch& sc) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    if (lane == 0) {
+        sc.warp[0][warp] = x;
+        sc.warp[1][warp] = y;
+    }
     __syncthreads();
+    x = sc.warp[0][lane];
+    y = sc.warp[1][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    __syncthreads();
+}
+
+// The sum of the threads before this one, and all threads' in total.  Two
+// counts below 2^31 fit one value: no carry crosses the halves.
+KRK_DEV long long block_scan(long long x, long long& total, PlanScratch& sc) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long upto = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) sc.warp[0][warp] = upto;
+    __syncthreads();
+    long long w = sc.warp[0][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+    __syncthreads();
+    return upto - x + (warp ? before : 0);
+}
+
+// The last i < n with first[i] <= x (first[0] <= x).
+KRK_DEV int bisect(const int* first, int n, int x) {
+    int lo = 0;
+    while (n > 1) {
+        const int half = n >> 1;
+        if (first[lo + half] <= x) {
+            lo += half;
+            n -= half;
+        } else {
+            n = half;
+        }
+    }
+    return lo;
+}
+
+KRK_DEV long long pages_for(long long tokens, int shift) { return (tokens + (1 << shift) - 1) >> shift; }
+
+// Rows [r0, r1) of positions and slots get those that `at` gives, four at a time.
+template <typename F>
+KRK_DEV void write_rows(const PagePlanArgs& a, int r0, int r1, int thread, int threads, F at) {
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.positions) | reinterpret_cast<uintptr_t>(a.slots)) & 15) == 0;
+    for (long long q = (r0 >> 2) + thread; q * 4 < r1; q += threads) {
+        const int r = (int)(q * 4), lo = max(r, r0), hi = (int)min((long long)r + 4, (long long)r1);
+        int pos[4], slot[4];
+        at(lo, hi, r, pos, slot);
+        if (wide && lo == r && hi == r + 4) {
+            *reinterpret_cast<int4*>(a.positions + r) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            *reinterpret_cast<int4*>(a.slots + r) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r + i >= lo && r + i < hi) {
+                    a.positions[r + i] = pos[i];
+                    a.slots[r + i] = slot[i];
+                }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_constant__ PagePlanArgs a) {
+    __shared__ PlanScratch sc;
+    const int tid = threadIdx.x, shift = a.page_shift, low = (1 << shift) - 1;
+    const int thread = cluster_rank() * PLAN_THREADS + tid, threads = cluster_blocks() * PLAN_THREADS;
+    if (tid == 0) sc.bad = 0;
     const int count = *a.free_count;
+    // what the step needs, and whether it fits
     long long tokens = 0, pages = 0;
-    int err = 0;
-    if (count < 0 || count > a.num_pages) err |= PAGES_BAD_LENGTH;
+    int err = count < 0 || count > a.num_pages ? PAGES_BAD_LENGTH : 0;
     for (int b = tid; b < a.B; b += PLAN_THREADS) {
         const long long len = a.lens[b], add = a.new_tokens[b];
         if (len < 0 || add < 0) {
             err |= PAGES_BAD_LENGTH;
             continue;
         }
-        const long long have = (len + P - 1) >> a.page_shift, want = (len + add + P - 1) >> a.page_shift;
+        const long long want = pages_for(len + add, shift);
         if (want > a.width) err |= PAGES_ROW_FULL;
         tokens += add;
-        pages += want - have;
+        pages += want - pages_for(len, shift);
     }
-    long long e0, e1, total_tokens, total_pages;
-    block_scan2(tokens, pages, e0, e1, total_tokens, total_pages, scratch);
-    if (total_tokens > a.rows) err |= PAGES_ROWS;
-    if (total_pages > count) err |= PAGES_EXHAUSTED;
-    if (err) atomicOr(&bad, err);
+    block_sum2(tokens, pages, sc);
+    if (tokens > a.rows) err |= PAGES_ROWS;
+    if (pages > count) err |= PAGES_EXHAUSTED;
+    if (err) atomicOr(&sc.bad, err);
     __syncthreads();
-    err = bad;
-    __syncthreads();
-    if (tid == 0) {
-        *a.status = err;
-        a.cu_new[0] = 0;
-    }
+    err = sc.bad;
     if (err) {
-        for (int b = tid; b < a.B; b += PLAN_THREADS) {
+        cluster_sync();  // all have read free_count and the lengths
+        for (int b = thread; b < a.B; b += threads) {
             a.lens_out[b] = a.lens[b];
             a.cu_new[b + 1] = 0;
         }
-        for (int r = tid; r < a.rows; r += PLAN_THREADS) {
-            a.slots[r] = -1;
-            a.positions[r] = 0;
+        write_rows(a, 0, a.rows, thread, threads, [](int, int, int, int* pos, int* slot) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pos[i] = 0;
+                slot[i] = -1;
+            }
+        });
+        if (thread == 0) {
+            *a.status = err;
+            a.cu_new[0] = 0;
+            *a.free_count_out = count;
         }
-        if (tid == 0) *a.free_count_out = count;
         return;
     }
-    long long base_t = 0, base_p = 0;
+    int base_t = 0, base_p = 0;
     for (int b0 = 0; b0 < a.B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid;
-        const long long len = b < a.B ? a.lens[b] : 0, add = b < a.B ? a.new_tokens[b] : 0;
-        const long long have = (len + P - 1) >> a.page_shift, want = (len + add + P - 1) >> a.page_shift;
-        long long t0, p0, tt, tp;
-        block_scan2(add, want - have, t0, p0, tt, tp, scratch);
-        t0 += base_t;
-        p0 += base_p;
-        if (b < a.B) {
-            int32_t* row = a.table + b * a.table_ld;
-            for (long long i = have; i < want; ++i) row[i] = a.free_pages[count - 1 - (p0 + i - have)];
-            for (long long i = 0; i < add; ++i) {
-                const int pos = (int)(len + i);
-                a.positions[t0 + i] = pos;
-                a.slots[t0 + i] = (row[pos >> a.page_shift] << a.page_shift) + (pos & (P - 1));
-            }
-            a.lens_out[b] = (int)(len + add);
-            a.cu_new[b + 1] = (int)(t0 + add);
+        const int b = b0 + tid, n = min(PLAN_THREADS, a.B - b0);
+        const int len = tid < n ? a.lens[b] : 0, add = tid < n ? a.new_tokens[b] : 0;
+        const int have = (int)pages_for(len, shift), lack = (int)pages_for((long long)len + add, shift) - have;
+        long long total;
+        const long long before = block_scan((long long)lack << 32 | (unsigned)add, total, sc);
+        sc.tokens[tid] = (int)before;
+        sc.pages[tid] = (int)(before >> 32);
+        sc.len[tid] = len;
+        sc.have[tid] = have;
+        const int tt = (int)total, tp = (int)(total >> 32);
+        __syncthreads();
+        cluster_sync();  // every block has read the chunk's lengths
+        if (tid < n && (tid & (cluster_blocks() - 1)) == cluster_rank()) {
+            a.lens_out[b] = len + add;
+            a.cu_new[b + 1] = base_t + (int)before + add;
         }
+        for (int j = thread; j < tp; j += threads) {
+            const int i = bisect(sc.pages, n, j);
+            a.table[(b0 + i) * a.table_ld + sc.have[i] + j - sc.pages[i]] = a.free_pages[count - 1 - base_p - j];
+        }
+        write_rows(a, base_t, base_t + tt, thread, threads, [&](int lo, int hi, int r, int* pos, int* slot) {
+            int i = bisect(sc.tokens, n, lo - base_t);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = r + k - base_t;
+                if (r + k < lo || r + k >= hi) continue;
+                while (i + 1 < n && sc.tokens[i + 1] <= at) ++i;
+                pos[k] = sc.len[i] + at - sc.tokens[i];
+                const int p = pos[k] >> shift;
+                const int page = p < sc.have[i] ? a.table[(b0 + i) * a.table_ld + p]
+                                                : a.free_pages[count - 1 - base_p - (sc.pages[i] + p - sc.have[i])];
+                slot[k] = (int)((unsigned)page << shift) + (pos[k] & low);
+            }
+        });
         base_t += tt;
         base_p += tp;
+        __syncthreads();
     }
-    for (int r = (int)base_t + tid; r < a.rows; r += PLAN_THREADS) {
-        a.slots[r] = -1;
-        a.positions[r] = 0;
+    write_rows(a, base_t, a.rows, thread, threads, [](int, int, int, int* pos, int* slot) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            pos[i] = 0;
+            slot[i] = -1;
+        }
+    });
+    if (thread == 0) {
+        *a.status = 0;
+        a.cu_new[0] = 0;
+        *a.free_count_out = count - base_p;
     }
-    if (tid == 0) *a.free_count_out = (int)(count - base_p);
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(PageReleaseArgs a) {
-    __shared__ long long scratch[66];
-    __shared__ int bad;
-    const int tid = threadIdx.x, P = 1 << a.page_shift;
-    if (tid == 0) bad = 0;
-    __syncthreads();
+__global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const __grid_constant__ PageReleaseArgs a) {
+    __shared__ PlanScratch sc;
+    const int tid = threadIdx.x, shift = a.page_shift;
+    const int thread = cluster_rank() * PLAN_THREADS + tid, threads = cluster_blocks() * PLAN_THREADS;
+    if (tid == 0) sc.bad = 0;
     const int count = *a.free_count;
-    long long pages = 0;
-    int err = 0;
-    if (count < 0 || count > a.num_pages) err |= PAGES_BAD_LENGTH;
+    long long pages = 0, unused = 0;
+    int err = count < 0 || count > a.num_pages ? PAGES_BAD_LENGTH : 0;
     for (int b = tid; b < a.B; b += PLAN_THREADS) {
         if (!a.done[b]) continue;
-        const long long len = a.lens[b], held = (len + P - 1) >> a.page_shift;
-        if (len < 0 || held > a.width) err |= PAGES_BAD_LENGTH;
-        else pages += held;
+        const long long len = a.lens[b], held = pages_for(len, shift);
+        if (len < 0 || held > a.width)
+            err |= PAGES_BAD_LENGTH;
+        else
+            pages += held;
     }
-    long long e0, e1, total, unused;
-    block_scan2(pages, 0, e0, e1, total, unused, scratch);
-    if (count + total > a.num_pages) err |= PAGES_OVERFLOW;
-    if (err) atomicOr(&bad, err);
+    block_sum2(pages, unused, sc);
+    if (count + pages > a.num_pages) err |= PAGES_OVERFLOW;
+    if (err) atomicOr(&sc.bad, err);
     __syncthreads();
-    err = bad;
-    __syncthreads();
-    if (tid == 0) *a.status = err;
-    if (err) {
-        for (int b = tid; b < a.B; b += PLAN_THREADS) a.lens_out[b] = a.lens[b];
-        if (tid == 0) *a.free_count_out = count;
-        return;
-    }
-    long long base = 0;
+    err = sc.bad;
+    int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid;
-        const bool done = b < a.B && a.done[b];
-        const int len = b < a.B ? a.lens[b] : 0;
-        const long long held = done ? ((long long)len + P - 1) >> a.page_shift : 0;
-        long long p0, x, tp, y;
-        block_scan2(held, 0, p0, x, tp, y, scratch);
-        p0 += base;
-        if (b < a.B) {
-            for (long long i = 0; i < held; ++i) a.free_pages[count + p0 + i] = a.table[b * a.table_ld + i];
-            a.lens_out[b] = done ? 0 : len;
+        const int b = b0 + tid, n = min(PLAN_THREADS, a.B - b0);
+        const int len = tid < n ? a.lens[b] : 0;
+        const bool gone = !err && tid < n && a.done[b];
+        long long total;
+        const int before = (int)block_scan(gone ? pages_for(len, shift) : 0, total, sc);
+        sc.pages[tid] = before;
+        __syncthreads();
+        cluster_sync();  // every block has read the chunk's lengths
+        if (tid < n && (tid & (cluster_blocks() - 1)) == cluster_rank()) a.lens_out[b] = gone ? 0 : len;
+        for (int j = thread; j < (int)total; j += threads) {
+            const int i = bisect(sc.pages, n, j);
+            a.free_pages[count + base + j] = a.table[(b0 + i) * a.table_ld + j - sc.pages[i]];
         }
-        base += tp;
+        base += (int)total;
+        __syncthreads();
     }
-    if (tid == 0) *a.free_count_out = (int)(count + base);
+    if (thread == 0) {
+        *a.status = err;
+        *a.free_count_out = count + base;
+    }
 }
 
-// One thread per pair (or unrotated element) of a row's head.
-template <typename T, typename C>
-__global__ void __launch_bounds__(256) rope_append_kernel(RopeAppendArgs a) {
-    const int half = a.rot / 2, per_head = a.dh - half, heads = a.Hq + 2 * a.Hkv;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)a.T * heads * per_head) return;
-    const int u = (int)(i % per_head), h = (int)(i / per_head % heads);
-    const long long t = i / per_head / heads;
-    const int slot = a.slots[t];
-    if (slot < 0) return;
-    if (slot >= a.num_slots) {
-        check_fail(CHK_TABLE);
-        return;
+template <typename... Args>
+cudaError_t launch_cluster(void (*kern)(Args...), bool one, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = one ? 1 : PLAN_CLUSTER;
+    cfg.blockDim = PLAN_THREADS;
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cfg.gridDim.x;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e == cudaSuccess) add_launches(1);
+    return e;
+}
+
+// ---------------------------------------------------------------- RoPE + append
+// Every input is read and every output written once, W elements (16 bytes) at
+// a time: HBM bounds it.  A block takes the heads of a few rows; the rows' cos
+// and sin are computed once a pair -- the turns, position times rate, reduced
+// to a fraction in 64 bits -- and shared by all heads through shared memory.  A
+// unit is W pairs (i, i + rot/2) of a query or key head, or 2 W neighbours that
+// are not rotated; a thread loads four units before it stores the first.
+constexpr int APPEND_THREADS = 256, APPEND_UNITS = 4, APPEND_ROWS = 8;
+
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<16> { using type = uint4; };
+template <>
+struct Raw<8> { using type = uint2; };
+template <>
+struct Raw<4> { using type = uint32_t; };
+template <>
+struct Raw<2> { using type = uint16_t; };
+
+template <typename T, int W>
+union Vec {
+    typename Raw<sizeof(T) * W>::type raw;
+    T e[W];
+    KRK_DEV Vec() {}
+};
+// f32 rows of 8 elements do not arise: W * sizeof(T) <= 16.
+template <typename T, int W>
+KRK_DEV void load_vec(Vec<T, W>& v, const T* p) {
+    v.raw = *reinterpret_cast<const typename Raw<sizeof(T) * W>::type*>(p);
+}
+template <typename T, int W>
+KRK_DEV void store_vec(T* p, const Vec<T, W>& v) {
+    *reinterpret_cast<typename Raw<sizeof(T) * W>::type*>(p) = v.raw;
+}
+template <typename T, int W>
+KRK_DEV void put(T* p, const float (&x)[W]) {
+    Vec<T, W> v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v.e[i] = from_f32<T>(x[i]);
+    store_vec<T, W>(p, v);
+}
+
+template <typename T, typename C, int W>
+__global__ void __launch_bounds__(APPEND_THREADS) rope_append_kernel(const __grid_constant__ RopeAppendArgs a,
+                                                                     int block_rows) {
+    extern __shared__ __align__(16) float turned[];  // [row][cos, sin][rot / 2]
+    __shared__ int slots[APPEND_ROWS];
+    const int half = a.rot / 2, units = a.dh / (2 * W), rot_units = half / W;
+    const int heads = a.Hq + 2 * a.Hkv, per_row = heads * units;
+    const int t0 = blockIdx.x * block_rows, rows = min(block_rows, a.T - t0);
+    if ((int)threadIdx.x < rows) {
+        const int slot = a.slots[t0 + threadIdx.x];
+        if (slot >= a.num_slots) check_fail(CHK_TABLE);
+        slots[threadIdx.x] = slot < a.num_slots ? slot : -1;
     }
-    const int lo = u < half ? u : u + half, hi = u < half ? u + half : lo;
-    const long long cell = (slot >> a.page_shift) * a.c_sp + (slot & ((1 << a.page_shift) - 1)) * a.c_st;
-    if (h >= a.Hq + a.Hkv) {
-        const int hv = h - a.Hq - a.Hkv;
-        const T* src = (const T*)a.v + t * a.v_st + hv * a.v_sh;
-        C* dst = (C*)a.vc + cell + hv * a.c_sh;
-        dst[lo] = from_f32<C>(to_f32(src[lo]));
-        if (hi != lo) dst[hi] = from_f32<C>(to_f32(src[hi]));
-        return;
-    }
-    const bool is_q = h < a.Hq;
-    const T* src = is_q ? (const T*)a.q + t * a.q_st + h * a.q_sh : (const T*)a.k + t * a.k_st + (h - a.Hq) * a.k_sh;
-    float x = to_f32(src[lo]), y = to_f32(src[hi]);
-    if (u < half) {
-        const double turns = (double)a.positions[t] * a.turns.f[u];
+    for (int i = threadIdx.x; i < rows * half; i += APPEND_THREADS) {
+        const int r = i / half, j = i - r * half;
+        const double turns = (double)a.positions[t0 + r] * a.turns.f[j];
         float sn, cs;
         sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
-        const float x0 = x, y0 = y;
-        x = x0 * cs - y0 * sn;
-        y = y0 * cs + x0 * sn;
+        turned[r * a.rot + j] = cs;
+        turned[r * a.rot + half + j] = sn;
     }
-    if (is_q) {
-        T* dst = (T*)a.q_out + t * a.qo_st + h * a.qo_sh;
-        dst[lo] = from_f32<T>(x);
-        if (hi != lo) dst[hi] = from_f32<T>(y);
-    } else {
-        C* dst = (C*)a.kc + cell + (h - a.Hq) * a.c_sh;
-        dst[lo] = from_f32<C>(x);
-        if (hi != lo) dst[hi] = from_f32<C>(y);
+    __syncthreads();
+    for (int base = 0; base < rows * per_row; base += APPEND_THREADS * APPEND_UNITS) {
+        Vec<T, W> lo[APPEND_UNITS], hi[APPEND_UNITS];
+        int row[APPEND_UNITS], head[APPEND_UNITS], unit[APPEND_UNITS];
+#pragma unroll
+        for (int k = 0; k < APPEND_UNITS; ++k) {
+            const int i = base + k * APPEND_THREADS + threadIdx.x;
+            row[k] = -1;
+            if (i >= rows * per_row) continue;
+            const int r = i / per_row, u = i - r * per_row, h = u / units;
+            if (slots[r] < 0) continue;
+            row[k] = r;
+            head[k] = h;
+            unit[k] = u - h * units;
+            const long long t = t0 + r;
+            const T* p = h < a.Hq           ? (const T*)a.q + t * a.q_st + h * a.q_sh
+                         : h < a.Hq + a.Hkv ? (const T*)a.k + t * a.k_st + (h - a.Hq) * a.k_sh
+                                            : (const T*)a.v + t * a.v_st + (h - a.Hq - a.Hkv) * a.v_sh;
+            const bool turn = unit[k] < rot_units && h < a.Hq + a.Hkv;
+            const int at = turn ? unit[k] * W : h < a.Hq + a.Hkv ? a.rot + (unit[k] - rot_units) * 2 * W : unit[k] * 2 * W;
+            load_vec<T, W>(lo[k], p + at);
+            load_vec<T, W>(hi[k], p + at + (turn ? half : W));
+        }
+#pragma unroll
+        for (int k = 0; k < APPEND_UNITS; ++k) {
+            if (row[k] < 0) continue;
+            const int h = head[k];
+            const bool turn = unit[k] < rot_units && h < a.Hq + a.Hkv;
+            const int at = turn ? unit[k] * W : h < a.Hq + a.Hkv ? a.rot + (unit[k] - rot_units) * 2 * W : unit[k] * 2 * W;
+            float x[W], y[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                x[i] = to_f32(lo[k].e[i]);
+                y[i] = to_f32(hi[k].e[i]);
+            }
+            if (turn) {
+                const float* cs = turned + row[k] * a.rot + unit[k] * W;
+                const float* sn = cs + half;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const float x0 = x[i], y0 = y[i];
+                    x[i] = x0 * cs[i] - y0 * sn[i];
+                    y[i] = y0 * cs[i] + x0 * sn[i];
+                }
+            }
+            const int next = at + (turn ? half : W);
+            if (h < a.Hq) {
+                T* p = (T*)a.q_out + (long long)(t0 + row[k]) * a.qo_st + h * a.qo_sh;
+                put<T, W>(p + at, x);
+                put<T, W>(p + next, y);
+            } else {
+                const int slot = slots[row[k]], hk = h < a.Hq + a.Hkv ? h - a.Hq : h - a.Hq - a.Hkv;
+                C* p = (C*)(h < a.Hq + a.Hkv ? a.kc : a.vc) + (slot >> a.page_shift) * a.c_sp +
+                       (slot & ((1 << a.page_shift) - 1)) * a.c_st + hk * a.c_sh;
+                put<C, W>(p + at, x);
+                put<C, W>(p + next, y);
+            }
+        }
     }
 }
 
-template <typename T, typename C>
-cudaError_t launch_append(const RopeAppendArgs& a, cudaStream_t s) {
-    const long long n = (long long)a.T * (a.Hq + 2 * a.Hkv) * (a.dh - a.rot / 2);
-    rope_append_kernel<T, C><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+template <typename T, typename C, int W>
+cudaError_t launch_append_w(const RopeAppendArgs& a, cudaStream_t s) {
+    const long long per_row = (long long)(a.Hq + 2 * a.Hkv) * (a.dh / (2 * W));
+    int rows = (int)(APPEND_THREADS * APPEND_UNITS / per_row);
+    rows = rows < 1 ? 1 : rows > APPEND_ROWS ? APPEND_ROWS : rows;
+    rope_append_kernel<T, C, W>
+        <<<(unsigned)((a.T + rows - 1) / rows), APPEND_THREADS, (size_t)rows * a.rot * sizeof(float), s>>>(a, rows);
     add_launches(1);
     return cudaGetLastError();
+}
+
+// The widest unit that divides the rotated half and what is left of a head.
+template <typename T, typename C>
+cudaError_t launch_append(const RopeAppendArgs& a, cudaStream_t s) {
+    auto fits = [&](int w) { return a.rot / 2 % w == 0 && (a.dh - a.rot) % (2 * w) == 0 && a.dh % (2 * w) == 0; };
+    if constexpr (sizeof(T) == 2) {
+        auto wide = [](const void* p, int64_t x, int64_t y) {
+            return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x % 8 == 0 && y % 8 == 0;
+        };
+        if (fits(8) && wide(a.k, a.k_st, a.k_sh) && wide(a.v, a.v_st, a.v_sh) && wide(a.kc, a.c_sp, a.c_st) &&
+            wide(a.vc, a.c_sh, 0) && (a.Hq == 0 || (wide(a.q, a.q_st, a.q_sh) && wide(a.q_out, a.qo_st, a.qo_sh))))
+            return launch_append_w<T, C, 8>(a, s);
+    }
+    if (fits(4)) return launch_append_w<T, C, 4>(a, s);
+    if (fits(2)) return launch_append_w<T, C, 2>(a, s);
+    return launch_append_w<T, C, 1>(a, s);
 }
 
 }  // namespace
 
 cudaError_t kv_page_plan(const PagePlanArgs& a, cudaStream_t s) {
-    page_plan_kernel<<<1, PLAN_THREADS, 0, s>>>(a);
-    add_launches(1);
-    return cudaGetLastError();
+    return launch_cluster(page_plan_kernel, a.rows <= PLAN_ONE_BLOCK, s, a);
 }
 
 cudaError_t kv_page_release(const PageReleaseArgs& a, cudaStream_t s) {
-    page_release_kernel<<<1, PLAN_THREADS, 0, s>>>(a);
-    add_launches(1);
-    return cudaGetLastError();
+    return launch_cluster(page_release_kernel, (long long)a.B * a.width <= PLAN_ONE_BLOCK, s, a);
 }
 
 // Powers of r = theta^(-2/rot) by repeated products in extended precision:
