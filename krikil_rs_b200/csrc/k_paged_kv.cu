@@ -293,12 +293,13 @@ cudaError_t launch_cluster(void (*kern)(Args...), bool one, cudaStream_t s, cons
 
 // ---------------------------------------------------------------- RoPE + append
 // Every input is read and every output written once, W elements (16 bytes) at
-// a time: HBM bounds it.  A block takes the heads of a few rows; the rows' cos
-// and sin are computed once a pair -- the turns, position times rate, reduced
-// to a fraction in 64 bits -- and shared by all heads through shared memory.  A
-// unit is W pairs (i, i + rot/2) of a query or key head, or 2 W neighbours that
-// are not rotated; a thread loads four units before it stores the first.
-constexpr int APPEND_THREADS = 256, APPEND_UNITS = 4, APPEND_ROWS = 8;
+// a time: HBM bounds it.  A unit is W pairs (i, i + rot/2) of a query or key
+// head, or 2 W neighbours that are not rotated; a thread keeps one unit and takes
+// it in two heads at once.  One wave of blocks takes equal runs of rows and
+// loads the next row before it stores the present one.  The rows' cos and sin
+// are computed eight rows at a time, once a pair for all heads: the turns,
+// position times rate, are reduced to a fraction in 64 bits.
+constexpr int APPEND_THREADS = 256, APPEND_HEADS = 2, APPEND_BATCH = 8, APPEND_BLOCKS = 3;
 
 template <int BYTES>
 struct Raw;
@@ -315,9 +316,9 @@ template <typename T, int W>
 union Vec {
     typename Raw<sizeof(T) * W>::type raw;
     T e[W];
+    uint32_t w[sizeof(T) * W / 4 ? sizeof(T) * W / 4 : 1];
     KRK_DEV Vec() {}
 };
-// f32 rows of 8 elements do not arise: W * sizeof(T) <= 16.
 template <typename T, int W>
 KRK_DEV void load_vec(Vec<T, W>& v, const T* p) {
     v.raw = *reinterpret_cast<const typename Raw<sizeof(T) * W>::type*>(p);
@@ -326,103 +327,177 @@ template <typename T, int W>
 KRK_DEV void store_vec(T* p, const Vec<T, W>& v) {
     *reinterpret_cast<typename Raw<sizeof(T) * W>::type*>(p) = v.raw;
 }
+KRK_DEV void to_f32x2(float& x, float& y, uint32_t u, __half) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+    x = f.x;
+    y = f.y;
+}
+KRK_DEV void to_f32x2(float& x, float& y, uint32_t u, __nv_bfloat16) {
+    x = __uint_as_float(u << 16);
+    y = __uint_as_float(u & 0xffff0000u);
+}
+KRK_DEV uint32_t from_f32x2(float x, float y, __half) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+KRK_DEV uint32_t from_f32x2(float x, float y, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T, int W>
+KRK_DEV void widen(float (&x)[W], const Vec<T, W>& v) {
+    if constexpr (sizeof(T) == 2 && W > 1) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) to_f32x2(x[2 * i], x[2 * i + 1], v.w[i], T());
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[i] = to_f32(v.e[i]);
+    }
+}
 template <typename T, int W>
 KRK_DEV void put(T* p, const float (&x)[W]) {
     Vec<T, W> v;
+    if constexpr (sizeof(T) == 2 && W > 1) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v.e[i] = from_f32<T>(x[i]);
+        for (int i = 0; i < W / 2; ++i) v.w[i] = from_f32x2(x[2 * i], x[2 * i + 1], T());
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v.e[i] = from_f32<T>(x[i]);
+    }
     store_vec<T, W>(p, v);
 }
 
+// How a block divides its rows: `side` rows at once, `lanes` threads of each
+// unit taking a row's heads; `depth` times.
+struct AppendShape {
+    int side, lanes, depth;
+};
+
 template <typename T, typename C, int W>
-__global__ void __launch_bounds__(APPEND_THREADS) rope_append_kernel(const __grid_constant__ RopeAppendArgs a,
-                                                                     int block_rows) {
-    extern __shared__ __align__(16) float turned[];  // [row][cos, sin][rot / 2]
-    __shared__ int slots[APPEND_ROWS];
-    const int half = a.rot / 2, units = a.dh / (2 * W), rot_units = half / W;
-    const int heads = a.Hq + 2 * a.Hkv, per_row = heads * units;
-    const int t0 = blockIdx.x * block_rows, rows = min(block_rows, a.T - t0);
-    if ((int)threadIdx.x < rows) {
-        const int slot = a.slots[t0 + threadIdx.x];
-        if (slot >= a.num_slots) check_fail(CHK_TABLE);
-        slots[threadIdx.x] = slot < a.num_slots ? slot : -1;
-    }
-    for (int i = threadIdx.x; i < rows * half; i += APPEND_THREADS) {
-        const int r = i / half, j = i - r * half;
-        const double turns = (double)a.positions[t0 + r] * a.turns.f[j];
-        float sn, cs;
-        sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
-        turned[r * a.rot + j] = cs;
-        turned[r * a.rot + half + j] = sn;
-    }
-    __syncthreads();
-    for (int base = 0; base < rows * per_row; base += APPEND_THREADS * APPEND_UNITS) {
-        Vec<T, W> lo[APPEND_UNITS], hi[APPEND_UNITS];
-        int row[APPEND_UNITS], head[APPEND_UNITS], unit[APPEND_UNITS];
+__global__ void __launch_bounds__(APPEND_THREADS, APPEND_BLOCKS)
+    rope_append_kernel(const __grid_constant__ RopeAppendArgs a, const AppendShape sh) {
+    extern __shared__ __align__(16) float turned[];  // [row of the batch][cos, sin][rot / 2]
+    const int half = a.rot / 2, units = a.dh / (2 * W), rot_units = half / W, heads = a.Hq + 2 * a.Hkv;
+    const int r = threadIdx.x / (sh.lanes * units), in_row = threadIdx.x - r * sh.lanes * units;
+    const int lane = in_row / units, unit = in_row - lane * units;
+    const long long t0 = (long long)blockIdx.x * sh.side * sh.depth;
+    const long long t1 = min(t0 + sh.side * sh.depth, (long long)a.T);
+    // where the unit's two parts lie in a rotated head and in a value head
+    const bool turns = unit < rot_units;
+    const int at = turns ? unit * W : a.rot + (unit - rot_units) * 2 * W, next = at + (turns ? half : W);
+    Vec<T, W> lo[APPEND_HEADS], hi[APPEND_HEADS];
+    int slot = -1;
+    auto load = [&](long long t, int h0) {
 #pragma unroll
-        for (int k = 0; k < APPEND_UNITS; ++k) {
-            const int i = base + k * APPEND_THREADS + threadIdx.x;
-            row[k] = -1;
-            if (i >= rows * per_row) continue;
-            const int r = i / per_row, u = i - r * per_row, h = u / units;
-            if (slots[r] < 0) continue;
-            row[k] = r;
-            head[k] = h;
-            unit[k] = u - h * units;
-            const long long t = t0 + r;
-            const T* p = h < a.Hq           ? (const T*)a.q + t * a.q_st + h * a.q_sh
-                         : h < a.Hq + a.Hkv ? (const T*)a.k + t * a.k_st + (h - a.Hq) * a.k_sh
-                                            : (const T*)a.v + t * a.v_st + (h - a.Hq - a.Hkv) * a.v_sh;
-            const bool turn = unit[k] < rot_units && h < a.Hq + a.Hkv;
-            const int at = turn ? unit[k] * W : h < a.Hq + a.Hkv ? a.rot + (unit[k] - rot_units) * 2 * W : unit[k] * 2 * W;
-            load_vec<T, W>(lo[k], p + at);
-            load_vec<T, W>(hi[k], p + at + (turn ? half : W));
-        }
-#pragma unroll
-        for (int k = 0; k < APPEND_UNITS; ++k) {
-            if (row[k] < 0) continue;
-            const int h = head[k];
-            const bool turn = unit[k] < rot_units && h < a.Hq + a.Hkv;
-            const int at = turn ? unit[k] * W : h < a.Hq + a.Hkv ? a.rot + (unit[k] - rot_units) * 2 * W : unit[k] * 2 * W;
-            float x[W], y[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                x[i] = to_f32(lo[k].e[i]);
-                y[i] = to_f32(hi[k].e[i]);
+        for (int i = 0; i < APPEND_HEADS; ++i) {
+            const int h = h0 + i * sh.lanes;
+            if (t >= t1 || h >= heads) continue;
+            if (h < a.Hq + a.Hkv) {
+                const T* p = h < a.Hq ? (const T*)a.q + t * a.q_st + h * a.q_sh
+                                      : (const T*)a.k + t * a.k_st + (h - a.Hq) * a.k_sh;
+                load_vec<T, W>(lo[i], p + at);
+                load_vec<T, W>(hi[i], p + next);
+            } else {
+                const T* p = (const T*)a.v + t * a.v_st + (h - a.Hq - a.Hkv) * a.v_sh + unit * 2 * W;
+                load_vec<T, W>(lo[i], p);
+                load_vec<T, W>(hi[i], p + W);
             }
-            if (turn) {
-                const float* cs = turned + row[k] * a.rot + unit[k] * W;
-                const float* sn = cs + half;
+        }
+    };
+    load(t0 + r, lane);
+    if (t0 + r < t1) slot = a.slots[t0 + r];
+    for (int d = 0; d < sh.depth; ++d) {
+        const int in_batch = d % APPEND_BATCH;
+        if (in_batch == 0) {
+            if (d > 0) __syncthreads();  // the batch before has been read
+            const long long first = t0 + (long long)d * sh.side;
+            const int rows = (int)min((long long)sh.side * APPEND_BATCH, t1 - first);
+            for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
+                const int row = i / half, j = i - row * half;
+                const double x = (double)a.positions[first + row] * a.turns.f[j];
+                float sn, cs;
+                sincospif(2.0f * (float)(x - rint(x)), &sn, &cs);
+                turned[row * a.rot + j] = cs;
+                turned[row * a.rot + half + j] = sn;
+            }
+            __syncthreads();
+        }
+        const long long t = t0 + (long long)d * sh.side + r, tn = t + sh.side;
+        int now = slot;
+        if (t >= t1 || now >= a.num_slots) {
+            if (t < t1) check_fail(CHK_TABLE);
+            now = -1;
+        }
+        if (tn < t1 && d + 1 < sh.depth) slot = a.slots[tn];
+        const float* cs = turned + (in_batch * sh.side + r) * a.rot + (turns ? unit * W : 0);
+        const long long cell = (now >> a.page_shift) * a.c_sp + (now & ((1 << a.page_shift) - 1)) * a.c_st;
+        for (int h0 = lane; h0 < heads;) {
+            Vec<T, W> lo_now[APPEND_HEADS], hi_now[APPEND_HEADS];
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const float x0 = x[i], y0 = y[i];
-                    x[i] = x0 * cs[i] - y0 * sn[i];
-                    y[i] = y0 * cs[i] + x0 * sn[i];
+            for (int i = 0; i < APPEND_HEADS; ++i) {
+                lo_now[i] = lo[i];
+                hi_now[i] = hi[i];
+            }
+            const int h1 = h0 + APPEND_HEADS * sh.lanes;
+            if (h1 < heads)
+                load(t, h1);
+            else if (d + 1 < sh.depth)
+                load(tn, lane);
+            if (now >= 0) {
+#pragma unroll
+                for (int i = 0; i < APPEND_HEADS; ++i) {
+                    const int h = h0 + i * sh.lanes;
+                    if (h >= heads) continue;
+                    float x[W], y[W];
+                    widen<T, W>(x, lo_now[i]);
+                    widen<T, W>(y, hi_now[i]);
+                    if (h >= a.Hq + a.Hkv) {
+                        C* p = (C*)a.vc + cell + (h - a.Hq - a.Hkv) * a.c_sh + unit * 2 * W;
+                        put<C, W>(p, x);
+                        put<C, W>(p + W, y);
+                        continue;
+                    }
+                    if (turns) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) {
+                            const float x0 = x[j], y0 = y[j], c = cs[j], s = cs[half + j];
+                            x[j] = fmaf(x0, c, -(y0 * s));
+                            y[j] = fmaf(y0, c, x0 * s);
+                        }
+                    }
+                    if (h < a.Hq) {
+                        T* p = (T*)a.q_out + t * a.qo_st + h * a.qo_sh;
+                        put<T, W>(p + at, x);
+                        put<T, W>(p + next, y);
+                    } else {
+                        C* p = (C*)a.kc + cell + (h - a.Hq) * a.c_sh;
+                        put<C, W>(p + at, x);
+                        put<C, W>(p + next, y);
+                    }
                 }
             }
-            const int next = at + (turn ? half : W);
-            if (h < a.Hq) {
-                T* p = (T*)a.q_out + (long long)(t0 + row[k]) * a.qo_st + h * a.qo_sh;
-                put<T, W>(p + at, x);
-                put<T, W>(p + next, y);
-            } else {
-                const int slot = slots[row[k]], hk = h < a.Hq + a.Hkv ? h - a.Hq : h - a.Hq - a.Hkv;
-                C* p = (C*)(h < a.Hq + a.Hkv ? a.kc : a.vc) + (slot >> a.page_shift) * a.c_sp +
-                       (slot & ((1 << a.page_shift) - 1)) * a.c_st + hk * a.c_sh;
-                put<C, W>(p + at, x);
-                put<C, W>(p + next, y);
-            }
+            h0 = h1;
         }
     }
 }
 
 template <typename T, typename C, int W>
 cudaError_t launch_append_w(const RopeAppendArgs& a, cudaStream_t s) {
-    const long long per_row = (long long)(a.Hq + 2 * a.Hkv) * (a.dh / (2 * W));
-    int rows = (int)(APPEND_THREADS * APPEND_UNITS / per_row);
-    rows = rows < 1 ? 1 : rows > APPEND_ROWS ? APPEND_ROWS : rows;
-    rope_append_kernel<T, C, W>
-        <<<(unsigned)((a.T + rows - 1) / rows), APPEND_THREADS, (size_t)rows * a.rot * sizeof(float), s>>>(a, rows);
+    const int units = a.dh / (2 * W), heads = a.Hq + 2 * a.Hkv;
+    AppendShape sh{1, (heads + APPEND_HEADS - 1) / APPEND_HEADS, 1};
+    if (sh.lanes > APPEND_THREADS / units) sh.lanes = APPEND_THREADS / units;  // several rounds of heads
+    sh.side = APPEND_THREADS / (sh.lanes * units);
+    if (sh.side > APPEND_BATCH) sh.side = APPEND_BATCH;
+    const int sms = paged_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    // One wave of blocks, each with its run of rows (16321 x 32/8 x 128 bf16: 69 us, 5.9 TB/s; 89 us with a block
+    // a row, whose start is not hidden).
+    const int threads = sh.side * sh.lanes * units;
+    const long long wave = (long long)sms * (APPEND_BLOCKS * APPEND_THREADS / threads) * sh.side;
+    sh.depth = (int)((a.T + wave - 1) / wave);
+    const long long rows = (long long)sh.side * sh.depth, batch = sh.depth < APPEND_BATCH ? sh.depth : APPEND_BATCH;
+    rope_append_kernel<T, C, W><<<(unsigned)((a.T + rows - 1) / rows), threads,
+                                  (size_t)sh.side * batch * a.rot * sizeof(float), s>>>(a, sh);
     add_launches(1);
     return cudaGetLastError();
 }

@@ -7,6 +7,9 @@
 
 namespace krk {
 
+// Multiprocessors of the current device, 0 if that cannot be read.
+int paged_sm_count();
+
 enum ElemType { ELEM_F32 = 0, ELEM_F16 = 1, ELEM_BF16 = 2 };  // KRK_TYPE_*
 
 // Status bits of the page planner and the release (KRK_PAGES_*).

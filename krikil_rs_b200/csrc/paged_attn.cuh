@@ -404,8 +404,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnA
 // Whether blocks take whole (request, heads): lengths up to `bound` are not worth a second kernel.
 inline bool pa_whole(int bound) { return bound <= PA_WHOLE_UNITS * PA_UNIT; }
 
-int paged_sm_count();  // of the current device, 0 if it cannot be read
-
 template <class E>
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     static DeviceOnce once;
