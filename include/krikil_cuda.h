@@ -497,10 +497,10 @@ KRK_API int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void
  * its window are never used, whatever they hold.
  * max_len: a bound of the lengths by which the launch is sized, 0 = width *
  * page_size; it moves the result by rounding at most.  work: 16-byte aligned
- * device scratch of krk_attn_paged_work_floats(B, Hq, Hkv, dh, that bound)
- * floats -- none (0) for short bounds -- with no initial contents, for calls
+ * device scratch of krk_attn_paged_work_floats(B, Hq, Hkv, dh, that bound,
+ * window) floats -- none (0) for little work, on the current device -- with no initial contents, for calls
  * that do not run at the same time. */
-KRK_API size_t krk_attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len);
+KRK_API size_t krk_attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int window);
 KRK_API int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void* kc, void* vc, int64_t c_sp,
                                     int64_t c_st, int64_t c_sh, int cache_type, const int32_t* table,
                                     int64_t table_ld, int width, int num_pages, int page_size, const int32_t* lens,

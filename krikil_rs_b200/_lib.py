@@ -80,7 +80,7 @@ _SIGS = {
     "krk_k_kv_page_release": (_i32, [_vp] * 3 + [_i64, _i32, _i32, _vp, _vp, _i32, _i32] + [_vp] * 4),
     "krk_k_rope_kv_append_paged": (_i32, [_vp, _i64, _i64] * 3 + [_i32, _vp, _i64, _i64, _vp, _vp] + [_i64] * 3
                                    + [_i32, _vp, _vp] + [_i32] * 7 + [_f32, _vp]),
-    "krk_attn_paged_work_floats": (C.c_size_t, [_i32] * 5),
+    "krk_attn_paged_work_floats": (C.c_size_t, [_i32] * 6),
     "krk_k_attn_decode_paged": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp] + [_i64] * 3 + [_i32, _vp, _i64]
                                 + [_i32] * 3 + [_vp] + [_i32] * 4 + [_f32, _i32, _i32, _vp, _i64, _i64, _vp, _vp,
                                                                     C.c_size_t, _vp]),

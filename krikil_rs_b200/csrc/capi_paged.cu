@@ -139,9 +139,10 @@ int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void* k, int
     return done(who, krk::rope_kv_append_paged(a, type, cache_type, (cudaStream_t)stream));
 }
 
-size_t krk_attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len) {
-    if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || dh < 4 || dh > 256 || dh % 4 || max_len < 0) return 0;
-    return krk::attn_paged_work_floats(B, Hq, Hkv, dh, max_len);
+size_t krk_attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int window) {
+    if (B <= 0 || Hkv <= 0 || Hq < Hkv || Hq % Hkv || dh < 4 || dh > 256 || dh % 4 || max_len < 0 || window < 0)
+        return 0;
+    return krk::attn_paged_work_floats(B, Hq, Hkv, dh, max_len, window);
 }
 
 int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void* kc, void* vc, int64_t c_sp,
@@ -170,7 +171,7 @@ int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void*
     const int shift = log2_exact(page_size);
     const int64_t cap = (int64_t)width << shift;
     const int bound = (int)(max_len > 0 && max_len < cap ? max_len : cap);
-    const size_t need = krk::attn_paged_work_floats(B, Hq, Hkv, dh, bound);
+    const size_t need = krk::attn_paged_work_floats(B, Hq, Hkv, dh, bound, window);
     if (need > 0 && (!work || work_floats < need || !aligned(work, 16)))
         return invalid(who, "work must be 16-byte aligned and hold " + std::to_string(need) + " floats");
     const krk::PagedAttnArgs a{q, q_sb, q_sh, kc, vc, c_sp, c_st, c_sh, table, table_ld, width, num_pages, shift,

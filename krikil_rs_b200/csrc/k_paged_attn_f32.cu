@@ -14,7 +14,7 @@
 namespace krk {
 namespace {
 
-template <int DC_, int GW>
+template <int DC_, int GW, int SLOTS_>
 struct F32Engine {
     using Act = float;
     using Cache = float;
@@ -25,8 +25,8 @@ struct F32Engine {
     static constexpr int KPL = 32 / LPK;               // keys side by side
     static constexpr int KT = J * KPL;                 // 16, 8 or 4 keys
     static constexpr int Q_BYTES = 0;
-    static constexpr int TILE_BYTES = 8 * 512, SLOTS = 1;
-    static constexpr int BLOCKS = 4;
+    static constexpr int TILE_BYTES = 8 * 512, SLOTS = SLOTS_;
+    static constexpr int BLOCKS = SLOTS == 1 ? 4 : 3;
     static constexpr float SCALE = 1.f;
 
     float4 q[GW][NL], acc[GW][NL];
@@ -125,9 +125,9 @@ struct F32Engine {
             if (LPK == 16) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             top = fmaxf(top, m[h]);
             const float ref = top == -INFINITY ? 0.f : top;
-            fade[h] = exp2f(m[h] - ref);
+            fade[h] = pa_exp2(m[h] - ref);
             m[h] = top;
-            s[h] = exp2f(x - ref);
+            s[h] = pa_exp2(x - ref);
             l[h] = l[h] * fade[h] + s[h];
         }
     }
@@ -187,9 +187,9 @@ struct F32Engine {
 
 template <int GW>
 cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
-    if (a.dh <= 64) return launch_paged_attn<F32Engine<64, GW>>(a, s);
-    if (a.dh <= 128) return launch_paged_attn<F32Engine<128, GW>>(a, s);
-    return launch_paged_attn<F32Engine<256, GW>>(a, s);
+    if (a.dh <= 64) return launch_paged_attn<F32Engine<64, GW, 1>, F32Engine<64, GW, 2>>(a, s);
+    if (a.dh <= 128) return launch_paged_attn<F32Engine<128, GW, 1>, F32Engine<128, GW, 2>>(a, s);
+    return launch_paged_attn<F32Engine<256, GW, 1>, F32Engine<256, GW, 2>>(a, s);
 }
 
 }  // namespace
@@ -206,9 +206,12 @@ int paged_sm_count() {
     return n;
 }
 
-size_t attn_paged_work_floats(int, int Hq, int Hkv, int dh, int max_len) {
-    if (pa_whole(max_len)) return 0;
-    const int share = Hq / Hkv, rows = 4 * share < PA_MAX_ROWS ? 4 * share : PA_MAX_ROWS;
+size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int window) {
+    // with as many pieces as any engine makes
+    const int sms = paged_sm_count(), share = Hq / Hkv, per_kv = (share + 15) / 16;
+    const int bound = pa_bound(max_len, window);
+    if (pa_clusters((long long)B * Hkv * per_kv, bound, sms > 0 ? sms : 148)) return 0;
+    const int rows = 4 * share < PA_MAX_ROWS ? 4 * share : PA_MAX_ROWS;
     return (size_t)PA_MAX_BLOCKS * (2 * (size_t)rows * (dh + 2) + 2);
 }
 
@@ -219,11 +222,13 @@ cudaError_t attn_decode_paged_f32(const PagedAttnArgs& a, cudaStream_t s) {
     return by_width<4>(a, s);
 }
 
-cudaError_t attn_decode_paged_half(const PagedAttnArgs& a, int act, int cache, cudaStream_t s);
+cudaError_t attn_decode_paged_f16(const PagedAttnArgs& a, bool act_f32, cudaStream_t s);
+cudaError_t attn_decode_paged_bf16(const PagedAttnArgs& a, bool act_f32, cudaStream_t s);
 
 cudaError_t attn_decode_paged(const PagedAttnArgs& a, int act, int cache, cudaStream_t s) {
-    if (act == ELEM_F32 && cache == ELEM_F32) return attn_decode_paged_f32(a, s);
-    return attn_decode_paged_half(a, act, cache, s);
+    if (cache == ELEM_F16) return attn_decode_paged_f16(a, act == ELEM_F32, s);
+    if (cache == ELEM_BF16) return attn_decode_paged_bf16(a, act == ELEM_F32, s);
+    return attn_decode_paged_f32(a, s);
 }
 
 }  // namespace krk

@@ -40,7 +40,7 @@ KRK_DEV unsigned cluster_rank() {
     return n;
 }
 KRK_DEV void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
 }
 
 // Sums of two values a thread over the block.

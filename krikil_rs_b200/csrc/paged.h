@@ -76,7 +76,7 @@ struct PagedAttnArgs {
     float* lse;                                      // [B][Hq] or nullptr
     float* work;
 };
-size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len);
+size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int window);
 cudaError_t attn_decode_paged(const PagedAttnArgs& a, int act, int cache, cudaStream_t s);
 
 }  // namespace krk

@@ -4,16 +4,24 @@
 // One token a request reads every visible key and value once and computes 4 dh
 // operations for each pair and query head, so for the up to some tens of heads
 // that share a cache head the cache's bytes bound it.  The frame therefore
-// divides bytes: the visible keys of every (request, cache head) are cut into
-// units of 64, and the units of the whole batch -- whatever the requests'
-// lengths -- are dealt to one resident wave of blocks in equal contiguous
-// shares.  A block works off its share piece by piece (a piece lies within one
-// request and one cache head, or up to four neighbours of it); its warps take
-// tiles of keys in turn, each with a running maximum and sum, and are merged in
-// shared memory at the piece's end.  A piece
-// that covers all of its keys is written as the result; otherwise its sums go
-// to the scratch, where attn_paged_join adds them up in the order of the
-// blocks, so that results do not depend on timing.
+// divides bytes, in one of two ways:
+//
+// Shares, for much work.  The visible keys of every (request, cache head) are
+// cut into units of 64, and the units of the whole batch -- whatever the
+// requests' lengths -- are dealt to one resident wave of blocks in equal
+// contiguous shares.  A block works off its share piece by piece (a piece lies
+// within one request and one cache head, or up to four neighbours of it).  A
+// piece that covers all of its keys is written as the result; otherwise its sums
+// go to the scratch, where paged_join_kernel adds them up in the order of the
+// blocks.
+//
+// Clusters, where latency counts: 1, 2, 4 or 8 blocks of a thread-block cluster
+// take equal parts of one piece and add up their sums through each other's shared
+// memory.  One kernel, no scratch and no look at the other requests.
+//
+// Either way a block's warps take tiles of keys in turn, each with a running
+// maximum and sum, and are merged in shared memory at the end; all orders are
+// fixed, so that results do not depend on timing.
 #pragma once
 #include <math.h>
 
@@ -25,7 +33,10 @@ namespace krk {
 
 constexpr int PA_THREADS = 128, PA_WARPS = 4;
 constexpr int PA_UNIT = 64;          // keys of one unit of work
-constexpr int PA_WHOLE_UNITS = 4;    // up to this many units a block takes a whole (request, head)
+constexpr int PA_CLUSTER = 8;        // blocks of a cluster, at most
+constexpr int PA_PART_UNITS = 2;     // units of a block down to which clusters grow
+constexpr int PA_CLUSTER_UNITS = 12; // units of a block up to which clusters are used
+constexpr int PA_JOIN = 512;         // threads of a join's block, at most
 constexpr int PA_MAX_BLOCKS = 592;   // blocks of a wave: four on each of 148 SMs
 constexpr int PA_MAX_ROWS = 32;      // query heads of a piece, at most
 constexpr int PA_SIDE_UNITS = 8;     // units a block from which on its warps take different cache heads
@@ -44,9 +55,16 @@ struct PagedParts {
 struct PagedShape {
     int side, groups;
     int per_kv;   // pieces for the query heads of one cache head
-    int rows;     // query heads of a piece
-    int whole;    // blocks take whole (request, heads)
+    int rows;     // query heads of a piece of one cache head
+    int cluster;  // blocks that share a piece, 0: shares of the whole batch
 };
+
+// 2^x to about a unit in the last place, 0 below 2^-126.
+KRK_DEV float pa_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 KRK_DEV int pa_len(const PagedAttnArgs& a, int b) {
     const int cap = (int)((long long)a.width << a.page_shift);
@@ -115,10 +133,11 @@ struct PagedTile {
     long long off;
     unsigned mask;  // the visible keys
 };
+// (Entries past the request's last page are read, and not used.)
 template <int KT>
-KRK_DEV int pa_page(const PagedAttnArgs& a, const int32_t* row, int key0, int k1) {
+KRK_DEV int pa_page(const PagedAttnArgs& a, const int32_t* row, int key0) {
     const int key = a.page_shift >= 4 ? key0 : key0 + (threadIdx.x & (KT - 1));
-    return key < k1 ? row[key >> a.page_shift] : -1;
+    return row[min(key >> a.page_shift, a.width - 1)];
 }
 template <int KT>
 KRK_DEV PagedTile pa_tile(const PagedAttnArgs& a, int page, int key0, int first, int k1) {
@@ -143,6 +162,29 @@ KRK_DEV PagedTile pa_tile(const PagedAttnArgs& a, int page, int key0, int first,
 // The element offset of key `key` of the tile (a fixed key for each lane).
 KRK_DEV long long pa_key(const PagedAttnArgs& a, const PagedTile& t, int key) {
     return a.page_shift >= 4 ? t.off + key * a.c_st : __shfl_sync(0xffffffffu, t.off, key);
+}
+
+KRK_DEV void pa_cluster_sync() {
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
+}
+// Shared memory of block `rank` of the cluster at this block's address `at`.
+KRK_DEV uint32_t pa_peer(uint32_t at, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
+}
+KRK_DEV float4 pa_peer_load4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at)
+                 : "memory");
+    return v;
+}
+KRK_DEV float2 pa_peer_load2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
 }
 
 // Barrier of the warps that share a group's queries.
@@ -172,6 +214,52 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 //   finish(obuf, m, l)          accumulators, maxima and sums of the warp to shared memory
 // A warp's ring has SLOTS slots for keys and as many for values; a slot is
 // filled again as soon as the warp has read it, with no barrier beyond the warp.
+// Adds up the sums of a cluster's blocks, each block a part of the elements.
+template <class E>
+KRK_DEV void pa_join_cluster(const PagedAttnArgs& a, const PagedShape& sh, const unsigned char* smem,
+                             const float2* sums, int b, int hk0, int head0, int rank) {
+    constexpr int LD = E::DC + 4, HW = E::HW;
+    const int G = a.Hq / a.Hkv, n4 = a.dh / 4, rows = sh.side * sh.rows;
+    const uint32_t sums_at = smem_addr(sums), acc_at = smem_addr(smem);
+    for (int i = rank * PA_THREADS + threadIdx.x; i < rows * n4; i += sh.cluster * PA_THREADS) {
+        const int r = i / n4, d = (i - r * n4) * 4, s = r / sh.rows, in_g = r - s * sh.rows;
+        if (head0 + in_g >= G) continue;
+        const int w0 = s * sh.groups + in_g / HW, h = in_g % HW;
+        const uint32_t ml_at = sums_at + (w0 * HW + h) * 8;
+        const uint32_t at = acc_at + w0 * 2 * E::SLOTS * E::TILE_BYTES + (h * LD + d) * 4;
+        float2 ml[PA_CLUSTER];
+        float4 x[PA_CLUSTER];
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int c = 0; c < PA_CLUSTER; ++c) {
+            ml[c] = make_float2(-INFINITY, 0.f);
+            x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c < sh.cluster) {
+                ml[c] = pa_peer_load2(pa_peer(ml_at, c));
+                x[c] = pa_peer_load4(pa_peer(at, c));
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < PA_CLUSTER; ++c) top = fmaxf(top, ml[c].x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < PA_CLUSTER; ++c) {
+            const float f = top == -INFINITY ? (ml[c].y == 0.f ? 0.f : ml[c].y) : pa_exp2(ml[c].x - top);
+            total = fmaf(f, ml[c].y, total);
+            o.x = fmaf(f, x[c].x, o.x);
+            o.y = fmaf(f, x[c].y, o.y);
+            o.z = fmaf(f, x[c].z, o.z);
+            o.w = fmaf(f, x[c].w, o.w);
+        }
+        const float inv = total == 0.f ? 0.f : 1.0f / total;
+        const long long head = (long long)(hk0 + s) * G + head0 + in_g;
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        store4((typename E::Act*)a.out + b * a.o_sb + head * a.o_sh + d, o);
+        if (a.lse && d == 0)
+            a.lse[(long long)b * a.Hq + head] = (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
+    }
+}
+
 template <class E>
 __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a,
                                                                            const PagedShape sh,
@@ -181,6 +269,7 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
     constexpr int KT = E::KT, HW = E::HW, LD = E::DC + 4, S = E::SLOTS, HALF = E::TILE_BYTES;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sm[PA_WARPS][HW], sl[PA_WARPS][HW], sf[PA_WARPS][HW];
+    __shared__ __align__(8) float2 sums[PA_MAX_ROWS];
     __shared__ long long warp_sums[PA_WARPS];
     __shared__ PagedShare share_out;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -192,22 +281,36 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
     const uint32_t ring_at = smem_addr(ring);
 
     PagedShare share;
-    if (sh.whole) {
-        share.b = blockIdx.x / pieces;
+    int pages[S + 1];
+    const int rank = sh.cluster > 1 ? blockIdx.x % sh.cluster : 0;
+    // a block with one part of one piece from the first key on reads its first pages beside the request's length
+    const bool early = sh.cluster == 1 && a.window == 0;
+    if (early) {
+#pragma unroll
+        for (int i = 0; i <= S; ++i)
+            pages[i] = pa_page<KT>(a, a.table + blockIdx.x / pieces * a.table_ld, (kwarp + i * kwarps) * KT);
+    }
+    if (sh.cluster) {
+        share.b = blockIdx.x / sh.cluster / pieces;
     } else {
         pdl_trigger();
         share = pa_share(a, pieces, &share_out, warp_sums);
     }
     int b = share.b, n = pa_len(a, b), first = pa_first(a, n), units = pa_units(n, first);
-    if (sh.whole) {
-        share.at = (long long)(blockIdx.x % pieces) * units;
-        share.size = units;
+    if (sh.cluster) {  // no unit for some blocks of a short request's cluster
+        const int u0 = (int)((long long)units * rank / sh.cluster);
+        share.at = (long long)(blockIdx.x / sh.cluster % pieces) * units + u0;
+        share.size = (int)((long long)units * (rank + 1) / sh.cluster) - u0;
     }
     int piece = (int)(share.at / units), unit = (int)(share.at % units);
+    if (sh.cluster) {  // (the place after a piece's last unit still belongs to it)
+        piece = blockIdx.x / sh.cluster % pieces;
+        unit = (int)(share.at - (long long)piece * units);
+    }
     long long left = share.size;
     int2 rec = make_int2(-1, -1);
 
-    while (left > 0) {
+    while (left > 0 || sh.cluster) {
         const int take = (int)min((long long)(units - unit), left);
         const int hk0 = piece / sh.per_kv * sh.side, head0 = piece % sh.per_kv * sh.rows;  // head0: within G
         const int hk = hk0 + set / sh.groups, head = head0 + set % sh.groups * HW;
@@ -221,9 +324,10 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
         int key = k0 + kwarp * KT;
         const int step = kwarps * KT;
         // the first tiles' pages, then the queries while they are on their way
-        int pages[S + 1];
+        if (!early) {
 #pragma unroll
-        for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step, k1);
+            for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step);
+        }
         e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, min(HW, G - head), qs, lane, kwarp,
                kwarps);
         if (E::Q_BYTES) pa_group_sync(set, kwarps);
@@ -249,7 +353,7 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
                 mask[S] = t.mask;
                 if (ahead < k1) e.issue(a, kc, t, ring_at + slot * HALF, lane);
                 cp_async_commit();
-                page = pa_page<KT>(a, row, ahead + step, k1);
+                page = pa_page<KT>(a, row, ahead + step);
                 e.weigh(mask[0], lane);
                 cp_async_wait<2 * S - 1>();
                 __syncwarp();
@@ -273,12 +377,14 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             float top = -INFINITY, total = 0.f;
             for (int w = w0; w < PA_WARPS; w += sets) top = fmaxf(top, sm[w][h]);
             for (int w = w0; w < PA_WARPS; w += sets) {
-                const float f = top == -INFINITY ? (sl[w][h] == 0.f ? 0.f : sl[w][h]) : exp2f(sm[w][h] - top);
+                const float f = top == -INFINITY ? (sl[w][h] == 0.f ? 0.f : sl[w][h]) : pa_exp2(sm[w][h] - top);
                 sf[w][h] = f;
                 total = fmaf(f, sl[w][h], total);
             }
             if (in_g < sh.rows && head0 + in_g < G) {
-                if (take == units) {
+                if (sh.cluster > 1) {
+                    sums[tid] = make_float2(top, total);
+                } else if (take == units) {
                     const float inv = total == 0.f ? 0.f : 1.0f / total;
                     for (int w = w0; w < PA_WARPS; w += sets) sf[w][h] *= inv;
                     if (a.lse)
@@ -305,11 +411,21 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
                 o.z = fmaf(f, x.z, o.z);
                 o.w = fmaf(f, x.w, o.w);
             }
-            if (take == units)
+            if (sh.cluster > 1)  // over the first of the warps' sums, which nobody else reads
+                *reinterpret_cast<float4*>(smem + (size_t)w0 * 2 * S * HALF + (h * LD + d) * 4) = o;
+            else if (take == units)
                 store4((T*)a.out + b * a.o_sb + ((long long)(hk0 + s) * G + head0 + in_g) * a.o_sh + d, o);
             else
                 *reinterpret_cast<float4*>(
                     parts.acc + (((long long)blockIdx.x * 2 + (unit == 0)) * rows + r) * a.dh + d) = o;
+        }
+        if (sh.cluster) {
+            if (sh.cluster > 1) {
+                pa_cluster_sync();
+                pa_join_cluster<E>(a, sh, smem, sums, b, hk0, head0, rank);
+                pa_cluster_sync();  // the others may still read this block's sums
+            }
+            return;
         }
         if (take != units) (unit == 0 ? rec.y : rec.x) = b * pieces + piece;
         left -= take;
@@ -324,19 +440,19 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
         }
         __syncthreads();  // the next piece's tiles go where this one's sums were
     }
-    if (!sh.whole && tid == 0) parts.rec[blockIdx.x] = rec;
+    if (tid == 0) parts.rec[blockIdx.x] = rec;
 }
 
 // Joins the partial results: block (c, r) looks whether block c of the
 // attention began a piece's keys without finishing them, and if so adds up query
 // head r of the piece over the blocks c, c + 1, ... that worked on it.
 template <typename T>
-__global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnArgs a, const PagedShape sh,
-                                                               const PagedParts parts, int blocks, float scale) {
+__global__ void __launch_bounds__(PA_JOIN) paged_join_kernel(const PagedAttnArgs a, const PagedShape sh,
+                                                            const PagedParts parts, int blocks, float scale) {
     __shared__ float weight[PA_MAX_BLOCKS + 1];
-    __shared__ float red[2][PA_WARPS];
-    __shared__ float4 sums[PA_THREADS];
-    const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+    __shared__ float red[2][32];
+    __shared__ float4 sums[PA_JOIN];
+    const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, threads = blockDim.x;
     pdl_wait();
     const int item = parts.rec[c].y;
     if (item < 0) return;
@@ -345,40 +461,56 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnA
     if (in_g >= G) return;
     const long long head = (long long)(piece / sh.per_kv * sh.side + r / sh.rows) * G + in_g;
     int count = 1;  // the blocks of an item are neighbours
-    for (int i = c + 1; i < blocks; i += PA_THREADS)
-        count += __syncthreads_count(i + tid < blocks && parts.rec[min(i + tid, blocks - 1)].x == item);
+    for (int i = c + 1; i < blocks; i += threads) {
+        const int here = __syncthreads_count(i + tid < blocks && parts.rec[min(i + tid, blocks - 1)].x == item);
+        count += here;
+        if (here < threads) break;
+    }
     // weights 2^(m - top) and the sum
     float top = -INFINITY, total = 0.f;
     auto ml = [&](int i) { return parts.ml[((long long)(c + i) * 2 + (i == 0)) * rows + r]; };
-    for (int i = tid; i < count; i += PA_THREADS) top = fmaxf(top, ml(i).x);
+    for (int i = tid; i < count; i += threads) top = fmaxf(top, ml(i).x);
     top = warp_max(top);
     if ((tid & 31) == 0) red[0][tid >> 5] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    for (int i = tid; i < count; i += PA_THREADS) {
+    for (int w = 0; w < threads / 32; ++w) top = fmaxf(top, red[0][w]);
+    for (int i = tid; i < count; i += threads) {
         const float2 x = ml(i);
-        const float f = top == -INFINITY ? (x.y == 0.f ? 0.f : x.y) : exp2f(x.x - top);
+        const float f = top == -INFINITY ? (x.y == 0.f ? 0.f : x.y) : pa_exp2(x.x - top);
         weight[i] = f;
         total = fmaf(f, x.y, total);
     }
     total = warp_sum(total);
     if ((tid & 31) == 0) red[1][tid >> 5] = total;
     __syncthreads();
-    total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    total = 0.f;
+    for (int w = 0; w < threads / 32; ++w) total += red[1][w];
     const float inv = total == 0.f ? 0.f : 1.0f / total;
-    // dh/4 threads a partial result, as many side by side as fit
-    const int n4 = a.dh / 4, side = PA_THREADS / n4, d = (tid % n4) * 4, s0 = tid / n4;
+    // dh/4 threads a partial result, as many side by side as fit, four loads of each on their way
+    const int n4 = a.dh / 4, side = threads / n4, d = (tid % n4) * 4, s0 = tid / n4;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (s0 < side) {
-#pragma unroll 8
-        for (int i = s0; i < count; i += side) {
-            const float4 x = *reinterpret_cast<const float4*>(
-                parts.acc + (((long long)(c + i) * 2 + (i == 0)) * rows + r) * a.dh + d);
-            const float f = weight[i];
-            o.x = fmaf(f, x.x, o.x);
-            o.y = fmaf(f, x.y, o.y);
-            o.z = fmaf(f, x.z, o.z);
-            o.w = fmaf(f, x.w, o.w);
+        for (int i0 = s0; i0 < count; i0 += 4 * side) {
+            float4 x[4];
+            float f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j * side;
+                f[j] = 0.f;
+                x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < count) {
+                    f[j] = weight[i];
+                    x[j] = *reinterpret_cast<const float4*>(
+                        parts.acc + (((long long)(c + i) * 2 + (i == 0)) * rows + r) * a.dh + d);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o.x = fmaf(f[j], x[j].x, o.x);
+                o.y = fmaf(f[j], x[j].y, o.y);
+                o.z = fmaf(f[j], x[j].z, o.z);
+                o.w = fmaf(f[j], x[j].w, o.w);
+            }
         }
     }
     sums[tid] = o;
@@ -401,49 +533,79 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join_kernel(const PagedAttnA
         a.lse[(long long)b * a.Hq + head] = (top + log2f(total * (1.0f / scale))) * 0.693147180559945309f;
 }
 
-// Whether blocks take whole (request, heads): lengths up to `bound` are not worth a second kernel.
-inline bool pa_whole(int bound) { return bound <= PA_WHOLE_UNITS * PA_UNIT; }
+// Blocks of a cluster for pieces of at most `bound` keys, 0: shares.  Clusters
+// grow while their blocks have more than PA_PART_UNITS units and all fit in a
+// wave of three a multiprocessor.
+inline int pa_clusters(long long items, int bound, int sms) {
+    const int units = (bound + PA_UNIT - 1) / PA_UNIT;
+    if (items > 3LL * sms) return 0;
+    int n = 1;
+    while (n < PA_CLUSTER && units > PA_PART_UNITS * n && items * 2 * n <= 3LL * sms) n *= 2;
+    return units <= PA_CLUSTER_UNITS * n ? n : 0;
+}
+inline int pa_bound(int max_len, int window) {  // of a piece's keys
+    return window > 0 && window < max_len ? window + PA_ALIGN : max_len;
+}
 
-template <class E>
+// E2: the engine with two slots a warp, for clusters.
+template <class E, class E2>
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
-    static DeviceOnce once;
-    constexpr size_t kRing = (size_t)PA_WARPS * 2 * E::SLOTS * E::TILE_BYTES;
     static_assert(E::HW * (E::DC + 4) * 4 <= 2 * E::SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
     const int G = a.Hq / a.Hkv, sms = paged_sm_count();
     if (sms <= 0) return cudaErrorInvalidDevice;
-    cudaError_t e = once.set_smem((const void*)paged_attn_kernel<E>, kRing + PA_WARPS * E::Q_BYTES);
-    if (e != cudaSuccess) return e;
-    const int slots = sms * E::BLOCKS < PA_MAX_BLOCKS ? sms * E::BLOCKS : PA_MAX_BLOCKS;
-    const int bound = a.window > 0 && a.window < a.max_len ? a.window + PA_ALIGN : a.max_len;
-    const long long units = (bound + PA_UNIT - 1) / PA_UNIT;
     PagedShape sh{1, 1, 1, 0, 0};
     while (sh.groups < PA_WARPS && sh.groups * E::HW < G) sh.groups *= 2;
     sh.per_kv = (G + sh.groups * E::HW - 1) / (sh.groups * E::HW);
     sh.rows = G < sh.groups * E::HW ? G : sh.groups * E::HW;
+    const int bound = pa_bound(a.max_len, a.window);
+    long long items = (long long)a.B * a.Hkv * sh.per_kv;
+    sh.cluster = pa_clusters(items, bound, sms);
+    if (sh.cluster) {
+        static DeviceOnce once;
+        constexpr size_t kRing = (size_t)PA_WARPS * 2 * E2::SLOTS * E2::TILE_BYTES;
+        cudaError_t e = once.set_smem((const void*)paged_attn_kernel<E2>, kRing + PA_WARPS * E2::Q_BYTES);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(items * sh.cluster));
+        cfg.blockDim = dim3(PA_THREADS);
+        cfg.dynamicSmemBytes = kRing + (size_t)sh.groups * E2::Q_BYTES;
+        cfg.stream = s;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = sh.cluster;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = sh.cluster > 1;
+        e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<E2>, a, sh, PagedParts{});
+        if (e == cudaSuccess) add_launches(1);
+        return e;
+    }
+    static DeviceOnce once;
+    constexpr size_t kRing = (size_t)PA_WARPS * 2 * E::SLOTS * E::TILE_BYTES;
+    cudaError_t e = once.set_smem((const void*)paged_attn_kernel<E>, kRing + PA_WARPS * E::Q_BYTES);
+    if (e != cudaSuccess) return e;
+    const int slots = sms * E::BLOCKS < PA_MAX_BLOCKS ? sms * E::BLOCKS : PA_MAX_BLOCKS;
+    const long long units = (bound + PA_UNIT - 1) / PA_UNIT;
     // With work for every block, warps take neighbouring cache heads of the same keys.
     while (sh.side * sh.groups < PA_WARPS && a.Hkv % (2 * sh.side) == 0 &&
-           (long long)a.B * (a.Hkv / sh.side / 2) * sh.per_kv * units >= PA_SIDE_UNITS * (long long)slots)
+           items / 2 * units >= PA_SIDE_UNITS * (long long)slots) {
         sh.side *= 2;
-    const size_t smem = kRing + (size_t)sh.side * sh.groups * E::Q_BYTES;
-    const long long items = (long long)a.B * (a.Hkv / sh.side) * sh.per_kv;
-    if (pa_whole(a.max_len)) {
-        sh.whole = 1;
-        paged_attn_kernel<E><<<(unsigned)items, PA_THREADS, smem, s>>>(a, sh, PagedParts{});
-        add_launches(1);
-        return cudaGetLastError();
+        items /= 2;
     }
     const int blocks = items * units < slots ? (int)(items * units) : slots, rows = sh.side * sh.rows;
     PagedParts parts;
     parts.acc = a.work;
     parts.ml = reinterpret_cast<float2*>(a.work + (size_t)PA_MAX_BLOCKS * 2 * rows * a.dh);
     parts.rec = reinterpret_cast<int2*>(parts.ml + (size_t)PA_MAX_BLOCKS * 2 * rows);
-    paged_attn_kernel<E><<<blocks, PA_THREADS, smem, s>>>(a, sh, parts);
+    paged_attn_kernel<E>
+        <<<blocks, PA_THREADS, kRing + (size_t)sh.side * sh.groups * E::Q_BYTES, s>>>(a, sh, parts);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     add_launches(1);
     PdlScope pdl(true);
-    e = launch_pdl(paged_join_kernel<typename E::Act>, dim3(blocks, rows), dim3(PA_THREADS), 0, s, a, sh, parts, blocks,
-                   E::SCALE);
+    // large blocks for the joins of many parts
+    e = launch_pdl(paged_join_kernel<typename E::Act>, dim3(blocks, rows),
+                   dim3(items * 16 <= blocks ? PA_JOIN : PA_THREADS), 0, s, a, sh, parts, blocks, E::SCALE);
     if (e == cudaSuccess) add_launches(1);
     return e;
 }

@@ -17,6 +17,7 @@
 // by a power of two (22 bits and a sign) or three bfloat16 parts (24 bits).
 // Half weights are scaled by 2^14, so that a key 2^-24 as likely as the
 // strongest still has 14 bits.
+#pragma once
 #include "paged_attn.cuh"
 
 namespace krk {
@@ -76,20 +77,21 @@ KRK_DEV void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
                  : "memory");
 }
 
-template <typename T, typename C, int DC_, bool WIDE>
+// DC: the elements of a row that are worked on, a multiple of 32 that is at least dh; SLOTS: of a warp's ring.
+template <typename T, typename C, int DC_, bool WIDE, int SLOTS_>
 struct HalfEngine {
     using Act = T;
     using Cache = C;
     static constexpr bool kSame = sizeof(T) == 2, kHalf = sizeof(__half) == 2 && std::is_same<C, __half>::value;
     static constexpr int DC = DC_, KT = 16, HW = 8;
     static constexpr int NB = DC / 32, NV = DC / 16;     // steps of the two products
-    static constexpr int ROW = DC * 2, CPR = DC / 8;      // bytes and 16-byte pieces of a row
+    static constexpr int CPR = DC <= 64 ? 8 : DC <= 128 ? 16 : 32, ROW = CPR * 16;  // a row's 16-byte pieces and bytes
     static constexpr int RPC = 32 / CPR;                  // rows of one copy
     static constexpr int QP = kSame ? 1 : kHalf ? 2 : 3;  // parts of a query
     static constexpr int PP = !kSame && !kHalf ? 3 : 2;   // parts of a weight
     static constexpr int Q_BYTES = QP * NB * 32 * 16;
-    static constexpr int TILE_BYTES = KT * ROW, SLOTS = 1;
-    static constexpr int BLOCKS = DC <= 128 ? 4 : 2;
+    static constexpr int TILE_BYTES = KT * ROW, SLOTS = SLOTS_;
+    static constexpr int BLOCKS = DC > 128 ? 2 : SLOTS == 1 ? 4 : 3;
     static constexpr float SCALE = kHalf ? 16384.f : 1.f;
 
     float acc[NV][4];
@@ -107,7 +109,7 @@ struct HalfEngine {
             for (int x = 0; x < 4; ++x) acc[i][x] = 0.f;
         c = a.scale * 1.44269504088896341f;
         for (int h = kwarp; h < HW; h += kwarps) {
-            float4 x[DC / 128 ? DC / 128 : 1];
+            float4 x[(DC + 127) / 128];
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < (DC + 127) / 128; ++i) {
@@ -235,10 +237,10 @@ struct HalfEngine {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         top = fmaxf(top, m);
         const float ref = top == -INFINITY ? 0.f : top;
-        fade = exp2f(m - ref);
+        fade = pa_exp2(m - ref);
         m = top;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = exp2f(s[i] - ref) * SCALE;
+        for (int i = 0; i < 4; ++i) s[i] = pa_exp2(s[i] - ref) * SCALE;
         l = l * fade + ((s[0] + s[1]) + (s[2] + s[3]));
     }
 
@@ -290,9 +292,11 @@ struct HalfEngine {
 
 template <typename T, typename C, bool WIDE>
 cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
-    if (a.dh <= 64) return launch_paged_attn<HalfEngine<T, C, 64, WIDE>>(a, s);
-    if (a.dh <= 128) return launch_paged_attn<HalfEngine<T, C, 128, WIDE>>(a, s);
-    return launch_paged_attn<HalfEngine<T, C, 256, WIDE>>(a, s);
+    if (a.dh <= 64) return launch_paged_attn<HalfEngine<T, C, 64, WIDE, 1>, HalfEngine<T, C, 64, WIDE, 2>>(a, s);
+    if (a.dh <= 96) return launch_paged_attn<HalfEngine<T, C, 96, WIDE, 1>, HalfEngine<T, C, 96, WIDE, 2>>(a, s);
+    if (a.dh <= 128) return launch_paged_attn<HalfEngine<T, C, 128, WIDE, 1>, HalfEngine<T, C, 128, WIDE, 2>>(a, s);
+    if (a.dh <= 192) return launch_paged_attn<HalfEngine<T, C, 192, WIDE, 1>, HalfEngine<T, C, 192, WIDE, 1>>(a, s);
+    return launch_paged_attn<HalfEngine<T, C, 256, WIDE, 1>, HalfEngine<T, C, 256, WIDE, 1>>(a, s);
 }
 
 template <typename T, typename C>
@@ -303,13 +307,5 @@ cudaError_t by_alignment(const PagedAttnArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
-
-cudaError_t attn_decode_paged_half(const PagedAttnArgs& a, int act, int cache, cudaStream_t s) {
-    if (act == ELEM_F32 && cache == ELEM_F16) return by_alignment<float, __half>(a, s);
-    if (act == ELEM_F32 && cache == ELEM_BF16) return by_alignment<float, __nv_bfloat16>(a, s);
-    if (act == ELEM_F16 && cache == ELEM_F16) return by_alignment<__half, __half>(a, s);
-    if (act == ELEM_BF16 && cache == ELEM_BF16) return by_alignment<__nv_bfloat16, __nv_bfloat16>(a, s);
-    return cudaErrorInvalidValue;
-}
 
 }  // namespace krk

@@ -331,8 +331,8 @@ def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000
     return q_out
 
 
-def attn_paged_work_floats(b: int, hq: int, hkv: int, dh: int, max_len: int) -> int:
-    return int(lib.krk_attn_paged_work_floats(b, hq, hkv, dh, max_len))
+def attn_paged_work_floats(b: int, hq: int, hkv: int, dh: int, max_len: int, window: int = 0) -> int:
+    return int(lib.krk_attn_paged_work_floats(b, hq, hkv, dh, max_len, window))
 
 
 def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, window: int = 0, max_len: int = 0,
@@ -360,7 +360,7 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
     cap = width * page_size
     bound = max_len if 0 < max_len < cap else cap
     if work is None:
-        need = lib.krk_attn_paged_work_floats(b, hq, hkv, dh, bound)
+        need = lib.krk_attn_paged_work_floats(b, hq, hkv, dh, bound, window)
         work_at = 0
         if need:
             work = torch.empty(need, device=dev, dtype=torch.float32)

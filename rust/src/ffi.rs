@@ -179,7 +179,8 @@ extern "C" {
                                       rot_dim: c_int, num_pages: c_int, page_size: c_int, theta: c_float,
                                       stream: *mut c_void) -> c_int;
     /// Returns a size, not a status.
-    pub fn krk_attn_paged_work_floats(b: c_int, hq: c_int, hkv: c_int, dh: c_int, max_len: c_int) -> usize;
+    pub fn krk_attn_paged_work_floats(b: c_int, hq: c_int, hkv: c_int, dh: c_int, max_len: c_int, window: c_int)
+                                      -> usize;
     pub fn krk_k_attn_decode_paged(q: *mut c_void, q_sb: i64, q_sh: i64, dtype: c_int, kc: *mut c_void,
                                    vc: *mut c_void, c_sp: i64, c_st: i64, c_sh: i64, cache_type: c_int,
                                    table: *const i32, table_ld: i64, width: c_int, num_pages: c_int,

@@ -308,9 +308,10 @@ def test_attention_is_repeatable_and_the_bound_only_sizes_it(act, cache):
 
 
 def test_scratch_that_is_too_small_is_refused():
-    pool = Pool([6400], 2, 64, 16, F32, seed=2)
+    pool = Pool([64000], 2, 64, 16, F32, seed=2)
     q = torch.randn(1, 4, 64, device=DEV)
-    need = K.attn_paged_work_floats(1, 4, 2, 64, 6400)
+    need = K.attn_paged_work_floats(1, 4, 2, 64, 64000)
+    assert need
     for work in (torch.empty(need - 1, device=DEV), torch.empty(need + 1, device=DEV)[1:]):
         with pytest.raises(KrikilError, match="work"):
             K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=work)

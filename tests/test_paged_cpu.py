@@ -97,9 +97,10 @@ def test_empty_steps_are_done_at_once():
 
 def test_sizes_of_the_attention_scratch():
     f = lib.krk_attn_paged_work_floats
-    assert f(4, 8, 8, 64, 100000) > 0 and f(4, 8, 8, 64, 1) == 0  # a short bound needs none
-    for bad in ((0, 8, 8, 64, 9999), (4, 8, 3, 64, 9999), (4, 8, 8, 62, 9999), (4, 0, 1, 64, 9999),
-                (4, 8, 0, 64, 9999), (4, 8, 8, 64, -1)):
+    assert f(4, 8, 8, 64, 100000, 0) > 0
+    assert f(4, 8, 8, 64, 1, 0) == 0 and f(4, 8, 8, 64, 100000, 100) == 0  # few keys need none
+    for bad in ((0, 8, 8, 64, 9999, 0), (4, 8, 3, 64, 9999, 0), (4, 8, 8, 62, 9999, 0), (4, 0, 1, 64, 9999, 0),
+                (4, 8, 0, 64, 9999, 0), (4, 8, 8, 64, -1, 0), (4, 8, 8, 64, 9999, -1)):
         assert f(*bad) == 0
 
 
