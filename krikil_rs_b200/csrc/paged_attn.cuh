@@ -35,7 +35,8 @@ constexpr int PA_THREADS = 128, PA_WARPS = 4;
 constexpr int PA_UNIT = 64;          // keys of one unit of work
 constexpr int PA_CLUSTER = 8;        // blocks of a cluster, at most
 constexpr int PA_PART_UNITS = 2;     // units of a block down to which clusters grow
-constexpr int PA_CLUSTER_UNITS = 12; // units of a block up to which clusters are used
+constexpr int PA_FULL_UNITS = 16;    // units of a block up to which clusters are used when they fill the device,
+constexpr int PA_FEW_UNITS = 4;      // and when they do not
 constexpr int PA_JOIN = 512;         // threads of a join's block, at most
 constexpr int PA_MAX_BLOCKS = 592;   // blocks of a wave: four on each of 148 SMs
 constexpr int PA_MAX_ROWS = 32;      // query heads of a piece, at most
@@ -56,6 +57,7 @@ struct PagedShape {
     int side, groups;
     int per_kv;   // pieces for the query heads of one cache head
     int rows;     // query heads of a piece of one cache head
+    int extra;    // units that a piece counts for beyond its own when work is shared out
     int cluster;  // blocks that share a piece, 0: shares of the whole batch
 };
 
@@ -79,20 +81,29 @@ KRK_DEV int pa_units(int n, int first) {
     return max(1, (keys + PA_UNIT - 1) / PA_UNIT);
 }
 
-// The first unit of this block's share: its request and its place among the
-// request's units over all heads; and the share's size.  All threads call it.
+// total * i / n, in 32 bits where they do.
+KRK_DEV long long pa_part(long long total, long long i, long long n) {
+    if (total < (1 << 21)) return (unsigned)total * (unsigned)i / (unsigned)n;  // i, n <= PA_MAX_BLOCKS
+    return total * i / n;
+}
+
+// Beginning and ending a piece costs a block about as much as a few units of one
+// cache head, so each piece counts for that much more: `extra` places come before
+// its units'.  This is the first place of a block's share -- its request and its
+// place in the request's pieces -- and the share's size.  All threads call it.
 struct PagedShare {
     int b;
     long long at, size;
 };
-KRK_DEV PagedShare pa_share(const PagedAttnArgs& a, int pieces, PagedShare* out, long long* warp_sums) {
+KRK_DEV PagedShare pa_share(const PagedAttnArgs& a, int pieces, int extra, PagedShare* out,
+                            long long* warp_sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = (a.B + PA_THREADS - 1) / PA_THREADS;
     const int b0 = min(a.B, tid * each), b1 = min(a.B, b0 + each);
     long long mine = 0;
     for (int b = b0; b < b1; ++b) {
         const int n = pa_len(a, b);
-        mine += (long long)pa_units(n, pa_first(a, n)) * pieces;
+        mine += (long long)(pa_units(n, pa_first(a, n)) + extra) * pieces;
     }
     long long upto = mine;
 #pragma unroll
@@ -109,14 +120,14 @@ KRK_DEV PagedShare pa_share(const PagedAttnArgs& a, int pieces, PagedShare* out,
     }
     // no empty share lies between two that have work: the join counts on neighbours
     const long long shares = min(total, (long long)gridDim.x), mine_at = min((long long)blockIdx.x, shares);
-    const long long s = total * mine_at / shares, e = total * min(mine_at + 1, shares) / shares;
+    const long long s = pa_part(total, mine_at, shares), e = pa_part(total, min(mine_at + 1, shares), shares);
     long long before = upto - mine;
     if (tid == 0 && s == e) *out = PagedShare{0, 0, 0};
     if (s < e && s >= before && s < upto) {
         int b = b0;
         for (;; ++b) {
             const int n = pa_len(a, b);
-            const long long u = (long long)pa_units(n, pa_first(a, n)) * pieces;
+            const long long u = (long long)(pa_units(n, pa_first(a, n)) + extra) * pieces;
             if (s < before + u) break;
             before += u;
         }
@@ -294,143 +305,150 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
         share.b = blockIdx.x / sh.cluster / pieces;
     } else {
         pdl_trigger();
-        share = pa_share(a, pieces, &share_out, warp_sums);
+        share = pa_share(a, pieces, sh.extra, &share_out, warp_sums);
     }
     int b = share.b, n = pa_len(a, b), first = pa_first(a, n), units = pa_units(n, first);
+    int piece, at = 0, unit, take;
     if (sh.cluster) {  // no unit for some blocks of a short request's cluster
-        const int u0 = (int)((long long)units * rank / sh.cluster);
-        share.at = (long long)(blockIdx.x / sh.cluster % pieces) * units + u0;
-        share.size = (int)((long long)units * (rank + 1) / sh.cluster) - u0;
-    }
-    int piece = (int)(share.at / units), unit = (int)(share.at % units);
-    if (sh.cluster) {  // (the place after a piece's last unit still belongs to it)
         piece = blockIdx.x / sh.cluster % pieces;
-        unit = (int)(share.at - (long long)piece * units);
+        unit = (int)((long long)units * rank / sh.cluster);
+        take = (int)((long long)units * (rank + 1) / sh.cluster) - unit;
+        share.size = 1;
+    } else {
+        piece = (int)(share.at / (units + sh.extra));
+        at = (int)(share.at % (units + sh.extra));
     }
     long long left = share.size;
     int2 rec = make_int2(-1, -1);
 
-    while (left > 0 || sh.cluster) {
-        const int take = (int)min((long long)(units - unit), left);
-        const int hk0 = piece / sh.per_kv * sh.side, head0 = piece % sh.per_kv * sh.rows;  // head0: within G
-        const int hk = hk0 + set / sh.groups, head = head0 + set % sh.groups * HW;
-        const int base = first & ~(PA_ALIGN - 1);
-        const int k0 = base + unit * PA_UNIT, k1 = min(n, base + (unit + take) * PA_UNIT);
-        const int32_t* row = a.table + b * a.table_ld;
-        const C* kc = (const C*)a.kc + hk * a.c_sh;
-        const C* vc = (const C*)a.vc + hk * a.c_sh;
+    while (left > 0) {
+        if (!sh.cluster) {
+            const int places = (int)min((long long)(units + sh.extra - at), left);
+            unit = max(0, at - sh.extra);
+            take = max(0, at + places - sh.extra) - unit;
+            left -= places;
+        }
+        if (sh.cluster || take > 0) {
+            const int hk0 = piece / sh.per_kv * sh.side, head0 = piece % sh.per_kv * sh.rows;  // head0: within G
+            const int hk = hk0 + set / sh.groups, head = head0 + set % sh.groups * HW;
+            const int base = first & ~(PA_ALIGN - 1);
+            const int k0 = base + unit * PA_UNIT, k1 = min(n, base + (unit + take) * PA_UNIT);
+            const int32_t* row = a.table + b * a.table_ld;
+            const C* kc = (const C*)a.kc + hk * a.c_sh;
+            const C* vc = (const C*)a.vc + hk * a.c_sh;
 
-        E e;
-        int key = k0 + kwarp * KT;
-        const int step = kwarps * KT;
-        // the first tiles' pages, then the queries while they are on their way
-        if (!early) {
+            E e;
+            int key = k0 + kwarp * KT;
+            const int step = kwarps * KT;
+            // the first tiles' pages, then the queries while they are on their way
+            if (!early) {
 #pragma unroll
-            for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step);
-        }
-        e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, min(HW, G - head), qs, lane, kwarp,
-               kwarps);
-        if (E::Q_BYTES) pa_group_sync(set, kwarps);
-        if (key < k1) {
-            unsigned mask[S + 1];
+                for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step);
+            }
+            e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, min(HW, G - head), qs, lane, kwarp,
+                   kwarps);
+            if (E::Q_BYTES) pa_group_sync(set, kwarps);
+            if (key < k1) {
+                unsigned mask[S + 1];
 #pragma unroll
-            for (int i = 0; i < S; ++i) {
-                const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
-                mask[i] = t.mask;
-                if (key + i * step < k1) e.issue(a, kc, t, ring_at + i * HALF, lane);
-                cp_async_commit();
-                if (key + i * step < k1) e.issue(a, vc, t, ring_at + (S + i) * HALF, lane);
-                cp_async_commit();
-            }
-            int page = pages[S];
-            for (int slot = 0;; slot = slot + 1 == S ? 0 : slot + 1) {
-                const int ahead = key + S * step;
-                cp_async_wait<2 * S - 1>();
-                __syncwarp();
-                e.scores(qs, ring + slot * HALF, lane);
-                __syncwarp();
-                const PagedTile t = pa_tile<KT>(a, page, ahead, first, k1);
-                mask[S] = t.mask;
-                if (ahead < k1) e.issue(a, kc, t, ring_at + slot * HALF, lane);
-                cp_async_commit();
-                page = pa_page<KT>(a, row, ahead + step);
-                e.weigh(mask[0], lane);
-                cp_async_wait<2 * S - 1>();
-                __syncwarp();
-                e.values(ring + (S + slot) * HALF, lane);
-                key += step;
-                if (key >= k1) break;
-                __syncwarp();
-                if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * HALF, lane);
-                cp_async_commit();
+                for (int i = 0; i < S; ++i) {
+                    const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
+                    mask[i] = t.mask;
+                    if (key + i * step < k1) e.issue(a, kc, t, ring_at + i * HALF, lane);
+                    cp_async_commit();
+                    if (key + i * step < k1) e.issue(a, vc, t, ring_at + (S + i) * HALF, lane);
+                    cp_async_commit();
+                }
+                int page = pages[S];
+                for (int slot = 0;; slot = slot + 1 == S ? 0 : slot + 1) {
+                    const int ahead = key + S * step;
+                    cp_async_wait<2 * S - 1>();
+                    __syncwarp();
+                    e.scores(qs, ring + slot * HALF, lane);
+                    __syncwarp();
+                    const PagedTile t = pa_tile<KT>(a, page, ahead, first, k1);
+                    mask[S] = t.mask;
+                    if (ahead < k1) e.issue(a, kc, t, ring_at + slot * HALF, lane);
+                    cp_async_commit();
+                    page = pa_page<KT>(a, row, ahead + step);
+                    e.weigh(mask[0], lane);
+                    cp_async_wait<2 * S - 1>();
+                    __syncwarp();
+                    e.values(ring + (S + slot) * HALF, lane);
+                    key += step;
+                    if (key >= k1) break;
+                    __syncwarp();
+                    if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * HALF, lane);
+                    cp_async_commit();
 #pragma unroll
-                for (int i = 0; i < S; ++i) mask[i] = mask[i + 1];
-            }
-        }
-        __syncwarp();  // the warp's sums go where its tiles were
-        e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
-        __syncthreads();
-        // each query head's factors for its warps' sums
-        const int rows = sh.side * sh.rows;
-        if (tid < sets * HW) {
-            const int w0 = tid / HW, h = tid % HW, in_g = w0 % sh.groups * HW + h;
-            float top = -INFINITY, total = 0.f;
-            for (int w = w0; w < PA_WARPS; w += sets) top = fmaxf(top, sm[w][h]);
-            for (int w = w0; w < PA_WARPS; w += sets) {
-                const float f = top == -INFINITY ? (sl[w][h] == 0.f ? 0.f : sl[w][h]) : pa_exp2(sm[w][h] - top);
-                sf[w][h] = f;
-                total = fmaf(f, sl[w][h], total);
-            }
-            if (in_g < sh.rows && head0 + in_g < G) {
-                if (sh.cluster > 1) {
-                    sums[tid] = make_float2(top, total);
-                } else if (take == units) {
-                    const float inv = total == 0.f ? 0.f : 1.0f / total;
-                    for (int w = w0; w < PA_WARPS; w += sets) sf[w][h] *= inv;
-                    if (a.lse)
-                        a.lse[(long long)b * a.Hq + (long long)(hk0 + w0 / sh.groups) * G + head0 + in_g] =
-                            (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
-                } else {
-                    parts.ml[((long long)blockIdx.x * 2 + (unit == 0)) * rows + w0 / sh.groups * sh.rows + in_g] =
-                        make_float2(top, total);
+                    for (int i = 0; i < S; ++i) mask[i] = mask[i + 1];
                 }
             }
-        }
-        __syncthreads();
-        const int n4 = a.dh / 4;
-        for (int i = tid; i < rows * n4; i += PA_THREADS) {
-            const int r = i / n4, d = (i - r * n4) * 4, s = r / sh.rows, in_g = r - s * sh.rows;
-            if (head0 + in_g >= G) continue;
-            const int w0 = s * sh.groups + in_g / HW, h = in_g % HW;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = w0; w < PA_WARPS; w += sets) {
-                const float f = sf[w][h];
-                const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * HALF + (h * LD + d) * 4);
-                o.x = fmaf(f, x.x, o.x);
-                o.y = fmaf(f, x.y, o.y);
-                o.z = fmaf(f, x.z, o.z);
-                o.w = fmaf(f, x.w, o.w);
+            __syncwarp();  // the warp's sums go where its tiles were
+            e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
+            __syncthreads();
+            // each query head's factors for its warps' sums
+            const int rows = sh.side * sh.rows;
+            if (tid < sets * HW) {
+                const int w0 = tid / HW, h = tid % HW, in_g = w0 % sh.groups * HW + h;
+                float top = -INFINITY, total = 0.f;
+                for (int w = w0; w < PA_WARPS; w += sets) top = fmaxf(top, sm[w][h]);
+                for (int w = w0; w < PA_WARPS; w += sets) {
+                    const float f = top == -INFINITY ? (sl[w][h] == 0.f ? 0.f : sl[w][h]) : pa_exp2(sm[w][h] - top);
+                    sf[w][h] = f;
+                    total = fmaf(f, sl[w][h], total);
+                }
+                if (in_g < sh.rows && head0 + in_g < G) {
+                    if (sh.cluster > 1) {
+                        sums[tid] = make_float2(top, total);
+                    } else if (take == units) {
+                        const float inv = total == 0.f ? 0.f : 1.0f / total;
+                        for (int w = w0; w < PA_WARPS; w += sets) sf[w][h] *= inv;
+                        if (a.lse)
+                            a.lse[(long long)b * a.Hq + (long long)(hk0 + w0 / sh.groups) * G + head0 + in_g] =
+                                (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
+                    } else {
+                        parts.ml[((long long)blockIdx.x * 2 + (unit == 0)) * rows + w0 / sh.groups * sh.rows + in_g] =
+                            make_float2(top, total);
+                    }
+                }
             }
-            if (sh.cluster > 1)  // over the first of the warps' sums, which nobody else reads
-                *reinterpret_cast<float4*>(smem + (size_t)w0 * 2 * S * HALF + (h * LD + d) * 4) = o;
-            else if (take == units)
-                store4((T*)a.out + b * a.o_sb + ((long long)(hk0 + s) * G + head0 + in_g) * a.o_sh + d, o);
-            else
-                *reinterpret_cast<float4*>(
-                    parts.acc + (((long long)blockIdx.x * 2 + (unit == 0)) * rows + r) * a.dh + d) = o;
-        }
-        if (sh.cluster) {
-            if (sh.cluster > 1) {
-                pa_cluster_sync();
-                pa_join_cluster<E>(a, sh, smem, sums, b, hk0, head0, rank);
-                pa_cluster_sync();  // the others may still read this block's sums
+            __syncthreads();
+            const int n4 = a.dh / 4;
+            for (int i = tid; i < rows * n4; i += PA_THREADS) {
+                const int r = i / n4, d = (i - r * n4) * 4, s = r / sh.rows, in_g = r - s * sh.rows;
+                if (head0 + in_g >= G) continue;
+                const int w0 = s * sh.groups + in_g / HW, h = in_g % HW;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int w = w0; w < PA_WARPS; w += sets) {
+                    const float f = sf[w][h];
+                    const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * HALF + (h * LD + d) * 4);
+                    o.x = fmaf(f, x.x, o.x);
+                    o.y = fmaf(f, x.y, o.y);
+                    o.z = fmaf(f, x.z, o.z);
+                    o.w = fmaf(f, x.w, o.w);
+                }
+                if (sh.cluster > 1)  // over the first of the warps' sums, which nobody else reads
+                    *reinterpret_cast<float4*>(smem + (size_t)w0 * 2 * S * HALF + (h * LD + d) * 4) = o;
+                else if (take == units)
+                    store4((T*)a.out + b * a.o_sb + ((long long)(hk0 + s) * G + head0 + in_g) * a.o_sh + d, o);
+                else
+                    *reinterpret_cast<float4*>(
+                        parts.acc + (((long long)blockIdx.x * 2 + (unit == 0)) * rows + r) * a.dh + d) = o;
             }
-            return;
+            if (sh.cluster) {
+                if (sh.cluster > 1) {
+                    pa_cluster_sync();
+                    pa_join_cluster<E>(a, sh, smem, sums, b, hk0, head0, rank);
+                    pa_cluster_sync();  // the others may still read this block's sums
+                }
+                return;
+            }
+            if (take != units) (unit == 0 ? rec.y : rec.x) = b * pieces + piece;
+            __syncthreads();  // the next piece's tiles go where this one's sums were
         }
-        if (take != units) (unit == 0 ? rec.y : rec.x) = b * pieces + piece;
-        left -= take;
         if (left <= 0) break;
-        unit = 0;
+        at = 0;
         if (++piece == pieces) {
             piece = 0;
             ++b;
@@ -438,7 +456,6 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             first = pa_first(a, n);
             units = pa_units(n, first);
         }
-        __syncthreads();  // the next piece's tiles go where this one's sums were
     }
     if (tid == 0) parts.rec[blockIdx.x] = rec;
 }
@@ -535,13 +552,16 @@ __global__ void __launch_bounds__(PA_JOIN) paged_join_kernel(const PagedAttnArgs
 
 // Blocks of a cluster for pieces of at most `bound` keys, 0: shares.  Clusters
 // grow while their blocks have more than PA_PART_UNITS units and all fit in a
-// wave of three a multiprocessor.
+// wave of three a multiprocessor; they are used for few units a block (bf16
+// 32 x 32/8 x 128: 29 us in clusters and 35 us in shares of 1000 keys each, 94
+// and 93 us of 4000; 1 x 32/8 x 128 of 8000 keys, when they cannot fill the
+// device: 25 and 20 us).
 inline int pa_clusters(long long items, int bound, int sms) {
     const int units = (bound + PA_UNIT - 1) / PA_UNIT;
     if (items > 3LL * sms) return 0;
     int n = 1;
     while (n < PA_CLUSTER && units > PA_PART_UNITS * n && items * 2 * n <= 3LL * sms) n *= 2;
-    return units <= PA_CLUSTER_UNITS * n ? n : 0;
+    return units <= (items * n >= sms ? PA_FULL_UNITS : PA_FEW_UNITS) * n ? n : 0;
 }
 inline int pa_bound(int max_len, int window) {  // of a piece's keys
     return window > 0 && window < max_len ? window + PA_ALIGN : max_len;
@@ -553,7 +573,7 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     static_assert(E::HW * (E::DC + 4) * 4 <= 2 * E::SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
     const int G = a.Hq / a.Hkv, sms = paged_sm_count();
     if (sms <= 0) return cudaErrorInvalidDevice;
-    PagedShape sh{1, 1, 1, 0, 0};
+    PagedShape sh{1, 1, 1, 0, 0, 0};
     while (sh.groups < PA_WARPS && sh.groups * E::HW < G) sh.groups *= 2;
     sh.per_kv = (G + sh.groups * E::HW - 1) / (sh.groups * E::HW);
     sh.rows = G < sh.groups * E::HW ? G : sh.groups * E::HW;
@@ -592,6 +612,9 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
         sh.side *= 2;
         items /= 2;
     }
+    // (of 0, 2 and 6 for one head: bf16 32 x 32/8 x 128 of 1 .. 2000 keys 48, 35 and 38 us, of 2000 each 55, 55 and
+    // 57 us; the same of 0, 1 and 2 for two, and more than 0 for four loses 2% where the keys are many)
+    sh.extra = sh.side == 1 ? 2 : sh.side == 2 ? 1 : 0;
     const int blocks = items * units < slots ? (int)(items * units) : slots, rows = sh.side * sh.rows;
     PagedParts parts;
     parts.acc = a.work;
