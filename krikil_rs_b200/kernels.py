@@ -191,23 +191,18 @@ def greedy(logits: torch.Tensor, seen: Optional[torch.Tensor] = None, penalty: f
 
 # ------------------------------------------------------ paged key-value cache
 # The wrappers' checks are a large part of a small call's time: each tensor's
-# type, device, shape and strides are read once, and scratch and small outputs
-# come from one allocation.
+# type, device, shape and strides are read once, and small outputs come from one
+# allocation.
 _TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = torch.cuda.current_device
 
 
-def _call_on(dev, fn, *args) -> None:
-    """fn(*args, stream) on dev's current stream, with dev current."""
-    index = dev.index
-    if index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, _raw_stream(index))
-    if status:
-        check(status)
+def _elsewhere(dev, fn, *args) -> int:
+    """fn(*args, stream) on dev's current stream with dev current, when another device is."""
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev.index))
 
 
 def _cuda_device(t):
@@ -216,12 +211,16 @@ def _cuda_device(t):
     return t.device
 
 
-def _elems(t, dims, dev, name):
-    """(type, shape, strides) of a float tensor whose last dimension is dense."""
+def _not_elems(name, dims, dev):
+    return ValueError(f"{name}: expected a float32, float16 or bfloat16 tensor of {dims} dimensions on {dev} whose "
+                      "last dimension is dense")
+
+
+def _elems3(t, dev, name):
+    """(type, shape, strides) of a float tensor [., ., dh] whose last dimension is dense."""
     kind, shape, strides = _TYPES.get(t.dtype), t.shape, t.stride()
-    if kind is None or len(shape) != dims or (strides[-1] != 1 and shape[-1] > 1) or t.device != dev:
-        raise ValueError(f"{name}: expected a float32, float16 or bfloat16 tensor of {dims} dimensions on {dev} "
-                         "whose last dimension is dense")
+    if kind is None or len(shape) != 3 or (strides[2] != 1 and shape[2] > 1) or t.device != dev:
+        raise _not_elems(name, 3, dev)
     return kind, shape, strides
 
 
@@ -233,14 +232,19 @@ def _ints(t, n, dev, name) -> int:
 
 
 def _table(t, dev):
+    """(rows, width, row stride) of a page table."""
     shape, strides = t.shape, t.stride()
     if t.dtype != torch.int32 or len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or t.device != dev:
         raise ValueError(f"table: expected an int32 [requests, pages] tensor on {dev} with dense rows")
-    return shape, max(strides[0], shape[1])
+    width, ld = shape[1], strides[0]
+    return shape[0], width, ld if ld > width else width
 
 
 def _pool(kc, vc, dev):
-    kind, shape, strides = _elems(kc, 4, dev, "kc")
+    """(type, shape, strides) of the two caches."""
+    kind, shape, strides = _TYPES.get(kc.dtype), kc.shape, kc.stride()
+    if kind is None or len(shape) != 4 or (strides[3] != 1 and shape[3] > 1) or kc.device != dev:
+        raise _not_elems("kc", 4, dev)
     if vc.dtype != kc.dtype or vc.shape != shape or vc.stride() != strides or vc.device != dev:
         raise ValueError("kc and vc: expected the same type, device, shape and strides")
     return kind, shape, strides
@@ -258,21 +262,33 @@ def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int
     not fit, in which case nothing was taken.  lens_out and free_count_out may be
     the inputs; they and the others are new tensors when not given."""
     dev = _cuda_device(table)
-    (b, width), ld = _table(table, dev)
+    b, width, ld = _table(table, dev)
     new_at, lens_at = _ints(new_tokens, b, dev, "new_tokens"), _ints(lens, b, dev, "lens")
     pages = free_pages.numel()
     free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
     padded = -rows % 4 + rows
-    buf = torch.empty(2 * padded + 2 * b + 3, device=dev, dtype=torch.int32)
-    positions, _, slots, _, cu, lens_new, count_new, status = buf.split(
-        [rows, padded - rows, rows, padded - rows, b + 1, b, 1, 1])
+    buf = lens.new_empty(2 * padded + 2 * b + 3)
+    positions, _, slots, _, cu, lens_new, count_new, status = buf.unsafe_split_with_sizes(
+        (rows, padded - rows, rows, padded - rows, b + 1, b, 1, 1))
+    at = buf.data_ptr()
+    cu_at = at + 8 * padded
     if lens_out is None:
-        lens_out = lens_new
+        lens_out, lens_out_at = lens_new, cu_at + 4 * b + 4
+    else:
+        lens_out_at = _ints(lens_out, b, dev, "lens_out")
     if free_count_out is None:
-        free_count_out = count_new
-    _call_on(dev, lib.krk_k_kv_page_plan, new_at, lens_at, table.data_ptr(), ld, b, width, free_at, count_at, pages,
-             page_size, _ints(lens_out, b, dev, "lens_out"), _ints(free_count_out, 1, dev, "free_count_out"),
-             cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), rows, status.data_ptr())
+        free_count_out, count_out_at = count_new, cu_at + 8 * b + 4
+    else:
+        count_out_at = _ints(free_count_out, 1, dev, "free_count_out")
+    args = (new_at, lens_at, table.data_ptr(), ld, b, width, free_at, count_at, pages, page_size, lens_out_at,
+            count_out_at, cu_at, at, at + 4 * padded, rows, cu_at + 8 * b + 8)
+    index = dev.index
+    if index == _current_device():
+        rc = lib.krk_k_kv_page_plan(*args, _raw_stream(index))
+    else:
+        rc = _elsewhere(dev, lib.krk_k_kv_page_plan, *args)
+    if rc:
+        check(rc)
     return lens_out, free_count_out, cu, positions, slots, status
 
 
@@ -281,19 +297,31 @@ def kv_page_release(done, lens, table, free_pages, free_count, page_size: int, l
     back on the stack free_pages, in place, and their lengths to 0.  Returns
     (lens_out, free_count_out, status)."""
     dev = _cuda_device(table)
-    (b, width), ld = _table(table, dev)
+    b, width, ld = _table(table, dev)
     if done.dtype not in (torch.bool, torch.uint8) or done.numel() != b or done.device != dev or not done.is_contiguous():
         raise ValueError(f"done: expected a contiguous bool or uint8 tensor of {b} elements on {dev}")
     lens_at, pages = _ints(lens, b, dev, "lens"), free_pages.numel()
     free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
-    lens_new, count_new, status = torch.empty(b + 2, device=dev, dtype=torch.int32).split([b, 1, 1])
+    buf = lens.new_empty(b + 2)
+    lens_new, count_new, status = buf.unsafe_split_with_sizes((b, 1, 1))
+    at = buf.data_ptr()
     if lens_out is None:
-        lens_out = lens_new
+        lens_out, lens_out_at = lens_new, at
+    else:
+        lens_out_at = _ints(lens_out, b, dev, "lens_out")
     if free_count_out is None:
-        free_count_out = count_new
-    _call_on(dev, lib.krk_k_kv_page_release, done.data_ptr(), lens_at, table.data_ptr(), ld, b, width, free_at,
-             count_at, pages, page_size, _ints(lens_out, b, dev, "lens_out"),
-             _ints(free_count_out, 1, dev, "free_count_out"), status.data_ptr())
+        free_count_out, count_out_at = count_new, at + 4 * b
+    else:
+        count_out_at = _ints(free_count_out, 1, dev, "free_count_out")
+    args = (done.data_ptr(), lens_at, table.data_ptr(), ld, b, width, free_at, count_at, pages, page_size, lens_out_at,
+            count_out_at, at + 4 * b + 4)
+    index = dev.index
+    if index == _current_device():
+        rc = lib.krk_k_kv_page_release(*args, _raw_stream(index))
+    else:
+        rc = _elsewhere(dev, lib.krk_k_kv_page_release, *args)
+    if rc:
+        check(rc)
     return lens_out, free_count_out, status
 
 
@@ -307,27 +335,35 @@ def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000
     are left as they were).  q may be None."""
     dev = _cuda_device(k)
     ctype, (pages, page_size, hkv, dh), (c_sp, c_st, c_sh, _) = _pool(kc, vc, dev)
-    type_, shape, (k_st, k_sh, _) = _elems(k, 3, dev, "k")
-    vtype, vshape, (v_st, v_sh, _) = _elems(v, 3, dev, "v")
+    kind, shape, (k_st, k_sh, _) = _elems3(k, dev, "k")
+    vkind, vshape, (v_st, v_sh, _) = _elems3(v, dev, "v")
     t = shape[0]
-    if shape[1] != hkv or shape[2] != dh or vshape != shape or vtype != type_:
+    if shape[1] != hkv or shape[2] != dh or vshape != shape or vkind != kind:
         raise ValueError(f"expected k and v of [T, {hkv}, {dh}] and one type")
-    slots_at, positions_at = _ints(slots, t, dev, "slots"), _ints(positions, t, dev, "positions")
     hq = q_at = q_st = q_sh = o_at = o_st = o_sh = 0
     if q is not None:
-        qtype, qshape, (q_st, q_sh, _) = _elems(q, 3, dev, "q")
+        qkind, qshape, (q_st, q_sh, _) = _elems3(q, dev, "q")
         hq = qshape[1]
-        if qshape[0] != t or qshape[2] != dh or qtype != type_:
+        if qshape[0] != t or qshape[2] != dh or qkind != kind:
             raise ValueError(f"expected q of [T, heads, {dh}] and k's type")
         if q_out is None:
-            q_out = q.new_empty(qshape)
-        otype, oshape, (o_st, o_sh, _) = _elems(q_out, 3, dev, "q_out")
-        if oshape != qshape or otype != qtype:
-            raise ValueError("q_out: expected q's shape and type")
+            q_out, o_st, o_sh = q.new_empty(qshape), hq * dh, dh
+        else:
+            okind, oshape, (o_st, o_sh, _) = _elems3(q_out, dev, "q_out")
+            if oshape != qshape or okind != kind:
+                raise ValueError("q_out: expected q's shape and type")
         q_at, o_at = q.data_ptr(), q_out.data_ptr()
-    _call_on(dev, lib.krk_k_rope_kv_append_paged, q_at, q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st,
-             v_sh, type_, o_at, o_st, o_sh, kc.data_ptr(), vc.data_ptr(), c_sp, c_st, c_sh, ctype, slots_at,
-             positions_at, t, hq, hkv, dh, dh if rot_dim is None else rot_dim, pages, page_size, theta)
+    args = (q_at, q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, kind, o_at, o_st, o_sh,
+            kc.data_ptr(), vc.data_ptr(), c_sp, c_st, c_sh, ctype, _ints(slots, t, dev, "slots"),
+            _ints(positions, t, dev, "positions"), t, hq, hkv, dh, dh if rot_dim is None else rot_dim, pages,
+            page_size, theta)
+    index = dev.index
+    if index == _current_device():
+        rc = lib.krk_k_rope_kv_append_paged(*args, _raw_stream(index))
+    else:
+        rc = _elsewhere(dev, lib.krk_k_rope_kv_append_paged, *args)
+    if rc:
+        check(rc)
     return q_out
 
 
@@ -345,23 +381,25 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
     when not given).  Returns out [B, Hq, dh], or (out, lse)."""
     dev = _cuda_device(q)
     ctype, (pages, page_size, hkv, dh), (c_sp, c_st, c_sh, _) = _pool(kc, vc, dev)
-    type_, shape, (q_sb, q_sh, _) = _elems(q, 3, dev, "q")
-    b, hq, _ = shape
-    (trows, width), ld = _table(table, dev)
-    if shape[2] != dh or trows != b:
+    kind, shape, (q_sb, q_sh, _) = _elems3(q, dev, "q")
+    b, hq, qdh = shape
+    rows, width, ld = _table(table, dev)
+    if qdh != dh or rows != b:
         raise ValueError(f"expected q of [B, heads, {dh}] and a table of B rows")
-    lens_at = _ints(lens, b, dev, "lens")
     if out is None:
-        out = q.new_empty(shape)
-    otype, oshape, (o_sb, o_sh, _) = _elems(out, 3, dev, "out")
-    if oshape != shape or otype != type_:
-        raise ValueError("out: expected q's shape and type")
-    lse = torch.empty((b, hq), device=dev, dtype=torch.float32) if return_lse else None
-    cap = width * page_size
-    bound = max_len if 0 < max_len < cap else cap
+        out, o_sb, o_sh = q.new_empty(shape), hq * dh, dh
+    else:
+        okind, oshape, (o_sb, o_sh, _) = _elems3(out, dev, "out")
+        if oshape != shape or okind != kind:
+            raise ValueError("out: expected q's shape and type")
+    lse, lse_at = None, None
+    if return_lse:
+        lse = torch.empty(b, hq, device=dev, dtype=torch.float32)
+        lse_at = lse.data_ptr()
     if work is None:
-        need = lib.krk_attn_paged_work_floats(b, hq, hkv, dh, bound, window)
-        work_at = 0
+        cap = width * page_size
+        need = lib.krk_attn_paged_work_floats(b, hq, hkv, dh, max_len if 0 < max_len < cap else cap, window)
+        work_at = None
         if need:
             work = torch.empty(need, device=dev, dtype=torch.float32)
             work_at = work.data_ptr()
@@ -369,8 +407,15 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
         if work.dtype != torch.float32 or work.device != dev or not work.is_contiguous():
             raise ValueError(f"work: expected a contiguous float32 tensor on {dev}")
         need, work_at = work.numel(), work.data_ptr()
-    _call_on(dev, lib.krk_k_attn_decode_paged, q.data_ptr(), q_sb, q_sh, type_, kc.data_ptr(), vc.data_ptr(), c_sp,
-             c_st, c_sh, ctype, table.data_ptr(), ld, width, pages, page_size, lens_at, b, hq, hkv, dh,
-             dh ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), o_sb, o_sh,
-             lse.data_ptr() if return_lse else None, work_at, need)
+    args = (q.data_ptr(), q_sb, q_sh, kind, kc.data_ptr(), vc.data_ptr(), c_sp, c_st, c_sh, ctype, table.data_ptr(),
+            ld, width, pages, page_size, _ints(lens, b, dev, "lens"), b, hq, hkv, dh,
+            dh ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), o_sb, o_sh, lse_at, work_at,
+            need)
+    index = dev.index
+    if index == _current_device():
+        rc = lib.krk_k_attn_decode_paged(*args, _raw_stream(index))
+    else:
+        rc = _elsewhere(dev, lib.krk_k_attn_decode_paged, *args)
+    if rc:
+        check(rc)
     return (out, lse) if return_lse else out
