@@ -12,36 +12,24 @@ namespace {
 // ---------------------------------------------------------------- the pages
 // Planning is two prefix sums over the requests -- of their new tokens and of
 // the pages that they lack -- and then independent writes: one entry a page and
-// a position and a slot a token.  A launch is one cluster of 1 or 8 blocks, one
-// kernel for every size: each block scans all requests itself (a few KB from
-// L2), so the blocks need nothing of each other but one barrier between the
-// last read of a chunk of requests and the first write, which lets the lengths
-// be updated in place.  Small steps are bound by latency; the writes of a large
-// one are dealt evenly to the cluster's threads, which find a token's or a
-// page's request by bisecting the chunk's prefix sums.
-constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_CLUSTER = 8;
-constexpr int PLAN_ONE_BLOCK = 8192;  // writes up to which one block does it
+// a position and a slot a token, found by bisecting a chunk's prefix sums.
+// Every block scans all requests itself (a few KB from L2), so blocks need
+// nothing of each other.  A small step, bound by latency, is one block's work.
+// A large one is dealt to the whole device by a kernel that writes only what no
+// block reads, and a second kernel of one block, which scans while the first
+// one writes, then updates what both have read: the lengths and the count may
+// be updated in place.  (249,880 prompt tokens: 438 us in one block, 19 us in a
+// cluster of eight, whose stores bound it, 6.0 us so.)
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_MIN_THREADS = 128;
+constexpr int PLAN_ONE_BLOCK = 4096;  // writes up to which one block does all
+enum PlanMode { PLAN_ALL, PLAN_FILL, PLAN_COMMIT };
 
 struct PlanScratch {
     long long warp[2][PLAN_WARPS + 1];
     int bad;
     // of a chunk's requests: tokens and pages before them, what they hold, their pages so far
-    int tokens[PLAN_THREADS + 1], pages[PLAN_THREADS + 1], len[PLAN_THREADS], have[PLAN_THREADS];
+    int tokens[PLAN_THREADS], pages[PLAN_THREADS], len[PLAN_THREADS], have[PLAN_THREADS];
 };
-
-KRK_DEV unsigned cluster_blocks() {
-    unsigned n;
-    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
-    return n;
-}
-KRK_DEV unsigned cluster_rank() {
-    unsigned n;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
-    return n;
-}
-KRK_DEV void cluster_sync() {
-    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
-}
 
 // Sums of two values a thread over the block.
 KRK_DEV void block_sum2(long long& x, long long& y, PlanScratch& sc) {
@@ -56,8 +44,9 @@ KRK_DEV void block_sum2(long long& x, long long& y, PlanScratch& sc) {
         sc.warp[1][warp] = y;
     }
     __syncthreads();
-    x = sc.warp[0][lane];
-    y = sc.warp[1][lane];
+    const bool in = lane < (int)(blockDim.x >> 5);
+    x = in ? sc.warp[0][lane] : 0;
+    y = in ? sc.warp[1][lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -78,7 +67,7 @@ KRK_DEV long long block_scan(long long x, long long& total, PlanScratch& sc) {
     }
     if (lane == 31) sc.warp[0][warp] = upto;
     __syncthreads();
-    long long w = sc.warp[0][lane];
+    long long w = lane < (int)(blockDim.x >> 5) ? sc.warp[0][lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const long long y = __shfl_up_sync(0xffffffffu, w, o);
@@ -129,16 +118,18 @@ KRK_DEV void write_rows(const PagePlanArgs& a, int r0, int r1, int thread, int t
     }
 }
 
+template <int MODE>
 __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_constant__ PagePlanArgs a) {
     __shared__ PlanScratch sc;
-    const int tid = threadIdx.x, shift = a.page_shift, low = (1 << shift) - 1;
-    const int thread = cluster_rank() * PLAN_THREADS + tid, threads = cluster_blocks() * PLAN_THREADS;
+    const int tid = threadIdx.x, nt = blockDim.x, shift = a.page_shift, low = (1 << shift) - 1;
+    const int thread = blockIdx.x * nt + tid, threads = gridDim.x * nt;
+    if (MODE == PLAN_FILL) pdl_trigger();
     if (tid == 0) sc.bad = 0;
     const int count = *a.free_count;
     // what the step needs, and whether it fits
     long long tokens = 0, pages = 0;
     int err = count < 0 || count > a.num_pages ? PAGES_BAD_LENGTH : 0;
-    for (int b = tid; b < a.B; b += PLAN_THREADS) {
+    for (int b = tid; b < a.B; b += nt) {
         const long long len = a.lens[b], add = a.new_tokens[b];
         if (len < 0 || add < 0) {
             err |= PAGES_BAD_LENGTH;
@@ -155,30 +146,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_co
     if (err) atomicOr(&sc.bad, err);
     __syncthreads();
     err = sc.bad;
-    if (err) {
-        cluster_sync();  // all have read free_count and the lengths
-        for (int b = thread; b < a.B; b += threads) {
-            a.lens_out[b] = a.lens[b];
-            a.cu_new[b + 1] = 0;
-        }
-        write_rows(a, 0, a.rows, thread, threads, [](int, int, int, int* pos, int* slot) {
+    if (MODE == PLAN_COMMIT) pdl_wait();  // the other kernel has read what is written here
+    auto padding = [](int, int, int, int* pos, int* slot) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                pos[i] = 0;
-                slot[i] = -1;
-            }
-        });
-        if (thread == 0) {
-            *a.status = err;
-            a.cu_new[0] = 0;
-            *a.free_count_out = count;
+        for (int i = 0; i < 4; ++i) {
+            pos[i] = 0;
+            slot[i] = -1;
         }
-        return;
-    }
+    };
     int base_t = 0, base_p = 0;
-    for (int b0 = 0; b0 < a.B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid, n = min(PLAN_THREADS, a.B - b0);
-        const int len = tid < n ? a.lens[b] : 0, add = tid < n ? a.new_tokens[b] : 0;
+    for (int b0 = 0; b0 < a.B; b0 += nt) {
+        const int b = b0 + tid, n = min(nt, a.B - b0);
+        const int len = tid < n ? a.lens[b] : 0, add = tid < n && !err ? a.new_tokens[b] : 0;
         const int have = (int)pages_for(len, shift), lack = (int)pages_for((long long)len + add, shift) - have;
         long long total;
         const long long before = block_scan((long long)lack << 32 | (unsigned)add, total, sc);
@@ -188,56 +167,54 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_co
         sc.have[tid] = have;
         const int tt = (int)total, tp = (int)(total >> 32);
         __syncthreads();
-        cluster_sync();  // every block has read the chunk's lengths
-        if (tid < n && (tid & (cluster_blocks() - 1)) == cluster_rank()) {
+        if (MODE != PLAN_FILL && tid < n) {
             a.lens_out[b] = len + add;
             a.cu_new[b + 1] = base_t + (int)before + add;
         }
-        for (int j = thread; j < tp; j += threads) {
-            const int i = bisect(sc.pages, n, j);
-            a.table[(b0 + i) * a.table_ld + sc.have[i] + j - sc.pages[i]] = a.free_pages[count - 1 - base_p - j];
-        }
-        write_rows(a, base_t, base_t + tt, thread, threads, [&](int lo, int hi, int r, int* pos, int* slot) {
-            int i = bisect(sc.tokens, n, lo - base_t);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int at = r + k - base_t;
-                if (r + k < lo || r + k >= hi) continue;
-                while (i + 1 < n && sc.tokens[i + 1] <= at) ++i;
-                pos[k] = sc.len[i] + at - sc.tokens[i];
-                const int p = pos[k] >> shift;
-                const int page = p < sc.have[i] ? a.table[(b0 + i) * a.table_ld + p]
-                                                : a.free_pages[count - 1 - base_p - (sc.pages[i] + p - sc.have[i])];
-                slot[k] = (int)((unsigned)page << shift) + (pos[k] & low);
+        if (MODE != PLAN_COMMIT) {
+            for (int j = thread; j < tp; j += threads) {
+                const int i = bisect(sc.pages, n, j);
+                a.table[(b0 + i) * a.table_ld + sc.have[i] + j - sc.pages[i]] = a.free_pages[count - 1 - base_p - j];
             }
-        });
+            write_rows(a, base_t, base_t + tt, thread, threads, [&](int lo, int hi, int r, int* pos, int* slot) {
+                int i = bisect(sc.tokens, n, lo - base_t);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int at = r + k - base_t;
+                    if (r + k < lo || r + k >= hi) continue;
+                    while (i + 1 < n && sc.tokens[i + 1] <= at) ++i;
+                    pos[k] = sc.len[i] + at - sc.tokens[i];
+                    const int p = pos[k] >> shift;
+                    const int page = p < sc.have[i]
+                                         ? a.table[(b0 + i) * a.table_ld + p]
+                                         : a.free_pages[count - 1 - base_p - (sc.pages[i] + p - sc.have[i])];
+                    slot[k] = (int)((unsigned)page << shift) + (pos[k] & low);
+                }
+            });
+        }
         base_t += tt;
         base_p += tp;
         __syncthreads();
     }
-    write_rows(a, base_t, a.rows, thread, threads, [](int, int, int, int* pos, int* slot) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            pos[i] = 0;
-            slot[i] = -1;
-        }
-    });
-    if (thread == 0) {
-        *a.status = 0;
+    if (MODE != PLAN_COMMIT) write_rows(a, base_t, a.rows, thread, threads, padding);
+    if (MODE != PLAN_FILL && tid == 0) {
+        *a.status = err;
         a.cu_new[0] = 0;
         *a.free_count_out = count - base_p;
     }
 }
 
+template <int MODE>
 __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const __grid_constant__ PageReleaseArgs a) {
     __shared__ PlanScratch sc;
-    const int tid = threadIdx.x, shift = a.page_shift;
-    const int thread = cluster_rank() * PLAN_THREADS + tid, threads = cluster_blocks() * PLAN_THREADS;
+    const int tid = threadIdx.x, nt = blockDim.x, shift = a.page_shift;
+    const int thread = blockIdx.x * nt + tid, threads = gridDim.x * nt;
+    if (MODE == PLAN_FILL) pdl_trigger();
     if (tid == 0) sc.bad = 0;
     const int count = *a.free_count;
     long long pages = 0, unused = 0;
     int err = count < 0 || count > a.num_pages ? PAGES_BAD_LENGTH : 0;
-    for (int b = tid; b < a.B; b += PLAN_THREADS) {
+    for (int b = tid; b < a.B; b += nt) {
         if (!a.done[b]) continue;
         const long long len = a.lens[b], held = pages_for(len, shift);
         if (len < 0 || held > a.width)
@@ -250,43 +227,52 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const __grid
     if (err) atomicOr(&sc.bad, err);
     __syncthreads();
     err = sc.bad;
+    if (MODE == PLAN_COMMIT) pdl_wait();  // the other kernel has read what is written here
     int base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += PLAN_THREADS) {
-        const int b = b0 + tid, n = min(PLAN_THREADS, a.B - b0);
+    for (int b0 = 0; b0 < a.B; b0 += nt) {
+        const int b = b0 + tid, n = min(nt, a.B - b0);
         const int len = tid < n ? a.lens[b] : 0;
         const bool gone = !err && tid < n && a.done[b];
         long long total;
         const int before = (int)block_scan(gone ? pages_for(len, shift) : 0, total, sc);
         sc.pages[tid] = before;
         __syncthreads();
-        cluster_sync();  // every block has read the chunk's lengths
-        if (tid < n && (tid & (cluster_blocks() - 1)) == cluster_rank()) a.lens_out[b] = gone ? 0 : len;
-        for (int j = thread; j < (int)total; j += threads) {
-            const int i = bisect(sc.pages, n, j);
-            a.free_pages[count + base + j] = a.table[(b0 + i) * a.table_ld + j - sc.pages[i]];
-        }
+        if (MODE != PLAN_FILL && tid < n) a.lens_out[b] = gone ? 0 : len;
+        if (MODE != PLAN_COMMIT)
+            for (int j = thread; j < (int)total; j += threads) {
+                const int i = bisect(sc.pages, n, j);
+                a.free_pages[count + base + j] = a.table[(b0 + i) * a.table_ld + j - sc.pages[i]];
+            }
         base += (int)total;
         __syncthreads();
     }
-    if (thread == 0) {
+    if (MODE != PLAN_FILL && tid == 0) {
         *a.status = err;
         *a.free_count_out = count + base;
     }
 }
 
-template <typename... Args>
-cudaError_t launch_cluster(void (*kern)(Args...), bool one, cudaStream_t s, const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = one ? 1 : PLAN_CLUSTER;
-    cfg.blockDim = PLAN_THREADS;
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cfg.gridDim.x;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+// One block for `writes` entries, or fill and commit.
+template <typename Args>
+cudaError_t launch_plan(void (*all)(Args), void (*fill)(Args), void (*commit)(Args), const Args& a, long long writes,
+                        cudaStream_t s) {
+    int nt = PLAN_MIN_THREADS;
+    while (nt < PLAN_THREADS && nt < a.B) nt *= 2;
+    if (writes <= PLAN_ONE_BLOCK) {
+        all<<<1, writes > nt ? PLAN_THREADS : nt, 0, s>>>(a);
+        add_launches(1);
+        return cudaGetLastError();
+    }
+    const int sms = paged_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    // four entries a thread, in one wave at most
+    const long long blocks = (writes + 4LL * nt - 1) / (4LL * nt), wave = (long long)sms * (2048 / nt);
+    fill<<<(unsigned)(blocks < wave ? blocks : wave), nt, 0, s>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    add_launches(1);
+    PdlScope pdl(true);
+    e = launch_pdl(commit, dim3(1), dim3(nt), 0, s, a);
     if (e == cudaSuccess) add_launches(1);
     return e;
 }
@@ -522,11 +508,13 @@ cudaError_t launch_append(const RopeAppendArgs& a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t kv_page_plan(const PagePlanArgs& a, cudaStream_t s) {
-    return launch_cluster(page_plan_kernel, a.rows <= PLAN_ONE_BLOCK, s, a);
+    return launch_plan(page_plan_kernel<PLAN_ALL>, page_plan_kernel<PLAN_FILL>, page_plan_kernel<PLAN_COMMIT>, a,
+                       a.rows, s);
 }
 
 cudaError_t kv_page_release(const PageReleaseArgs& a, cudaStream_t s) {
-    return launch_cluster(page_release_kernel, (long long)a.B * a.width <= PLAN_ONE_BLOCK, s, a);
+    return launch_plan(page_release_kernel<PLAN_ALL>, page_release_kernel<PLAN_FILL>,
+                       page_release_kernel<PLAN_COMMIT>, a, (long long)a.B * a.width, s);
 }
 
 // Powers of r = theta^(-2/rot) by repeated products in extended precision:
