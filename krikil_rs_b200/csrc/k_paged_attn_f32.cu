@@ -46,19 +46,32 @@ struct F32Engine {
             }
         }
     }
-    // A lane copies what it reads itself: load i of a tile fills 512 consecutive bytes.
+    // A lane copies what it reads itself: load i of a tile fills 512 consecutive bytes.  A whole tile on one page
+    // takes an addition a copy.
     KRK_DEV void issue(const PagedAttnArgs& a, const float* base, const PagedTile& t, uint32_t to, int lane) {
         constexpr unsigned kAll = (1u << KT) - 1;
+        const int d = (lane & (LPK - 1)) * 4;
+        to += lane * 16;
+        if (t.mask == kAll && a.page_shift >= 4) {
+            const float* p = base + (t.off + (lane / LPK) * a.c_st + d);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+#pragma unroll
+                for (int i = 0; i < NL; ++i)
+                    pa_copy<16>(to + (j * NL + i) * 512, p + i * LPK * 4, d + i * LPK * 4 < a.dh);
+                p += KPL * a.c_st;
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int key = j * KPL + lane / LPK;
-            const bool seen = t.mask == kAll || (t.mask >> key & 1u);
+            const bool seen = t.mask >> key & 1u;
             const long long off = pa_key(a, t, key);
-            const float* p = seen ? base + off + (lane & (LPK - 1)) * 4 : base;
+            const float* p = seen ? base + off + d : base;
 #pragma unroll
             for (int i = 0; i < NL; ++i)
-                pa_copy<16>(to + lane * 16 + (j * NL + i) * 512, p + (seen ? i * LPK * 4 : 0),
-                            seen && ((lane & (LPK - 1)) + i * LPK) * 4 < a.dh);
+                pa_copy<16>(to + (j * NL + i) * 512, p + (seen ? i * LPK * 4 : 0), seen && d + i * LPK * 4 < a.dh);
         }
     }
 

@@ -157,13 +157,29 @@ struct HalfEngine {
     KRK_DEV void issue(const PagedAttnArgs& a, const C* base, const PagedTile& t, uint32_t to, int lane) {
         const int chunk = lane & (CPR - 1), row0 = lane / CPR;
         const bool in = chunk * 8 < a.dh, more = chunk * 8 + 4 < a.dh;
+        to += row0 * ROW;
+        if (t.mask == 0xffffu && a.page_shift >= 4) {  // a whole tile on one page: an addition a copy
+            const C* p = base + (t.off + row0 * a.c_st + chunk * 8);
+#pragma unroll
+            for (int j = 0; j < KT / RPC; ++j) {
+                const uint32_t at = to + j * RPC * ROW + (((chunk ^ row0) ^ (j * RPC & 7)) << 4);
+                if (WIDE) {
+                    pa_copy<16>(at, p, in);
+                } else {
+                    pa_copy<8>(at, p, in);
+                    pa_copy<8>(at + 8, p + 4, more);
+                }
+                p += RPC * a.c_st;
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < KT / RPC; ++j) {
             const int row = j * RPC + row0;
-            const bool seen = t.mask == 0xffffu || (t.mask >> row & 1u);
+            const bool seen = t.mask >> row & 1u;
             const long long off = pa_key(a, t, row);
             const C* p = seen ? base + off + chunk * 8 : base;
-            const uint32_t at = to + row * ROW + ((chunk ^ (row & 7)) << 4);
+            const uint32_t at = to + j * RPC * ROW + (((chunk ^ row0) ^ (j * RPC & 7)) << 4);
             if (WIDE) {
                 pa_copy<16>(at, p, seen && in);
             } else {
