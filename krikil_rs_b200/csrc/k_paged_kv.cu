@@ -285,7 +285,7 @@ cudaError_t launch_plan(void (*all)(Args), void (*fill)(Args), void (*commit)(Ar
 // loads the next row before it stores the present one.  The rows' cos and sin
 // are computed eight rows at a time, once a pair for all heads: the turns,
 // position times rate, are reduced to a fraction in 64 bits.
-constexpr int APPEND_THREADS = 256, APPEND_HEADS = 2, APPEND_BATCH = 8, APPEND_BLOCKS = 3;
+constexpr int APPEND_THREADS = 256, APPEND_HEADS = 2, APPEND_BATCH = 8, APPEND_SIDE = 8, APPEND_BLOCKS = 3;
 
 template <int BYTES>
 struct Raw;
@@ -473,7 +473,9 @@ cudaError_t launch_append_w(const RopeAppendArgs& a, cudaStream_t s) {
     AppendShape sh{1, (heads + APPEND_HEADS - 1) / APPEND_HEADS, 1};
     if (sh.lanes > APPEND_THREADS / units) sh.lanes = APPEND_THREADS / units;  // several rounds of heads
     sh.side = APPEND_THREADS / (sh.lanes * units);
-    if (sh.side > APPEND_BATCH) sh.side = APPEND_BATCH;
+    // (48 KB of cos and sin at most)
+    while (sh.side > 1 && (size_t)sh.side * APPEND_BATCH * a.rot * sizeof(float) > 48 * 1024) --sh.side;
+    if (sh.side > APPEND_SIDE) sh.side = APPEND_SIDE;
     const int sms = paged_sm_count();
     if (sms <= 0) return cudaErrorInvalidDevice;
     // One wave of blocks, each with its run of rows (16321 x 32/8 x 128 bf16: 69 us, 5.9 TB/s; 89 us with a block

@@ -456,6 +456,33 @@ def test_append_layouts_padding_and_bad_slots(act, cache, pad, dh, layout):
     assert (raw == 5.0).all()
 
 
+@pytest.mark.parametrize("act,cache,t,hq,hkv,dh", [
+    (F16, F16, 30000, 1, 1, 256), (BF16, BF16, 30011, 1, 1, 256), (F32, F32, 9001, 2, 1, 256), (F32, BF16, 40003, 0, 1, 64),
+    (BF16, BF16, 700, 128, 16, 128), (F32, F16, 601, 71, 71, 76), (F16, F16, 333, 40, 8, 192)])
+def test_append_long_runs_of_rows_and_many_heads(act, cache, t, hq, hkv, dh):
+    """Few heads, so that a block takes several rows side by side in long runs, and more heads than a block's threads
+    take at once."""
+    g = gen(t)
+    page, pages = 64, -(-t // 64)
+    q = torch.randn(t, hq, dh, generator=g, device=DEV).to(act) if hq else None
+    k, v = (torch.randn(t, hkv, dh, generator=g, device=DEV).to(act) for _ in range(2))
+    slots = torch.randperm(pages * page, generator=g, device=DEV)[:t].int()
+    slots[::17] = -1
+    positions = torch.randint(0, 10 ** 6, (t,), generator=g, device=DEV, dtype=torch.int32)
+    kc, vc = (torch.full((pages, page, hkv, dh), 9.0, device=DEV, dtype=cache) for _ in range(2))
+    keep = slots >= 0
+    out = torch.full((t, hq, dh), 3.0, device=DEV, dtype=act) if hq else None
+    assert K.rope_kv_append_paged(q, k, v, kc, vc, slots, positions, q_out=out) is out
+    if hq:
+        close(out[keep], *rotated(q[keep], positions[keep], dh))
+        assert (out[~keep] == 3.0).all()
+    at = slots[keep].long()
+    close(kc.view(-1, hkv, dh)[at], *rotated(k[keep], positions[keep], dh))
+    assert torch.equal(vc.view(-1, hkv, dh)[at], v[keep].to(cache))
+    kc.view(-1, hkv, dh)[at] = 9.0
+    assert (kc == 9.0).all()
+
+
 def test_append_stores_the_nearest_values():
     """float32 values into 16-bit caches: the values' own rounding (to even at ties, overflow to infinity), the
     last of what fits; NaN and infinities stay."""
@@ -597,7 +624,59 @@ def test_page_requests_that_do_not_fit():
     assert release([False, False], [1, 1], 5)[0] & PAGES_BAD_LENGTH
 
 
+def test_large_plans_replayed_from_a_graph():
+    """Steps of thousands of tokens and releases of thousands of pages, which take two kernels each, updating the
+    lengths and the count in place, captured once and replayed."""
+    batch, width, page, rows = 40, 400, 16, 50000
+    rng = np.random.default_rng(2)
+    books = Books(batch, width, 9000, page, seed=3)
+    d = device_books(books, batch)
+    new_d, done_d = torch.zeros(batch, device=DEV, dtype=torch.int32), torch.zeros(batch, device=DEV, dtype=torch.bool)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        released = K.kv_page_release(done_d, d["lens"], d["table"], d["free"], d["count"], page, lens_out=d["lens"],
+                                     free_count_out=d["count"])
+        planned = K.kv_page_plan(new_d, d["lens"], d["table"], d["free"], d["count"], page, rows,
+                                 lens_out=d["lens"], free_count_out=d["count"])
+    for step in range(6):
+        done = rng.random(batch) < 0.3
+        books.release(done)
+        new = [int(x) for x in rng.integers(0, 1200, batch)]
+        want = books.fits(new, rows)
+        new_d.copy_(i32(new))
+        done_d.copy_(torch.tensor(done, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert released[2].item() == 0 and planned[5].item() == want
+        p, sl = books.plan(new) if not want else ([], [])
+        assert planned[3][:len(p)].tolist() == p and planned[4][:len(p)].tolist() == sl
+        assert (planned[4][len(p):] == -1).all() and not planned[3][len(p):].any()
+        assert planned[2].tolist() == [0] + (np.cumsum(new).tolist() if not want else [0] * batch)
+        same_books(d, books)
+
+
 # ------------------------------------------------------------------ together
+def test_two_streams_at_once():
+    """Calls on two streams that share the pages, each with its own scratch and outputs, in both ways that work is
+    divided."""
+    for lens in ([700, 64, 1], [40000, 3, 9000]):
+        pool = Pool(lens, 2, 64, 16, BF16, seed=31)
+        qs = [torch.randn(3, 8, 64, generator=gen(i), device=DEV).to(BF16) for i in range(2)]
+        want = [K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens) for q in qs]
+        streams = [torch.cuda.Stream() for _ in qs]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(20):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(K.attn_decode_paged(qs[i], pool.kc, pool.vc, pool.table, pool.lens))
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 @pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
 @pytest.mark.parametrize("hq,hkv,dh,page", [(8, 8, 76, 16), (8, 2, 128, 8)])
 def test_serving_steps_of_requests_that_come_and_go(act, cache, hq, hkv, dh, page):
