@@ -29,7 +29,7 @@ struct F32Engine {
     static constexpr int BLOCKS = SLOTS == 1 ? 4 : 3;
     static constexpr float SCALE = 1.f;
 
-    float4 q[GW][NL], acc[GW][NL];
+    float2 q[GW][NL][2], acc[GW][NL][2];  // pairs for the packed multiply-adds
     float s[GW], m[GW], l[GW], fade[GW], c;
 
     KRK_DEV void init(const PagedAttnArgs& a, const float* qp, int heads, unsigned char*, int lane, int, int) {
@@ -41,8 +41,10 @@ struct F32Engine {
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
                 const int d = ((lane & (LPK - 1)) + i * LPK) * 4;
-                acc[h][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                q[h][i] = h < heads && d < a.dh ? load4(qp + h * a.q_sh + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 x = h < heads && d < a.dh ? load4(qp + h * a.q_sh + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                acc[h][i][0] = acc[h][i][1] = make_float2(0.f, 0.f);
+                q[h][i][0] = make_float2(x.x, x.y);
+                q[h][i][1] = make_float2(x.z, x.w);
             }
         }
     }
@@ -113,15 +115,13 @@ struct F32Engine {
             float x[J];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                x[j] = 0.f;
+                float2 y = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int i = 0; i < NL; ++i) {
-                    const float4 y = k[j * NL + i];
-                    x[j] = fmaf(y.x, q[h][i].x, x[j]);
-                    x[j] = fmaf(y.y, q[h][i].y, x[j]);
-                    x[j] = fmaf(y.z, q[h][i].z, x[j]);
-                    x[j] = fmaf(y.w, q[h][i].w, x[j]);
+                    y = __ffma2_rn(make_float2(k[j * NL + i].x, k[j * NL + i].y), q[h][i][0], y);
+                    y = __ffma2_rn(make_float2(k[j * NL + i].z, k[j * NL + i].w), q[h][i][1], y);
                 }
+                x[j] = y.x + y.y;
             }
             s[h] = fold(x, lane);
         }
@@ -152,22 +152,20 @@ struct F32Engine {
 #pragma unroll
         for (int h = 0; h < GW; ++h) {
 #pragma unroll
-            for (int i = 0; i < NL; ++i) {
-                acc[h][i].x *= fade[h];
-                acc[h][i].y *= fade[h];
-                acc[h][i].z *= fade[h];
-                acc[h][i].w *= fade[h];
-            }
+            for (int i = 0; i < NL; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    acc[h][i][e].x *= fade[h];
+                    acc[h][i][e].y *= fade[h];
+                }
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const float p = __shfl_sync(0xffffffffu, s[h], side + lane_of(j));
+                const float w = __shfl_sync(0xffffffffu, s[h], side + lane_of(j));
+                const float2 p = make_float2(w, w);
 #pragma unroll
                 for (int i = 0; i < NL; ++i) {
-                    const float4 y = v[j * NL + i];
-                    acc[h][i].x = fmaf(p, y.x, acc[h][i].x);
-                    acc[h][i].y = fmaf(p, y.y, acc[h][i].y);
-                    acc[h][i].z = fmaf(p, y.z, acc[h][i].z);
-                    acc[h][i].w = fmaf(p, y.w, acc[h][i].w);
+                    acc[h][i][0] = __ffma2_rn(p, make_float2(v[j * NL + i].x, v[j * NL + i].y), acc[h][i][0]);
+                    acc[h][i][1] = __ffma2_rn(p, make_float2(v[j * NL + i].z, v[j * NL + i].w), acc[h][i][1]);
                 }
             }
         }
@@ -185,7 +183,7 @@ struct F32Engine {
             }
 #pragma unroll
             for (int i = 0; i < NL; ++i) {
-                float4 o = acc[h][i];
+                float4 o = make_float4(acc[h][i][0].x, acc[h][i][0].y, acc[h][i][1].x, acc[h][i][1].y);
                 if (LPK == 16) {
                     o.x += __shfl_xor_sync(0xffffffffu, o.x, 16);
                     o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
