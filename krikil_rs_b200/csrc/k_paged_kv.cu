@@ -21,7 +21,8 @@ namespace {
 // be updated in place.  (249,880 prompt tokens: 438 us in one block, 19 us in a
 // cluster of eight, whose stores bound it, 6.0 us so.)
 constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_MIN_THREADS = 128;
-constexpr int PLAN_ONE_BLOCK = 4096;  // writes up to which one block does all
+constexpr int PLAN_ONE_BLOCK = 4096;  // writes up to which one block does all (61 requests' 7800 tokens: 8.3 us, 5.8 us
+                                      // in two kernels; 1024 requests' 4096: 7.7 and 9.4 us)
 enum PlanMode { PLAN_ALL, PLAN_FILL, PLAN_COMMIT };
 
 struct PlanScratch {

@@ -17,7 +17,9 @@
 //
 // Clusters, where latency counts: 1, 2, 4 or 8 blocks of a thread-block cluster
 // take equal parts of one piece and add up their sums through each other's shared
-// memory.  One kernel, no scratch and no look at the other requests.
+// memory.  One kernel, no scratch and no look at the other requests.  What bounds
+// it is a chain of latencies: launch, length, page, first keys, about 1 us a tile
+// of each warp, the merge (8 x 76 f32: 5.5 us of 32 keys, 9.4 us of 1000).
 //
 // Either way a block's warps take tiles of keys in turn, each with a running
 // maximum and sum, and are merged in shared memory at the end; all orders are
@@ -225,6 +227,8 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 //   finish(obuf, m, l)          accumulators, maxima and sums of the warp to shared memory
 // A warp's ring has SLOTS slots for keys and as many for values; a slot is
 // filled again as soon as the warp has read it, with no barrier beyond the warp.
+// (The same tiles held in registers, loads issued as early: f32 1024 x 8 x 76 in
+// 604 us, 271 us from a ring; bf16 128 x 32/8 x 128 in 435 us, 331 us.)
 // Adds up the sums of a cluster's blocks, each block a part of the elements.
 template <class E>
 KRK_DEV void pa_join_cluster(const PagedAttnArgs& a, const PagedShape& sh, const unsigned char* smem,
@@ -567,7 +571,8 @@ inline int pa_bound(int max_len, int window) {  // of a piece's keys
     return window > 0 && window < max_len ? window + PA_ALIGN : max_len;
 }
 
-// E2: the engine with two slots a warp, for clusters.
+// E2: the engine with two slots a warp, for clusters, whose few blocks leave room for it (bf16 32 x 32/8 x 128 of 1000
+// keys: 26.5 us, 29.7 us with one).
 template <class E, class E2>
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     static_assert(E::HW * (E::DC + 4) * 4 <= 2 * E::SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
@@ -606,7 +611,10 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int slots = sms * E::BLOCKS < PA_MAX_BLOCKS ? sms * E::BLOCKS : PA_MAX_BLOCKS;
     const long long units = (bound + PA_UNIT - 1) / PA_UNIT;
-    // With work for every block, warps take neighbouring cache heads of the same keys.
+    // With work for every block, warps take neighbouring cache heads of the same keys: a token's heads lie side by
+    // side, and rows of 304 bytes share sectors (f32 1024 x 8 x 76, 128 .. 384 keys: 245 us, 291 us with one head a
+    // block; bf16 128 x 32/8 x 128 the same either way; from 2 units a block on instead of 8, bf16 8 x 32/8 x 128 of
+    // 8000 keys takes 72 us instead of 54).
     while (sh.side * sh.groups < PA_WARPS && a.Hkv % (2 * sh.side) == 0 &&
            items / 2 * units >= PA_SIDE_UNITS * (long long)slots) {
         sh.side *= 2;
@@ -626,7 +634,7 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     add_launches(1);
     PdlScope pdl(true);
-    // large blocks for the joins of many parts
+    // large blocks for the joins of many parts (f16 1 x 16/2 x 256 of 131071 keys, 148 parts: 58 us, 63 us without)
     e = launch_pdl(paged_join_kernel<typename E::Act>, dim3(blocks, rows),
                    dim3(items * 16 <= blocks ? PA_JOIN : PA_THREADS), 0, s, a, sh, parts, blocks, E::SCALE);
     if (e == cudaSuccess) add_launches(1);

@@ -347,7 +347,7 @@ def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000
         if qshape[0] != t or qshape[2] != dh or qkind != kind:
             raise ValueError(f"expected q of [T, heads, {dh}] and k's type")
         if q_out is None:
-            q_out, o_st, o_sh = q.new_empty(qshape), hq * dh, dh
+            q_out, o_st, o_sh = q.new_empty(t, hq, dh), hq * dh, dh
         else:
             okind, oshape, (o_st, o_sh, _) = _elems3(q_out, dev, "q_out")
             if oshape != qshape or okind != kind:
@@ -387,7 +387,7 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
     if qdh != dh or rows != b:
         raise ValueError(f"expected q of [B, heads, {dh}] and a table of B rows")
     if out is None:
-        out, o_sb, o_sh = q.new_empty(shape), hq * dh, dh
+        out, o_sb, o_sh = q.new_empty(b, hq, dh), hq * dh, dh
     else:
         okind, oshape, (o_sb, o_sh, _) = _elems3(out, dev, "out")
         if oshape != shape or okind != kind:
