@@ -494,7 +494,8 @@ KRK_API int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void
  * zeros and lse -inf.  Lengths past width * page_size are cut there and
  * negative ones read as 0; keys on pages outside the pool are left out (both
  * reported by checked builds).  Cache cells past a request's length or before
- * its window are never used, whatever they hold.
+ * its window are never used, whatever they hold (16-bit rows are read in aligned
+ * 16-byte pieces, so that up to 8 bytes beside a row may be read along).
  * max_len: a bound of the lengths by which the launch is sized, 0 = width *
  * page_size; it moves the result by rounding at most.  work: 16-byte aligned
  * device scratch of krk_attn_paged_work_floats(B, Hq, Hkv, dh, that bound,

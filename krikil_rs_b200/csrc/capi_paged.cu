@@ -174,6 +174,10 @@ int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void*
     const size_t need = krk::attn_paged_work_floats(B, Hq, Hkv, dh, bound, window);
     if (need > 0 && (!work || work_floats < need || !aligned(work, 16)))
         return invalid(who, "work must be 16-byte aligned and hold " + std::to_string(need) + " floats");
+    // (the engines choose by the strides, and a dimension of one element has none)
+    if (num_pages == 1) c_sp = 0;
+    if (page_size == 1) c_st = 0;
+    if (Hkv == 1) c_sh = 0;
     const krk::PagedAttnArgs a{q, q_sb, q_sh, kc, vc, c_sp, c_st, c_sh, table, table_ld, width, num_pages, shift,
                                lens, B, Hq, Hkv, dh, scale, window,
                                bound, out, o_sb, o_sh, lse, work};

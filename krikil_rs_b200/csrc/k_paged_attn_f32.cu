@@ -34,7 +34,8 @@ struct F32Engine {
     float2 q[GW][NL][2], acc[GW][NL][2];  // pairs for the packed multiply-adds
     float s[GW], m[GW], l[GW], fade[GW], c;
 
-    KRK_DEV void init(const PagedAttnArgs& a, const float* qp, int heads, unsigned char*, int lane, int, int) {
+    KRK_DEV void init(const PagedAttnArgs& a, const float* qp, const float*, const float*, int heads, unsigned char*,
+                      int lane, int, int) {
         c = a.scale * 1.44269504088896341f;
 #pragma unroll
         for (int h = 0; h < GW; ++h) {
@@ -108,7 +109,7 @@ struct F32Engine {
         return r;
     }
 
-    KRK_DEV void scores(const unsigned char*, const unsigned char* from, int lane) {
+    KRK_DEV void scores(const unsigned char*, unsigned char* from, int lane) {
         float4 k[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const float4*>(from + lane * 16 + j * 512);

@@ -219,7 +219,7 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 }
 
 // E: an engine.  Its warp holds KT keys of a tile and HW query heads:
-//   init(a, q, heads, qs)       loads a warp's queries (or prepares them in shared memory)
+//   init(a, q, k, v, heads, qs) loads a warp's queries (or prepares them in shared memory)
 //   issue(base, tile, to)       starts the copies of a tile's keys or values to a ring slot
 //   scores(qs, from)            q . k of the slot's keys
 //   weigh(mask)                 softmax step over the visible keys of the tile
@@ -349,8 +349,8 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
 #pragma unroll
                 for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step);
             }
-            e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, min(HW, G - head), qs, lane, kwarp,
-                   kwarps);
+            e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, kc, vc, min(HW, G - head), qs,
+                   lane, kwarp, kwarps);
             if (E::Q_BYTES) pa_group_sync(set, kwarps);
             if (key < k1) {
                 unsigned mask[S + 1];

@@ -14,8 +14,9 @@
 // up to 8192 keys, 2.15 GB: 331 us, 6.5 TB/s); with few keys a call, latency
 // bounds it, and with 16 query heads a cache head, whose tiles two warps copy, L1
 // (128 heads over 8: 222 us for 168 us of bytes).  Rows that are not 16-byte
-// aligned or not a multiple of 8 elements are copied 8 bytes at a time (bf16 heads
-// of 76: 173 us for 100 us of bytes).
+// aligned, or not a multiple of 8 elements, are shifted in place when all of a
+// head's lie alike (bf16 64 x 32/8 x 76: 140 us for 100 us of bytes, 173 us when
+// they were copied 8 bytes at a time, as they still are when tokens differ).
 //
 // Precision: the products are exact and added in 32 bits, and a tile's sum is
 // folded into the float32 accumulators once a tile.  A float32 weight is the
@@ -84,8 +85,14 @@ KRK_DEV void load_matrices_t(uint32_t (&r)[4], uint32_t at) {
                  : "memory");
 }
 
-// DC: the elements of a row that are worked on, a multiple of 32 that is at least dh; SLOTS: of a warp's ring.
-template <typename T, typename C, int DC_, bool WIDE, int SLOTS_>
+// How rows lie: 8-byte pieces only; every row of a cache head at the same place within 16 bytes; all on 16 bytes.
+enum RowAlign { ROWS_NARROW, ROWS_SHIFTED, ROWS_WIDE };
+
+// DC: the elements of a row that are worked on, a multiple of 32 that is at least dh (dh + 4 for shifted rows); SLOTS:
+// of a warp's ring.  Shifted rows are copied from the 16-byte boundary before them, and everything -- queries, products,
+// results -- is moved up by the `before` elements in between; what the copies bring along of other rows is cleared in
+// the keys, where it would meet a query, and dropped with the results' columns in the values.
+template <typename T, typename C, int DC_, int ALIGN, int SLOTS_>
 struct HalfEngine {
     using Act = T;
     using Cache = C;
@@ -103,11 +110,16 @@ struct HalfEngine {
 
     float acc[NV][4];
     float s[4], m, l, c, fade;
+    int before_k, before_v;  // 0 or 4
+    int dh;
 
     // Lays the parts of the group's queries out as the first operand's registers.  Each warp of a group prepares
     // every kwarps-th head.
-    KRK_DEV void init(const PagedAttnArgs& a, const T* q, int heads, unsigned char* qs, int lane, int kwarp,
-                      int kwarps) {
+    KRK_DEV void init(const PagedAttnArgs& a, const T* q, const C* kc, const C* vc, int heads, unsigned char* qs,
+                      int lane, int kwarp, int kwarps) {
+        dh = a.dh;
+        before_k = ALIGN == ROWS_SHIFTED && (reinterpret_cast<uintptr_t>(kc) & 15) ? 4 : 0;
+        before_v = ALIGN == ROWS_SHIFTED && (reinterpret_cast<uintptr_t>(vc) & 15) ? 4 : 0;
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
@@ -120,8 +132,8 @@ struct HalfEngine {
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < (DC + 127) / 128; ++i) {
-                const int d = (i * 32 + lane) * 4;
-                x[i] = h < heads && d < a.dh ? load4(q + h * a.q_sh + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int d = (i * 32 + lane) * 4 - before_k;
+                x[i] = h < heads && d >= 0 && d < a.dh ? load4(q + h * a.q_sh + d) : make_float4(0.f, 0.f, 0.f, 0.f);
                 most = fmaxf(most, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
             }
             float up = 1.f;
@@ -163,14 +175,15 @@ struct HalfEngine {
 
     KRK_DEV void issue(const PagedAttnArgs& a, const C* base, const PagedTile& t, uint32_t to, int lane) {
         const int chunk = lane & (CPR - 1), row0 = lane / CPR;
-        const bool in = chunk * 8 < a.dh, more = chunk * 8 + 4 < a.dh;
+        const int before = ALIGN == ROWS_SHIFTED && (reinterpret_cast<uintptr_t>(base) & 15) ? 4 : 0;
+        const bool in = chunk * 8 < a.dh + before, more = chunk * 8 + 4 < a.dh;
         to += row0 * ROW;
         if (t.mask == 0xffffu && a.page_shift >= 4) {  // a whole tile on one page: an addition a copy
-            const C* p = base + (t.off + row0 * a.c_st + chunk * 8);
+            const C* p = base + (t.off + row0 * a.c_st + chunk * 8 - before);
 #pragma unroll
             for (int j = 0; j < KT / RPC; ++j) {
                 const uint32_t at = to + j * RPC * ROW + (((chunk ^ row0) ^ (j * RPC & 7)) << 4);
-                if (WIDE) {
+                if (ALIGN != ROWS_NARROW) {
                     pa_copy<16>(at, p, in);
                 } else {
                     pa_copy<8>(at, p, in);
@@ -185,9 +198,9 @@ struct HalfEngine {
             const int row = j * RPC + row0;
             const bool seen = t.mask >> row & 1u;
             const long long off = pa_key(a, t, row);
-            const C* p = seen ? base + off + chunk * 8 : base;
+            const C* p = seen ? base + off + chunk * 8 - before : base - before;
             const uint32_t at = to + j * RPC * ROW + (((chunk ^ row0) ^ (j * RPC & 7)) << 4);
-            if (WIDE) {
+            if (ALIGN != ROWS_NARROW) {
                 pa_copy<16>(at, p, seen && in);
             } else {
                 pa_copy<8>(at, p, seen && in);
@@ -196,7 +209,20 @@ struct HalfEngine {
         }
     }
 
-    KRK_DEV void scores(const unsigned char* qs, const unsigned char* from, int lane) {
+    // Clears the four elements before and behind each of the tile's keys in their first and last 16 bytes.
+    KRK_DEV void clear_edges(unsigned char* from, int lane) {
+        const int end = dh + before_k;
+        unsigned char* row = from + (lane & 15) * ROW;
+        if (lane < 16) {
+            if (before_k) *reinterpret_cast<uint2*>(row + ((lane & 7) << 4)) = make_uint2(0u, 0u);
+        } else {
+            if (end & 4) *reinterpret_cast<uint2*>(row + (((end >> 3) ^ (lane & 7)) << 4) + 8) = make_uint2(0u, 0u);
+        }
+        __syncwarp();
+    }
+
+    KRK_DEV void scores(const unsigned char* qs, unsigned char* from, int lane) {
+        if (ALIGN == ROWS_SHIFTED) clear_edges(from, lane);
         float d0[4], d1[4], e0[4], e1[4];
         const uint4* qf = reinterpret_cast<const uint4*>(qs) + lane;
         const uint32_t at = smem_addr(from) + (lane & 7) * ROW;
@@ -304,29 +330,35 @@ struct HalfEngine {
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float* o = obuf + 2 * t * (DC + 4) + i * 16 + r;
-            o[0] = acc[i][0];
-            o[DC + 4] = acc[i][1];
+            float* o = obuf + 2 * t * (DC + 4) + i * 16 + r - before_v;
+            if (ALIGN != ROWS_SHIFTED || i * 16 + r >= before_v) {
+                o[0] = acc[i][0];
+                o[DC + 4] = acc[i][1];
+            }
             o[8] = acc[i][2];
             o[DC + 12] = acc[i][3];
         }
     }
 };
 
-template <typename T, typename C, bool WIDE>
+template <typename T, typename C, int ALIGN>
 cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
-    if (a.dh <= 64) return launch_paged_attn<HalfEngine<T, C, 64, WIDE, 1>, HalfEngine<T, C, 64, WIDE, 2>>(a, s);
-    if (a.dh <= 96) return launch_paged_attn<HalfEngine<T, C, 96, WIDE, 1>, HalfEngine<T, C, 96, WIDE, 2>>(a, s);
-    if (a.dh <= 128) return launch_paged_attn<HalfEngine<T, C, 128, WIDE, 1>, HalfEngine<T, C, 128, WIDE, 2>>(a, s);
-    if (a.dh <= 192) return launch_paged_attn<HalfEngine<T, C, 192, WIDE, 1>, HalfEngine<T, C, 192, WIDE, 1>>(a, s);
-    return launch_paged_attn<HalfEngine<T, C, 256, WIDE, 1>, HalfEngine<T, C, 256, WIDE, 1>>(a, s);
+    const int width = ALIGN == ROWS_SHIFTED ? a.dh + 4 : a.dh;
+    if (width <= 64) return launch_paged_attn<HalfEngine<T, C, 64, ALIGN, 1>, HalfEngine<T, C, 64, ALIGN, 2>>(a, s);
+    if (width <= 96) return launch_paged_attn<HalfEngine<T, C, 96, ALIGN, 1>, HalfEngine<T, C, 96, ALIGN, 2>>(a, s);
+    if (width <= 128) return launch_paged_attn<HalfEngine<T, C, 128, ALIGN, 1>, HalfEngine<T, C, 128, ALIGN, 2>>(a, s);
+    if (width <= 192) return launch_paged_attn<HalfEngine<T, C, 192, ALIGN, 1>, HalfEngine<T, C, 192, ALIGN, 1>>(a, s);
+    return launch_paged_attn<HalfEngine<T, C, 256, ALIGN, 1>, HalfEngine<T, C, 256, ALIGN, 1>>(a, s);
 }
 
 template <typename T, typename C>
 cudaError_t by_alignment(const PagedAttnArgs& a, cudaStream_t s) {
-    const bool wide = a.dh % 8 == 0 && a.c_sp % 8 == 0 && a.c_st % 8 == 0 && a.c_sh % 8 == 0 &&
-                      (reinterpret_cast<uintptr_t>(a.kc) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.vc) & 15) == 0;
-    return wide ? by_width<T, C, true>(a, s) : by_width<T, C, false>(a, s);
+    const bool same = a.c_sp % 8 == 0 && a.c_st % 8 == 0;
+    const bool wide = same && a.dh % 8 == 0 && a.c_sh % 8 == 0 && (reinterpret_cast<uintptr_t>(a.kc) & 15) == 0 &&
+                      (reinterpret_cast<uintptr_t>(a.vc) & 15) == 0;
+    if (wide) return by_width<T, C, ROWS_WIDE>(a, s);
+    if (same && a.dh <= 252) return by_width<T, C, ROWS_SHIFTED>(a, s);
+    return by_width<T, C, ROWS_NARROW>(a, s);
 }
 
 }  // namespace

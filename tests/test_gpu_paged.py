@@ -234,14 +234,15 @@ def test_one_dominant_key_and_a_long_faint_tail(act, cache):
 
 
 @pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
-def test_infinities_and_nan_stay_where_they_are(act, cache):
+@pytest.mark.parametrize("dh,pad", [(64, 0), (64, 4), (76, 0), (76, 4), (120, 12)])
+def test_infinities_and_nan_stay_where_they_are(act, cache, dh, pad):
     """A NaN key reaches its own request and cache head alone; a key of score -inf gets weight 0, and a row
     of nothing but -inf scores gives zeros; an infinite value of a visible key leaves its own column not finite
     (infinite or, where the product of a weight's parts is undefined, NaN) and nothing else."""
     def make(seed):
-        return Pool([64, 90, 33, 5], 2, 64, 16, cache, seed=seed)
+        return Pool([64, 90, 33, 5], 2, dh, 16, cache, seed=seed, pad=pad)
     pool = make(7)
-    q = torch.rand(4, 4, 64, generator=gen(4), device=DEV).to(act) + 0.5
+    q = torch.rand(4, 4, dh, generator=gen(4), device=DEV).to(act) + 0.5
     clean, _ = check_attn(pool, q)
     def at(b, j):
         return int(pool.table[b, j // 16]), j % 16
@@ -255,7 +256,7 @@ def test_infinities_and_nan_stay_where_they_are(act, cache):
     pool.kc[at(2, 10)][1] = -float("inf")
     out, lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, return_lse=True)
     pool.k[2][10, 1] = -1e4  # a weight of 0 in 32 bits
-    ref, rl, tol, ltol = attn_reference(pool, q, 1 / 8)
+    ref, rl, tol, ltol = attn_reference(pool, q, 1 / math.sqrt(dh))
     # sum |q k| of the key that was moved away has no part in the others' rounding
     assert ((out.double() - ref).abs() <= tol).all() and not lse.isnan().any()
     pool = make(7)
@@ -270,6 +271,23 @@ def test_infinities_and_nan_stay_where_they_are(act, cache):
     assert not out[0, :2, 5].isfinite().any()
     out[0, :2, 5] = clean[0, :2, 5]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("dh,pad,page", [(64, 4, 16), (76, 0, 16), (76, 0, 4), (76, 4, 16), (12, 0, 16), (128, 4, 32),
+                                         (252, 0, 16), (256, 4, 16)])
+def test_nan_in_the_neighbouring_heads(act, cache, dh, pad, page):
+    """Three cache heads of which the outer ones are NaN throughout: the one between, whose rows may begin and end
+    within the same 16 bytes, is what it was."""
+    pool = Pool([70, 9, 0, 33], 3, dh, page, cache, seed=6, pad=pad)
+    q = torch.randn(4, 6, dh, generator=gen(4), device=DEV).to(act)
+    clean, lse = check_attn(pool, q)
+    for c in (pool.kc, pool.vc):
+        c[:, :, 0] = float("nan")
+        c[:, :, 2] = float("nan")
+    out, got = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, return_lse=True)
+    assert torch.equal(out[:, 2:4], clean[:, 2:4]) and torch.equal(got[:, 2:4], lse[:, 2:4])
+    assert out[:2, [0, 1, 4, 5]].isnan().all()
 
 
 @pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
