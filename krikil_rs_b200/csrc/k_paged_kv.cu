@@ -282,7 +282,9 @@ cudaError_t launch_plan(void (*all)(Args), void (*fill)(Args), void (*commit)(Ar
 // Every input is read and every output written once, W elements (16 bytes) at
 // a time: HBM bounds it.  A unit is W pairs (i, i + rot/2) of a query or key
 // head, or 2 W neighbours that are not rotated; a thread keeps one unit and takes
-// it in two heads at once.  One wave of blocks takes equal runs of rows and
+// it in two heads at once.  Where half a head is an odd number of half units (76 =
+// 2 x 38 of four), units are RAGGED: the second parts are taken in two pieces, and
+// the last unit is half of one.  One wave of blocks takes equal runs of rows and
 // loads the next row before it stores the present one.  The rows' cos and sin
 // are computed eight rows at a time, once a pair for all heads: the turns,
 // position times rate, are reduced to a fraction in 64 bits.
@@ -302,6 +304,7 @@ struct Raw<2> { using type = uint16_t; };
 template <typename T, int W>
 union Vec {
     typename Raw<sizeof(T) * W>::type raw;
+    typename Raw<W == 1 ? sizeof(T) : sizeof(T) * W / 2>::type part[2];
     T e[W];
     uint32_t w[sizeof(T) * W / 4 ? sizeof(T) * W / 4 : 1];
     KRK_DEV Vec() {}
@@ -309,6 +312,13 @@ union Vec {
 template <typename T, int W>
 KRK_DEV void load_vec(Vec<T, W>& v, const T* p) {
     v.raw = *reinterpret_cast<const typename Raw<sizeof(T) * W>::type*>(p);
+}
+// The same from half the alignment, the second part only if `whole`.
+template <typename T, int W>
+KRK_DEV void load_parts(Vec<T, W>& v, const T* p, bool whole) {
+    using R = typename Raw<W == 1 ? sizeof(T) : sizeof(T) * W / 2>::type;
+    v.part[0] = reinterpret_cast<const R*>(p)[0];
+    if (whole) v.part[1] = reinterpret_cast<const R*>(p)[1];
 }
 template <typename T, int W>
 KRK_DEV void store_vec(T* p, const Vec<T, W>& v) {
@@ -354,23 +364,38 @@ KRK_DEV void put(T* p, const float (&x)[W]) {
     store_vec<T, W>(p, v);
 }
 
+template <typename T, int W>
+KRK_DEV void put_parts(T* p, const float (&x)[W], bool whole) {
+    if constexpr (W > 1) {
+        float a[W / 2], b[W / 2];
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+            a[i] = x[i];
+            b[i] = x[W / 2 + i];
+        }
+        put<T, W / 2>(p, a);
+        if (whole) put<T, W / 2>(p + W / 2, b);
+    }
+}
+
 // How a block divides its rows: `side` rows at once, `lanes` threads of each
 // unit taking a row's heads; `depth` times.
 struct AppendShape {
     int side, lanes, depth;
 };
 
-template <typename T, typename C, int W>
+template <typename T, typename C, int W, bool RAGGED>
 __global__ void __launch_bounds__(APPEND_THREADS, APPEND_BLOCKS)
     rope_append_kernel(const __grid_constant__ RopeAppendArgs a, const AppendShape sh) {
     extern __shared__ __align__(16) float turned[];  // [row of the batch][cos, sin][rot / 2]
-    const int half = a.rot / 2, units = a.dh / (2 * W), rot_units = half / W, heads = a.Hq + 2 * a.Hkv;
+    const int half = a.rot / 2, units = RAGGED ? (half + W / 2) / W : a.dh / (2 * W);
+    const int rot_units = RAGGED ? units : half / W, heads = a.Hq + 2 * a.Hkv;
     const int r = threadIdx.x / (sh.lanes * units), in_row = threadIdx.x - r * sh.lanes * units;
     const int lane = in_row / units, unit = in_row - lane * units;
     const long long t0 = (long long)blockIdx.x * sh.side * sh.depth;
     const long long t1 = min(t0 + sh.side * sh.depth, (long long)a.T);
     // where the unit's two parts lie in a rotated head and in a value head
-    const bool turns = unit < rot_units;
+    const bool turns = unit < rot_units, whole = !RAGGED || unit < units - 1;
     const int at = turns ? unit * W : a.rot + (unit - rot_units) * 2 * W, next = at + (turns ? half : W);
     Vec<T, W> lo[APPEND_HEADS], hi[APPEND_HEADS];
     int slot = -1;
@@ -383,11 +408,14 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_BLOCKS)
                 const T* p = h < a.Hq ? (const T*)a.q + t * a.q_st + h * a.q_sh
                                       : (const T*)a.k + t * a.k_st + (h - a.Hq) * a.k_sh;
                 load_vec<T, W>(lo[i], p + at);
-                load_vec<T, W>(hi[i], p + next);
+                if (RAGGED)
+                    load_parts<T, W>(hi[i], p + next, whole);
+                else
+                    load_vec<T, W>(hi[i], p + next);
             } else {
                 const T* p = (const T*)a.v + t * a.v_st + (h - a.Hq - a.Hkv) * a.v_sh + unit * 2 * W;
                 load_vec<T, W>(lo[i], p);
-                load_vec<T, W>(hi[i], p + W);
+                if (whole) load_vec<T, W>(hi[i], p + W);
             }
         }
     };
@@ -441,12 +469,13 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_BLOCKS)
                     if (h >= a.Hq + a.Hkv) {
                         C* p = (C*)a.vc + cell + (h - a.Hq - a.Hkv) * a.c_sh + unit * 2 * W;
                         put<C, W>(p, x);
-                        put<C, W>(p + W, y);
+                        if (whole) put<C, W>(p + W, y);
                         continue;
                     }
                     if (turns) {
 #pragma unroll
                         for (int j = 0; j < W; ++j) {
+                            if (j >= W / 2 && !whole) break;
                             const float x0 = x[j], y0 = y[j], c = cs[j], s = cs[half + j];
                             x[j] = fmaf(x0, c, -(y0 * s));
                             y[j] = fmaf(y0, c, x0 * s);
@@ -454,12 +483,24 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_BLOCKS)
                     }
                     if (h < a.Hq) {
                         T* p = (T*)a.q_out + t * a.qo_st + h * a.qo_sh;
-                        put<T, W>(p + at, x);
-                        put<T, W>(p + next, y);
+                        if (RAGGED && !whole)
+                            put_parts<T, W>(p + at, x, false);
+                        else
+                            put<T, W>(p + at, x);
+                        if (RAGGED)
+                            put_parts<T, W>(p + next, y, whole);
+                        else
+                            put<T, W>(p + next, y);
                     } else {
                         C* p = (C*)a.kc + cell + (h - a.Hq) * a.c_sh;
-                        put<C, W>(p + at, x);
-                        put<C, W>(p + next, y);
+                        if (RAGGED && !whole)
+                            put_parts<C, W>(p + at, x, false);
+                        else
+                            put<C, W>(p + at, x);
+                        if (RAGGED)
+                            put_parts<C, W>(p + next, y, whole);
+                        else
+                            put<C, W>(p + next, y);
                     }
                 }
             }
@@ -468,9 +509,9 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_BLOCKS)
     }
 }
 
-template <typename T, typename C, int W>
+template <typename T, typename C, int W, bool RAGGED = false>
 cudaError_t launch_append_w(const RopeAppendArgs& a, cudaStream_t s) {
-    const int units = a.dh / (2 * W), heads = a.Hq + 2 * a.Hkv;
+    const int units = RAGGED ? (a.rot / 2 + W / 2) / W : a.dh / (2 * W), heads = a.Hq + 2 * a.Hkv;
     AppendShape sh{1, (heads + APPEND_HEADS - 1) / APPEND_HEADS, 1};
     if (sh.lanes > APPEND_THREADS / units) sh.lanes = APPEND_THREADS / units;  // several rounds of heads
     sh.side = APPEND_THREADS / (sh.lanes * units);
@@ -485,7 +526,7 @@ cudaError_t launch_append_w(const RopeAppendArgs& a, cudaStream_t s) {
     const long long wave = (long long)sms * (APPEND_BLOCKS * APPEND_THREADS / threads) * sh.side;
     sh.depth = (int)((a.T + wave - 1) / wave);
     const long long rows = (long long)sh.side * sh.depth, batch = sh.depth < APPEND_BATCH ? sh.depth : APPEND_BATCH;
-    rope_append_kernel<T, C, W><<<(unsigned)((a.T + rows - 1) / rows), threads,
+    rope_append_kernel<T, C, W, RAGGED><<<(unsigned)((a.T + rows - 1) / rows), threads,
                                   (size_t)sh.side * batch * a.rot * sizeof(float), s>>>(a, sh);
     add_launches(1);
     return cudaGetLastError();
@@ -504,6 +545,7 @@ cudaError_t launch_append(const RopeAppendArgs& a, cudaStream_t s) {
             return launch_append_w<T, C, 8>(a, s);
     }
     if (fits(4)) return launch_append_w<T, C, 4>(a, s);
+    if (a.rot == a.dh && a.dh % 8 == 4) return launch_append_w<T, C, 4, true>(a, s);
     if (fits(2)) return launch_append_w<T, C, 2>(a, s);
     return launch_append_w<T, C, 1>(a, s);
 }

@@ -415,7 +415,8 @@ def close(got, ref, tol):
 @pytest.mark.parametrize("t,hq,hkv,dh,rot,page,far", [
     (1, 8, 8, 76, 76, 16, 2048), (37, 32, 8, 128, 128, 16, 10 ** 6), (300, 4, 1, 64, 32, 1, 2 ** 31 - 1),
     (65, 7, 7, 80, 40, 8, 32768), (5, 2, 2, 256, 256, 256, 10 ** 6), (129, 1, 1, 4, 2, 4, 100),
-    (40, 6, 2, 96, 0, 16, 1000), (1111, 12, 4, 192, 190, 32, 5000)])
+    (40, 6, 2, 96, 0, 16, 1000), (1111, 12, 4, 192, 190, 32, 5000), (33, 3, 1, 4, 4, 8, 100), (70, 5, 5, 12, 12, 16, 999),
+    (21, 2, 1, 252, 252, 16, 4000), (300, 9, 3, 36, 36, 32, 70000), (50, 4, 2, 76, 38, 16, 2048)])
 def test_append_types_heads_and_positions(act, cache, t, hq, hkv, dh, rot, page, far):
     g = gen(t + dh)
     pages = -(-t // page) + 2
