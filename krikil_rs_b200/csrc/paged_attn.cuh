@@ -1,5 +1,5 @@
 // Decode attention over a paged key-value cache: the kernel's frame, shared by
-// the float32 and the 16-bit engines (k_paged_attn_f32.cu, k_paged_attn_half.cu).
+// the float32 and the 16-bit engines (k_paged_attn_f32.cu, paged_attn_half.cuh).
 //
 // One token a request reads every visible key and value once and computes 4 dh
 // operations for each pair and query head, so for the up to some tens of heads
@@ -229,6 +229,7 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 // filled again as soon as the warp has read it, with no barrier beyond the warp.
 // (The same tiles held in registers, loads issued as early: f32 1024 x 8 x 76 in
 // 604 us, 271 us from a ring; bf16 128 x 32/8 x 128 in 435 us, 331 us.)
+
 // Adds up the sums of a cluster's blocks, each block a part of the elements.
 template <class E>
 KRK_DEV void pa_join_cluster(const PagedAttnArgs& a, const PagedShape& sh, const unsigned char* smem,
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
                                                                            const PagedParts parts) {
     using T = typename E::Act;
     using C = typename E::Cache;
-    constexpr int KT = E::KT, HW = E::HW, LD = E::DC + 4, S = E::SLOTS, HALF = E::TILE_BYTES;
+    constexpr int KT = E::KT, HW = E::HW, LD = E::DC + 4, S = E::SLOTS, SLOT = E::TILE_BYTES;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float sm[PA_WARPS][HW], sl[PA_WARPS][HW], sf[PA_WARPS][HW];
     __shared__ __align__(8) float2 sums[PA_MAX_ROWS];
@@ -291,8 +292,8 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
     const int G = a.Hq / a.Hkv, pieces = a.Hkv / sh.side * sh.per_kv;
     // warp -> (keys, cache head, query heads)
     const int sets = sh.side * sh.groups, kwarps = PA_WARPS / sets, kwarp = warp / sets, set = warp % sets;
-    unsigned char* ring = smem + (size_t)warp * 2 * S * HALF;
-    unsigned char* qs = smem + (size_t)PA_WARPS * 2 * S * HALF + (size_t)set * E::Q_BYTES;
+    unsigned char* ring = smem + (size_t)warp * 2 * S * SLOT;
+    unsigned char* qs = smem + (size_t)PA_WARPS * 2 * S * SLOT + (size_t)set * E::Q_BYTES;
     const uint32_t ring_at = smem_addr(ring);
 
     PagedShare share;
@@ -358,9 +359,9 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
                 for (int i = 0; i < S; ++i) {
                     const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
                     mask[i] = t.mask;
-                    if (key + i * step < k1) e.issue(a, kc, t, ring_at + i * HALF, lane);
+                    if (key + i * step < k1) e.issue(a, kc, t, ring_at + i * SLOT, lane);
                     cp_async_commit();
-                    if (key + i * step < k1) e.issue(a, vc, t, ring_at + (S + i) * HALF, lane);
+                    if (key + i * step < k1) e.issue(a, vc, t, ring_at + (S + i) * SLOT, lane);
                     cp_async_commit();
                 }
                 int page = pages[S];
@@ -368,21 +369,21 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
                     const int ahead = key + S * step;
                     cp_async_wait<2 * S - 1>();
                     __syncwarp();
-                    e.scores(qs, ring + slot * HALF, lane);
+                    e.scores(qs, ring + slot * SLOT, lane);
                     __syncwarp();
                     const PagedTile t = pa_tile<KT>(a, page, ahead, first, k1);
                     mask[S] = t.mask;
-                    if (ahead < k1) e.issue(a, kc, t, ring_at + slot * HALF, lane);
+                    if (ahead < k1) e.issue(a, kc, t, ring_at + slot * SLOT, lane);
                     cp_async_commit();
                     page = pa_page<KT>(a, row, ahead + step);
                     e.weigh(mask[0], lane);
                     cp_async_wait<2 * S - 1>();
                     __syncwarp();
-                    e.values(ring + (S + slot) * HALF, lane);
+                    e.values(ring + (S + slot) * SLOT, lane);
                     key += step;
                     if (key >= k1) break;
                     __syncwarp();
-                    if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * HALF, lane);
+                    if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * SLOT, lane);
                     cp_async_commit();
 #pragma unroll
                     for (int i = 0; i < S; ++i) mask[i] = mask[i + 1];
@@ -426,14 +427,14 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int w = w0; w < PA_WARPS; w += sets) {
                     const float f = sf[w][h];
-                    const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * HALF + (h * LD + d) * 4);
+                    const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * SLOT + (h * LD + d) * 4);
                     o.x = fmaf(f, x.x, o.x);
                     o.y = fmaf(f, x.y, o.y);
                     o.z = fmaf(f, x.z, o.z);
                     o.w = fmaf(f, x.w, o.w);
                 }
                 if (sh.cluster > 1)  // over the first of the warps' sums, which nobody else reads
-                    *reinterpret_cast<float4*>(smem + (size_t)w0 * 2 * S * HALF + (h * LD + d) * 4) = o;
+                    *reinterpret_cast<float4*>(smem + (size_t)w0 * 2 * S * SLOT + (h * LD + d) * 4) = o;
                 else if (take == units)
                     store4((T*)a.out + b * a.o_sb + ((long long)(hk0 + s) * G + head0 + in_g) * a.o_sh + d, o);
                 else
