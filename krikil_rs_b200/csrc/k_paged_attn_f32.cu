@@ -16,7 +16,8 @@
 namespace krk {
 namespace {
 
-template <int DC_, int GW, int SLOTS_>
+// PART: rows are not whole sectors of 32 bytes, and are copied through L1.
+template <int DC_, int GW, int SLOTS_, bool PART>
 struct F32Engine {
     using Act = float;
     using Cache = float;
@@ -63,7 +64,7 @@ struct F32Engine {
             for (int j = 0; j < J; ++j) {
 #pragma unroll
                 for (int i = 0; i < NL; ++i)
-                    pa_copy<16>(to + (j * NL + i) * 512, p + i * LPK * 4, d + i * LPK * 4 < a.dh);
+                    pa_copy<16, PART>(to + (j * NL + i) * 512, p + i * LPK * 4, d + i * LPK * 4 < a.dh);
                 p += KPL * a.c_st;
             }
             return;
@@ -199,11 +200,11 @@ struct F32Engine {
     }
 };
 
-template <int GW>
+template <int GW, bool PART>
 cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
-    if (a.dh <= 64) return launch_paged_attn<F32Engine<64, GW, 1>, F32Engine<64, GW, 2>>(a, s);
-    if (a.dh <= 128) return launch_paged_attn<F32Engine<128, GW, 1>, F32Engine<128, GW, 2>>(a, s);
-    return launch_paged_attn<F32Engine<256, GW, 1>, F32Engine<256, GW, 2>>(a, s);
+    if (a.dh <= 64) return launch_paged_attn<F32Engine<64, GW, 1, PART>, F32Engine<64, GW, 2, PART>>(a, s);
+    if (a.dh <= 128) return launch_paged_attn<F32Engine<128, GW, 1, PART>, F32Engine<128, GW, 2, PART>>(a, s);
+    return launch_paged_attn<F32Engine<256, GW, 1, PART>, F32Engine<256, GW, 2, PART>>(a, s);
 }
 
 }  // namespace
@@ -231,9 +232,8 @@ size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int w
 
 cudaError_t attn_decode_paged_f32(const PagedAttnArgs& a, cudaStream_t s) {
     const int G = a.Hq / a.Hkv;
-    if (G == 1) return by_width<1>(a, s);
-    if (G == 2) return by_width<2>(a, s);
-    return by_width<4>(a, s);
+    if (G == 1) return a.dh % 8 ? by_width<1, true>(a, s) : by_width<1, false>(a, s);
+    return G == 2 ? by_width<2, false>(a, s) : by_width<4, false>(a, s);
 }
 
 cudaError_t attn_decode_paged_f16(const PagedAttnArgs& a, bool act_f32, cudaStream_t s);

@@ -208,14 +208,19 @@ KRK_DEV void pa_group_sync(int group, int warps) {
         __syncwarp();
 }
 
-// Asynchronous copy of BYTES (16 or 8) to shared memory; zeros, and no access, when !take.
-template <int BYTES>
+// Asynchronous copy of BYTES (16 or 8) to shared memory; zeros, and no access, when !take.  L1: rows that begin or end
+// inside a sector find the half that a neighbouring head's warp has fetched in L1 (f32 64 x 8 x 76 of 4096 keys: 217 us,
+// 237 us past L1).  It costs where rows are whole sectors (f32 heads of 80: 232 and 225 us), where several query heads
+// slow a tile down (f32 8/2 heads of 76: 96 and 90 us) and for the shorter 16-bit rows (f32 queries on bf16 heads of 76:
+// 232 and 161 us).
+template <int BYTES, bool L1 = false>
 KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
     const int n = take ? BYTES : 0;
-    if (BYTES == 16)
+    if (BYTES == 16 && !L1)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to), "l"(from), "r"(n) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;\n" ::"r"(to), "l"(from), "r"(n), "n"(BYTES)
+                     : "memory");
 }
 
 // E: an engine.  Its warp holds KT keys of a tile and HW query heads:
