@@ -92,18 +92,20 @@ enum RowAlign { ROWS_NARROW, ROWS_SHIFTED, ROWS_WIDE };
 // of a warp's ring.  Shifted rows are copied from the 16-byte boundary before them, and everything -- queries, products,
 // results -- is moved up by the `before` elements in between; what the copies bring along of other rows is cleared in
 // the keys, where it would meet a query, and dropped with the results' columns in the values.
-template <typename T, typename C, int DC_, int ALIGN, int SLOTS_>
+template <typename T, typename C, int DC_, int ALIGN, int SLOTS_, int HW_>
 struct HalfEngine {
     using Act = T;
     using Cache = C;
     static constexpr bool kSame = sizeof(T) == 2, kHalf = sizeof(__half) == 2 && std::is_same<C, __half>::value;
-    static constexpr int DC = DC_, KT = 16, HW = 8;
+    static constexpr int DC = DC_, KT = 16, HW = HW_;
+    static constexpr bool kPacked = HW == 4;  // parts lie in the rows and columns of four heads that are not there
     static constexpr int NB = DC / 32, NV = DC / 16;     // steps of the two products
     static constexpr int CPR = DC <= 64 ? 8 : DC <= 128 ? 16 : 32, ROW = CPR * 16;  // a row's 16-byte pieces and bytes
     static constexpr int RPC = 32 / CPR;                  // rows of one copy
     static constexpr int QP = kSame ? 1 : kHalf ? 2 : 3;  // parts of a query
     static constexpr int PP = !kSame && !kHalf ? 3 : 2;   // parts of a weight
-    static constexpr int Q_BYTES = QP * NB * 32 * 16;
+    static constexpr int QA = kPacked ? (QP + 1) / 2 : QP;  // eights of rows of the first operand
+    static constexpr int Q_BYTES = QA * NB * 32 * 16;
     static constexpr int TILE_BYTES = KT * ROW, SLOTS = SLOTS_;
     static constexpr int BLOCKS = DC > 128 ? 2 : SLOTS == 1 ? 4 : 3;
     static constexpr float SCALE = kHalf ? 16384.f : 1.f;
@@ -144,14 +146,15 @@ struct HalfEngine {
                 if (d >= DC) continue;
                 float4 y = make_float4(x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up);
 #pragma unroll
-                for (int p = 0; p < QP; ++p) {
+                for (int p = 0; p < (kPacked ? 2 * QA : QA); ++p) {  // (a part beyond the last is zero)
+                    const int row = kPacked ? p * 4 + h : p * 8 + h;
                     uint32_t* to = reinterpret_cast<uint32_t*>(qs) +
-                                   ((p * NB + d / 32) * 32 + h * 4 + d % 8 / 2) * 4 + d % 32 / 8;
-                    to[0] = pack_rest(y.x, y.y, C());
-                    to[4] = pack_rest(y.z, y.w, C());
+                                   ((row / 8 * NB + d / 32) * 32 + row % 8 * 4 + d % 8 / 2) * 4 + d % 32 / 8;
+                    to[0] = p < QP ? pack_rest(y.x, y.y, C()) : 0u;
+                    to[4] = p < QP ? pack_rest(y.z, y.w, C()) : 0u;
                 }
             }
-            if (QP == 2 && lane / 4 == h) c *= 1.0f / up;
+            if (QP == 2 && lane / 4 % HW == h) c *= 1.0f / up;
         }
         if (QP == 2) {  // the other warps' heads: the same scales again
             for (int h = 0; h < HW; ++h) {
@@ -162,7 +165,7 @@ struct HalfEngine {
                     most = fmaxf(most, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
                 }
                 const float up = row_scale(warp_max(most));
-                if (lane / 4 == h) c *= 1.0f / up;
+                if (lane / 4 % HW == h) c *= 1.0f / up;
             }
         }
     }
@@ -233,7 +236,7 @@ struct HalfEngine {
             load_matrices(k0, at + (((i * 4 + piece) ^ turn) << 4));
             load_matrices(k1, at + 8 * ROW + (((i * 4 + piece) ^ turn) << 4));
             const uint4 h = qf[i * 32];
-            const uint4 r = QP > 1 ? qf[(NB + i) * 32] : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 r = QA > 1 ? qf[(NB + i) * 32] : make_uint4(0u, 0u, 0u, 0u);
             if (i == 0) {
                 mma_first(d0, h.x, r.x, h.y, r.y, k0[0], k0[1], C());
                 mma_first(d1, h.x, r.x, h.y, r.y, k1[0], k1[1], C());
@@ -243,7 +246,7 @@ struct HalfEngine {
             }
             mma(d0, h.z, r.z, h.w, r.w, k0[2], k0[3], C());
             mma(d1, h.z, r.z, h.w, r.w, k1[2], k1[3], C());
-            if (QP > 2) {
+            if (QA > 2) {
                 const uint4 t = qf[(2 * NB + i) * 32];
                 if (i == 0) {
                     mma_first(e0, t.x, 0u, t.y, 0u, k0[0], k0[1], C());
@@ -256,14 +259,27 @@ struct HalfEngine {
                 mma(e1, t.z, 0u, t.w, 0u, k1[2], k1[3], C());
             }
         }
-        if (QP <= 2) {
+        if (QA <= 2) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) e0[i] = e1[i] = 0.f;
+        }
+        if (kPacked) {  // rows 0-3, 4-7 and 8-11 hold the parts of the same four heads: every lane gets all three
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                apart(d0[i], d0[2 + i], e0[i], lane);
+                apart(d1[i], d1[2 + i], e1[i], lane);
+            }
         }
         s[0] = joined(d0[0], d0[2], e0[0]);
         s[1] = joined(d0[1], d0[3], e0[1]);
         s[2] = joined(d1[0], d1[2], e1[0]);
         s[3] = joined(d1[1], d1[3], e1[1]);
+    }
+    static KRK_DEV void apart(float& low, float& high, float& third, int lane) {
+        const float other = __shfl_xor_sync(0xffffffffu, low, 16);
+        if (QP > 2) third = __shfl_sync(0xffffffffu, high, lane & 15);
+        high = lane < 16 ? other : low;
+        low = lane < 16 ? low : other;
     }
     // The parts' products; an infinite key's first part decides (the others may be infinite the other way, or NaN).
     static KRK_DEV float joined(float first, float second, float third) {
@@ -294,14 +310,23 @@ struct HalfEngine {
     }
 
     KRK_DEV void values(const unsigned char* from, int lane) {
-        const float f0 = __shfl_sync(0xffffffffu, fade, (lane & 3) * 8);
-        const float f1 = __shfl_sync(0xffffffffu, fade, (lane & 3) * 8 + 4);
+        // of the accumulators' columns 2 (lane % 4) and the one after it
+        const float f0 = __shfl_sync(0xffffffffu, fade, (lane & 3) * 8 % (HW * 4));
+        const float f1 = __shfl_sync(0xffffffffu, fade, ((lane & 3) * 8 + 4) % (HW * 4));
         uint32_t p[PP][2];
 #pragma unroll
         for (int i = 0; i < PP; ++i) {
             p[i][0] = pack_rest(s[0], s[1], C());
             p[i][1] = pack_rest(s[2], s[3], C());
         }
+        if (kPacked) {  // columns 0-3 take the first part, 4-7 the second, and the third goes by itself
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                p[0][x] = lane < 16 ? p[0][x] : p[1][x];
+                if (PP > 2) p[1][x] = lane < 16 ? p[PP - 1][x] : 0u;
+            }
+        }
+        constexpr int PA = kPacked ? PP - 1 : PP;
         // matrices: keys 0-7 and 8-15 of the pieces 2i and 2i + 1
         const int key = (lane >> 4) * 8 + (lane & 7), piece = lane >> 3 & 1, turn = lane & 7;
         const uint32_t at = smem_addr(from) + key * ROW;
@@ -310,9 +335,9 @@ struct HalfEngine {
             uint32_t v[4];
             load_matrices_t(v, at + (((i * 2 + piece) ^ turn) << 4));
             float d[4];
-            mma_first(d, v[0], v[1], v[2], v[3], p[PP - 1][0], p[PP - 1][1], C());
+            mma_first(d, v[0], v[1], v[2], v[3], p[PA - 1][0], p[PA - 1][1], C());
 #pragma unroll
-            for (int x = PP - 2; x >= 0; --x) mma(d, v[0], v[1], v[2], v[3], p[x][0], p[x][1], C());
+            for (int x = PA - 2; x >= 0; --x) mma(d, v[0], v[1], v[2], v[3], p[x][0], p[x][1], C());
             acc[i][0] = fmaf(acc[i][0], f0, d[0]);
             acc[i][1] = fmaf(acc[i][1], f1, d[1]);
             acc[i][2] = fmaf(acc[i][2], f0, d[2]);
@@ -324,9 +349,16 @@ struct HalfEngine {
         const int r = lane >> 2, t = lane & 3;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) {
+        if (t == 0 && r < HW) {
             sm[r] = m;
             sl[r] = l;
+        }
+        if (kPacked) {  // the columns of the parts
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[i][x] += __shfl_xor_sync(0xffffffffu, acc[i][x], 2);
+            if (t > 1) return;
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -341,14 +373,27 @@ struct HalfEngine {
     }
 };
 
-template <typename T, typename C, int ALIGN>
+template <typename T, typename C, int ALIGN, int HW>
 cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
     const int width = ALIGN == ROWS_SHIFTED ? a.dh + 4 : a.dh;
-    if (width <= 64) return launch_paged_attn<HalfEngine<T, C, 64, ALIGN, 1>, HalfEngine<T, C, 64, ALIGN, 2>>(a, s);
-    if (width <= 96) return launch_paged_attn<HalfEngine<T, C, 96, ALIGN, 1>, HalfEngine<T, C, 96, ALIGN, 2>>(a, s);
-    if (width <= 128) return launch_paged_attn<HalfEngine<T, C, 128, ALIGN, 1>, HalfEngine<T, C, 128, ALIGN, 2>>(a, s);
-    if (width <= 192) return launch_paged_attn<HalfEngine<T, C, 192, ALIGN, 1>, HalfEngine<T, C, 192, ALIGN, 1>>(a, s);
-    return launch_paged_attn<HalfEngine<T, C, 256, ALIGN, 1>, HalfEngine<T, C, 256, ALIGN, 1>>(a, s);
+    if (width <= 64)
+        return launch_paged_attn<HalfEngine<T, C, 64, ALIGN, 1, HW>, HalfEngine<T, C, 64, ALIGN, 2, HW>>(a, s);
+    if (width <= 96)
+        return launch_paged_attn<HalfEngine<T, C, 96, ALIGN, 1, HW>, HalfEngine<T, C, 96, ALIGN, 2, HW>>(a, s);
+    if (width <= 128)
+        return launch_paged_attn<HalfEngine<T, C, 128, ALIGN, 1, HW>, HalfEngine<T, C, 128, ALIGN, 2, HW>>(a, s);
+    if (width <= 192)
+        return launch_paged_attn<HalfEngine<T, C, 192, ALIGN, 1, HW>, HalfEngine<T, C, 192, ALIGN, 1, HW>>(a, s);
+    return launch_paged_attn<HalfEngine<T, C, 256, ALIGN, 1, HW>, HalfEngine<T, C, 256, ALIGN, 1, HW>>(a, s);
+}
+
+// Up to four heads of float32 queries lie packed, their parts in the rows and columns of the four that are missing (f32
+// queries on bf16 pages, 1024 x 8 x 76: 148 us, 161 us in eights; on f16 pages 147 and 162 us).
+template <typename T, typename C, int ALIGN>
+cudaError_t by_heads(const PagedAttnArgs& a, cudaStream_t s) {
+    if constexpr (sizeof(T) == 4)
+        if (a.Hq / a.Hkv <= 4) return by_width<T, C, ALIGN, 4>(a, s);
+    return by_width<T, C, ALIGN, 8>(a, s);
 }
 
 template <typename T, typename C>
@@ -356,9 +401,9 @@ cudaError_t by_alignment(const PagedAttnArgs& a, cudaStream_t s) {
     const bool same = a.c_sp % 8 == 0 && a.c_st % 8 == 0;
     const bool wide = same && a.dh % 8 == 0 && a.c_sh % 8 == 0 && (reinterpret_cast<uintptr_t>(a.kc) & 15) == 0 &&
                       (reinterpret_cast<uintptr_t>(a.vc) & 15) == 0;
-    if (wide) return by_width<T, C, ROWS_WIDE>(a, s);
-    if (same && a.dh <= 252) return by_width<T, C, ROWS_SHIFTED>(a, s);
-    return by_width<T, C, ROWS_NARROW>(a, s);
+    if (wide) return by_heads<T, C, ROWS_WIDE>(a, s);
+    if (same && a.dh <= 252) return by_heads<T, C, ROWS_SHIFTED>(a, s);
+    return by_width<T, C, ROWS_NARROW, 8>(a, s);
 }
 
 }  // namespace
