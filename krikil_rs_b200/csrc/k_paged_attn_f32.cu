@@ -8,9 +8,9 @@
 // query; the eight partial sums are added over the LPK lanes by exchanging
 // halves -- four, two, one, so that each lane ends with one key's score after
 // 8 or 9 shuffles instead of 8 x 5 -- and one exponential a lane weighs the
-// tile.  HBM bounds it for heads that fill their lanes (256 x 8 x 128 of 2048
-// keys, 4.3 GB: 619 us, 6.9 TB/s); heads of 76 use 19 of 32 lanes, and issue and
-// shared memory come close (1024 x 8 x 76: 245 us, 5.2 TB/s).
+// tile.  HBM bounds it (256 x 8 x 128 of 2048 keys, 4.3 GB: 619 us, 6.9 TB/s;
+// 1024 x 8 x 76, whose rows share sectors: 235 us, 5.4 TB/s); with four query heads
+// a warp the shuffles do (1024 x 8/2 x 76: 92 us for 51 us of bytes).
 #include "paged_attn.cuh"
 
 namespace krk {

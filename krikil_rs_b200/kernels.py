@@ -266,6 +266,8 @@ def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int
     new_at, lens_at = _ints(new_tokens, b, dev, "new_tokens"), _ints(lens, b, dev, "lens")
     pages = free_pages.numel()
     free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
+    if rows < 0:
+        raise ValueError("rows must not be negative")
     padded = -rows % 4 + rows
     buf = lens.new_empty(2 * padded + 2 * b + 3)
     positions, _, slots, _, cu, lens_new, count_new, status = buf.unsafe_split_with_sizes(

@@ -836,5 +836,7 @@ def test_wrappers_refuse_what_does_not_belong_together():
                 (two, pool.lens, pool.table[0], free, one), (two, pool.lens.cpu(), pool.table, free, one)):
         with pytest.raises(ValueError):
             K.kv_page_plan(*bad, 16, 4)
+    with pytest.raises(ValueError, match="rows"):
+        K.kv_page_plan(two, pool.lens, pool.table, free, one, 16, -1)
     with pytest.raises(ValueError):
         K.kv_page_release(two, *(pool.lens, pool.table, free, one), 16)
