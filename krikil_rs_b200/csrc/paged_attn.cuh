@@ -235,6 +235,28 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 // (The same tiles held in registers, loads issued as early: f32 1024 x 8 x 76 in
 // 604 us, 271 us from a ring; bf16 128 x 32/8 x 128 in 435 us, 331 us.)
 
+// One part of a head's sums, with maximum m and sum l, onto others; top: the largest maximum of all.
+KRK_DEV void pa_add(float4& o, float& total, const float4& x, float m, float l, float top) {
+    // (no visible key at all: weight 0, or NaN if the sum is)
+    const float f = top == -INFINITY ? (l == 0.f ? 0.f : l) : pa_exp2(m - top);
+    total = fmaf(f, l, total);
+    o.x = fmaf(f, x.x, o.x);
+    o.y = fmaf(f, x.y, o.y);
+    o.z = fmaf(f, x.z, o.z);
+    o.w = fmaf(f, x.w, o.w);
+}
+// Elements d .. d + 3 of a query head's result from its sums, and with the first of them its logarithm.
+template <class E>
+KRK_DEV void pa_result(const PagedAttnArgs& a, int b, long long head, int d, float4 o, float top, float total) {
+    float inv;  // within a unit in the last place
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(total));
+    if (total == 0.f) inv = 0.f;
+    store4((typename E::Act*)a.out + b * a.o_sb + head * a.o_sh + d,
+           make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+    if (a.lse && d == 0)
+        a.lse[(long long)b * a.Hq + head] = (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
+}
+
 // Adds up the sums of a cluster's blocks, each block a part of the elements.
 template <class E>
 KRK_DEV void pa_join_cluster(const PagedAttnArgs& a, const PagedShape& sh, const unsigned char* smem,
@@ -264,20 +286,8 @@ KRK_DEV void pa_join_cluster(const PagedAttnArgs& a, const PagedShape& sh, const
         for (int c = 0; c < PA_CLUSTER; ++c) top = fmaxf(top, ml[c].x);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < PA_CLUSTER; ++c) {
-            const float f = top == -INFINITY ? (ml[c].y == 0.f ? 0.f : ml[c].y) : pa_exp2(ml[c].x - top);
-            total = fmaf(f, ml[c].y, total);
-            o.x = fmaf(f, x[c].x, o.x);
-            o.y = fmaf(f, x[c].y, o.y);
-            o.z = fmaf(f, x[c].z, o.z);
-            o.w = fmaf(f, x[c].w, o.w);
-        }
-        const float inv = total == 0.f ? 0.f : 1.0f / total;
-        const long long head = (long long)(hk0 + s) * G + head0 + in_g;
-        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        store4((typename E::Act*)a.out + b * a.o_sb + head * a.o_sh + d, o);
-        if (a.lse && d == 0)
-            a.lse[(long long)b * a.Hq + head] = (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
+        for (int c = 0; c < PA_CLUSTER; ++c) pa_add(o, total, x[c], ml[c].x, ml[c].y, top);
+        pa_result<E>(a, b, (long long)(hk0 + s) * G + head0 + in_g, d, o, top, total);
     }
 }
 
@@ -289,7 +299,7 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
     using C = typename E::Cache;
     constexpr int KT = E::KT, HW = E::HW, LD = E::DC + 4, S = E::SLOTS, SLOT = E::TILE_BYTES;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float sm[PA_WARPS][HW], sl[PA_WARPS][HW], sf[PA_WARPS][HW];
+    __shared__ float sm[PA_WARPS][HW], sl[PA_WARPS][HW];
     __shared__ __align__(8) float2 sums[PA_MAX_ROWS];
     __shared__ long long warp_sums[PA_WARPS];
     __shared__ PagedShare share_out;
@@ -350,25 +360,31 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             E e;
             int key = k0 + kwarp * KT;
             const int step = kwarps * KT;
-            // the first tiles' pages, then the queries while they are on their way
+            // the first tiles, and the queries while they are on their way
             if (!early) {
 #pragma unroll
                 for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step);
+            }
+            unsigned mask[S + 1];
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                if (key + i * step < k1) {
+                    const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
+                    mask[i] = t.mask;
+                    e.issue(a, kc, t, ring_at + i * SLOT, lane);
+                    cp_async_commit();
+                    e.issue(a, vc, t, ring_at + (S + i) * SLOT, lane);
+                    cp_async_commit();
+                } else {
+                    mask[i] = 0u;
+                    cp_async_commit();
+                    cp_async_commit();
+                }
             }
             e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, kc, vc, min(HW, G - head), qs,
                    lane, kwarp, kwarps);
             if (E::Q_BYTES) pa_group_sync(set, kwarps);
             if (key < k1) {
-                unsigned mask[S + 1];
-#pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
-                    mask[i] = t.mask;
-                    if (key + i * step < k1) e.issue(a, kc, t, ring_at + i * SLOT, lane);
-                    cp_async_commit();
-                    if (key + i * step < k1) e.issue(a, vc, t, ring_at + (S + i) * SLOT, lane);
-                    cp_async_commit();
-                }
                 int page = pages[S];
                 for (int slot = 0;; slot = slot + 1 == S ? 0 : slot + 1) {
                     const int ahead = key + S * step;
@@ -397,54 +413,40 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             __syncwarp();  // the warp's sums go where its tiles were
             e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
             __syncthreads();
-            // each query head's factors for its warps' sums
-            const int rows = sh.side * sh.rows;
-            if (tid < sets * HW) {
-                const int w0 = tid / HW, h = tid % HW, in_g = w0 % sh.groups * HW + h;
-                float top = -INFINITY, total = 0.f;
-                for (int w = w0; w < PA_WARPS; w += sets) top = fmaxf(top, sm[w][h]);
-                for (int w = w0; w < PA_WARPS; w += sets) {
-                    const float f = top == -INFINITY ? (sl[w][h] == 0.f ? 0.f : sl[w][h]) : pa_exp2(sm[w][h] - top);
-                    sf[w][h] = f;
-                    total = fmaf(f, sl[w][h], total);
-                }
-                if (in_g < sh.rows && head0 + in_g < G) {
-                    if (sh.cluster > 1) {
-                        sums[tid] = make_float2(top, total);
-                    } else if (take == units) {
-                        const float inv = total == 0.f ? 0.f : 1.0f / total;
-                        for (int w = w0; w < PA_WARPS; w += sets) sf[w][h] *= inv;
-                        if (a.lse)
-                            a.lse[(long long)b * a.Hq + (long long)(hk0 + w0 / sh.groups) * G + head0 + in_g] =
-                                (top + log2f(total * (1.0f / E::SCALE))) * 0.693147180559945309f;
-                    } else {
-                        parts.ml[((long long)blockIdx.x * 2 + (unit == 0)) * rows + w0 / sh.groups * sh.rows + in_g] =
-                            make_float2(top, total);
-                    }
-                }
-            }
-            __syncthreads();
-            const int n4 = a.dh / 4;
+            // Each thread joins its four elements over the head's warps by itself: one barrier, and the warps' loads
+            // side by side (with the factors computed once a head between two barriers, f32 1 x 8 x 76 of 96 keys
+            // took 6.9 us instead of 5.8).
+            const int rows = sh.side * sh.rows, n4 = a.dh / 4;
             for (int i = tid; i < rows * n4; i += PA_THREADS) {
                 const int r = i / n4, d = (i - r * n4) * 4, s = r / sh.rows, in_g = r - s * sh.rows;
                 if (head0 + in_g >= G) continue;
                 const int w0 = s * sh.groups + in_g / HW, h = in_g % HW;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int w = w0; w < PA_WARPS; w += sets) {
-                    const float f = sf[w][h];
-                    const float4 x = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * SLOT + (h * LD + d) * 4);
-                    o.x = fmaf(f, x.x, o.x);
-                    o.y = fmaf(f, x.y, o.y);
-                    o.z = fmaf(f, x.z, o.z);
-                    o.w = fmaf(f, x.w, o.w);
+                float mw[PA_WARPS], lw[PA_WARPS];
+                float4 x[PA_WARPS];
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    const bool his = (w & (sets - 1)) == w0;
+                    mw[w] = his ? sm[w][h] : -INFINITY;
+                    lw[w] = his ? sl[w][h] : 0.f;
+                    x[w] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (his) x[w] = *reinterpret_cast<const float4*>(smem + (size_t)w * 2 * S * SLOT + (h * LD + d) * 4);
                 }
-                if (sh.cluster > 1)  // over the first of the warps' sums, which nobody else reads
+                const float top = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
+                float total = 0.f;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) pa_add(o, total, x[w], mw[w], lw[w], top);
+                const long long head = (long long)(hk0 + s) * G + head0 + in_g;
+                if (sh.cluster > 1) {  // over the first of the warps' sums, which nobody else reads
                     *reinterpret_cast<float4*>(smem + (size_t)w0 * 2 * S * SLOT + (h * LD + d) * 4) = o;
-                else if (take == units)
-                    store4((T*)a.out + b * a.o_sb + ((long long)(hk0 + s) * G + head0 + in_g) * a.o_sh + d, o);
-                else
-                    *reinterpret_cast<float4*>(
-                        parts.acc + (((long long)blockIdx.x * 2 + (unit == 0)) * rows + r) * a.dh + d) = o;
+                    if (d == 0) sums[w0 * HW + h] = make_float2(top, total);
+                } else if (take == units) {
+                    pa_result<E>(a, b, head, d, o, top, total);
+                } else {
+                    const long long at_row = ((long long)blockIdx.x * 2 + (unit == 0)) * rows + r;
+                    *reinterpret_cast<float4*>(parts.acc + at_row * a.dh + d) = o;
+                    if (d == 0) parts.ml[at_row] = make_float2(top, total);
+                }
             }
             if (sh.cluster) {
                 if (sh.cluster > 1) {
