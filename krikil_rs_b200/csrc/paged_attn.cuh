@@ -37,8 +37,8 @@ constexpr int PA_THREADS = 128, PA_WARPS = 4;
 constexpr int PA_UNIT = 64;          // keys of one unit of work
 constexpr int PA_CLUSTER = 8;        // blocks of a cluster, at most
 constexpr int PA_PART_UNITS = 2;     // units of a block down to which clusters grow
-constexpr int PA_FULL_UNITS = 16;    // units of a block up to which clusters are used when they fill the device,
-constexpr int PA_FEW_UNITS = 4;      // and when they do not
+constexpr int PA_FULL_UNITS = 24;    // units of a block up to which clusters are used when they fill the device,
+constexpr int PA_FEW_UNITS = 8;      // and when they do not
 constexpr int PA_JOIN = 512;         // threads of a join's block, at most
 constexpr int PA_MAX_BLOCKS = 592;   // blocks of a wave: four on each of 148 SMs
 constexpr int PA_MAX_ROWS = 32;      // query heads of a piece, at most
@@ -578,10 +578,13 @@ __global__ void __launch_bounds__(PA_JOIN) paged_join_kernel(const PagedAttnArgs
 
 // Blocks of a cluster for pieces of at most `bound` keys, 0: shares.  Clusters
 // grow while their blocks have more than PA_PART_UNITS units and all fit in a
-// wave of three a multiprocessor; they are used for few units a block (bf16
-// 32 x 32/8 x 128: 29 us in clusters and 35 us in shares of 1000 keys each, 94
-// and 93 us of 4000; 1 x 32/8 x 128 of 8000 keys, when they cannot fill the
-// device: 25 and 20 us).
+// wave of three a multiprocessor; they are used for few units a block, since they
+// last as long as the longest request.  (In clusters and in shares, bf16
+// 32 x 32/8 x 128: 25.5 and 32.8 us of 1000 keys each, 18.7 and 20.3 of 1 .. 1000,
+// 43.5 and 51.5 of 2000, 33.8 and 32.6 of 1 .. 2000; f32 on bf16 48 x 12/4 x 80, 31
+// units a block: 48.9 and 53.7 us of 4000, 38.0 and 33.0 of 1 .. 4000.  When they
+// cannot fill the device, bf16 1 x 32/8 x 128: 12.2 and 15.4 us of 4000 keys, 17.4
+// and 16.9 of 8000.)
 inline int pa_clusters(long long items, int bound, int sms) {
     const int units = (bound + PA_UNIT - 1) / PA_UNIT;
     if (items > 3LL * sms) return 0;
@@ -645,7 +648,11 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     // (of 0, 2 and 6 for one head: bf16 32 x 32/8 x 128 of 1 .. 2000 keys 48, 35 and 38 us, of 2000 each 55, 55 and
     // 57 us; the same of 0, 1 and 2 for two, and more than 0 for four loses 2% where the keys are many)
     sh.extra = sh.side == 1 ? 2 : sh.side == 2 ? 1 : 0;
-    const int blocks = items * units < slots ? (int)(items * units) : slots, rows = sh.side * sh.rows;
+    int blocks = items * units < slots ? (int)(items * units) : slots;
+    const int rows = sh.side * sh.rows;
+    // a whole number of shares a piece, if that costs few blocks: requests of one length are cut evenly (bf16
+    // 64 x 32/8 x 128 of 4000 keys: 173 us, 178 us with 592 blocks)
+    if (items <= blocks && blocks / items * items * 5 >= 4LL * blocks) blocks = (int)(blocks / items * items);
     PagedParts parts;
     parts.acc = a.work;
     parts.ml = reinterpret_cast<float2*>(a.work + (size_t)PA_MAX_BLOCKS * 2 * rows * a.dh);
