@@ -303,6 +303,25 @@ def test_pages_outside_the_pool_are_left_out(act, cache, page):
 
 
 @pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("page,window", [(4, 30), (16, 1), (16, 50), (64, 200), (2, 333)])
+def test_what_lies_before_the_window_does_not_matter(act, cache, page, window):
+    """Cells before the window hold NaN, and whole pages before it are gone from the table."""
+    lens = [5, 64, 65, 400, 1500, 0]
+    pool = Pool(lens, 2, 76, page, cache, seed=page)
+    q = torch.randn(len(lens), 6, 76, generator=gen(9), device=DEV).to(act)
+    want, lse = check_attn(pool, q, window=window)
+    for b, n in enumerate(lens):
+        for j in range(max(0, n - window)):
+            if j // page == max(0, n - window) // page:  # the page on which the window begins
+                at = int(pool.table[b, j // page]), j % page
+                pool.kc[at] = float("nan")
+                pool.vc[at] = float("nan")
+        pool.table[b, :max(0, n - window) // page] = -1
+    got, got_lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, window=window, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(got_lse, lse)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
 def test_lengths_outside_the_table(act, cache):
     """Longer than width * page_size: cut there; negative: empty."""
     pool = Pool([64, 64, 64], 2, 64, 16, cache, seed=2)

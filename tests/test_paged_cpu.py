@@ -71,7 +71,7 @@ def test_append_refuses(what, value, word):
 
 
 @pytest.mark.parametrize("what,value,word", POOL + TABLE + TYPES + HEAD + [
-    ("B", -1, "B must"), ("Hq", 0, "Hq"), ("Hkv", 0, "Hkv"), ("Hq", 7, "multiple"), ("Hq", 65536, "65535"),
+    ("B", -1, "B must"), ("B", 1 << 30, "B * Hq"), ("Hq", 0, "Hq"), ("Hkv", 0, "Hkv"), ("Hq", 7, "multiple"), ("Hq", 65536, "65535"),
     ("scale", float("nan"), "scale"), ("scale", float("inf"), "scale"), ("window", -1, "window"),
     ("max_len", -1, "max_len"), ("table", None, "null"), ("lens", None, "null"),
     ("o_sb", 0, "shorter"), ("o_sh", 32, "shorter")]
