@@ -180,7 +180,7 @@ int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void*
     if (Hkv == 1) c_sh = 0;
     const krk::PagedAttnArgs a{q, q_sb, q_sh, kc, vc, c_sp, c_st, c_sh, table, table_ld, width, num_pages, shift,
                                lens, B, Hq, Hkv, dh, scale, window,
-                               bound, out, o_sb, o_sh, lse, work};
+                               bound, out, o_sb, o_sh, lse, work, work ? work_floats : 0};
     return done(who, krk::attn_decode_paged(a, type, cache_type, (cudaStream_t)stream));
 }
 

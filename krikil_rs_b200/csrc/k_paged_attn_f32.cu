@@ -222,18 +222,21 @@ int paged_sm_count() {
 }
 
 size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int window) {
-    // with as many pieces as any engine makes
-    const int sms = paged_sm_count(), share = Hq / Hkv, per_kv = (share + 15) / 16;
-    const int bound = pa_bound(max_len, window);
-    if (pa_clusters((long long)B * Hkv * per_kv, bound, sms > 0 ? sms : 148)) return 0;
+    // the types are not known here: scratch if any engine takes shares, for as many rows as any makes
+    const int sms = paged_sm_count(), share = Hq / Hkv, bound = pa_bound(max_len, window);
     const int rows = 4 * share < PA_MAX_ROWS ? 4 * share : PA_MAX_ROWS;
-    return (size_t)PA_MAX_BLOCKS * (2 * (size_t)rows * (dh + 2) + 2);
+    const int heads[] = {pa_heads_f32(share), share <= PA_HEADS_PACKED ? PA_HEADS_PACKED : PA_HEADS_HALF, PA_HEADS_HALF};
+    for (int h : heads)
+        if (!pa_shape(B, Hq, Hkv, h, bound, sms > 0 ? sms : 148).cluster) return pa_scratch_floats(rows, dh);
+    return 0;
 }
 
 cudaError_t attn_decode_paged_f32(const PagedAttnArgs& a, cudaStream_t s) {
-    const int G = a.Hq / a.Hkv;
-    if (G == 1) return a.dh % 8 ? by_width<1, true>(a, s) : by_width<1, false>(a, s);
-    return G == 2 ? by_width<2, false>(a, s) : by_width<4, false>(a, s);
+    switch (pa_heads_f32(a.Hq / a.Hkv)) {
+        case 1: return a.dh % 8 ? by_width<1, true>(a, s) : by_width<1, false>(a, s);
+        case 2: return by_width<2, false>(a, s);
+        default: return by_width<4, false>(a, s);
+    }
 }
 
 cudaError_t attn_decode_paged_f16(const PagedAttnArgs& a, bool act_f32, cudaStream_t s);

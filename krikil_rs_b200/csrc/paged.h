@@ -74,7 +74,8 @@ struct PagedAttnArgs {
     int max_len;                                     // a bound of the lengths that the launch is sized for
     void* out; int64_t o_sb, o_sh;
     float* lse;                                      // [B][Hq] or nullptr
-    float* work;
+    float* work;                                     // of work_floats, nullptr when clusters take the call
+    size_t work_floats;
 };
 size_t attn_paged_work_floats(int B, int Hq, int Hkv, int dh, int max_len, int window);
 cudaError_t attn_decode_paged(const PagedAttnArgs& a, int act, int cache, cudaStream_t s);

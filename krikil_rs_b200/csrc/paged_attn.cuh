@@ -595,21 +595,36 @@ inline int pa_clusters(long long items, int bound, int sms) {
 inline int pa_bound(int max_len, int window) {  // of a piece's keys
     return window > 0 && window < max_len ? window + PA_ALIGN : max_len;
 }
+// How a launch divides its work, by its engine's query heads a warp.  The size of the scratch and the launch are both
+// taken from here: the rule above is not monotone in the pieces, so that a size from another number of them may find
+// clusters, which need no scratch, where the launch takes shares.
+inline PagedShape pa_shape(int B, int Hq, int Hkv, int heads, int bound, int sms) {
+    const int G = Hq / Hkv;
+    PagedShape sh{1, 1, 1, 0, 0, 0};
+    while (sh.groups < PA_WARPS && sh.groups * heads < G) sh.groups *= 2;
+    sh.per_kv = (G + sh.groups * heads - 1) / (sh.groups * heads);
+    sh.rows = G < sh.groups * heads ? G : sh.groups * heads;
+    sh.cluster = pa_clusters((long long)B * Hkv * sh.per_kv, bound, sms);
+    return sh;
+}
+inline size_t pa_scratch_floats(int rows, int dh) {  // of shares with pieces of `rows` query heads
+    return (size_t)PA_MAX_BLOCKS * (2 * (size_t)rows * (dh + 2) + 2);
+}
+// Query heads a warp of the engines that may take a call of G heads a cache head: on float32 pages, on 16-bit pages,
+// and on 16-bit pages with the parts of float32 queries packed.
+inline int pa_heads_f32(int G) { return G == 1 ? 1 : G == 2 ? 2 : 4; }
+constexpr int PA_HEADS_HALF = 8, PA_HEADS_PACKED = 4;
 
 // E2: the engine with two slots a warp, for clusters, whose few blocks leave room for it (bf16 32 x 32/8 x 128 of 1000
 // keys: 26.5 us, 29.7 us with one).
 template <class E, class E2>
 cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     static_assert(E::HW * (E::DC + 4) * 4 <= 2 * E::SLOTS * E::TILE_BYTES, "a warp's sums fit in its ring");
-    const int G = a.Hq / a.Hkv, sms = paged_sm_count();
+    const int sms = paged_sm_count();
     if (sms <= 0) return cudaErrorInvalidDevice;
-    PagedShape sh{1, 1, 1, 0, 0, 0};
-    while (sh.groups < PA_WARPS && sh.groups * E::HW < G) sh.groups *= 2;
-    sh.per_kv = (G + sh.groups * E::HW - 1) / (sh.groups * E::HW);
-    sh.rows = G < sh.groups * E::HW ? G : sh.groups * E::HW;
     const int bound = pa_bound(a.max_len, a.window);
+    PagedShape sh = pa_shape(a.B, a.Hq, a.Hkv, E::HW, bound, sms);
     long long items = (long long)a.B * a.Hkv * sh.per_kv;
-    sh.cluster = pa_clusters(items, bound, sms);
     if (sh.cluster) {
         static DeviceOnce once;
         constexpr size_t kRing = (size_t)PA_WARPS * 2 * E2::SLOTS * E2::TILE_BYTES;
@@ -650,6 +665,7 @@ cudaError_t launch_paged_attn(const PagedAttnArgs& a, cudaStream_t s) {
     sh.extra = sh.side == 1 ? 2 : sh.side == 2 ? 1 : 0;
     int blocks = items * units < slots ? (int)(items * units) : slots;
     const int rows = sh.side * sh.rows;
+    if (!a.work || a.work_floats < pa_scratch_floats(rows, a.dh)) return cudaErrorInvalidValue;
     // a whole number of shares a piece, if that costs few blocks: requests of one length are cut evenly (bf16
     // 64 x 32/8 x 128 of 4000 keys: 173 us, 178 us with 592 blocks)
     if (items <= blocks && blocks / items * items * 5 >= 4LL * blocks) blocks = (int)(blocks / items * items);

@@ -98,7 +98,7 @@ struct HalfEngine {
     using Cache = C;
     static constexpr bool kSame = sizeof(T) == 2, kHalf = sizeof(__half) == 2 && std::is_same<C, __half>::value;
     static constexpr int DC = DC_, KT = 16, HW = HW_;
-    static constexpr bool kPacked = HW == 4;  // parts lie in the rows and columns of four heads that are not there
+    static constexpr bool kPacked = HW == PA_HEADS_PACKED;  // parts lie in the rows and columns of four heads that are not there
     static constexpr int NB = DC / 32, NV = DC / 16;     // steps of the two products
     static constexpr int CPR = DC <= 64 ? 8 : DC <= 128 ? 16 : 32, ROW = CPR * 16;  // a row's 16-byte pieces and bytes
     static constexpr int RPC = 32 / CPR;                  // rows of one copy
@@ -392,8 +392,8 @@ cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
 template <typename T, typename C, int ALIGN>
 cudaError_t by_heads(const PagedAttnArgs& a, cudaStream_t s) {
     if constexpr (sizeof(T) == 4)
-        if (a.Hq / a.Hkv <= 4) return by_width<T, C, ALIGN, 4>(a, s);
-    return by_width<T, C, ALIGN, 8>(a, s);
+        if (a.Hq / a.Hkv <= PA_HEADS_PACKED) return by_width<T, C, ALIGN, PA_HEADS_PACKED>(a, s);
+    return by_width<T, C, ALIGN, PA_HEADS_HALF>(a, s);
 }
 
 template <typename T, typename C>
@@ -403,7 +403,7 @@ cudaError_t by_alignment(const PagedAttnArgs& a, cudaStream_t s) {
                       (reinterpret_cast<uintptr_t>(a.vc) & 15) == 0;
     if (wide) return by_heads<T, C, ROWS_WIDE>(a, s);
     if (same && a.dh <= 252) return by_heads<T, C, ROWS_SHIFTED>(a, s);
-    return by_width<T, C, ROWS_NARROW, 8>(a, s);
+    return by_width<T, C, ROWS_NARROW, PA_HEADS_HALF>(a, s);
 }
 
 }  // namespace

@@ -355,6 +355,19 @@ def test_scratch_that_is_too_small_is_refused():
     K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=torch.empty(need, device=DEV))
 
 
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("b,hq,dh,page,longest,window", [
+    (10, 32, 64, 16, 8192, 0), (10, 17, 128, 64, 5000, 0), (7, 48, 64, 8, 6000, 0), (4, 71, 80, 32, 12000, 0),
+    (5, 64, 76, 16, 9000, 0), (10, 24, 64, 4, 9000, 5000)])
+def test_many_heads_on_one_cache_head(act, cache, b, hq, dh, page, longest, window):
+    """17 and more query heads a cache head, at bounds where the number of pieces, which differs from type to type,
+    decides between clusters and shares: whichever a type takes has its scratch."""
+    lens = [longest, 0, 1, longest // 2] + [longest - 17 * i for i in range(b - 4)]
+    pool = Pool(lens, 1, dh, page, cache, seed=hq)
+    assert K.attn_paged_work_floats(b, hq, 1, dh, pool.table.shape[1] * page, window) > 0
+    check_attn(pool, torch.randn(b, hq, dh, generator=gen(hq), device=DEV).to(act), window=window)
+
+
 @pytest.mark.parametrize("act,cache", [(F32, F32), (F32, BF16), (BF16, BF16), (F16, F16)])
 def test_attention_replayed_from_a_graph_on_another_stream(act, cache):
     """A captured call follows the lengths, table and queries that it finds at replay, beside eager calls of the

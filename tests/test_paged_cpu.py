@@ -104,6 +104,45 @@ def test_sizes_of_the_attention_scratch():
         assert f(*bad) == 0
 
 
+def clusters(items, units, sms):
+    """Whether a launch of so many pieces of so many 64-key units takes clusters, which need no scratch (shares do):
+    up to 8 blocks a piece in a wave of three a multiprocessor, 24 units a block, 8 when the device is not full."""
+    if items > 3 * sms:
+        return False
+    n = 1
+    while n < 8 and units > 2 * n and items * 2 * n <= 3 * sms:
+        n *= 2
+    return units <= (24 if items * n >= sms else 8) * n
+
+
+def pieces(g, heads):
+    """Of a cache head with g query heads, `heads` of them a warp, 1, 2 or 4 warps side by side."""
+    groups = 1 if g <= heads else 2 if g <= 2 * heads else 4
+    return -(-g // (groups * heads))
+
+
+def test_scratch_for_every_launch_that_takes_shares():
+    """The types are not known to the size of the scratch, and engines differ in their pieces: whichever takes shares
+    must have got some."""
+    f = lib.krk_attn_paged_work_floats
+    sms = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148
+    bounds = [1, 64, 65, 128, 129, 500, 1000, 1500, 2048, 3000, 4096, 4097, 5000, 6144, 6145, 8000, 8192, 10000, 12288,
+              12289, 16000, 20000, 24576, 32768]
+    for g in range(1, 129):
+        engines = {1 if g == 1 else 2 if g == 2 else 4, 8}
+        for heads in [*range(1, 160), 161, 199, 222, 223, 296, 297, 444, 445, 500]:  # B * Hkv
+            for n in bounds:
+                if not all(clusters(heads * pieces(g, e), -(-n // 64), sms) for e in engines):
+                    assert f(heads, g, 1, 64, n, 0) > 0, (g, heads, n)
+
+
+@pytest.mark.parametrize("b,hq,hkv,dh,n,window", [(10, 32, 1, 64, 8192, 0), (10, 32, 1, 128, 8000, 0),
+                                                  (5, 64, 2, 64, 4097, 0), (8, 48, 1, 128, 100000, 6000),
+                                                  (4, 71, 1, 64, 12000, 0), (3, 128, 1, 64, 12288, 0)])
+def test_scratch_for_many_heads_on_one_cache_head(b, hq, hkv, dh, n, window):
+    assert lib.krk_attn_paged_work_floats(b, hq, hkv, dh, n, window) > 0
+
+
 def test_wrappers_refuse_cpu_tensors():
     i = torch.zeros(2, dtype=torch.int32)
     x = torch.zeros(2, 2, 64)
