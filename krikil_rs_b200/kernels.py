@@ -236,8 +236,13 @@ def _table(t, dev):
     shape, strides = t.shape, t.stride()
     if t.dtype != torch.int32 or len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or t.device != dev:
         raise ValueError(f"table: expected an int32 [requests, pages] tensor on {dev} with dense rows")
-    width, ld = shape[1], strides[0]
-    return shape[0], width, ld if ld > width else width
+    rows, width = shape
+    ld = strides[0]
+    if ld < width:  # the stride of a single row does not matter
+        if rows > 1:
+            raise ValueError("table: rows that overlap (an expanded row?) must be copied out first")
+        ld = width
+    return rows, width, ld
 
 
 def _pool(kc, vc, dev):

@@ -872,3 +872,20 @@ def test_wrappers_refuse_what_does_not_belong_together():
         K.kv_page_plan(two, pool.lens, pool.table, free, one, 16, -1)
     with pytest.raises(ValueError):
         K.kv_page_release(two, *(pool.lens, pool.table, free, one), 16)
+
+
+def test_wrappers_refuse_an_expanded_table():
+    """One row for several requests (stride 0): refused by every call, before anything is read or written."""
+    pool = Pool([40], 2, 64, 16, F32, seed=2)
+    q = torch.randn(2, 4, 64, device=DEV)
+    two, free, one = i32([40, 40]), i32([0, 1]), i32([1])
+    shared = pool.table.expand(2, -1)
+    with pytest.raises(ValueError, match="table"):
+        K.attn_decode_paged(q, pool.kc, pool.vc, shared, two)
+    with pytest.raises(ValueError, match="table"):
+        K.kv_page_plan(i32([1, 1]), two, shared, free, one, 16, 4)
+    with pytest.raises(ValueError, match="table"):
+        K.kv_page_release(torch.tensor([True, False], device=DEV), two, shared, free, one, 16)
+    out = K.attn_decode_paged(q, pool.kc, pool.vc, shared.contiguous(), two)
+    alone = K.attn_decode_paged(q[:1], pool.kc, pool.vc, pool.table, pool.lens)
+    assert torch.equal(out[:1], alone)

@@ -143,6 +143,19 @@ def test_scratch_for_many_heads_on_one_cache_head(b, hq, hkv, dh, n, window):
     assert lib.krk_attn_paged_work_floats(b, hq, hkv, dh, n, window) > 0
 
 
+def test_table_rows_that_lie_closer_than_their_width_are_refused():
+    """A row expanded over the requests, or a sliding view: rows must not be taken to lie `width` apart."""
+    cpu = torch.device("cpu")
+    row = torch.arange(6, dtype=torch.int32)
+    for bad in (row[None].expand(3, 6), row.as_strided((3, 4), (1, 1)), row[:1].expand(2, 1)):
+        with pytest.raises(ValueError, match="table"):
+            K._table(bad, cpu)
+    assert K._table(row[None], cpu) == (1, 6, 6) and K._table(row.expand(1, 6), cpu) == (1, 6, 6)
+    assert K._table(row.as_strided((1, 6), (0, 1)), cpu) == (1, 6, 6)  # one row: its stride does not matter
+    assert K._table(torch.zeros(3, 9, dtype=torch.int32)[:, 2:7], cpu) == (3, 5, 9)
+    assert K._table(row[None][:0], cpu) == (0, 6, 6)
+
+
 def test_wrappers_refuse_cpu_tensors():
     i = torch.zeros(2, dtype=torch.int32)
     x = torch.zeros(2, 2, 64)
