@@ -387,6 +387,10 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
     holds).  `work` is scratch of attn_paged_work_floats floats (allocated here
     when not given).  Returns out [B, Hq, dh], or (out, lse)."""
     dev = _cuda_device(q)
+    index = dev.index
+    if index != _current_device():  # the scratch is sized for the current device
+        with torch.cuda.device(dev):
+            return attn_decode_paged(q, kc, vc, table, lens, scale, window, max_len, out, work, return_lse)
     ctype, (pages, page_size, hkv, dh), (c_sp, c_st, c_sh, _) = _pool(kc, vc, dev)
     kind, shape, (q_sb, q_sh, _) = _elems3(q, dev, "q")
     b, hq, qdh = shape
@@ -418,11 +422,7 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
             ld, width, pages, page_size, _ints(lens, b, dev, "lens"), b, hq, hkv, dh,
             dh ** -0.5 if scale is None else scale, window, max_len, out.data_ptr(), o_sb, o_sh, lse_at, work_at,
             need)
-    index = dev.index
-    if index == _current_device():
-        rc = lib.krk_k_attn_decode_paged(*args, _raw_stream(index))
-    else:
-        rc = _elsewhere(dev, lib.krk_k_attn_decode_paged, *args)
+    rc = lib.krk_k_attn_decode_paged(*args, _raw_stream(index))
     if rc:
         check(rc)
     return (out, lse) if return_lse else out

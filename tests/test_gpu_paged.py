@@ -889,3 +889,49 @@ def test_wrappers_refuse_an_expanded_table():
     out = K.attn_decode_paged(q, pool.kc, pool.vc, shared.contiguous(), two)
     alone = K.attn_decode_paged(q[:1], pool.kc, pool.vc, pool.table, pool.lens)
     assert torch.equal(out[:1], alone)
+
+
+def test_calls_run_with_their_tensors_device_current(monkeypatch):
+    """With another device current, every library call -- the size of the scratch, which depends on the device, too --
+    is made with the tensors' device current, on that device's stream, and the other device is current again behind
+    it.  (The other device is pretended: what the wrappers ask and set is stood in for.)"""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, dev):
+            self.index = dev.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append((name, current[0]))
+                return getattr(lib, name)(*args)
+            return call
+
+    lib = K.lib
+    pool = Pool([9000, 40], 2, 64, 16, BF16, seed=2)
+    q = torch.randn(2, 4, 64, device=DEV).to(BF16)
+    slots, new = i32([-1, 3]), i32([0, 0])
+    free, count = i32(range(pool.pages)), i32([2])
+
+    def calls():
+        b = K.rope_kv_append_paged(q, q[:, :2], q[:, :2], pool.kc, pool.vc, slots, slots)[1]
+        a = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, return_lse=True)
+        c = K.kv_page_plan(new, pool.lens, pool.table, free, count, 16, 4)
+        d = K.kv_page_release(new.bool(), pool.lens, pool.table, free, count, 16)
+        return [*a, b, *c, *d]
+
+    here = calls()
+    monkeypatch.setattr(K, "lib", Lib())
+    monkeypatch.setattr(K, "_current_device", lambda: current[0])
+    monkeypatch.setattr(K.torch.cuda, "device", Device)
+    current[0] = 1
+    there = calls()
+    assert all(torch.equal(x, y) for x, y in zip(here, there))
+    assert len(seen) == 5 and all(dev == 0 for _, dev in seen) and current[0] == 1, seen
