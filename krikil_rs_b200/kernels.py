@@ -205,6 +205,12 @@ def _elsewhere(dev, fn, *args) -> int:
         return fn(*args, _raw_stream(dev.index))
 
 
+def _number(x, name) -> None:
+    """Refuses what does not fit the 31 bits that the library takes (more would be cut off on the way)."""
+    if x >> 31:
+        raise ValueError(f"{name} must lie between 0 and 2^31 - 1")
+
+
 def _cuda_device(t):
     if not t.is_cuda:
         raise ValueError("expected CUDA tensors")
@@ -271,8 +277,8 @@ def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int
     new_at, lens_at = _ints(new_tokens, b, dev, "new_tokens"), _ints(lens, b, dev, "lens")
     pages = free_pages.numel()
     free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
-    if rows < 0:
-        raise ValueError("rows must not be negative")
+    _number(rows, "rows")
+    _number(page_size, "page_size")
     padded = -rows % 4 + rows
     buf = lens.new_empty(2 * padded + 2 * b + 3)
     positions, _, slots, _, cu, lens_new, count_new, status = buf.unsafe_split_with_sizes(
@@ -307,6 +313,7 @@ def kv_page_release(done, lens, table, free_pages, free_count, page_size: int, l
     b, width, ld = _table(table, dev)
     if done.dtype not in (torch.bool, torch.uint8) or done.numel() != b or done.device != dev or not done.is_contiguous():
         raise ValueError(f"done: expected a contiguous bool or uint8 tensor of {b} elements on {dev}")
+    _number(page_size, "page_size")
     lens_at, pages = _ints(lens, b, dev, "lens"), free_pages.numel()
     free_at, count_at = _ints(free_pages, pages, dev, "free_pages"), _ints(free_count, 1, dev, "free_count")
     buf = lens.new_empty(b + 2)
@@ -360,10 +367,12 @@ def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000
             if oshape != qshape or okind != kind:
                 raise ValueError("q_out: expected q's shape and type")
         q_at, o_at = q.data_ptr(), q_out.data_ptr()
+    rot_dim = dh if rot_dim is None else rot_dim
+    _number(rot_dim, "rot_dim")
     args = (q_at, q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, kind, o_at, o_st, o_sh,
             kc.data_ptr(), vc.data_ptr(), c_sp, c_st, c_sh, ctype, _ints(slots, t, dev, "slots"),
-            _ints(positions, t, dev, "positions"), t, hq, hkv, dh, dh if rot_dim is None else rot_dim, pages,
-            page_size, theta)
+            _ints(positions, t, dev, "positions"), t, hq, hkv, dh, rot_dim, pages, page_size,
+            theta)
     index = dev.index
     if index == _current_device():
         rc = lib.krk_k_rope_kv_append_paged(*args, _raw_stream(index))
@@ -403,6 +412,8 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
         okind, oshape, (o_sb, o_sh, _) = _elems3(out, dev, "out")
         if oshape != shape or okind != kind:
             raise ValueError("out: expected q's shape and type")
+    _number(window, "window")
+    _number(max_len, "max_len")
     lse, lse_at = None, None
     if return_lse:
         lse = torch.empty(b, hq, device=dev, dtype=torch.float32)

@@ -935,3 +935,24 @@ def test_calls_run_with_their_tensors_device_current(monkeypatch):
     there = calls()
     assert all(torch.equal(x, y) for x, y in zip(here, there))
     assert len(seen) == 5 and all(dev == 0 for _, dev in seen) and current[0] == 1, seen
+
+
+@pytest.mark.parametrize("far", [2 ** 32, -2 ** 32, 2 ** 31, -1])
+def test_wrappers_refuse_numbers_past_31_bits(far):
+    """A window of 2^32 + 5 is not one of 5."""
+    pool = Pool([40], 2, 64, 16, F32, seed=2)
+    q = torch.randn(1, 4, 64, device=DEV)
+    free, one = i32([0, 1]), i32([1])
+    with pytest.raises(ValueError, match="window"):
+        K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, window=far + 5 * (far > 2))
+    with pytest.raises(ValueError, match="max_len"):
+        K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, max_len=far)
+    with pytest.raises(ValueError, match="rot_dim"):
+        K.rope_kv_append_paged(q, q[:, :2], q[:, :2], pool.kc, pool.vc, one, one, rot_dim=far + 64 * (far > 2))
+    for size in (dict(page_size=far + 16 * (far > 2), rows=4), dict(page_size=16, rows=far)):
+        with pytest.raises(ValueError, match="page_size" if size["rows"] == 4 else "rows"):
+            K.kv_page_plan(one, pool.lens, pool.table, free, one, **size)
+    with pytest.raises(ValueError, match="page_size"):
+        K.kv_page_release(one.bool(), pool.lens, pool.table, free, one, far + 16 * (far > 2))
+    wide = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, window=2 ** 31 - 1, max_len=2 ** 31 - 1)
+    assert torch.equal(wide, K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens))
