@@ -448,7 +448,8 @@ KRK_API int krk_k_wait_probe(const float* src16, int polls, int copy, int32_t* s
  * overlap.  *status is 0, or the KRK_PAGES_* bits of what does not fit: then
  * nothing is taken (table untouched, lens_out = lens, free_count_out =
  * free_count), cu_new is 0 and every slot -1.  Page ids on the list are copied
- * as they are. */
+ * as they are; a token whose page lies outside the pool gets slot -1 (reported
+ * by checked builds). */
 KRK_API int krk_k_kv_page_plan(const int32_t* new_tokens, const int32_t* lens, int32_t* table, int64_t table_ld,
                                int B, int width, const int32_t* free_pages, const int32_t* free_count, int num_pages,
                                int page_size, int32_t* lens_out, int32_t* free_count_out, int32_t* cu_new,

@@ -189,7 +189,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_co
                     const int page = p < sc.have[i]
                                          ? a.table[(b0 + i) * a.table_ld + p]
                                          : a.free_pages[count - 1 - base_p - (sc.pages[i] + p - sc.have[i])];
-                    slot[k] = (int)((unsigned)page << shift) + (pos[k] & low);
+                    const bool in = (unsigned)page < (unsigned)a.num_pages;  // (another's slots may wrap into the pool)
+                    if (!in) check_fail(CHK_TABLE);
+                    slot[k] = in ? (page << shift) + (pos[k] & low) : -1;
                 }
             });
         }

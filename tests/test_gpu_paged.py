@@ -956,3 +956,31 @@ def test_wrappers_refuse_numbers_past_31_bits(far):
         K.kv_page_release(one.bool(), pool.lens, pool.table, free, one, far + 16 * (far > 2))
     wide = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, window=2 ** 31 - 1, max_len=2 ** 31 - 1)
     assert torch.equal(wide, K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens))
+
+
+@pytest.mark.parametrize("page", [1, 4, 64, 65536])
+@pytest.mark.parametrize("tokens", [3, 6000])
+def test_planned_slots_of_pages_outside_the_pool(page, tokens):
+    """Ids that are no pages, on the stack or in a row: copied as they are, and their tokens get slot -1, also where
+    id * page_size leaves 32 bits and comes back to a slot of the pool."""
+    per = -(-tokens // page)
+    bad = [2 ** 32 // page % 2 ** 31 + 1, -1, 2 * per + 4, 2 ** 31 - 1, -2 ** 31]
+    num_pages = 2 * per + 4
+    free = list(range(num_pages))
+    held = bad[::-1]  # a request that holds five pages, all of them gone, the last one with a token to spare
+    table = i32([held + [7] * (per + 1), [7] * (per + 6)])
+    for i, x in enumerate(bad):
+        if num_pages - 1 - i >= 0:
+            free[num_pages - 1 - i] = x
+    new, lens = [tokens, tokens], [5 * page - (page > 1), 0]
+    out = K.kv_page_plan(i32(new), i32(lens), table, i32(free), i32([num_pages]), page, 2 * tokens)
+    assert out[5].item() == 0
+    rows = [list(held), []]
+    want = []
+    for b in range(2):
+        while len(rows[b]) < -(-(lens[b] + new[b]) // page):
+            rows[b].append(free.pop())
+        assert table[b, :len(rows[b])].tolist() == rows[b]
+        at = [(j // page, j % page) for j in range(lens[b], lens[b] + new[b])]
+        want += [rows[b][p] * page + o if 0 <= rows[b][p] < num_pages else -1 for p, o in at]
+    assert out[4].tolist() == want and out[3].tolist() == [j for b in range(2) for j in range(lens[b], lens[b] + new[b])]
