@@ -457,9 +457,12 @@ KRK_API int krk_k_kv_page_plan(const int32_t* new_tokens, const int32_t* lens, i
 
 /* Puts the pages of every request with done_mask[b] != 0 back on the stack, in
  * request order and each request's pages in table order, and sets lens_out[b]
- * to 0 (lens[b] for the others); the table is left as it is.  Pages belong to one
- * request each: a caller that shares pages among requests keeps count of them itself.  Aliasing and
- * *status as above: with a bit set nothing changes. */
+ * to 0 (lens[b] for the others); the table is left as it is.  A negative entry is
+ * skipped: a caller that gives back pages which a window has left behind, before
+ * their request has finished, sets their entries to -1 (an entry that stays is
+ * put on the stack once more, and two requests get that page).  Pages belong to
+ * one request each: a caller that shares pages among requests keeps count of them
+ * itself.  Aliasing and *status as above: with a bit set nothing changes. */
 KRK_API int krk_k_kv_page_release(const uint8_t* done_mask, const int32_t* lens, const int32_t* table,
                                   int64_t table_ld, int B, int width, int32_t* free_pages,
                                   const int32_t* free_count, int num_pages, int page_size, int32_t* lens_out,

@@ -207,6 +207,34 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const __grid_co
     }
 }
 
+// Puts entries 0 .. n - 1, which `id` gives, on the stack in their order, without the negative ones; returns how many.
+// `id` may read them from the stack itself, where they lie in the same order from the first one on.
+template <typename F>
+KRK_DEV int push_pages(int32_t* stack, int n, PlanScratch& sc, F id) {
+    const int tid = threadIdx.x, nt = blockDim.x;
+    int kept = 0;
+    for (int j0 = 0; j0 < n; j0 += nt) {
+        const bool mine = tid < n - j0;
+        const int page = mine ? id(j0 + tid) : -1;
+        if (__syncthreads_and(page >= 0 || !mine)) {
+            if (mine) stack[kept + tid] = page;
+            kept += min(nt, n - j0);
+        } else {
+            long long total;
+            const int before = (int)block_scan(page >= 0, total, sc);
+            if (page >= 0) stack[kept + before] = page;
+            kept += (int)total;
+        }
+    }
+    return kept;
+}
+
+// Negative entries of a row are pages that the caller has given back already.  The rule is that there are none: the
+// entries are written as they are, and one block closes the gaps behind them if there are any.  The kernel that fills
+// leaves word of gaps in the status, which the commit writes in any case (were the word there by chance, nothing would
+// be found to close).  Only when the entries would not fit with the negative ones does one block count them first.
+constexpr int PAGES_GAPS = INT32_MIN;
+
 template <int MODE>
 __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const __grid_constant__ PageReleaseArgs a) {
     __shared__ PlanScratch sc;
@@ -226,32 +254,69 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_release_kernel(const __grid
             pages += held;
     }
     block_sum2(pages, unused, sc);
-    if (count + pages > a.num_pages) err |= PAGES_OVERFLOW;
+    if (pages > INT32_MAX) err |= PAGES_OVERFLOW;
+    const bool fits = count + pages <= a.num_pages;
     if (err) atomicOr(&sc.bad, err);
     __syncthreads();
     err = sc.bad;
+    if (err && !fits) err |= PAGES_OVERFLOW;
+    if (MODE == PLAN_FILL && (err || !fits)) return;
     if (MODE == PLAN_COMMIT) pdl_wait();  // the other kernel has read what is written here
-    int base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += nt) {
-        const int b = b0 + tid, n = min(nt, a.B - b0);
-        const int len = tid < n ? a.lens[b] : 0;
-        const bool gone = !err && tid < n && a.done[b];
-        long long total;
-        const int before = (int)block_scan(gone ? pages_for(len, shift) : 0, total, sc);
-        sc.pages[tid] = before;
-        __syncthreads();
-        if (MODE != PLAN_FILL && tid < n) a.lens_out[b] = gone ? 0 : len;
-        if (MODE != PLAN_COMMIT)
-            for (int j = thread; j < (int)total; j += threads) {
-                const int i = bisect(sc.pages, n, j);
-                a.free_pages[count + base + j] = a.table[(b0 + i) * a.table_ld + j - sc.pages[i]];
-            }
-        base += (int)total;
-        __syncthreads();
+    // The requests, a chunk of them at a time: use(b0, n, len, gone, total) with this thread's request and the entries of
+    // all that are gone, of which entry(b0, n, j) is one.
+    auto walk = [&](auto use) {
+        for (int b0 = 0; b0 < a.B; b0 += nt) {
+            const int b = b0 + tid, n = min(nt, a.B - b0);
+            const int len = tid < n ? a.lens[b] : 0;
+            const bool gone = !err && tid < n && a.done[b];
+            long long total;
+            const int before = (int)block_scan(gone ? pages_for(len, shift) : 0, total, sc);
+            sc.pages[tid] = before;
+            __syncthreads();
+            use(b0, n, len, gone, (int)total);
+            __syncthreads();
+        }
+    };
+    auto entry = [&](int b0, int n, int j) {
+        const int i = bisect(sc.pages, n, j);
+        return a.table[(b0 + i) * a.table_ld + j - sc.pages[i]];
+    };
+    if (MODE != PLAN_FILL && !err && !fits) {
+        long long real = 0;
+        walk([&](int b0, int n, int, bool, int total) {
+            for (int j = tid; j < total; j += nt) real += entry(b0, n, j) >= 0;
+        });
+        block_sum2(real, unused, sc);
+        if (count + real > a.num_pages) err = PAGES_OVERFLOW;
     }
-    if (MODE != PLAN_FILL && tid == 0) {
+    int32_t* stack = a.free_pages + count;
+    int kept = 0;
+    bool gaps = false;
+    walk([&](int b0, int n, int len, bool gone, int total) {
+        if (MODE != PLAN_FILL && tid < n) a.lens_out[b0 + tid] = gone ? 0 : len;
+        if (MODE != PLAN_FILL && !fits) {
+            kept += push_pages(stack + kept, total, sc, [&](int j) { return entry(b0, n, j); });
+            return;
+        }
+        if (MODE != PLAN_COMMIT)
+            for (int j = thread; j < total; j += threads) {
+                const int page = entry(b0, n, j);
+                stack[kept + j] = page;
+                gaps |= page < 0;
+            }
+        kept += total;
+    });
+    if (MODE == PLAN_FILL) {
+        if (gaps) *a.status = PAGES_GAPS;
+        return;
+    }
+    if (MODE == PLAN_ALL) gaps = __syncthreads_or(gaps);
+    if (MODE == PLAN_COMMIT) gaps = fits && __ldcg(a.status) == PAGES_GAPS;
+    if (gaps) kept = push_pages(stack, kept, sc, [&](int j) { return stack[j]; });
+    __syncthreads();  // the word has been read
+    if (tid == 0) {
         *a.status = err;
-        *a.free_count_out = count + base;
+        *a.free_count_out = count + kept;
     }
 }
 

@@ -307,8 +307,9 @@ def kv_page_plan(new_tokens, lens, table, free_pages, free_count, page_size: int
 
 def kv_page_release(done, lens, table, free_pages, free_count, page_size: int, lens_out=None, free_count_out=None):
     """Puts the pages of the requests whose done flag (bool or uint8 [B]) is set
-    back on the stack free_pages, in place, and their lengths to 0.  Returns
-    (lens_out, free_count_out, status)."""
+    back on the stack free_pages, in place, and their lengths to 0.  Negative
+    entries of their rows are skipped: set those of pages that were given back
+    before (behind a window) to -1.  Returns (lens_out, free_count_out, status)."""
     dev = _cuda_device(table)
     b, width, ld = _table(table, dev)
     if done.dtype not in (torch.bool, torch.uint8) or done.numel() != b or done.device != dev or not done.is_contiguous():

@@ -984,3 +984,101 @@ def test_planned_slots_of_pages_outside_the_pool(page, tokens):
         at = [(j // page, j % page) for j in range(lens[b], lens[b] + new[b])]
         want += [rows[b][p] * page + o if 0 <= rows[b][p] < num_pages else -1 for p, o in at]
     assert out[4].tolist() == want and out[3].tolist() == [j for b in range(2) for j in range(lens[b], lens[b] + new[b])]
+
+
+@pytest.mark.parametrize("batch,width,page,most", [(1, 6, 16, 96), (5, 40, 4, 160), (700, 5, 8, 40), (60, 300, 16, 4800),
+                                                   (1500, 33, 1, 33), (3, 9000, 2, 18000), (2048, 2, 8, 16)])
+@pytest.mark.parametrize("gone", [0.0, 0.001, 0.3, 1.0])
+@pytest.mark.parametrize("full", [False, True])
+def test_release_skips_entries_that_were_given_back(batch, width, page, most, gone, full):
+    """Negative entries of finished rows are left out, the others keep their order.  Where all of a pool's pages come
+    back (`full`), the entries with the negative ones are more than the stack holds; one page fewer, and nothing
+    changes."""
+    rng = np.random.default_rng(batch + width)
+    lens = [int(x) for x in rng.integers(0, most + 1, batch)]
+    done = rng.random(batch) < 0.7
+    held = [-(-n // page) for n in lens]
+    ids = iter(rng.permutation(sum(held) + 5).tolist())
+    rows = [[next(ids) for _ in range(n)] for n in held]
+    left = list(ids)
+    for row in rows:
+        for i in range(len(row)):
+            if rng.random() < gone:
+                left.append(row[i])
+                row[i] = -1 if i % 2 else -2 ** 31
+    num_pages = sum(held) + 5
+    back = [x for row, d in zip(rows, done) if d for x in row if x >= 0]
+    if full:  # the pages that stay with their requests are not of this pool
+        num_pages = len(left) + len(back)
+    free = left + [77] * (num_pages - len(left))
+    table = i32([row + [5] * (width - len(row)) for row in rows])
+
+    def release(free, lens_d, count):
+        return K.kv_page_release(torch.tensor(done, device=DEV), lens_d, table, free, count, page, lens_out=lens_d,
+                                 free_count_out=count)[2].item()
+
+    stack, lens_d, count = i32(free), i32(lens), i32([len(left)])
+    assert release(stack, lens_d, count) == 0
+    assert lens_d.tolist() == [0 if d else n for n, d in zip(lens, done)]
+    assert count.item() == len(left) + len(back)
+    assert stack[:count.item()].tolist() == left + back
+    if full and back:
+        if num_pages > 1:
+            short, lens_d, count = i32(free[:-1]), i32(lens), i32([min(len(left), num_pages - 1)])
+            assert release(short, lens_d, count) == PAGES_OVERFLOW
+            assert lens_d.tolist() == lens and short.tolist() == free[:-1] and count.item() == len(left)
+
+
+@pytest.mark.parametrize("hq,hkv,dh,page,window", [(4, 2, 64, 4, 10), (8, 8, 76, 16, 40)])
+def test_serving_with_pages_given_back_behind_a_window(hq, hkv, dh, page, window):
+    """Requests of one token a step whose pages go back as the window leaves them behind: no page is ever held twice,
+    and attention is that of plain attention over the window."""
+    batch, width, num_pages = 5, 24, 40
+    rng = np.random.default_rng(page)
+    g = gen(page)
+    kc, vc = (torch.full((num_pages, page, hkv, dh), float("nan"), device=DEV) for _ in range(2))
+    d = dict(lens=i32([0] * batch), table=i32([[-1] * width] * batch), free=i32(list(range(num_pages))),
+             count=i32([num_pages]))
+    keys = [[[], []] for _ in range(batch)]
+    for step in range(3 * width * page // 4):
+        lens = d["lens"].tolist()
+        done = [n >= width * page or (n > 0 and rng.random() < 0.01) for n in lens]
+        kw = dict(lens_out=d["lens"], free_count_out=d["count"])
+        status = K.kv_page_release(torch.tensor(done, device=DEV), d["lens"], d["table"], d["free"], d["count"], page,
+                                   **kw)[2]
+        new = [1 if n and not x else int(rng.integers(0, 2 * page)) for n, x in zip(lens, done)]
+        plan = K.kv_page_plan(i32(new), d["lens"], d["table"], d["free"], d["count"], page, 16 * page, **kw)
+        assert status.item() == 0 and plan[5].item() == 0
+        rows = sum(new)
+        q, k, v = (torch.randn(16 * page, h, dh, generator=g, device=DEV) for h in (hq, hkv, hkv))
+        K.rope_kv_append_paged(q, k, v, kc, vc, plan[4], plan[3], rot_dim=0, q_out=q)
+        owner = [b for b in range(batch) for _ in range(new[b])]
+        for b in range(batch):
+            if done[b]:
+                keys[b] = [[], []]
+        for r, b in enumerate(owner):
+            keys[b][0].append(k[r])
+            keys[b][1].append(v[r])
+        view = Pool.__new__(Pool)
+        view.lens_h = d["lens"].tolist()
+        assert view.lens_h == [len(x[0]) for x in keys] and rows == len(owner)
+        view.k = [torch.stack(x[0]) if x[0] else None for x in keys]
+        view.v = [torch.stack(x[1]) if x[1] else None for x in keys]
+        last = q[(plan[2][1:] - 1).clamp_min(0).long()]
+        out = K.attn_decode_paged(last, kc, vc, d["table"], d["lens"], window=window)
+        if step % 7 == 0:
+            ref, _, tol, _ = attn_reference(view, last, 1 / math.sqrt(dh), window)
+            assert ((out.double() - ref).abs() <= tol).all()
+        # what the next token's window has left behind goes back
+        table, free = d["table"].tolist(), d["free"][:d["count"].item()].tolist()
+        for b, n in enumerate(view.lens_h):
+            for i in range(max(0, n + 1 - window) // page):
+                if table[b][i] >= 0:
+                    free.append(table[b][i])
+                    table[b][i] = -1
+            assert all(x >= 0 for x in table[b][max(0, n + 1 - window) // page:-(-n // page)])
+        here = [x for b, n in enumerate(view.lens_h) for x in table[b][:-(-n // page)] if x >= 0]
+        assert sorted(here + free) == list(range(num_pages))
+        d["table"].copy_(i32(table))
+        d["free"][:len(free)] = i32(free)
+        d["count"].fill_(len(free))
