@@ -27,6 +27,7 @@ struct F32Engine {
     static constexpr int J = 8 / NL;                   // key steps of a tile
     static constexpr int KPL = 32 / LPK;               // keys side by side
     static constexpr int KT = J * KPL;                 // 16, 8 or 4 keys
+    static constexpr bool PARTS = false;
     static constexpr int Q_BYTES = 0;
     static constexpr int TILE_BYTES = 8 * 512, SLOTS = SLOTS_;
     static constexpr int BLOCKS = SLOTS == 1 ? 4 : 3;
@@ -148,6 +149,9 @@ struct F32Engine {
             l[h] = l[h] * fade[h] + s[h];
         }
     }
+    KRK_DEV bool spoilt() const { return false; }
+    KRK_DEV void resume(const PagedAttnArgs&, const float*, const float*, float) {}
+    template <bool AGAIN>
     KRK_DEV void values(const unsigned char* from, int lane) {
         float4 v[8];
 #pragma unroll

@@ -228,7 +228,8 @@ KRK_DEV void pa_copy(uint32_t to, const void* from, bool take) {
 //   issue(base, tile, to)       starts the copies of a tile's keys or values to a ring slot
 //   scores(qs, from)            q . k of the slot's keys
 //   weigh(mask)                 softmax step over the visible keys of the tile
-//   values(from)                weighted values into the accumulators
+//   values<again>(from)         weighted values into the accumulators
+//   spoilt()                    whether sums are NaN that may not be, and the tiles are to be taken again
 //   finish(obuf, m, l)          accumulators, maxima and sums of the warp to shared memory
 // A warp's ring has SLOTS slots for keys and as many for values; a slot is
 // filled again as soon as the warp has read it, with no barrier beyond the warp.
@@ -291,6 +292,76 @@ KRK_DEV void pa_join_cluster(const PagedAttnArgs& a, const PagedShape& sh, const
     }
 }
 
+// A warp's tiles of a piece: the keys from `key` on, `step` apart, up to k1.  pages: of the first tiles; prepare: run
+// while those are on their way.
+template <class E, bool AGAIN, class F>
+KRK_DEV void pa_tiles(E& e, const PagedAttnArgs& a, const int32_t* row, const typename E::Cache* kc,
+                      const typename E::Cache* vc, unsigned char* ring, const unsigned char* qs,
+                      const int (&pages)[E::SLOTS + 1], int key, int step, int first, int k1, int lane, F prepare) {
+    constexpr int KT = E::KT, S = E::SLOTS, SLOT = E::TILE_BYTES;
+    const uint32_t ring_at = smem_addr(ring);
+    unsigned mask[S + 1];
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        if (key + i * step < k1) {
+            const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
+            mask[i] = t.mask;
+            e.issue(a, kc, t, ring_at + i * SLOT, lane);
+            cp_async_commit();
+            e.issue(a, vc, t, ring_at + (S + i) * SLOT, lane);
+            cp_async_commit();
+        } else {
+            mask[i] = 0u;
+            cp_async_commit();
+            cp_async_commit();
+        }
+    }
+    prepare();
+    if (key >= k1) return;
+    int page = pages[S];
+    for (int slot = 0;; slot = slot + 1 == S ? 0 : slot + 1) {
+        const int ahead = key + S * step;
+        cp_async_wait<2 * S - 1>();
+        __syncwarp();
+        e.scores(qs, ring + slot * SLOT, lane);
+        __syncwarp();
+        const PagedTile t = pa_tile<KT>(a, page, ahead, first, k1);
+        mask[S] = t.mask;
+        if (ahead < k1) e.issue(a, kc, t, ring_at + slot * SLOT, lane);
+        cp_async_commit();
+        page = pa_page<KT>(a, row, ahead + step);
+        e.weigh(mask[0], lane);
+        cp_async_wait<2 * S - 1>();
+        __syncwarp();
+        e.template values<AGAIN>(ring + (S + slot) * SLOT, lane);
+        key += step;
+        if (key >= k1) break;
+        __syncwarp();
+        if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * SLOT, lane);
+        cp_async_commit();
+#pragma unroll
+        for (int i = 0; i < S; ++i) mask[i] = mask[i + 1];
+    }
+}
+
+// The same once more for a warp whose sums are NaN and may not be, up to its sums in shared memory.  A call by itself,
+// since its registers would cost the loop that is always taken (16 query heads a cache head, bf16 64 x 128/8 x 128:
+// 239 us; 264 us with the parts apart in every tile, 248 us with infinite values left to come out as NaN).
+template <class E>
+__device__ __noinline__ void pa_again(float c, const PagedAttnArgs& a, const int32_t* row, const typename E::Cache* kc,
+                                      const typename E::Cache* vc, unsigned char* ring, const unsigned char* qs, int key,
+                                      int step, int first, int k1, float* sm, float* sl) {
+    const int lane = threadIdx.x & 31;
+    E e;
+    e.resume(a, kc, vc, c);
+    int pages[E::SLOTS + 1];
+#pragma unroll
+    for (int i = 0; i <= E::SLOTS; ++i) pages[i] = pa_page<E::KT>(a, row, key + i * step);
+    pa_tiles<E, true>(e, a, row, kc, vc, ring, qs, pages, key, step, first, k1, lane, [] {});
+    __syncwarp();
+    e.finish(reinterpret_cast<float*>(ring), sm, sl, lane);
+}
+
 template <class E>
 __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a,
                                                                            const PagedShape sh,
@@ -309,7 +380,6 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
     const int sets = sh.side * sh.groups, kwarps = PA_WARPS / sets, kwarp = warp / sets, set = warp % sets;
     unsigned char* ring = smem + (size_t)warp * 2 * S * SLOT;
     unsigned char* qs = smem + (size_t)PA_WARPS * 2 * S * SLOT + (size_t)set * E::Q_BYTES;
-    const uint32_t ring_at = smem_addr(ring);
 
     PagedShare share;
     int pages[S + 1];
@@ -358,60 +428,23 @@ __global__ void __launch_bounds__(PA_THREADS, E::BLOCKS) paged_attn_kernel(const
             const C* vc = (const C*)a.vc + hk * a.c_sh;
 
             E e;
-            int key = k0 + kwarp * KT;
+            const int key = k0 + kwarp * KT;
             const int step = kwarps * KT;
             // the first tiles, and the queries while they are on their way
             if (!early) {
 #pragma unroll
                 for (int i = 0; i <= S; ++i) pages[i] = pa_page<KT>(a, row, key + i * step);
             }
-            unsigned mask[S + 1];
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                if (key + i * step < k1) {
-                    const PagedTile t = pa_tile<KT>(a, pages[i], key + i * step, first, k1);
-                    mask[i] = t.mask;
-                    e.issue(a, kc, t, ring_at + i * SLOT, lane);
-                    cp_async_commit();
-                    e.issue(a, vc, t, ring_at + (S + i) * SLOT, lane);
-                    cp_async_commit();
-                } else {
-                    mask[i] = 0u;
-                    cp_async_commit();
-                    cp_async_commit();
-                }
-            }
-            e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, kc, vc, min(HW, G - head), qs,
-                   lane, kwarp, kwarps);
-            if (E::Q_BYTES) pa_group_sync(set, kwarps);
-            if (key < k1) {
-                int page = pages[S];
-                for (int slot = 0;; slot = slot + 1 == S ? 0 : slot + 1) {
-                    const int ahead = key + S * step;
-                    cp_async_wait<2 * S - 1>();
-                    __syncwarp();
-                    e.scores(qs, ring + slot * SLOT, lane);
-                    __syncwarp();
-                    const PagedTile t = pa_tile<KT>(a, page, ahead, first, k1);
-                    mask[S] = t.mask;
-                    if (ahead < k1) e.issue(a, kc, t, ring_at + slot * SLOT, lane);
-                    cp_async_commit();
-                    page = pa_page<KT>(a, row, ahead + step);
-                    e.weigh(mask[0], lane);
-                    cp_async_wait<2 * S - 1>();
-                    __syncwarp();
-                    e.values(ring + (S + slot) * SLOT, lane);
-                    key += step;
-                    if (key >= k1) break;
-                    __syncwarp();
-                    if (ahead < k1) e.issue(a, vc, t, ring_at + (S + slot) * SLOT, lane);
-                    cp_async_commit();
-#pragma unroll
-                    for (int i = 0; i < S; ++i) mask[i] = mask[i + 1];
-                }
-            }
+            pa_tiles<E, false>(e, a, row, kc, vc, ring, qs, pages, key, step, first, k1, lane, [&] {
+                e.init(a, (const T*)a.q + b * a.q_sb + ((long long)hk * G + head) * a.q_sh, kc, vc, min(HW, G - head),
+                       qs, lane, kwarp, kwarps);
+                if (E::Q_BYTES) pa_group_sync(set, kwarps);
+            });
             __syncwarp();  // the warp's sums go where its tiles were
-            e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
+            if (E::PARTS && e.spoilt())
+                pa_again<E>(e.c, a, row, kc, vc, ring, qs, key, step, first, k1, sm[warp], sl[warp]);
+            else
+                e.finish(reinterpret_cast<float*>(ring), sm[warp], sl[warp], lane);
             __syncthreads();
             // Each thread joins its four elements over the head's warps by itself: one barrier, and the warps' loads
             // side by side (with the factors computed once a head between two barriers, f32 1 x 8 x 76 of 96 keys

@@ -105,6 +105,7 @@ struct HalfEngine {
     static constexpr int QP = kSame ? 1 : kHalf ? 2 : 3;  // parts of a query
     static constexpr int PP = !kSame && !kHalf ? 3 : 2;   // parts of a weight
     static constexpr int QA = kPacked ? (QP + 1) / 2 : QP;  // eights of rows of the first operand
+    static constexpr bool PARTS = true;
     static constexpr int Q_BYTES = QA * NB * 32 * 16;
     static constexpr int TILE_BYTES = KT * ROW, SLOTS = SLOTS_;
     static constexpr int BLOCKS = DC > 128 ? 2 : SLOTS == 1 ? 4 : 3;
@@ -115,20 +116,23 @@ struct HalfEngine {
     int before_k, before_v;  // 0 or 4
     int dh;
 
-    // Lays the parts of the group's queries out as the first operand's registers.  Each warp of a group prepares
-    // every kwarps-th head.
-    KRK_DEV void init(const PagedAttnArgs& a, const T* q, const C* kc, const C* vc, int heads, unsigned char* qs,
-                      int lane, int kwarp, int kwarps) {
+    KRK_DEV void resume(const PagedAttnArgs& a, const C* kc, const C* vc, float scale) {
         dh = a.dh;
         before_k = ALIGN == ROWS_SHIFTED && (reinterpret_cast<uintptr_t>(kc) & 15) ? 4 : 0;
         before_v = ALIGN == ROWS_SHIFTED && (reinterpret_cast<uintptr_t>(vc) & 15) ? 4 : 0;
+        c = scale;
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int x = 0; x < 4; ++x) acc[i][x] = 0.f;
-        c = a.scale * 1.44269504088896341f;
+    }
+    // Lays the parts of the group's queries out as the first operand's registers.  Each warp of a group prepares
+    // every kwarps-th head.
+    KRK_DEV void init(const PagedAttnArgs& a, const T* q, const C* kc, const C* vc, int heads, unsigned char* qs,
+                      int lane, int kwarp, int kwarps) {
+        resume(a, kc, vc, a.scale * 1.44269504088896341f);
         for (int h = kwarp; h < HW; h += kwarps) {
             float4 x[(DC + 127) / 128];
             float most = 0.f;
@@ -309,11 +313,20 @@ struct HalfEngine {
         l = l * fade + ((s[0] + s[1]) + (s[2] + s[3]));
     }
 
+    // AGAIN: every weight that is not 0 taken for 2^-14 as well.  Where that product is infinite it is the result: a part
+    // of the weight may be 0 there, or negative, and spoil it.
+    template <bool AGAIN>
     KRK_DEV void values(const unsigned char* from, int lane) {
         // of the accumulators' columns 2 (lane % 4) and the one after it
         const float f0 = __shfl_sync(0xffffffffu, fade, (lane & 3) * 8 % (HW * 4));
         const float f1 = __shfl_sync(0xffffffffu, fade, ((lane & 3) * 8 + 4) % (HW * 4));
-        uint32_t p[PP][2];
+        uint32_t p[PP][2], some[2];
+        if (AGAIN) {
+            constexpr uint32_t kSmall = kHalf ? 0x0400u : 0x3880u;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                some[x] = (s[2 * x] > 0.f ? kSmall : 0u) | (s[2 * x + 1] > 0.f ? kSmall << 16 : 0u);
+        }
 #pragma unroll
         for (int i = 0; i < PP; ++i) {
             p[i][0] = pack_rest(s[0], s[1], C());
@@ -338,13 +351,27 @@ struct HalfEngine {
             mma_first(d, v[0], v[1], v[2], v[3], p[PA - 1][0], p[PA - 1][1], C());
 #pragma unroll
             for (int x = PA - 2; x >= 0; --x) mma(d, v[0], v[1], v[2], v[3], p[x][0], p[x][1], C());
+            if (AGAIN) {
+                float y[4];
+                mma_first(y, v[0], v[1], v[2], v[3], some[0], some[1], C());
+#pragma unroll
+                for (int x = 0; x < 4; ++x) d[x] = fabsf(y[x]) == INFINITY ? y[x] : d[x];
+            }
             acc[i][0] = fmaf(acc[i][0], f0, d[0]);
             acc[i][1] = fmaf(acc[i][1], f1, d[1]);
             acc[i][2] = fmaf(acc[i][2], f0, d[2]);
             acc[i][3] = fmaf(acc[i][3], f1, d[3]);
         }
     }
-
+    // NaN among the warp's sums: an infinite value may be behind it, and the tiles are taken once more, in parts.
+    KRK_DEV bool spoilt() const {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) bad |= acc[i][x] != acc[i][x];
+        return __any_sync(0xffffffffu, bad);
+    }
     KRK_DEV void finish(float* obuf, float* sm, float* sl, int lane) {
         const int r = lane >> 2, t = lane & 3;
         l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -357,7 +384,10 @@ struct HalfEngine {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) acc[i][x] += __shfl_xor_sync(0xffffffffu, acc[i][x], 2);
+                for (int x = 0; x < 4; ++x) {
+                    const float rest = __shfl_xor_sync(0xffffffffu, acc[i][x], 2);
+                    acc[i][x] = fabsf(acc[i][x]) == INFINITY ? acc[i][x] : acc[i][x] + rest;
+                }
             if (t > 1) return;
         }
 #pragma unroll

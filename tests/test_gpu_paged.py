@@ -1082,3 +1082,55 @@ def test_serving_with_pages_given_back_behind_a_window(hq, hkv, dh, page, window
         d["table"].copy_(i32(table))
         d["free"][:len(free)] = i32(free)
         d["count"].fill_(len(free))
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page,lens", [
+    (4, 4, 64, 16, [1, 40, 300, 0]), (8, 2, 76, 16, [17, 3, 129]), (16, 2, 128, 4, [64, 1000]), (17, 1, 96, 32, [333, 2]),
+    (4, 2, 192, 16, [50, 50]), (2, 1, 256, 8, [31, 700]), (8, 1, 64, 64, [30000, 5, 70])])
+def test_infinite_values_of_visible_keys(act, cache, hq, hkv, dh, page, lens):
+    """An infinite value makes its column infinite, one of each sign NaN, whatever a weight's parts are (a weight of 1,
+    which a 16-bit type holds exactly, included); nothing else changes."""
+    def fill(n, h, d, g):
+        return 0.1 * torch.randn(n, h, d, generator=g, device=DEV), torch.randn(n, h, d, generator=g, device=DEV)
+    pool = Pool(lens, hkv, dh, page, cache, seed=hq, fill=fill)
+    q = torch.randn(len(lens), hq, dh, generator=gen(4), device=DEV).to(act)
+    clean, lse = check_attn(pool, q)
+    inf = float("inf")
+    want = clean.clone().float()
+    share = hq // hkv
+    for b, n in enumerate(lens):
+        marks = [(0, 0, inf), (n - 1, 1, -inf), (n // 2, dh - 1, inf), (n // 3, dh // 2, -inf), (n // 2, dh // 2, -inf),
+                 (0, 5, inf), (n - 1, 5, inf)]
+        if n > 1:
+            marks += [(0, 9, inf), (n - 1, 9, -inf)]
+        for j, d, x in marks if n else []:
+            h = (j + d) % hkv
+            if d in (5, 9):  # both of one head
+                h = d % hkv
+            pool.vc[int(pool.table[b, j // page]), j % page, h, d] = x
+            cells = want[b, h * share:(h + 1) * share, d]
+            cells[:] = float("nan") if (cells == -x).any() else x
+    out, got = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, return_lse=True)
+    assert torch.equal(got, lse)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.float().nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh", [(1, 1, 64), (4, 2, 76), (16, 1, 128)])
+@pytest.mark.parametrize("far", [10.0, 27.0, 35.0, 60.0])
+def test_infinite_values_of_faint_keys(act, cache, hq, hkv, dh, far):
+    """A weight of e^-far is not 0 in 32 bits, and times infinity is infinity."""
+    def fill(n, h, d, g):
+        k = torch.zeros(n, h, d, device=DEV)
+        k[:, :, 0] = torch.arange(n, device=DEV)[:, None] % 2 * -far
+        return k, torch.randn(n, h, d, generator=g, device=DEV)
+    pool = Pool([2, 40], hkv, dh, 16, cache, seed=8, fill=fill)
+    q = torch.zeros(2, hq, dh, device=DEV, dtype=act)
+    q[:, :, 0] = 1.0
+    want, _ = check_attn(pool, q, scale=1.0)
+    for b, j, d, x in ((0, 1, 3, float("inf")), (1, 39, 2, -float("inf")), (1, 5, dh - 1, float("inf"))):
+        pool.vc[int(pool.table[b, j // 16]), j % 16, :, d] = x
+        want[b, :, d] = x
+    assert torch.equal(K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, scale=1.0), want)
