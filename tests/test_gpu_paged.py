@@ -1134,3 +1134,111 @@ def test_infinite_values_of_faint_keys(act, cache, hq, hkv, dh, far):
         pool.vc[int(pool.table[b, j // 16]), j % 16, :, d] = x
         want[b, :, d] = x
     assert torch.equal(K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, scale=1.0), want)
+
+
+# ------------------------------------------------------------------ attention in shares
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_scratch_of_nan_and_bounds_that_are_too_small(act, cache):
+    """Long keys, which go through the scratch: what it held before does not matter, calls repeat bit for bit, and a
+    bound below the lengths sizes the launch and nothing else."""
+    lens = [40000, 0, 9000, 12]
+    pool = Pool(lens, 2, 128, 16, cache, seed=12)
+    q = torch.randn(4, 8, 128, generator=gen(3), device=DEV).to(act)
+    need = K.attn_paged_work_floats(4, 8, 2, 128, 40000)
+    assert need > 0
+    first, first_lse = check_attn(pool, q)
+    for fill in (float("nan"), float("inf"), -1.0):
+        work = torch.full((need + 8,), fill, device=DEV)
+        out, lse = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, work=work, return_lse=True)
+        assert torch.equal(first, out) and torch.equal(first_lse, lse)
+        assert not torch.equal(work[:need].nan_to_num(5.0), torch.full_like(work[:need], fill).nan_to_num(5.0))
+        assert torch.equal(work[need:].nan_to_num(5.0), torch.full_like(work[need:], fill).nan_to_num(5.0))
+    work = torch.full((need,), float("nan"), device=DEV)
+    for bound in (1, 5000, 13000, 20000, 2 ** 31 - 1):
+        if bound > 12500:
+            assert K.attn_paged_work_floats(4, 8, 2, 128, min(bound, 40000)) > 0
+        check_attn(pool, q, max_len=bound, work=work)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page", [(8, 2, 64, 16), (17, 1, 76, 64), (40, 1, 128, 4)])
+def test_shares_replayed_from_a_graph(act, cache, hq, hkv, dh, page):
+    """The captured pair of kernels follows the lengths, table and queries that it finds, whatever its scratch holds,
+    beside eager calls that run at the same time with their own."""
+    most = 30016
+    pool = Pool([most] * 3, hkv, dh, page, cache, seed=21)
+    q = torch.randn(3, hq, dh, generator=gen(3), device=DEV).to(act)
+    now, s = i32([10, 0, 20000]), torch.cuda.Stream()
+    need = K.attn_paged_work_floats(3, hq, hkv, dh, most)
+    assert need > 0
+    out, work = torch.empty_like(q), torch.empty(need, device=DEV)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now, out=out, work=work)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now, out=out, work=work)
+    for step, lens in enumerate(([most, 0, 64], [0, 0, 0], [most] * 3, [1, 20000, 29999], [17, 16, 65])):
+        now.copy_(i32(lens))
+        q.copy_(torch.randn(3, hq, dh, generator=gen(step), device=DEV).to(act))
+        work.fill_(float("nan"))
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            g.replay()
+            g.replay()
+        eager = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, now)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        view = Pool.__new__(Pool)
+        view.lens_h, view.k, view.v = lens, [k[:n] for k, n in zip(pool.k, lens)], [v[:n] for v, n in zip(pool.v, lens)]
+        ref, _, tol, _ = attn_reference(view, q, 1 / math.sqrt(dh))
+        assert ((out.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page,window", [(2, 2, 64, 16, 0), (8, 8, 76, 32, 0), (16, 8, 36, 16, 0),
+                                                   (24, 2, 96, 64, 0), (32, 4, 128, 8, 0), (32, 8, 128, 16, 1500),
+                                                   (6, 2, 252, 16, 0)])
+def test_large_batches_take_neighbouring_heads_together(act, cache, hq, hkv, dh, page, window):
+    """Batches with 8 units of 64 keys and more for each of 592 blocks when two heads of the cache go together: a
+    block's warps then take two or four neighbouring ones.  Random values against 64 bits; then every weight 1 and
+    values that are whole numbers, so that a key of another head or request shows, exactly."""
+    batch = 600 // hkv + 60
+    lens = [int(2000 * (i + 0.5) / batch) for i in np.random.default_rng(hq).permutation(batch)]
+    lens[3] = lens[-1] = 0
+    longest = -(-max(lens) // page) * page
+    units = -(-(min(longest, window + 16) if window else longest) // 64)
+    assert batch * hkv // 2 * units >= 8 * 592 and K.attn_paged_work_floats(batch, hq, hkv, dh, longest, window) > 0
+
+    def fill(n, h, d, g):
+        return (torch.randn(n, h, d, generator=g, device=DEV),
+                torch.randint(-8, 9, (n, h, d), generator=g, device=DEV).float())
+    pool = Pool(lens, hkv, dh, page, cache, seed=dh, fill=fill)
+    q = torch.randn(batch, hq, dh, generator=gen(7), device=DEV).to(act)
+    first, _ = check_attn(pool, q, window=window)
+    again = K.attn_decode_paged(q, pool.kc, pool.vc, pool.table, pool.lens, window=window)
+    assert torch.equal(first, again)
+    out, lse = K.attn_decode_paged(torch.zeros_like(q), pool.kc, pool.vc, pool.table, pool.lens, window=window,
+                                   return_lse=True)
+    for i, n in enumerate(lens):
+        seen = min(n, window) if window else n
+        mean = pool.v[i][n - seen:].double().sum(0).repeat_interleave(hq // hkv, 0) / max(1, seen)
+        tol = (8 * U + half_step(act)) * mean.abs() + torch.finfo(act).tiny
+        assert ((out[i].double() - mean).abs() <= tol).all(), (i, n)
+        want = math.log(seen) if seen else -math.inf
+        assert torch.allclose(lse[i].double(), torch.full_like(lse[i].double(), want), rtol=8 * U, atol=8 * U)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("hq,hkv,dh,page,lens,window", [
+    (33, 1, 64, 16, [30000, 0, 9000], 0), (40, 1, 76, 4, [16000, 16001], 0), (64, 1, 128, 32, [20000], 0),
+    (66, 2, 80, 16, [14000, 1, 15000], 0), (71, 1, 192, 64, [13000], 0), (128, 1, 256, 16, [13000, 5], 0),
+    (40, 1, 64, 16, [60000, 40], 20000)])
+def test_many_query_heads_in_shares(act, cache, hq, hkv, dh, page, lens, window):
+    """More query heads a cache head than a block takes at once, over keys that go through the scratch."""
+    pool = Pool(lens, hkv, dh, page, cache, seed=hq)
+    q = torch.randn(len(lens), hq, dh, generator=gen(hq), device=DEV).to(act)
+    assert K.attn_paged_work_floats(len(lens), hq, hkv, dh, pool.table.shape[1] * page, window) > 0
+    check_attn(pool, q, window=window)
