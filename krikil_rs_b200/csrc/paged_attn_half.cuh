@@ -173,11 +173,11 @@ struct HalfEngine {
             }
         }
     }
-    // The power of two that brings the row's largest element to 2^14 .. 2^15 (at most 2^+-100; 1 for zeros,
-    // infinities and NaN).
+    // The power of two that brings the row's largest element to 2^14 .. 2^15 (at most 2^126, whose inverse is a normal
+    // number; 1 for zeros, infinities and NaN).
     static KRK_DEV float row_scale(float most) {
         if (!(most > 0.f) || most == INFINITY) return 1.f;
-        return exp2f((float)min(100, max(-100, 14 - ilogbf(most))));
+        return exp2f((float)min(126, 14 - ilogbf(most)));
     }
 
     KRK_DEV void issue(const PagedAttnArgs& a, const C* base, const PagedTile& t, uint32_t to, int lane) {

@@ -1242,3 +1242,13 @@ def test_many_query_heads_in_shares(act, cache, hq, hkv, dh, page, lens, window)
     q = torch.randn(len(lens), hq, dh, generator=gen(hq), device=DEV).to(act)
     assert K.attn_paged_work_floats(len(lens), hq, hkv, dh, pool.table.shape[1] * page, window) > 0
     check_attn(pool, q, window=window)
+
+
+@pytest.mark.parametrize("cache", [F32, F16, BF16])
+@pytest.mark.parametrize("hq,dh", [(4, 64), (8, 76), (34, 128)])
+@pytest.mark.parametrize("power", [-118, -100, 100, 114, 116, 118, 122])
+def test_float32_queries_of_any_size(cache, hq, dh, power):
+    """Queries far from 1 under a scale that brings the scores back: no part of them leaves its type."""
+    pool = Pool([130, 17], 2, dh, 16, cache, seed=14)
+    q = torch.randn(2, hq, dh, generator=gen(3), device=DEV) * 2.0 ** power
+    check_attn(pool, q, scale=2.0 ** -power / math.sqrt(dh))
