@@ -65,3 +65,45 @@ def test_checked_build_reports_bad_lengths_pages_and_slots():
     env = dict(os.environ, KRIKIL_CHECKED="1", PYTHONPATH=ROOT)
     r = subprocess.run([sys.executable, "-c", CHILD], cwd=ROOT, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "checked ok" in r.stdout, r.stdout + r.stderr
+
+
+PLAN_CHILD = r'''
+import ctypes as C
+import torch
+from krikil_rs_b200 import kernels as K
+from krikil_rs_b200._lib import lib, CHECK_TABLE, OK
+
+assert lib.krk_checked_build() == 1
+dev = torch.device("cuda:0")
+
+def status():
+    torch.cuda.synchronize()
+    b = C.c_uint32()
+    assert lib.krk_check_status(C.byref(b), 1) == OK
+    return b.value
+
+def i32(v):
+    return torch.tensor(v, device=dev, dtype=torch.int32)
+
+for new in (3, 5000):  # in one block, and in two kernels
+    pages = 2 * -(-new // 4) + 2
+    table = torch.full((2, pages), 7, device=dev, dtype=torch.int32)
+    free = torch.arange(pages, device=dev, dtype=torch.int32)
+    lens, count = i32([0, 0]), i32([pages])
+    out = K.kv_page_plan(i32([new, new]), lens, table, free, count, 4, 2 * new)
+    assert out[5].item() == 0 and status() == 0
+    free[pages - 1] = 2 ** 30 + 1  # * 4 is 4 in 32 bits
+    out = K.kv_page_plan(i32([new, new]), lens, table, free, count, 4, 2 * new)
+    assert out[5].item() == 0 and status() == CHECK_TABLE and (out[4][:3] == -1).all()
+    held = i32([8, 4])
+    table[:, :2] = i32([[-1, 3], [4, -1]])  # a page given back: skipped, and nothing amiss
+    out = K.kv_page_release(torch.tensor([True, True], device=dev), held, table, free, i32([0]), 4)
+    assert out[2].item() == 0 and out[1].item() == 2 and free[:2].tolist() == [3, 4] and status() == 0
+print("checked ok")
+'''
+
+
+def test_checked_build_reports_planned_tokens_on_no_page():
+    env = dict(os.environ, KRIKIL_CHECKED="1", PYTHONPATH=ROOT)
+    r = subprocess.run([sys.executable, "-c", PLAN_CHILD], cwd=ROOT, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "checked ok" in r.stdout, r.stdout + r.stderr
