@@ -16,6 +16,9 @@ result by (2 s + 2 (n + 32) u) max |v| and h |result|, and the logarithm by s +
 2 (n + 32) u + 2u |lse|.  Exact tests (whole-number values under equal weights)
 hold the long sums."""
 import math
+import os
+import re
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -1252,3 +1255,43 @@ def test_float32_queries_of_any_size(cache, hq, dh, power):
     pool = Pool([130, 17], 2, dh, 16, cache, seed=14)
     q = torch.randn(2, hq, dh, generator=gen(3), device=DEV) * 2.0 ** power
     check_attn(pool, q, scale=2.0 ** -power / math.sqrt(dh))
+
+
+def test_the_serving_step_of_the_readme():
+    """The step as README.md has it: requests without a new token first and last, then a step that does not fit."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "README.md"), encoding="utf-8") as f:
+        code = next(x for x in re.findall(r"```python\n(.*?)```", f.read(), re.S) if "kv_page_plan" in x)
+    hq, hkv, dh, page, batch = 4, 2, 64, 4, 4
+    g = gen(1)
+    layers = [SimpleNamespace(kc=torch.full((9, page, hkv, dh), float("nan"), device=DEV),
+                              vc=torch.full((9, page, hkv, dh), float("nan"), device=DEV)) for _ in range(2)]
+    names = dict(layers=layers, lens=i32([0] * batch), count=i32([9]), free_pages=i32(list(range(9))), page_size=page,
+                 table=torch.full((batch, 8), -1, device=DEV, dtype=torch.int32), rows=batch, bound=32)
+    kept = [[[[], []] for _ in range(batch)] for _ in layers]
+    for step in range(12):
+        new = [0, 1, int(step % 3 == 0), 0] if step < 10 else [0, 1, 1, 0]
+        names["new_tokens"] = i32(new)
+        for l in layers:
+            l.q, l.k, l.v = (torch.randn(batch, h, dh, generator=g, device=DEV) for h in (hq, hkv, hkv))
+        exec(code, names)
+        for i, l in enumerate(layers):
+            q = K.rope_kv_append_paged(l.q, l.k, l.v, l.kc.clone(), l.vc.clone(), names["slots"], names["positions"])
+            owner = [b for b in range(batch) if new[b]]
+            for r, b in enumerate(owner):
+                j = names["lens"].tolist()[b] - 1
+                cell = names["table"][b, j // page].long(), j % page
+                kept[i][b][0].append(l.kc[cell].clone())
+                kept[i][b][1].append(l.v[r])
+            view = Pool.__new__(Pool)
+            view.lens_h = [len(x[0]) for x in kept[i]]
+            assert view.lens_h == names["lens"].tolist()
+            view.k, view.v = ([torch.stack(x[c]) if x[c] else None for x in kept[i]] for c in (0, 1))
+            mine = torch.zeros(batch, hq, dh, device=DEV)
+            mine[owner] = q[:len(owner)]
+            ref, _, tol, _ = attn_reference(view, mine, 1 / math.sqrt(dh))
+            assert ((l.out.double() - ref).abs() <= tol)[owner].all()
+    names["new_tokens"], before = i32([1, 1, 1, 2]), [l.kc.clone() for l in layers]  # five tokens in four rows
+    with pytest.raises(MemoryError):
+        exec(code, names)
+    assert all(torch.equal(l.kc.nan_to_num(9.0), x.nan_to_num(9.0)) for l, x in zip(layers, before))
