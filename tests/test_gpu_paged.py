@@ -1295,3 +1295,62 @@ def test_the_serving_step_of_the_readme():
     with pytest.raises(MemoryError):
         exec(code, names)
     assert all(torch.equal(l.kc.nan_to_num(9.0), x.nan_to_num(9.0)) for l, x in zip(layers, before))
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+@pytest.mark.parametrize("batch,hq,hkv,dh,page", [(100003, 1, 1, 4, 1), (66000, 3, 3, 8, 2), (30011, 8, 4, 12, 4)])
+def test_very_many_requests(act, cache, batch, hq, hkv, dh, page):
+    """Tens of thousands of requests of 0 to 5 tokens, planned, appended and attended."""
+    g = gen(batch)
+    new = torch.randint(0, 6, (batch,), generator=g, device=DEV, dtype=torch.int32)
+    tokens, width = int(new.sum()), -(-5 // page)
+    need = int(((new + page - 1) // page).sum())
+    free = torch.randperm(need + 3, generator=g, device=DEV).int()
+    table = torch.full((batch, width), -1, device=DEV, dtype=torch.int32)
+    lens, count, cu, positions, slots, status = K.kv_page_plan(new, torch.zeros_like(new), table, free, i32([need + 3]),
+                                                               page, tokens + 5)
+    assert status.item() == 0 and count.item() == 3 and torch.equal(lens, new)
+    assert torch.equal(cu[1:].long(), torch.cumsum(new.long(), 0)) and (slots[tokens:] == -1).all()
+    row = torch.repeat_interleave(torch.arange(batch, device=DEV), new.long())
+    at = torch.arange(tokens, device=DEV) - cu[row].long()
+    assert torch.equal(positions[:tokens].long(), at)
+    page_of = table[row, at // page].long()
+    assert torch.equal(slots[:tokens].long(), page_of * page + at % page)
+    held = page_of[at % page == 0]
+    assert held.unique().numel() == need  # no page twice
+    kc, vc = (torch.full((need + 3, page, hkv, dh), float("nan"), device=DEV, dtype=cache) for _ in range(2))
+    k = torch.randn(tokens + 5, hkv, dh, generator=g, device=DEV).to(act)
+    v = torch.randint(-8, 9, (tokens + 5, hkv, dh), generator=g, device=DEV).to(act)
+    K.rope_kv_append_paged(None, k, v, kc, vc, slots, positions, rot_dim=0)
+    assert torch.equal(kc[page_of, at % page], k[:tokens].to(cache))
+    out, lse = K.attn_decode_paged(torch.zeros(batch, hq, dh, device=DEV, dtype=act), kc, vc, table, lens,
+                                   return_lse=True)
+    total = torch.zeros(batch, hkv, dh, device=DEV, dtype=torch.float64).index_add_(0, row, v[:tokens].double())
+    mean = (total / new.clamp_min(1)[:, None, None]).repeat_interleave(hq // hkv, 1)
+    assert ((out.double() - mean).abs() <= (8 * U + half_step(act)) * mean.abs() + torch.finfo(act).tiny).all()
+    want = torch.log(new.double())[:, None].expand(-1, hq)
+    assert torch.equal(lse == -math.inf, want == -math.inf)
+    assert (lse.double() - want).abs()[new > 0].max() <= 16 * U
+    done = torch.rand(batch, generator=g, device=DEV) < 0.5
+    after, left, status = K.kv_page_release(done, lens, table, free, count, page)
+    assert status.item() == 0 and torch.equal(after, torch.where(done, 0, new))
+    back = table[row, at // page][(at % page == 0) & done[row]]
+    assert left.item() == 3 + back.numel() and torch.equal(free[3:left.item()], back)
+
+
+@pytest.mark.parametrize("act,cache", TYPES, ids=IDS)
+def test_one_query_and_one_cache_for_all(act, cache):
+    """Inputs that are read only may be broadcast: one query row expanded over requests and heads, values that are the
+    keys themselves."""
+    pool = Pool([33, 0, 200], 2, 64, 16, cache, seed=3)
+    one = torch.randn(1, 1, 64, generator=gen(1), device=DEV).to(act)
+    pool.vc, pool.v = pool.kc, pool.k
+    a, _ = check_attn(pool, one.expand(3, 8, 64))
+    b, _ = check_attn(pool, one.expand(3, 8, 64).contiguous())
+    assert torch.equal(a, b)
+    kv = one.expand(5, 2, 64)
+    kc, vc = torch.zeros(2, 4, 2, 64, device=DEV, dtype=cache), torch.zeros(2, 4, 2, 64, device=DEV, dtype=cache)
+    K.rope_kv_append_paged(None, kv, kv, kc, vc, i32([0, 1, 2, 7, -1]), i32([0] * 5))
+    for c in (kc, vc):
+        cells = c.view(8, 2, 64)
+        assert torch.equal(cells[[0, 1, 2, 7]], one.to(cache).expand(4, 2, 64)) and not cells[3:7].any()
