@@ -157,7 +157,7 @@ int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int type, void*
     if (B < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq > 65535 || (int64_t)B * Hq > INT32_MAX)
         return invalid(who, "B must not be negative, Hq a positive multiple of Hkv of at most 65535, B * Hq below 2^31");
     if (dh < 4 || dh > 256 || dh % 4) return invalid(who, "dh must be a multiple of 4 of at most 256");
-    if (!std::isfinite(scale)) return invalid(who, "scale must be finite");
+    if (!std::isfinite(scale * 1.44269504088896341f)) return invalid(who, "scale (times log2(e)) must be finite");
     if (window < 0 || max_len < 0) return invalid(who, "window and max_len must not be negative");
     if (table_ld < width) return invalid(who, "table_ld is shorter than the table's width");
     if (B == 0) return KRK_OK;

@@ -169,3 +169,9 @@ def test_wrappers_refuse_cpu_tensors():
         K.rope_kv_append_paged(x, x, x, pool, pool, i, i)
     with pytest.raises(ValueError, match="CUDA"):
         K.attn_decode_paged(x, pool, pool, table, i)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+def test_a_scale_that_leaves_32_bits_in_base_two_is_refused(scale):
+    """Scores are taken times log2(e): such a scale would make NaN of a score of 0."""
+    refused(lib.krk_k_attn_decode_paged, ATTN, "scale", scale, "scale")
