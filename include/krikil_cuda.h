@@ -420,9 +420,14 @@ KRK_API int krk_k_wait_probe(const float* src16, int polls, int copy, int32_t* s
  * back to the host, so the step can be captured into a CUDA graph.
  *
  * q, k, v, out are all of `type`, the caches of `cache_type` (KRK_TYPE_*):
- * equal, or a 16-bit cache under float32 activations.  Computation is in 32
- * bits or more throughout, and rounded once when written.  dh is a multiple of
- * 4 of at most 256; pointers are aligned to four elements and strides are
+ * equal, or a 16-bit cache under float32 activations.  Sums, softmax statistics
+ * and angles are kept in 32 bits or more, and results rounded once when written.
+ * On 16-bit pages the factors of the products are 16-bit too, in parts whose
+ * exact products are added in 32 bits: a float32 query is two half parts (22
+ * bits and a sign, relative to the largest element of its head) or three
+ * bfloat16 parts (24 bits), a softmax weight two half parts (22 bits, at least
+ * 2^-38 of the largest), two bfloat16 parts (16 bits) or, under float32 queries,
+ * three (24 bits).  dh is a multiple of 4 of at most 256; pointers are aligned to four elements and strides are
  * multiples of four; the last dimension is dense.  The calls run on the current
  * device, to which `stream` and all pointers belong. */
 #define KRK_TYPE_F32 0
@@ -475,8 +480,8 @@ KRK_API int krk_k_kv_page_release(const uint8_t* done_mask, const int32_t* lens,
  * k, v and q_out likewise (q_out may be q with its strides).  Row t goes to
  * slots[t]; a row with a negative slot is padding: neither the caches nor its
  * q_out are written, and its other inputs do not matter.  A slot past the pool
- * is skipped the same way (reported by checked builds); two rows with the same
- * slot leave either one's key and value.  Angles are positions[t] *
+ * is skipped the same way (reported by checked builds).  No two rows may have the
+ * same slot: its cell would hold a mixture of theirs.  Angles are positions[t] *
  * theta^(-2i/rot_dim) reduced in 64 bits, so they hold at any int32 position
  * (krk_k_rope_kv_attn_decode keeps the reference's 32-bit product).  Hq may be
  * 0 (q and q_out unused).  q, k, v are only read. */
@@ -498,7 +503,9 @@ KRK_API int krk_k_rope_kv_append_paged(void* q, int64_t q_st, int64_t q_sh, void
  * token, so lens is what krk_k_kv_page_plan left.  A request of length 0 gets
  * zeros and lse -inf.  Lengths past width * page_size are cut there and
  * negative ones read as 0; keys on pages outside the pool are left out (both
- * reported by checked builds).  Cache cells past a request's length or before
+ * reported by checked builds).  scale may have any sign and size up to 2^127 /
+ * log2(e).  An infinite value of a visible key makes its element infinite, as in
+ * 32 bits.  Cache cells past a request's length or before
  * its window are never used, whatever they hold (16-bit rows are read in aligned
  * 16-byte pieces, so that up to 8 bytes beside a row may be read along).
  * max_len: a bound of the lengths by which the launch is sized, 0 = width *

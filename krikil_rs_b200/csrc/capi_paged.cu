@@ -1,6 +1,7 @@
 // C entry points of the paged key-value cache: argument checks, then the
-// launchers of k_paged_kv.cu and k_paged_attn.cu.  Nothing is launched by a
-// refused call.
+// launchers of k_paged_kv.cu and of the attention (paged_attn.cuh, with its
+// engines in k_paged_attn_f32.cu, k_paged_attn_f16.cu and k_paged_attn_bf16.cu).
+// Nothing is launched by a refused call.
 #include <cuda_runtime.h>
 
 #include <cmath>

@@ -610,8 +610,10 @@ __global__ void __launch_bounds__(PA_JOIN) paged_join_kernel(const PagedAttnArgs
 }
 
 // Blocks of a cluster for pieces of at most `bound` keys, 0: shares.  Clusters
-// grow while their blocks have more than PA_PART_UNITS units and all fit in a
-// wave of three a multiprocessor; they are used for few units a block, since they
+// grow while their blocks have more than PA_PART_UNITS units and there are at most
+// three a multiprocessor -- one wave, except for 16-bit heads of more than 128
+// elements, of which two are resident (bf16 25 x 32/8 x 256 of 1500 keys, 400
+// blocks: 63.5 us for 48 us of bytes); they are used for few units a block, since they
 // last as long as the longest request.  (In clusters and in shares, bf16
 // 32 x 32/8 x 128: 25.5 and 32.8 us of 1000 keys each, 18.7 and 20.3 of 1 .. 1000,
 // 43.5 and 51.5 of 2000, 33.8 and 32.6 of 1 .. 2000; f32 on bf16 48 x 12/4 x 80, 31

@@ -13,9 +13,9 @@
 // Keys and values are read once at up to the copy rate (bf16 128 x 32/8 x 128,
 // up to 8192 keys, 2.15 GB: 331 us, 6.5 TB/s); with few keys a call, latency
 // bounds it, and with 16 query heads a cache head, whose tiles two warps copy, L1
-// (128 heads over 8: 222 us for 168 us of bytes).  Rows that are not 16-byte
+// (64 x 128/8 x 128, up to 8192 keys: 244 us for 168 us of bytes).  Rows that are not 16-byte
 // aligned, or not a multiple of 8 elements, are shifted in place when all of a
-// head's lie alike (bf16 64 x 32/8 x 76: 140 us for 100 us of bytes, 173 us when
+// head's lie alike (bf16 64 x 32/8 x 76: 139 us for 100 us of bytes, 173 us when
 // they were copied 8 bytes at a time, as they still are when tokens differ).
 //
 // Precision: the products are exact and added in 32 bits, and a tile's sum is
@@ -24,7 +24,9 @@
 // pages: 24 bits), and a float32 query of two half parts after scaling its row
 // by a power of two (22 bits and a sign) or three bfloat16 parts (24 bits).
 // Half weights are scaled by 2^14, so that a key 2^-24 as likely as the
-// strongest still has 14 bits.
+// strongest still has 14 bits.  A part may be 0 where the weight is not: infinite
+// values, which that would turn into NaN, are looked for in a second pass by warps
+// whose sums are NaN.
 #pragma once
 #include "paged_attn.cuh"
 
@@ -418,7 +420,7 @@ cudaError_t by_width(const PagedAttnArgs& a, cudaStream_t s) {
 }
 
 // Up to four heads of float32 queries lie packed, their parts in the rows and columns of the four that are missing (f32
-// queries on bf16 pages, 1024 x 8 x 76: 148 us, 161 us in eights; on f16 pages 147 and 162 us).
+// queries on bf16 pages, 1024 x 8 x 76: 146 us, 161 us in eights; on f16 pages 147 and 162 us).
 template <typename T, typename C, int ALIGN>
 cudaError_t by_heads(const PagedAttnArgs& a, cudaStream_t s) {
     if constexpr (sizeof(T) == 4)

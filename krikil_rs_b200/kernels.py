@@ -345,7 +345,7 @@ def rope_kv_append_paged(q, k, v, kc, vc, slots, positions, theta: float = 10000
     """Rotates q [T, Hq, dh] and k [T, Hkv, dh] by their positions (int32 [T];
     rotate-half on the first rot_dim elements, all by default) and writes k and
     v to the slots (int32 [T], -1: padding) of the pages kc, vc [pages,
-    page_size, Hkv, dh].  Strided views are fine as long as dh is dense.
+    page_size, Hkv, dh]; no two rows may have the same slot.  Strided views are fine as long as dh is dense.
     Returns the rotated q (q_out, which may be q; padding rows of a given q_out
     are left as they were).  q may be None."""
     dev = _cuda_device(k)
