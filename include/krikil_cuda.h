@@ -5,8 +5,8 @@
  * The reference is a Rust library whose public surface is src/lib.rs:1-6; its
  * model API (src/model.rs) is what a Rust `build.rs` + `extern "C"` binding of
  * this header replaces.  Each entry point below names the reference interface
- * it stands in for.  All computation is fp32, on the GPU (the paged cache's
- * operators also take 16-bit elements); there is no CPU
+ * it stands in for.  All computation is fp32, on the GPU (the operators of
+ * the paged cache, of layers over state slots and of log probabilities also take 16-bit elements); there is no CPU
  * fallback -- if the device or the kernels are unusable, calls fail with
  * KRK_CUDA and krk_last_error() says why.
  *
@@ -521,6 +521,68 @@ KRK_API int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int typ
                                     int64_t o_sb, int64_t o_sh, float* lse, float* work, size_t work_floats,
                                     void* stream);
 
+/* ------------------------------------------- recurrent layers over state slots
+ * The convolution and the state space scan of layers whose decay belongs to each
+ * channel and state (no counterpart in the reference, whose layers have one
+ * decay a head: krk_k_conv_ssd_step / krk_k_conv_ssd_scan), for servers: packed
+ * requests of different lengths, or one token of each, with the requests' states
+ * in a pool of slots.
+ *
+ * Packed: request s (of S) owns rows cu[s] .. cu[s+1]-1 of T; rows of no request
+ * are left alone.  cu is not trusted: its values are cut to [0, T], and a request
+ * that ends before it begins is empty.  Single tokens: request b owns row b.
+ * Slots: request s continues from slot init[s] -- below 0: it begins, from zeros
+ * -- and leaves its state in slot slots[s].  slots NULL: slot s; init NULL: the
+ * slot it goes to.  A request of no rows leaves there what it continues from.  A
+ * request whose slot is negative is padding, and one with a slot or init past the
+ * pool is treated the same (reported by checked builds, as are cut values of
+ * cu): its rows and all slots are left alone.  No two requests may have the same
+ * slot, nor may one continue from a slot that another one goes to; several may
+ * continue from the same one.  The step between two slots is state_stride
+ * elements.  state NULL (with slots and init NULL and num_slots 0; packed
+ * requests only): every request begins, and nothing is kept.
+ *
+ * x, dt, z, b, c and out are of `type` (KRK_TYPE_*), weights and scan states
+ * float32; everything is computed in 32 bits and rounded once when written.
+ * Element (t, i) of a [T][.] tensor is p[t*p_st + i]; pointers are aligned to
+ * their elements, and 16-byte aligned rows are read and written 16 bytes at a
+ * time.  The calls run on the current device, to which `stream` and all pointers
+ * belong; they need no scratch and can be captured into a CUDA graph. */
+
+/* Causal depthwise convolution of width W (2, 3 or 4) over C channels:
+ *   out[t][c] = act(bias[c] + sum_j weight[c*W + j] x[t - (W-1) + j][c]),
+ * act(y) = y * sigmoid(y) with silu != 0, else y; bias may be NULL.  The state
+ * [W-1][C], of x's type, holds the request's last W-1 rows of x, the latest
+ * last.  out must not overlap x. */
+KRK_API int krk_k_causal_conv(void* x, int64_t x_st, const float* weight, const float* bias, void* out, int64_t o_st,
+                              int type, void* state, int64_t state_stride, int num_slots, const int32_t* slots,
+                              const int32_t* init, const int32_t* cu, int T, int S, int C, int W, int silu,
+                              void* stream);
+KRK_API int krk_k_causal_conv_step(void* x, int64_t x_st, const float* weight, const float* bias, void* out,
+                                   int64_t o_st, int type, void* state, int64_t state_stride, int num_slots,
+                                   const int32_t* slots, const int32_t* init, int B, int C, int W, int silu,
+                                   void* stream);
+
+/* Selective state space scan over D channels of N (at most 256) states, which
+ * share b and c [T][G][N] in G groups of D / G consecutive channels: with delta
+ * = softplus(dt[t][i] + dt_bias[i]),
+ *   h[n] = exp(delta a[i*N + n]) h[n] + delta x[t][i] b[t][g][n],
+ *   out[t][i] = (sum_n h[n] c[t][g][n] + d[i] x[t][i]) * z[t][i] * sigmoid(z[t][i]).
+ * a [D][N] is the decay itself (negative, as -exp(A_log)); d, dt_bias (zeros) and
+ * z (no gate) may be NULL.  The state is [D][N].  out may be x, dt or z with
+ * their strides, and must not overlap the others. */
+KRK_API int krk_k_selective_scan(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z, int64_t z_st, void* b,
+                                 int64_t b_st, int64_t b_sg, void* c, int64_t c_st, int64_t c_sg, void* out,
+                                 int64_t o_st, int type, const float* a, const float* d, const float* dt_bias,
+                                 float* state, int64_t state_stride, int num_slots, const int32_t* slots,
+                                 const int32_t* init, const int32_t* cu, int T, int S, int D, int N, int G,
+                                 void* stream);
+KRK_API int krk_k_selective_step(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z, int64_t z_st, void* b,
+                                 int64_t b_st, int64_t b_sg, void* c, int64_t c_st, int64_t c_sg, void* out,
+                                 int64_t o_st, int type, const float* a, const float* d, const float* dt_bias,
+                                 float* state, int64_t state_stride, int num_slots, const int32_t* slots,
+                                 const int32_t* init, int B, int D, int N, int G, void* stream);
+
 /* Greedy pick (src/sampler.rs:50-80) per row of logits [B][ld]: repetition
  * penalty on tokens whose bit is set in seen [B][vocab/32] (seen may be NULL;
  * penalty 1 disables it), then the first maximum; tok [B]. */
@@ -533,6 +595,18 @@ KRK_API int krk_k_greedy(const float* logits, int64_t ld, int vocab, int B, uint
  * seen when seen is not NULL.  temperature <= 1e-6 is krk_k_greedy. */
 KRK_API int krk_k_sample(const float* logits, int64_t ld, int vocab, int B, uint32_t* seen, float temperature,
                          float top_p, int top_k, float penalty, uint32_t* rng_state, uint32_t* tok, void* stream);
+
+/* Log probabilities under softmax of each row of logits [R][V] (of `type`, row r
+ * at logits + r*ld; computed in 32 bits): logprobs[r*K + k] of token tokens[r*K +
+ * k], entropy[r] (may be NULL; natural logarithm), and the `top` (at most 64)
+ * largest logits' ids and log probabilities, the largest first and of equal ones
+ * the lower id.  A negative token asks for nothing and gets 0; one of at least V
+ * gets -inf (reported by checked builds).  A logit of -inf is a masked token.  A
+ * row with nothing else gives every token -inf and entropy 0; one with a NaN or
+ * +inf logit gives NaN (its ids are still in order, NaN taken for -inf). */
+KRK_API int krk_k_token_logprobs(void* logits, int64_t ld, int type, int R, int V, const int32_t* tokens, int K,
+                                 float* logprobs, float* entropy, int top, int32_t* top_ids, float* top_logprobs,
+                                 void* stream);
 
 /* StdRng::seed_from_u64(seed) as sampler state: 8 ChaCha12 key words from
  * rand_core's PCG32 expansion, then the next keystream word's index (0, 0);

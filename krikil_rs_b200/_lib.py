@@ -84,6 +84,15 @@ _SIGS = {
     "krk_k_attn_decode_paged": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp] + [_i64] * 3 + [_i32, _vp, _i64]
                                 + [_i32] * 3 + [_vp] + [_i32] * 4 + [_f32, _i32, _i32, _vp, _i64, _i64, _vp, _vp,
                                                                     C.c_size_t, _vp]),
+    "krk_k_causal_conv": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
+        _i32, _i32, _i32, _i32, _vp]),
+    "krk_k_causal_conv_step": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32,
+        _i32, _i32, _i32, _vp]),
+    "krk_k_selective_scan": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+        _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "krk_k_selective_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+        _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
+    "krk_k_token_logprobs": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp]),
     # include/krikil_text.h
     "krk_tokenizer_load": (_i32, [C.c_char_p, C.POINTER(_vp)]),
     "krk_tokenizer_free": (_i32, [_vp]),

@@ -1,0 +1,186 @@
+// Short causal depthwise convolution over packed requests and over single
+// tokens, with the rows before a request in a pool of state slots:
+//   y[t] = act(bias + sum_j w[j] x[t - (W-1) + j]).
+// Bound by memory: each element of x is read once from HBM (the W-1 rows that
+// runs share come from L2) and each of y written once.
+#include "kernels.h"
+#include "paged.h"
+#include "recurrent.cuh"
+
+namespace krk {
+namespace {
+
+constexpr int CONV_THREADS = 128;
+
+// One thread: V channels; their taps, bias, and the window of W-1 rows.
+template <typename T, int W, int V>
+struct ConvColumn {
+    const ConvArgs& a;
+    int c;
+    float w[W][V], bias[V];
+
+    KRK_DEV ConvColumn(const ConvArgs& args, int channel) : a(args), c(channel) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[j][i] = a.w[(int64_t)(c + i) * W + j];
+            bias[i] = a.bias ? a.bias[c + i] : 0.0f;
+        }
+    }
+    KRK_DEV const T* row(int t) const { return (const T*)a.x + t * a.x_st + c; }
+    KRK_DEV T* kept(int slot, int k) const { return (T*)a.slot.state + slot * a.slot.stride + (int64_t)k * a.C + c; }
+    // Row t of a request whose rows begin at `begin`: a packed row, or one of the W-1 before them.
+    KRK_DEV Pack<T, V> tap(int t, int begin, int from) const {
+        if (t >= begin) return load_pack<T, V>(row(t));
+        if (from >= 0) return load_pack<T, V>(kept(from, W - 1 + t - begin));
+        Pack<T, V> zero;
+#pragma unroll
+        for (int i = 0; i < V; ++i) zero.v[i] = from_f32<T>(0.0f);
+        return zero;
+    }
+    KRK_DEV void put(int t, const float (&win)[W - 1][V], const float (&x)[V]) const {
+        Pack<T, V> y;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float s = bias[i];
+#pragma unroll
+            for (int j = 0; j < W - 1; ++j) s = fmaf(w[j][i], win[j][i], s);
+            s = fmaf(w[W - 1][i], x[i], s);
+            y.v[i] = from_f32<T>(a.silu ? fast_silu(s) : s);
+        }
+        store_pack<T, V>((T*)a.out + t * a.o_st + c, y);
+    }
+    // Rows [i, j) of a request that begins at `begin`.
+    KRK_DEV void run(int i, int j, int begin, int from) const {
+        if (i >= j) return;
+        float win[W - 1][V];
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) {
+            const Pack<T, V> p = tap(i - (W - 1) + k, begin, from);
+#pragma unroll
+            for (int v = 0; v < V; ++v) win[k][v] = to_f32(p.v[v]);
+        }
+        for (int t = i; t < j; ++t) {
+            const Pack<T, V> p = load_pack<T, V>(row(t));
+            float x[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = to_f32(p.v[v]);
+            put(t, win, x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int k = 0; k + 1 < W - 1; ++k) win[k][v] = win[k + 1][v];
+                win[W - 2][v] = x[v];
+            }
+        }
+    }
+    // The W-1 rows that the request ends with, into its slot (which may be the one that they are read from).
+    KRK_DEV void keep(const Span& span, int to, int from) const {
+        if (to < 0) return;
+        Pack<T, V> last[W - 1];
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) last[k] = tap(span.end - (W - 1) + k, span.begin, from);
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) store_pack<T, V>(kept(to, k), last[k]);
+    }
+};
+
+// The number of requests that begin before row r (their beginnings ascend): a
+// warp looks at 32 of them at a time.
+KRK_DEV int requests_before(const int32_t* cu, int S, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = S;  // the answer lies in [lo, lo + n]
+    while (n > 0) {
+        const int step = (n + 31) / 32, i = lo + (lane + 1) * step - 1;
+        const bool before = i < lo + n && cu[i] < r;
+        const int k = __popc(__ballot_sync(0xffffffffu, before));
+        const int end = lo + n;
+        lo += k * step;
+        n = min(step - 1, end - lo);
+    }
+    return lo;
+}
+
+// A block takes `rows` packed rows of CONV_THREADS * V channels, and the
+// requests that begin there: it keeps their states, and computes their first
+// W-1 rows even past its own, so that whatever reads a request's old state is
+// the thread that writes the new one.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(CONV_THREADS) conv_kernel(ConvArgs a, int rows, int side) {
+    const int chunk = blockIdx.x / side, c = ((blockIdx.x - chunk * side) * CONV_THREADS + threadIdx.x) * V;
+    const int r0 = chunk * rows;
+    const bool last = r0 >= a.T - rows;
+    const int r1 = last ? a.T : r0 + rows;
+    int s = chunk == 0 ? 0 : requests_before(a.cu, a.S, r0);
+    if (c >= a.C) return;
+    const ConvColumn<T, W, V> col(a, c);
+    int to, from;
+    if (s > 0) {
+        const Span span = request_rows(a.cu, s - 1, a.T);
+        if (span.end > r0 && request_slots(a.slot, s - 1, to, from))
+            col.run(max(r0, min(span.begin + W - 1, span.end)), min(span.end, r1), span.begin, from);
+    }
+    for (; s < a.S; ++s) {
+        const Span span = request_rows(a.cu, s, a.T);
+        if (!last && span.begin >= r1) break;
+        if (!request_slots(a.slot, s, to, from)) continue;
+        col.run(span.begin, min(span.end, max(r1, span.begin + W - 1)), span.begin, from);
+        col.keep(span, to, from);
+    }
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(CONV_THREADS) conv_step_kernel(ConvArgs a, int side) {
+    const int t = blockIdx.x / side, c = ((blockIdx.x - t * side) * CONV_THREADS + threadIdx.x) * V;
+    int to, from;
+    if (c >= a.C || !request_slots(a.slot, t, to, from)) return;
+    const ConvColumn<T, W, V> col(a, c);
+    col.run(t, t + 1, t, from);
+    col.keep({t, t + 1}, to, from);
+}
+
+bool fits(const void* p, int64_t stride, size_t bytes, size_t elem) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * elem % bytes == 0;
+}
+
+template <typename T, int W, int V>
+cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
+    const int side = (a.C + CONV_THREADS * V - 1) / (CONV_THREADS * V);
+    if (!a.cu) {
+        if ((int64_t)a.T * side > INT32_MAX) return cudaErrorInvalidValue;
+        conv_step_kernel<T, W, V><<<a.T * side, CONV_THREADS, 0, s>>>(a, side);
+    } else {
+        const int sms = paged_sm_count();
+        if (sms <= 0) return cudaErrorInvalidDevice;
+        const int64_t share = (int64_t)a.T * side / (sms * 16);
+        const int rows = share < 8 ? 8 : share > 64 ? 64 : (int)share;
+        const int64_t blocks = (int64_t)(a.T > 0 ? (a.T + (int64_t)rows - 1) / rows : 1) * side;
+        if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+        conv_kernel<T, W, V><<<(unsigned)blocks, CONV_THREADS, 0, s>>>(a, rows, side);
+    }
+    add_launches(1);
+    return cudaGetLastError();
+}
+
+template <typename T, int W>
+cudaError_t conv_width(const ConvArgs& a, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const bool wide = a.C % V == 0 && fits(a.x, a.T > 1 ? a.x_st : 0, 16, sizeof(T)) &&
+                      fits(a.out, a.T > 1 ? a.o_st : 0, 16, sizeof(T)) &&
+                      fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, 16, sizeof(T));
+    return wide ? launch_conv<T, W, V>(a, s) : launch_conv<T, W, 1>(a, s);
+}
+
+template <typename T>
+cudaError_t conv_type(const ConvArgs& a, int W, cudaStream_t s) {
+    return W == 2 ? conv_width<T, 2>(a, s) : W == 3 ? conv_width<T, 3>(a, s) : conv_width<T, 4>(a, s);
+}
+
+}  // namespace
+
+cudaError_t causal_conv(const ConvArgs& a, int W, int type, cudaStream_t s) {
+    return type == ELEM_F32 ? conv_type<float>(a, W, s)
+                            : type == ELEM_F16 ? conv_type<__half>(a, W, s) : conv_type<__nv_bfloat16>(a, W, s);
+}
+
+}  // namespace krk

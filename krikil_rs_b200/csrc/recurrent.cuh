@@ -1,0 +1,61 @@
+// Device helpers of the recurrent layers: the rows and the state slots of a
+// packed request, neither of which is trusted.
+#pragma once
+#include "elem.cuh"
+#include "recurrent.h"
+
+namespace krk {
+
+struct Span {
+    int begin, end;  // rows [begin, end) of the packed ones
+};
+
+KRK_DEV int clamp_row(int r, int T) { return r < 0 ? 0 : r > T ? T : r; }
+
+KRK_DEV Span request_rows(const int32_t* cu, int s, int T) {
+    const int i = cu[s], j = cu[s + 1], begin = clamp_row(i, T), end = clamp_row(j, T);
+    if (begin != i || end != j || end < begin) check_fail(CHK_POSITION);
+    return {begin, end < begin ? begin : end};
+}
+
+// The slot that request s leaves its state in and the one it continues from
+// (below 0: nothing); false for padding, whose rows are left alone.
+KRK_DEV bool request_slots(const SlotArgs& a, int s, int& to, int& from) {
+    to = from = -1;
+    if (!a.state) return true;
+    const int t = a.slots ? a.slots[s] : s;
+    if (t < 0) return false;
+    const int f = a.init ? a.init[s] : t;
+    if (t >= a.num_slots || f >= a.num_slots) {
+        check_fail(CHK_TABLE);
+        return false;
+    }
+    to = t;
+    from = f;
+    return true;
+}
+
+// x * sigmoid(x) on the exponential unit (ex2 and rcp, each within 2^-22).
+KRK_DEV float fast_silu(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504088896341f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return x * r;
+}
+KRK_DEV float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// V consecutive elements in one access.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+template <typename T, int V>
+KRK_DEV Pack<T, V> load_pack(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+template <typename T, int V>
+KRK_DEV void store_pack(T* p, const Pack<T, V>& x) { *reinterpret_cast<Pack<T, V>*>(p) = x; }
+
+}  // namespace krk

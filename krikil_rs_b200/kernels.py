@@ -438,3 +438,176 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
     if rc:
         check(rc)
     return (out, lse) if return_lse else out
+
+
+# ------------------------------------------- recurrent layers over state slots
+def _rows2(t, dev, name):
+    """(type, rows, width, row stride) of a float tensor [rows, width] whose last dimension is dense."""
+    kind, shape, strides = _TYPES.get(t.dtype), t.shape, t.stride()
+    if kind is None or len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or t.device != dev:
+        raise _not_elems(name, 2, dev)
+    return kind, shape[0], shape[1], strides[0]
+
+
+def _same_rows(t, kind, rows, width, dev, name):
+    """(address, row stride) of a tensor like x; (None, 0) of None."""
+    if t is None:
+        return None, 0
+    k, r, w, st = _rows2(t, dev, name)
+    if k != kind or r != rows or w != width:
+        raise ValueError(f"{name}: expected [{rows}, {width}] of x's type")
+    return t.data_ptr(), st
+
+
+def _weights(t, shape, dev, name):
+    """The address of a dense float32 tensor of this shape (None: None)."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.shape != shape or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous float32 tensor of {tuple(shape)} on {dev}")
+    return t.data_ptr()
+
+
+def _slot_args(state, shape, dtype, slots, init, requests, dev):
+    """The pool's address, slot stride and size, and the addresses of slots and init."""
+    if state is None:
+        if slots is not None or init is not None:
+            raise ValueError("slots and init need a state")
+        return None, 0, 0, None, None
+    have, strides = state.shape, state.stride()
+    if state.dtype != dtype or state.device != dev or have[1:] != shape or (
+            shape[1] > 1 and strides[2] != 1) or (shape[0] > 1 and strides[1] != shape[1]):
+        raise ValueError(f"state: expected {dtype} [slots, {shape[0]}, {shape[1]}] on {dev} with dense slots")
+    if slots is None and have[0] < requests:
+        raise ValueError(f"state: expected a slot for each of {requests} requests, or their slots")
+    return (state.data_ptr(), strides[0], have[0],
+            None if slots is None else _ints(slots, requests, dev, "slots"),
+            None if init is None else _ints(init, requests, dev, "init"))
+
+
+def _call(dev, fn, args) -> None:
+    index = dev.index
+    rc = fn(*args, _raw_stream(index)) if index == _current_device() else _elsewhere(dev, fn, *args)
+    if rc:
+        check(rc)
+
+
+def _conv_args(x, weight, bias, state, slots, init, out, requests):
+    dev = _cuda_device(x)
+    kind, rows, ch, x_st = _rows2(x, dev, "x")
+    if len(weight.shape) != 2 or weight.shape[0] != ch:
+        raise ValueError(f"weight: expected [{ch}, width]")
+    width = weight.shape[1]
+    slot = _slot_args(state, (width - 1, ch), x.dtype, slots, init, rows if requests is None else requests, dev)
+    if out is None:
+        out = x.new_empty(rows, ch)
+    out_at, o_st = _same_rows(out, kind, rows, ch, dev, "out")
+    return dev, out, (x.data_ptr(), x_st, _weights(weight, (ch, width), dev, "weight"),
+                      _weights(bias, (ch,), dev, "bias"), out_at, o_st, kind, *slot), rows, ch, width
+
+
+def _requests(cu, dev):
+    """(address, number of requests) of packed requests' offsets."""
+    n = cu.numel()
+    if n < 1:
+        raise ValueError("cu: expected the requests' offsets, one more than there are requests")
+    return _ints(cu, n, dev, "cu"), n - 1
+
+
+def causal_conv(x, weight, cu, bias=None, state=None, slots=None, init=None, silu: bool = True, out=None):
+    """Causal depthwise convolution of packed requests: x [T, C], weight [C, W]
+    (W 2 to 4) and bias [C] float32, then x * sigmoid(x) unless silu is False.
+    Request s owns rows cu[s] .. cu[s+1]-1 (cu int32 [S+1]); its last W-1 rows go
+    to slot slots[s] (int32 [S]; -1: padding, left alone; None: slot s) of state
+    [slots, W-1, C] of x's type, and those before it come from slot init[s] (-1:
+    it begins; None: the same slot).  Without a state every request begins.
+    Returns out [T, C], whose rows of no request are left as they were."""
+    cu_at, requests = _requests(cu, x.device)
+    dev, out, args, rows, ch, width = _conv_args(x, weight, bias, state, slots, init, out, requests)
+    _call(dev, lib.krk_k_causal_conv, (*args, cu_at, rows, requests, ch, width, int(silu)))
+    return out
+
+
+def causal_conv_step(x, weight, state, slots=None, bias=None, init=None, silu: bool = True, out=None):
+    """causal_conv of one token a request: row b of x [B, C] is request b's."""
+    dev, out, args, rows, ch, width = _conv_args(x, weight, bias, state, slots, init, out, None)
+    _call(dev, lib.krk_k_causal_conv_step, (*args, rows, ch, width, int(silu)))
+    return out
+
+
+def _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests):
+    dev = _cuda_device(x)
+    kind, rows, ch, x_st = _rows2(x, dev, "x")
+    if len(a.shape) != 2 or a.shape[0] != ch:
+        raise ValueError(f"a: expected [{ch}, states]")
+    n = a.shape[1]
+
+    def grouped(t, name):
+        if len(t.shape) == 2:
+            k, r, w, st = _rows2(t, dev, name)
+            g, sg = 1, w
+        else:
+            k, (r, g, w), (st, sg, _) = _elems3(t, dev, name)
+        if k != kind or r != rows or w != n:
+            raise ValueError(f"{name}: expected [{rows}, {n}] or [{rows}, groups, {n}] of x's type")
+        return t.data_ptr(), st, sg, g
+
+    b_at, b_st, b_sg, groups = grouped(b, "b")
+    c_at, c_st, c_sg, c_groups = grouped(c, "c")
+    if c_groups != groups or not groups or ch % groups:
+        raise ValueError(f"b and c: expected as many groups, dividing {ch} channels")
+    dt_at, dt_st = _same_rows(dt, kind, rows, ch, dev, "dt")
+    z_at, z_st = _same_rows(z, kind, rows, ch, dev, "z")
+    slot = _slot_args(state, (ch, n), torch.float32, slots, init, rows if requests is None else requests, dev)
+    if out is None:
+        out = x.new_empty(rows, ch)
+    out_at, o_st = _same_rows(out, kind, rows, ch, dev, "out")
+    return dev, out, (x.data_ptr(), x_st, dt_at, dt_st, z_at, z_st, b_at, b_st, b_sg, c_at, c_st, c_sg, out_at, o_st,
+                      kind, _weights(a, (ch, n), dev, "a"), _weights(d, (ch,), dev, "d"),
+                      _weights(dt_bias, (ch,), dev, "dt_bias"), *slot), (ch, n, groups), rows
+
+
+def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None, slots=None, init=None, out=None):
+    """Selective state space scan of packed requests: x, dt and the gate z [T, D],
+    b and c [T, N] or [T, G, N] of one type; the decay a [D, N] (negative), the
+    skip d [D] and dt_bias [D] float32.  With delta = softplus(dt + dt_bias), h =
+    exp(delta a) h + delta x b and out = (h . c + d x) * z * sigmoid(z).  Requests
+    and slots as for causal_conv; state is float32 [slots, D, N].  Returns out
+    [T, D] (which may be x, dt or z), whose rows of no request are left as they
+    were."""
+    cu_at, requests = _requests(cu, x.device)
+    dev, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
+    _call(dev, lib.krk_k_selective_scan, (*args, cu_at, rows, requests, *sizes))
+    return out
+
+
+def selective_step(x, dt, a, b, c, state, slots=None, d=None, z=None, dt_bias=None, init=None, out=None):
+    """selective_scan of one token a request: row t of x [B, D] is request t's."""
+    dev, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, None)
+    _call(dev, lib.krk_k_selective_step, (*args, rows, *sizes))
+    return out
+
+
+def token_logprobs(logits, tokens=None, top: int = 0):
+    """Log probabilities under softmax of each row of logits [R, V]: of tokens
+    (int32 [R] or [R, K]; negative: none asked, 0), the entropy [R], and the ids
+    and log probabilities [R, top] of the largest logits (at most 64), the lower
+    id first among equal ones.  Returns (logprobs like tokens, or None; entropy;
+    top_ids; top_logprobs), float32 and int32."""
+    dev = _cuda_device(logits)
+    kind, rows, vocab, ld = _rows2(logits, dev, "logits")
+    _number(top, "top")
+    asked, tokens_at = 0, None
+    if tokens is not None:
+        if len(tokens.shape) not in (1, 2) or tokens.shape[0] != rows:
+            raise ValueError(f"tokens: expected [{rows}] or [{rows}, tokens]")
+        asked = 1 if len(tokens.shape) == 1 else tokens.shape[1]
+        tokens_at = _ints(tokens, rows * asked, dev, "tokens")
+    buf = torch.empty(rows * (asked + 1 + 2 * top), device=dev, dtype=torch.float32)
+    at, (lp, entropy, ids, best) = buf.data_ptr(), buf.unsafe_split_with_sizes((rows * asked, rows, rows * top, rows * top))
+    ids_at = at + 4 * rows * (asked + 1)
+    _call(dev, lib.krk_k_token_logprobs,
+          (logits.data_ptr(), ld, kind, rows, vocab, tokens_at, asked, at, at + 4 * rows * asked, top, ids_at,
+           ids_at + 4 * rows * top))
+    return (None if tokens is None else lp.view(tokens.shape), entropy, ids.view(torch.int32).view(rows, top),
+            best.view(rows, top))

@@ -188,6 +188,31 @@ extern "C" {
                                    scale: c_float, window: c_int, max_len: c_int, out: *mut c_void, o_sb: i64,
                                    o_sh: i64, lse: *mut c_float, work: *mut c_float, work_floats: usize,
                                    stream: *mut c_void) -> c_int;
+    pub fn krk_k_causal_conv(x: *mut c_void, x_st: i64, weight: *const c_float, bias: *const c_float,
+                             out: *mut c_void, o_st: i64, dtype: c_int, state: *mut c_void, state_stride: i64,
+                             num_slots: c_int, slots: *const i32, init: *const i32, cu: *const i32, rows: c_int,
+                             requests: c_int, channels: c_int, width: c_int, silu: c_int,
+                             stream: *mut c_void) -> c_int;
+    pub fn krk_k_causal_conv_step(x: *mut c_void, x_st: i64, weight: *const c_float, bias: *const c_float,
+                                  out: *mut c_void, o_st: i64, dtype: c_int, state: *mut c_void, state_stride: i64,
+                                  num_slots: c_int, slots: *const i32, init: *const i32, rows: c_int,
+                                  channels: c_int, width: c_int, silu: c_int, stream: *mut c_void) -> c_int;
+    pub fn krk_k_selective_scan(x: *mut c_void, x_st: i64, dt: *mut c_void, dt_st: i64, z: *mut c_void, z_st: i64,
+                                b: *mut c_void, b_st: i64, b_sg: i64, c: *mut c_void, c_st: i64, c_sg: i64,
+                                out: *mut c_void, o_st: i64, dtype: c_int, a: *const c_float, d: *const c_float,
+                                dt_bias: *const c_float, state: *mut c_float, state_stride: i64, num_slots: c_int,
+                                slots: *const i32, init: *const i32, cu: *const i32, rows: c_int, requests: c_int,
+                                channels: c_int, states: c_int, groups: c_int, stream: *mut c_void) -> c_int;
+    pub fn krk_k_selective_step(x: *mut c_void, x_st: i64, dt: *mut c_void, dt_st: i64, z: *mut c_void, z_st: i64,
+                                b: *mut c_void, b_st: i64, b_sg: i64, c: *mut c_void, c_st: i64, c_sg: i64,
+                                out: *mut c_void, o_st: i64, dtype: c_int, a: *const c_float, d: *const c_float,
+                                dt_bias: *const c_float, state: *mut c_float, state_stride: i64, num_slots: c_int,
+                                slots: *const i32, init: *const i32, rows: c_int, channels: c_int, states: c_int,
+                                groups: c_int, stream: *mut c_void) -> c_int;
+    pub fn krk_k_token_logprobs(logits: *mut c_void, ld: i64, dtype: c_int, rows: c_int, vocab: c_int,
+                                tokens: *const i32, asked: c_int, logprobs: *mut c_float, entropy: *mut c_float,
+                                top: c_int, top_ids: *mut i32, top_logprobs: *mut c_float,
+                                stream: *mut c_void) -> c_int;
     pub fn krk_k_wait_probe(src16: *const c_float, polls: c_int, copy: c_int, status: *mut i32,
                             stream: *mut c_void) -> c_int;
     pub fn krk_k_greedy(logits: *const c_float, ld: i64, vocab: c_int, b: c_int, seen: *mut u32, penalty: c_float,

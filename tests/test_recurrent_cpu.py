@@ -1,0 +1,106 @@
+"""Refusals of the entry points of recurrent layers over state slots and of the log probabilities.  Arguments are
+checked before a device is touched, so these run without a GPU: a refused call answers INVALID and names the fault, a
+sound one gets as far as the missing device."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from krikil_rs_b200 import _lib, kernels as K  # noqa: E402
+from krikil_rs_b200._lib import lib  # noqa: E402
+
+P = 4096  # a placeholder address, aligned to 16 bytes: never read
+FAR = 1 << 40
+
+SLOT = dict(state=P, stride=4096, num_slots=8, slots=P, init=P)
+CONV = dict(x=P, x_st=64, weight=P, bias=P, out=FAR, o_st=64, type=0, **SLOT, cu=P, T=5, S=2, C=64, W=4, silu=1,
+            stream=None)
+CONV_STEP = dict(x=P, x_st=64, weight=P, bias=P, out=FAR, o_st=64, type=0, **SLOT, B=2, C=64, W=4, silu=1,
+                 stream=None)
+SCAN = dict(x=P, x_st=64, dt=P, dt_st=64, z=P, z_st=64, b=P, b_st=16, b_sg=16, c=P, c_st=16, c_sg=16, out=FAR, o_st=64,
+            type=0, a=P, d=P, dt_bias=P, **SLOT, cu=P, T=5, S=2, D=64, N=16, G=1, stream=None)
+STEP = dict(x=P, x_st=64, dt=P, dt_st=64, z=P, z_st=64, b=P, b_st=16, b_sg=16, c=P, c_st=16, c_sg=16, out=FAR, o_st=64,
+            type=0, a=P, d=P, dt_bias=P, **SLOT, B=2, D=64, N=16, G=1, stream=None)
+LOGPROBS = dict(logits=P, ld=100, type=0, R=3, V=100, tokens=P, K=1, lp=P, entropy=P, top=5, ids=P, best=P, stream=None)
+
+
+def refused(fn, base, what, value, word):
+    args = dict(base)
+    args.update(zip(what, value) if isinstance(what, tuple) else [(what, value)])
+    assert list(args) == list(base)
+    assert fn(*args.values()) == _lib.INVALID, (what, value)
+    assert word in lib.krk_last_error().decode(), lib.krk_last_error()
+
+
+POOL = [("num_slots", 0, "num_slots"), ("num_slots", -1, "num_slots"), ("stride", 100, "stride"), ("state", P + 2, "state")]
+BARE = [("state", None, "need a state"), (("state", "slots", "init"), (None, None, None), "need a state")]
+CONV_FAULTS = POOL + [("type", 3, "type"), ("type", -1, "type"), ("W", 1, "width"), ("W", 5, "width"), ("C", 0, "channels"),
+                      ("C", 1 << 25, "channels"), ("weight", None, "weight"), ("weight", P + 2, "aligned"),
+                      ("bias", P + 2, "aligned"), ("x", None, "x and out"), ("out", None, "x and out"),
+                      ("x", P + 2, "aligned"), ("out", P + 2, "aligned"), ("o_st", 63, "overlap"),
+                      ("out", P, "overlap x"), ("out", P + 4 * 32, "overlap x"),
+                      (("x_st", "o_st", "out"), (100, 100, P + 4 * 63), "overlap x"),
+                      (("x_st", "o_st", "out"), (100, 100, P + 4 * 137), "overlap x")]
+
+
+@pytest.mark.parametrize("what,value,word", CONV_FAULTS + BARE + [("cu", None, "null"), ("T", -1, "rows"), ("S", -1, "rows")])
+def test_conv_refuses(what, value, word):
+    refused(lib.krk_k_causal_conv, CONV, what, value, word)
+
+
+@pytest.mark.parametrize("what,value,word", CONV_FAULTS + [("state", None, "null"), ("B", -1, "rows")])
+def test_conv_step_refuses(what, value, word):
+    refused(lib.krk_k_causal_conv_step, CONV_STEP, what, value, word)
+
+
+SCAN_FAULTS = POOL + [("type", 3, "type"), ("N", 0, "N must"), ("N", 257, "N must"), ("D", 0, "D must"), ("G", 0, "D must"),
+                      ("G", 3, "D must"), ("D", 1 << 25, "D must"), ("a", None, "a must"), ("a", P + 1, "a must"),
+                      ("d", P + 1, "aligned"), ("dt_bias", P + 1, "aligned"), ("z", P + 1, "aligned"),
+                      ("o_st", 63, "overlap")] + [(n, None, "must be set") for n in ("x", "dt", "b", "c", "out")] + [
+                          (n, P + 2, "aligned") for n in ("x", "dt", "b", "c", "out")]
+
+
+@pytest.mark.parametrize("what,value,word", SCAN_FAULTS + BARE + [("cu", None, "null"), ("T", -1, "rows"), ("S", -1, "rows")])
+def test_scan_refuses(what, value, word):
+    refused(lib.krk_k_selective_scan, SCAN, what, value, word)
+
+
+@pytest.mark.parametrize("what,value,word", SCAN_FAULTS + [("state", None, "null"), ("B", -1, "rows")])
+def test_step_refuses(what, value, word):
+    refused(lib.krk_k_selective_step, STEP, what, value, word)
+
+
+@pytest.mark.parametrize("what,value,word", [
+    ("type", 3, "type"), ("R", -1, "R and K"), ("K", -1, "R and K"), ("V", 0, "V positive"), ("top", -1, "top"),
+    ("top", 65, "top"), (("top", "V"), (5, 4), "top"), ("logits", None, "logits"), ("logits", P + 2, "aligned"),
+    ("tokens", None, "null"), ("lp", None, "null"), ("ids", None, "null"), ("best", None, "null")])
+def test_logprobs_refuses(what, value, word):
+    refused(lib.krk_k_token_logprobs, LOGPROBS, what, value, word)
+
+
+def test_calls_of_nothing_are_fine():
+    for fn, base, none in ((lib.krk_k_causal_conv, CONV, ("S", 0)), (lib.krk_k_causal_conv_step, CONV_STEP, ("B", 0)),
+                           (lib.krk_k_selective_scan, SCAN, ("S", 0)), (lib.krk_k_selective_step, STEP, ("B", 0)),
+                           (lib.krk_k_token_logprobs, LOGPROBS, ("R", 0))):
+        assert fn(*dict(base, **dict([none])).values()) == _lib.OK
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would read the placeholder addresses")
+def test_sound_calls_reach_the_device():
+    columns = dict(CONV, x_st=128, o_st=128, out=P + 4 * 64)  # two halves of one matrix
+    for fn, args in ((lib.krk_k_causal_conv, CONV), (lib.krk_k_causal_conv, columns),
+                     (lib.krk_k_causal_conv_step, CONV_STEP), (lib.krk_k_selective_scan, SCAN),
+                     (lib.krk_k_selective_scan, dict(SCAN, z=None, d=None, dt_bias=None, state=None, stride=0, num_slots=0,
+                                                     slots=None, init=None)),
+                     (lib.krk_k_selective_step, STEP), (lib.krk_k_token_logprobs, LOGPROBS),
+                     (lib.krk_k_token_logprobs, dict(LOGPROBS, entropy=None, top=0, ids=None, best=None))):
+        assert fn(*args.values()) == _lib.CUDA, lib.krk_last_error()
+
+
+def test_wrappers_want_cuda_tensors():
+    x, w, cu = torch.zeros(3, 8), torch.zeros(8, 4), torch.zeros(2, dtype=torch.int32)
+    a, bc, state = torch.zeros(8, 4), torch.zeros(3, 4), torch.zeros(3, 8, 4)
+    for call in (lambda: K.causal_conv(x, w, cu), lambda: K.causal_conv_step(x, w, torch.zeros(3, 3, 8)),
+                 lambda: K.selective_scan(x, x, a, bc, bc, cu), lambda: K.selective_step(x, x, a, bc, bc, state),
+                 lambda: K.token_logprobs(x)):
+        with pytest.raises(ValueError, match="CUDA|cuda"):
+            call()
