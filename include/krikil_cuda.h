@@ -547,7 +547,7 @@ KRK_API int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int typ
  * Element (t, i) of a [T][.] tensor is p[t*p_st + i]; pointers are aligned to
  * their elements, and 16-byte aligned rows are read and written 16 bytes at a
  * time.  The calls run on the current device, to which `stream` and all pointers
- * belong; they need no scratch and can be captured into a CUDA graph. */
+ * belong, and can be captured into a CUDA graph. */
 
 /* Causal depthwise convolution of width W (2, 3 or 4) over C channels:
  *   out[t][c] = act(bias[c] + sum_j weight[c*W + j] x[t - (W-1) + j][c]),
@@ -570,13 +570,19 @@ KRK_API int krk_k_causal_conv_step(void* x, int64_t x_st, const float* weight, c
  *   out[t][i] = (sum_n h[n] c[t][g][n] + d[i] x[t][i]) * z[t][i] * sigmoid(z[t][i]).
  * a [D][N] is the decay itself (negative, as -exp(A_log)); d, dt_bias (zeros) and
  * z (no gate) may be NULL.  The state is [D][N].  out may be x, dt or z with
- * their strides, and must not overlap the others. */
+ * their strides, and must not overlap the others.  max_len: a bound of the
+ * requests' rows, 0 = T, which moves the results by rounding at most.  work:
+ * 16-byte aligned device scratch of krk_selective_scan_work_floats(T, D, N, G,
+ * max_len) floats, with which long requests are walked in pieces at once -- none
+ * (0) when no request can be so long, on the current device -- with no initial
+ * contents, for calls that do not run at the same time. */
+KRK_API size_t krk_selective_scan_work_floats(int T, int D, int N, int G, int max_len);
 KRK_API int krk_k_selective_scan(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z, int64_t z_st, void* b,
                                  int64_t b_st, int64_t b_sg, void* c, int64_t c_st, int64_t c_sg, void* out,
                                  int64_t o_st, int type, const float* a, const float* d, const float* dt_bias,
                                  float* state, int64_t state_stride, int num_slots, const int32_t* slots,
                                  const int32_t* init, const int32_t* cu, int T, int S, int D, int N, int G,
-                                 void* stream);
+                                 int max_len, float* work, size_t work_floats, void* stream);
 KRK_API int krk_k_selective_step(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z, int64_t z_st, void* b,
                                  int64_t b_st, int64_t b_sg, void* c, int64_t c_st, int64_t c_sg, void* out,
                                  int64_t o_st, int type, const float* a, const float* d, const float* dt_bias,

@@ -88,8 +88,9 @@ _SIGS = {
         _i32, _i32, _i32, _i32, _vp]),
     "krk_k_causal_conv_step": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32,
         _i32, _i32, _i32, _vp]),
+    "krk_selective_scan_work_floats": (C.c_size_t, [_i32] * 5),
     "krk_k_selective_scan": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
-        _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+        _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, C.c_size_t, _vp]),
     "krk_k_selective_step": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
         _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     "krk_k_token_logprobs": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp]),

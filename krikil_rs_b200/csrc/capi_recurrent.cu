@@ -82,7 +82,7 @@ int krk_k_causal_conv(void* x, int64_t x_st, const float* weight, const float* b
     const char* who = "causal_conv";
     if (!cu) return invalid(who, "null pointer");
     const krk::ConvArgs a{x, x_st, weight, bias, out, o_st, {state, state_stride, num_slots, slots, init}, cu, T, S, C,
-                          silu != 0};
+                          silu != 0, false};
     return conv_call(who, a, W, type, (cudaStream_t)stream);
 }
 
@@ -92,11 +92,12 @@ int krk_k_causal_conv_step(void* x, int64_t x_st, const float* weight, const flo
     const char* who = "causal_conv_step";
     if (!state) return invalid(who, "null pointer");
     const krk::ConvArgs a{x, x_st, weight, bias, out, o_st, {state, state_stride, num_slots, slots, init}, nullptr, B,
-                          B, C, silu != 0};
+                          B, C, silu != 0, false};
     return conv_call(who, a, W, type, (cudaStream_t)stream);
 }
 
-static int scan_call(const char* who, const krk::ScanArgs& a, int type, cudaStream_t stream) {
+static int scan_call(const char* who, const krk::ScanArgs& a, int type, int max_len, float* work, size_t work_floats,
+                     cudaStream_t stream) {
     const int es = elem_size(type);
     if (!es) return invalid(who, "unknown element type");
     if (a.T < 0 || a.S < 0) return invalid(who, "rows and requests must not be negative");
@@ -109,19 +110,30 @@ static int scan_call(const char* who, const krk::ScanArgs& a, int type, cudaStre
     if (a.T > 0 && (!readable(a.x, es) || !readable(a.dt, es) || !readable(a.b, es) || !readable(a.c, es) ||
                     (a.z && !readable(a.z, es)) || !writable(a.out, a.o_st, a.T, a.D, es)))
         return invalid(who, "x, dt, b, c and out must be set and aligned to their elements, rows of out must not overlap");
-    return done(who, a.cu ? krk::selective_scan(a, type, stream) : krk::selective_step(a, type, stream));
+    if (!a.cu) return done(who, krk::selective_step(a, type, stream));
+    if (max_len < 0) return invalid(who, "max_len must not be negative");
+    const size_t need = krk::scan_work_floats(a.T, a.D, a.N, a.G, max_len);
+    if (need > 0 && (!work || work_floats < need || !aligned(work, 16)))
+        return krk::report_error(KRK_INVALID, std::string(who) + ": work must be 16-byte aligned and hold " +
+                                                  std::to_string(need) + " floats");
+    return done(who, krk::selective_scan(a, type, max_len, work, stream));
+}
+
+size_t krk_selective_scan_work_floats(int T, int D, int N, int G, int max_len) {
+    if (T <= 0 || D <= 0 || N <= 0 || N > krk::SCAN_MAX_STATES || G <= 0 || D % G || max_len < 0) return 0;
+    return krk::scan_work_floats(T, D, N, G, max_len);
 }
 
 int krk_k_selective_scan(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z, int64_t z_st, void* b, int64_t b_st,
                          int64_t b_sg, void* c, int64_t c_st, int64_t c_sg, void* out, int64_t o_st, int type,
                          const float* a, const float* d, const float* dt_bias, float* state, int64_t state_stride,
                          int num_slots, const int32_t* slots, const int32_t* init, const int32_t* cu, int T, int S,
-                         int D, int N, int G, void* stream) {
+                         int D, int N, int G, int max_len, float* work, size_t work_floats, void* stream) {
     const char* who = "selective_scan";
     if (!cu) return invalid(who, "null pointer");
     const krk::ScanArgs s{x, x_st, dt, dt_st, z, z_st, b, b_st, b_sg, c, c_st, c_sg, out, o_st, a, d, dt_bias,
                           {state, state_stride, num_slots, slots, init}, cu, T, S, D, N, G};
-    return scan_call(who, s, type, (cudaStream_t)stream);
+    return scan_call(who, s, type, max_len, work, work_floats, (cudaStream_t)stream);
 }
 
 int krk_k_selective_step(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z, int64_t z_st, void* b, int64_t b_st,
@@ -133,7 +145,7 @@ int krk_k_selective_step(void* x, int64_t x_st, void* dt, int64_t dt_st, void* z
     if (!state) return invalid(who, "null pointer");
     const krk::ScanArgs s{x, x_st, dt, dt_st, z, z_st, b, b_st, b_sg, c, c_st, c_sg, out, o_st, a, d, dt_bias,
                           {state, state_stride, num_slots, slots, init}, nullptr, B, B, D, N, G};
-    return scan_call(who, s, type, (cudaStream_t)stream);
+    return scan_call(who, s, type, 0, nullptr, 0, (cudaStream_t)stream);
 }
 
 int krk_k_token_logprobs(void* logits, int64_t ld, int type, int R, int V, const int32_t* tokens, int K,

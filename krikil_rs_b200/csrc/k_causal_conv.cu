@@ -11,6 +11,7 @@ namespace krk {
 namespace {
 
 constexpr int CONV_THREADS = 128;
+constexpr int CONV_GROUP = 4;  // rows whose loads are on their way together
 
 // One thread: V channels; their taps, bias, and the window of W-1 rows.
 template <typename T, int W, int V>
@@ -20,10 +21,19 @@ struct ConvColumn {
     float w[W][V], bias[V];
 
     KRK_DEV ConvColumn(const ConvArgs& args, int channel) : a(args), c(channel) {
+        __align__(16) float flat[V * W];
+        const float* from = a.w + (int64_t)c * W;
+        if (V % 4 == 0 && a.aligned) {
+#pragma unroll
+            for (int i = 0; i < V * W / 4; ++i) reinterpret_cast<float4*>(flat)[i] = reinterpret_cast<const float4*>(from)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V * W; ++i) flat[i] = from[i];
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) w[j][i] = a.w[(int64_t)(c + i) * W + j];
+            for (int j = 0; j < W; ++j) w[j][i] = flat[i * W + j];
             bias[i] = a.bias ? a.bias[c + i] : 0.0f;
         }
     }
@@ -60,17 +70,24 @@ struct ConvColumn {
 #pragma unroll
             for (int v = 0; v < V; ++v) win[k][v] = to_f32(p.v[v]);
         }
-        for (int t = i; t < j; ++t) {
-            const Pack<T, V> p = load_pack<T, V>(row(t));
-            float x[V];
+        for (int t = i; t < j; t += CONV_GROUP) {
+            Pack<T, V> p[CONV_GROUP];
 #pragma unroll
-            for (int v = 0; v < V; ++v) x[v] = to_f32(p.v[v]);
-            put(t, win, x);
+            for (int u = 0; u < CONV_GROUP; ++u)
+                if (t + u < j) p[u] = load_pack<T, V>(row(t + u));
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
+            for (int u = 0; u < CONV_GROUP; ++u) {
+                if (t + u >= j) break;
+                float x[V];
 #pragma unroll
-                for (int k = 0; k + 1 < W - 1; ++k) win[k][v] = win[k + 1][v];
-                win[W - 2][v] = x[v];
+                for (int v = 0; v < V; ++v) x[v] = to_f32(p[u].v[v]);
+                put(t + u, win, x);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+#pragma unroll
+                    for (int k = 0; k + 1 < W - 1; ++k) win[k][v] = win[k + 1][v];
+                    win[W - 2][v] = x[v];
+                }
             }
         }
     }
@@ -129,14 +146,37 @@ __global__ void __launch_bounds__(CONV_THREADS) conv_kernel(ConvArgs a, int rows
     }
 }
 
-template <typename T, int W, int V>
+// One row a request: a thread takes R of them, with the same taps.
+template <typename T, int W, int V, int R>
 __global__ void __launch_bounds__(CONV_THREADS) conv_step_kernel(ConvArgs a, int side) {
-    const int t = blockIdx.x / side, c = ((blockIdx.x - t * side) * CONV_THREADS + threadIdx.x) * V;
-    int to, from;
-    if (c >= a.C || !request_slots(a.slot, t, to, from)) return;
+    const int t0 = blockIdx.x / side * R;
+    const int c = ((blockIdx.x - blockIdx.x / side * side) * CONV_THREADS + threadIdx.x) * V;
+    if (c >= a.C) return;
     const ConvColumn<T, W, V> col(a, c);
-    col.run(t, t + 1, t, from);
-    col.keep({t, t + 1}, to, from);
+    int to[R], from[R];
+    bool live[R];
+    Pack<T, V> rows[R][W];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        live[r] = t0 + r < a.T && request_slots(a.slot, t0 + r, to[r], from[r]);
+        if (!live[r]) continue;
+#pragma unroll
+        for (int k = 0; k < W; ++k) rows[r][k] = col.tap(t0 + r - (W - 1) + k, t0 + r, from[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (!live[r]) continue;
+        float win[W - 1][V], x[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) win[k][v] = to_f32(rows[r][k].v[v]);
+            x[v] = to_f32(rows[r][W - 1].v[v]);
+        }
+        col.put(t0 + r, win, x);
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) store_pack<T, V>(col.kept(to[r], k), rows[r][k + 1]);
+    }
 }
 
 bool fits(const void* p, int64_t stride, size_t bytes, size_t elem) {
@@ -146,12 +186,17 @@ bool fits(const void* p, int64_t stride, size_t bytes, size_t elem) {
 template <typename T, int W, int V>
 cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
     const int side = (a.C + CONV_THREADS * V - 1) / (CONV_THREADS * V);
+    const int sms = paged_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
     if (!a.cu) {
-        if ((int64_t)a.T * side > INT32_MAX) return cudaErrorInvalidValue;
-        conv_step_kernel<T, W, V><<<a.T * side, CONV_THREADS, 0, s>>>(a, side);
+        // two requests a thread once every multiprocessor has a full set of threads
+        const int64_t units = (int64_t)a.T * side;
+        if (units > INT32_MAX) return cudaErrorInvalidValue;
+        if (units >= (int64_t)sms * 2048 / CONV_THREADS)
+            conv_step_kernel<T, W, V, 2><<<(a.T + 1) / 2 * side, CONV_THREADS, 0, s>>>(a, side);
+        else
+            conv_step_kernel<T, W, V, 1><<<(unsigned)units, CONV_THREADS, 0, s>>>(a, side);
     } else {
-        const int sms = paged_sm_count();
-        if (sms <= 0) return cudaErrorInvalidDevice;
         const int64_t share = (int64_t)a.T * side / (sms * 16);
         const int rows = share < 8 ? 8 : share > 64 ? 64 : (int)share;
         const int64_t blocks = (int64_t)(a.T > 0 ? (a.T + (int64_t)rows - 1) / rows : 1) * side;
@@ -163,7 +208,8 @@ cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
 }
 
 template <typename T, int W>
-cudaError_t conv_width(const ConvArgs& a, cudaStream_t s) {
+cudaError_t conv_width(ConvArgs a, cudaStream_t s) {
+    a.aligned = fits(a.w, 0, 16, 4);
     constexpr int V = 16 / sizeof(T);
     const bool wide = a.C % V == 0 && fits(a.x, a.T > 1 ? a.x_st : 0, 16, sizeof(T)) &&
                       fits(a.out, a.T > 1 ? a.o_st : 0, 16, sizeof(T)) &&

@@ -1,0 +1,8 @@
+// The selective scan of half activations.
+#include "selective_scan.cuh"
+
+namespace krk {
+cudaError_t selective_scan_f16(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
+    return scan_type<__half>(a, work, rows, s);
+}
+}  // namespace krk

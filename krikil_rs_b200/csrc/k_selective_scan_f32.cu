@@ -1,0 +1,8 @@
+// The selective scan of float32 activations.
+#include "selective_scan.cuh"
+
+namespace krk {
+cudaError_t selective_scan_f32(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
+    return scan_type<float>(a, work, rows, s);
+}
+}  // namespace krk

@@ -48,6 +48,28 @@ KRK_DEV float fast_exp2(float x) {
     return y;
 }
 
+// A decay in powers of two; finite, since rows that step by nothing step by 0 times it.
+KRK_DEV float scan_rate(float a) {
+    const float r = a * 1.44269504088896341f;
+    return r < -3.0e38f ? -3.0e38f : r;
+}
+
+// log(1 + e^v) as max(v, 0) + 2 atanh(w / (2 + w)), w = e^-|v|, by atanh's series (its argument is at most 1/3: the
+// first term left out is 2^-26 of the whole), which keeps the small steps that negative arguments make.
+KRK_DEV float step_width(float v) {
+    const float w = fast_exp2(fabsf(v) * -1.44269504088896341f);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(2.0f + w));
+    const float s = w * r, q = s * s;
+    float p = fmaf(q, 2.0f / 13.0f, 2.0f / 11.0f);
+    p = fmaf(p, q, 2.0f / 9.0f);
+    p = fmaf(p, q, 2.0f / 7.0f);
+    p = fmaf(p, q, 2.0f / 5.0f);
+    p = fmaf(p, q, 2.0f / 3.0f);
+    p = fmaf(p, q, 2.0f);
+    return fmaf(s, p, fmaxf(v, 0.0f));
+}
+
 // V consecutive elements in one access.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {

@@ -25,10 +25,16 @@ struct ConvArgs {
     const int32_t* cu;                           // [S+1]; nullptr: one row a request
     int T, S, C;
     bool silu;
+    bool aligned;                                // w on 16 bytes (the launcher's own)
 };
 cudaError_t causal_conv(const ConvArgs& a, int W, int type, cudaStream_t s);
 
 constexpr int SCAN_MAX_STATES = 256;
+constexpr int SCAN_THREADS = 128;
+constexpr int SCAN_BLOCKS = 4;  // blocks a multiprocessor, by registers
+constexpr int SCAN_LANE = 16;   // states a lane holds, if there are as many
+constexpr int SCAN_ALONE = 7;   // a request of up to so many pieces is not split
+constexpr int SCAN_PIECE = 64;  // fewest rows of one
 struct ScanArgs {
     const void* x; int64_t x_st;                 // (t, d) at t*x_st + d
     const void* dt; int64_t dt_st;
@@ -42,7 +48,12 @@ struct ScanArgs {
     const int32_t* cu;                           // [S+1]; nullptr: one row a request
     int T, S, D, N, G;
 };
-cudaError_t selective_scan(const ScanArgs& a, int type, cudaStream_t s);
+// The scan's split of long requests: scratch of so many floats lets requests of
+// up to max_len rows be walked in pieces of scan_piece_rows rows (0: they are not).
+int scan_piece_rows(int T, int D, int N, int G, int max_len);
+size_t scan_work_floats(int T, int D, int N, int G, int max_len);
+constexpr int64_t scan_split_room(int64_t T, int rows) { return T / rows * 8 / 7 + 2; }
+cudaError_t selective_scan(const ScanArgs& a, int type, int max_len, float* work, cudaStream_t s);
 cudaError_t selective_step(const ScanArgs& a, int type, cudaStream_t s);
 
 constexpr int LOGPROBS_MAX_TOP = 64;

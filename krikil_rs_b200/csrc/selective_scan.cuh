@@ -1,0 +1,361 @@
+// Selective state space scan over packed requests, with the requests' states in
+// a pool of slots.  With delta = softplus(dt + bias), channel d's N states and
+// output are
+//   h[n] = exp(delta A[d][n]) h[n] + delta x B[n],   y = (sum_n h[n] C[n] + D x) silu(z).
+//
+// Bound by the exponential unit: N exponentials a row and channel, two for
+// delta and two for the gate, at 16 a clock and multiprocessor.  So everything
+// else is kept small beside them.  K lanes share a channel and hold SPT of its
+// states each in registers; a channel's delta, gate and output are its lanes'
+// own work (of four rows, each lane has its part of them), and only B and C,
+// which all channels of a group read, go through shared memory, where a block
+// converts them once for its 128 / K channels.  The multiply-adds are packed in
+// pairs of states.
+//
+// A request is walked row by row; walking requests in pieces at once costs about
+// twice the work (a first walk finds each piece's own state and sum of delta, a
+// short kernel carries the states from piece to piece, and the last walk starts
+// from them), so that only a request of more than its share is split: one that
+// alone would take longer than twice what the whole call takes when it is shared
+// out evenly.
+#pragma once
+#include "kernels.h"
+#include "paged.h"
+#include "recurrent.cuh"
+
+namespace krk {
+namespace {
+
+constexpr int SCAN_GROUP = 4;  // rows whose outputs are formed together
+
+template <int K, int SPT>
+struct ScanShape {
+    static constexpr int CH = SCAN_THREADS / K, NP = K * SPT;
+    static constexpr int ROWS = NP <= 32 ? 32 : 1024 / NP;           // a tile of B and C
+    static constexpr int F = 2 * ROWS * NP / SCAN_THREADS;           // elements of them that a thread stages
+    static constexpr int OWN = K < SCAN_GROUP ? SCAN_GROUP / K : 1;  // rows of a group whose delta and output a lane forms
+    static constexpr int SHARE = K < SCAN_GROUP ? 1 : K / SCAN_GROUP;  // lanes that form the same one
+};
+
+// How a request is split.
+struct ScanSplit {
+    int rows;       // a piece's
+    float* start;   // [pieces of split requests][D][N]: the states that pieces start from
+    float* sum;     // [pieces of split requests][D]: their sums of delta
+    int room;       // pieces of split requests that there is room for: more come from offsets that do not ascend
+};
+KRK_DEV int scan_pieces(int n, int rows) { return rows > 0 && n > (int64_t)SCAN_ALONE * rows ? (n - 1) / rows + 1 : 1; }
+
+// The piece-th piece of all requests' (or of the split ones' alone, or of those
+// each one's first): its request, its place there, and the place of the
+// request's first one among the split ones'.  request < 0: there are not so many.
+struct ScanPiece {
+    int request, at, first;
+};
+enum ScanCount { COUNT_ALL, COUNT_SPLIT, COUNT_FIRST };
+KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piece, ScanCount count) {
+    __shared__ int warp_sum[2][SCAN_THREADS / 32];
+    __shared__ ScanPiece found;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int before = 0, before_split = 0;
+    if (tid == 0) found.request = -1;
+    __syncthreads();
+    for (int s0 = 0; s0 < S; s0 += SCAN_THREADS) {
+        const int s = s0 + tid;
+        int n = 0, m = 0;
+        if (s < S) {
+            const int begin = clamp_row(cu[s], T), end = clamp_row(cu[s + 1], T);
+            n = scan_pieces(end - begin, rows);
+            m = n > 1 ? n : 0;
+            if (count != COUNT_ALL) n = count == COUNT_SPLIT ? m : m > 0;
+        }
+        int x = n, y = m;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) x += p, y += q;
+        }
+        if (lane == 31) warp_sum[0][warp] = x, warp_sum[1][warp] = y;
+        __syncthreads();
+        int all = 0, all_split = 0;
+#pragma unroll
+        for (int w = 0; w < SCAN_THREADS / 32; ++w) {
+            if (w == warp) x += all, y += all_split;
+            all += warp_sum[0][w];
+            all_split += warp_sum[1][w];
+        }
+        const int at = piece - before - (x - n);
+        if (at >= 0 && at < n) found = {s, at, before_split + y - m};
+        before += all;
+        before_split += all_split;
+        __syncthreads();
+        if (found.request >= 0) break;
+    }
+    return found;
+}
+
+// Sums each of v's rows over K lanes.  While a lane holds several rows it keeps
+// half of them and gives the others away: with K < R lane i ends with rows
+// i * R/K .. of the R, else lanes i * K/R .. with row i.
+template <int R, int K>
+KRK_DEV void sum_rows(float (&v)[R], int lane) {
+    int n = R / 2;
+#pragma unroll
+    for (int off = K / 2; off > 0; off /= 2) {
+        if (n > 0) {
+            const bool upper = lane & off;
+#pragma unroll
+            for (int i = 0; i < R / 2; ++i)
+                if (i < n) {
+                    const float mine = upper ? v[i + n] : v[i], theirs = upper ? v[i] : v[i + n];
+                    v[i] = mine + __shfl_xor_sync(0xffffffffu, theirs, off);
+                }
+            n /= 2;
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+        }
+    }
+}
+
+// CARRY: the first walk of split requests, which leaves each piece's state from
+// zeros, for the piece behind it, and its sum of delta.
+template <typename T, int K, int SPT, bool PADDED, bool CARRY>
+__global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArgs a, ScanSplit split, int side) {
+    using Sh = ScanShape<K, SPT>;
+    constexpr int CH = Sh::CH, NP = Sh::NP, ROWS = Sh::ROWS, F = Sh::F, OWN = Sh::OWN, U = SCAN_GROUP;
+    __shared__ __align__(16) float s_bc[2][ROWS][2][NP];
+
+    const int tid = threadIdx.x, lane = tid % K, ch = tid / K, per = a.D / a.G;
+    const int block = blockIdx.x / side, cb = blockIdx.x - block * side, sides = side / a.G;
+    const int g = cb / sides, ch0 = (cb - g * sides) * CH;  // within the group
+    const bool open = ch < per - ch0;
+    const int d = g * per + (open ? ch0 + ch : 0);
+    const ScanPiece piece = split.rows > 0 ? find_piece(a.cu, a.S, a.T, split.rows, block, CARRY ? COUNT_SPLIT : COUNT_ALL) : ScanPiece{block, 0, 0};
+    if (piece.request < 0) return;
+    const Span span = request_rows(a.cu, piece.request, a.T);
+    int to, from;
+    if (!request_slots(a.slot, piece.request, to, from)) return;
+    const int pieces = scan_pieces(span.end - span.begin, split.rows);
+    const bool last = piece.at == pieces - 1;
+    if (pieces > 1 && (piece.first < 0 || piece.first > split.room - pieces)) return;
+    if (CARRY && last) return;
+    const int begin = span.begin + piece.at * split.rows, end = last ? span.end : begin + split.rows;
+
+    // States 4 (q K + lane) .. + 3 of the channel for q < SPT / 4: lanes read B and C side by side.
+    const auto state_of = [&](int j) { return 4 * (j / 4 * K + lane) + j % 4; };
+    float2 h[SPT / 2], rate[SPT / 2];
+    {
+        const float* old = CARRY ? nullptr
+                           : pieces > 1 ? split.start + (int64_t)(piece.first + piece.at) * a.D * a.N
+                           : from >= 0 ? (const float*)a.slot.state + from * a.slot.stride : nullptr;
+#pragma unroll
+        for (int j = 0; j < SPT; ++j) {
+            const int n = state_of(j);
+            const bool in = open && (!PADDED || n < a.N);
+            const int64_t at = (int64_t)d * a.N + n;
+            const float r = in ? scan_rate(a.a[at]) : 0.0f;
+            const float v = in && old ? old[at] : 0.0f;
+            (j % 2 ? rate[j / 2].y : rate[j / 2].x) = r;
+            (j % 2 ? h[j / 2].y : h[j / 2].x) = v;
+        }
+    }
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = !CARRY && a.d ? a.d[d] : 0.0f;
+    const T* xp = (const T*)a.x + d;
+    const T* dtp = (const T*)a.dt + d;
+    const T* zp = (const T*)a.z + d;
+    const T* bp = (const T*)a.b + g * a.b_sg;
+    const T* cp = (const T*)a.c + g * a.c_sg;
+    const T zero = from_f32<T>(0.0f);
+
+    // A thread's rows of a group, on their way while the group before is computed.
+    const int own = lane / Sh::SHARE * OWN;
+    T xr[OWN], dtr[OWN], zr[OWN];
+    const auto fetch = [&](int t0) {
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int t = t0 + own + o;
+            const bool in = open && t < end;
+            xr[o] = in ? xp[t * a.x_st] : zero;
+            dtr[o] = in ? dtp[t * a.dt_st] : zero;
+            if (!CARRY) zr[o] = in && a.z ? zp[t * a.z_st] : zero;
+        }
+    };
+    // And its elements of the next tile of B and C.
+    T bcr[F];
+    const auto fetch_bc = [&](int t0) {
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            const int i = f * SCAN_THREADS + tid, t = t0 + i / (2 * NP), n = i % NP;
+            const bool is_c = i / NP % 2;
+            const bool in = t < end && (!PADDED || n < a.N) && !(CARRY && is_c);
+            bcr[f] = in ? (is_c ? cp + t * a.c_st : bp + t * a.b_st)[n] : zero;
+        }
+    };
+    const auto stage_bc = [&](int buffer) {
+#pragma unroll
+        for (int f = 0; f < F; ++f) (&s_bc[buffer][0][0][0])[f * SCAN_THREADS + tid] = to_f32(bcr[f]);
+    };
+
+    float total = 0.0f;
+    if (begin < end) {
+        fetch(begin);
+        fetch_bc(begin);
+        stage_bc(0);
+    }
+    __syncthreads();
+    int buffer = 0;
+    for (int t0 = begin; t0 < end; t0 += ROWS, buffer ^= 1) {
+        const bool more = t0 + ROWS < end;
+        if (more) fetch_bc(t0 + ROWS);
+        const int rows = min(ROWS, end - t0);
+        for (int r0 = 0; r0 < rows; r0 += U) {
+            float step[U], put[U], gate[OWN], skipped[OWN];
+#pragma unroll
+            for (int o = 0; o < OWN; ++o) {
+                const float x = to_f32(xr[o]);
+                // rows behind the last one step by nothing: the states stay
+                const float delta = t0 + r0 + own + o < end ? step_width(to_f32(dtr[o]) + bias) : 0.0f;
+                step[o] = delta;
+                put[o] = delta * x;
+                if (!CARRY) {
+                    skipped[o] = skip * x;
+                    gate[o] = a.z ? fast_silu(to_f32(zr[o])) : 1.0f;
+                }
+            }
+            fetch(t0 + r0 + U);
+            if (K > 1) {
+                float mine[OWN], mine_put[OWN];
+#pragma unroll
+                for (int o = 0; o < OWN; ++o) mine[o] = step[o], mine_put[o] = put[o];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    step[u] = __shfl_sync(0xffffffffu, mine[u % OWN], u / OWN * Sh::SHARE, K);
+                    put[u] = __shfl_sync(0xffffffffu, mine_put[u % OWN], u / OWN * Sh::SHARE, K);
+                }
+            }
+            float y[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float4* b = reinterpret_cast<const float4*>(s_bc[buffer][r0 + u][0]) + lane;
+                const float4* c = reinterpret_cast<const float4*>(s_bc[buffer][r0 + u][1]) + lane;
+                const float2 st = make_float2(step[u], step[u]), pt = make_float2(put[u], put[u]);
+                float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int q = 0; q < SPT / 4; ++q) {
+                    const float4 b4 = b[q * K];
+                    const float4 c4 = CARRY ? b4 : c[q * K];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int j = 2 * q + i;
+                        const float2 e = __fmul2_rn(st, rate[j]);
+                        const float2 decay = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                        h[j] = __ffma2_rn(decay, h[j], __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y)));
+                        if (!CARRY) {
+                            float2 live = h[j];
+                            if (PADDED) {  // an infinite x makes no NaN of states that are not there
+                                if (state_of(2 * j) >= a.N) live.x = 0.0f;
+                                if (state_of(2 * j + 1) >= a.N) live.y = 0.0f;
+                            }
+                            acc = __ffma2_rn(live, i ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y), acc);
+                        }
+                    }
+                }
+                if (CARRY)
+                    total += step[u];
+                else
+                    y[u] = acc.x + acc.y;
+            }
+            if (!CARRY) {
+                sum_rows<U, K>(y, lane);
+#pragma unroll
+                for (int o = 0; o < OWN; ++o) {
+                    const int t = t0 + r0 + own + o;
+                    if (open && t < end && lane % Sh::SHARE == 0)
+                        ((T*)a.out)[t * a.o_st + d] = from_f32<T>((y[o] + skipped[o]) * gate[o]);
+                }
+            }
+        }
+        if (more) stage_bc(buffer ^ 1);
+        __syncthreads();
+    }
+
+    float* kept = CARRY ? split.start + (int64_t)(piece.first + piece.at + 1) * a.D * a.N
+                  : last && to >= 0 ? (float*)a.slot.state + to * a.slot.stride : nullptr;
+    if (!open || !kept) return;
+#pragma unroll
+    for (int j = 0; j < SPT; ++j) {
+        const int n = state_of(j);
+        if (!PADDED || n < a.N) kept[(int64_t)d * a.N + n] = j % 2 ? h[j / 2].y : h[j / 2].x;
+    }
+    if (CARRY && lane == 0) split.sum[(int64_t)(piece.first + piece.at) * a.D + d] = total;
+}
+
+// Carries a split request's states from piece to piece: start[c] becomes the
+// state that piece c starts from.  A thread a state, `blocks` blocks a request.
+__global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanArgs a, ScanSplit split, int blocks) {
+    const int place = blockIdx.x / blocks;
+    const int64_t at = (int64_t)(blockIdx.x - place * blocks) * SCAN_THREADS + threadIdx.x, size = (int64_t)a.D * a.N;
+    const ScanPiece piece = find_piece(a.cu, a.S, a.T, split.rows, place, COUNT_FIRST);
+    if (piece.request < 0) return;
+    const Span span = request_rows(a.cu, piece.request, a.T);
+    int to, from;
+    if (at >= size || !request_slots(a.slot, piece.request, to, from)) return;
+    const int pieces = scan_pieces(span.end - span.begin, split.rows), d = (int)(at / a.N);
+    if (piece.first < 0 || piece.first > split.room - pieces) return;
+    const float rate = scan_rate(a.a[at]);
+    float h = from >= 0 ? ((const float*)a.slot.state)[from * a.slot.stride + at] : 0.0f;
+    float* start = split.start + piece.first * size + at;
+    const float* sum = split.sum + (int64_t)piece.first * a.D + d;
+    start[0] = h;
+    for (int c = 1; c < pieces; ++c) {
+        h = fmaf(fast_exp2(rate * sum[(int64_t)(c - 1) * a.D]), h, start[c * size]);
+        start[c * size] = h;
+    }
+}
+
+// ---------------------------------------------------------------- the launches
+template <typename T, int K, int SPT, bool PADDED>
+cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStream_t s) {
+    using Sh = ScanShape<K, SPT>;
+    const int64_t side = (int64_t)((a.D / a.G + Sh::CH - 1) / Sh::CH) * a.G;
+    ScanSplit split{0, nullptr, nullptr, 0};
+    int64_t pieces = a.S;
+    if (piece_rows > 0) {
+        const int64_t room = scan_split_room(a.T, piece_rows), states = (int64_t)a.D * a.N;
+        split = {piece_rows, work, work + room * states, (int)room};
+        pieces = a.S + a.T / piece_rows;
+        const int64_t blocks = (states + SCAN_THREADS - 1) / SCAN_THREADS;
+        const int64_t requests = a.T / (SCAN_ALONE * (int64_t)piece_rows);  // that can be split
+        if (side * room > INT32_MAX || blocks * requests > INT32_MAX) return cudaErrorInvalidValue;
+        scan_kernel<T, K, SPT, PADDED, true><<<(unsigned)(side * room), SCAN_THREADS, 0, s>>>(a, split, (int)side);
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        scan_carry_kernel<<<(unsigned)(blocks * requests), SCAN_THREADS, 0, s>>>(a, split, (int)blocks);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        add_launches(2);
+    }
+    if (side * pieces > INT32_MAX) return cudaErrorInvalidValue;
+    scan_kernel<T, K, SPT, PADDED, false><<<(unsigned)(side * pieces), SCAN_THREADS, 0, s>>>(a, split, (int)side);
+    add_launches(1);
+    return cudaGetLastError();
+}
+
+template <typename T, int K, int SPT>
+cudaError_t scan_padded(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
+    return a.N == K * SPT ? launch_scan<T, K, SPT, false>(a, work, rows, s) : launch_scan<T, K, SPT, true>(a, work, rows, s);
+}
+
+template <typename T>
+cudaError_t scan_type(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
+    if (a.N <= 4) return scan_padded<T, 1, 4>(a, work, rows, s);
+    if (a.N <= 8) return scan_padded<T, 1, 8>(a, work, rows, s);
+    if (a.N <= 16) return scan_padded<T, 1, 16>(a, work, rows, s);
+    if (a.N <= 32) return scan_padded<T, 2, 16>(a, work, rows, s);
+    if (a.N <= 64) return scan_padded<T, 4, 16>(a, work, rows, s);
+    if (a.N <= 128) return scan_padded<T, 8, 16>(a, work, rows, s);
+    return scan_padded<T, 16, 16>(a, work, rows, s);
+}
+
+}  // namespace
+}  // namespace krk

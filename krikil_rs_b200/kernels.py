@@ -567,17 +567,40 @@ def _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
                       _weights(dt_bias, (ch,), dev, "dt_bias"), *slot), (ch, n, groups), rows
 
 
-def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None, slots=None, init=None, out=None):
+def selective_scan_work_floats(rows: int, channels: int, states: int, groups: int = 1, max_len: int = 0) -> int:
+    return int(lib.krk_selective_scan_work_floats(rows, channels, states, groups, max_len))
+
+
+def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None, slots=None, init=None, out=None,
+                   max_len: int = 0, work=None):
     """Selective state space scan of packed requests: x, dt and the gate z [T, D],
     b and c [T, N] or [T, G, N] of one type; the decay a [D, N] (negative), the
     skip d [D] and dt_bias [D] float32.  With delta = softplus(dt + dt_bias), h =
     exp(delta a) h + delta x b and out = (h . c + d x) * z * sigmoid(z).  Requests
-    and slots as for causal_conv; state is float32 [slots, D, N].  Returns out
-    [T, D] (which may be x, dt or z), whose rows of no request are left as they
-    were."""
+    and slots as for causal_conv; state is float32 [slots, D, N].  max_len, a
+    bound of the requests' rows (0: T), only sizes the launch; `work` is scratch
+    of selective_scan_work_floats floats (allocated here when not given).  Returns
+    out [T, D] (which may be x, dt or z), whose rows of no request are left as
+    they were."""
     cu_at, requests = _requests(cu, x.device)
     dev, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
-    _call(dev, lib.krk_k_selective_scan, (*args, cu_at, rows, requests, *sizes))
+    index = dev.index
+    if index != _current_device():  # the scratch is sized for the current device
+        with torch.cuda.device(dev):
+            return selective_scan(x, dt, a, b, c, cu, d, z, dt_bias, state, slots, init, out, max_len, work)
+    _number(max_len, "max_len")
+    if work is None:
+        need, work_at = lib.krk_selective_scan_work_floats(rows, *sizes, max_len), None
+        if need:
+            work = torch.empty(need, device=dev, dtype=torch.float32)
+            work_at = work.data_ptr()
+    else:
+        if work.dtype != torch.float32 or work.device != dev or not work.is_contiguous():
+            raise ValueError(f"work: expected a contiguous float32 tensor on {dev}")
+        need, work_at = work.numel(), work.data_ptr()
+    rc = lib.krk_k_selective_scan(*args, cu_at, rows, requests, *sizes, max_len, work_at, need, _raw_stream(index))
+    if rc:
+        check(rc)
     return out
 
 

@@ -197,12 +197,16 @@ extern "C" {
                                   out: *mut c_void, o_st: i64, dtype: c_int, state: *mut c_void, state_stride: i64,
                                   num_slots: c_int, slots: *const i32, init: *const i32, rows: c_int,
                                   channels: c_int, width: c_int, silu: c_int, stream: *mut c_void) -> c_int;
+    /// Returns a size, not a status.
+    pub fn krk_selective_scan_work_floats(rows: c_int, channels: c_int, states: c_int, groups: c_int, max_len: c_int)
+                                          -> usize;
     pub fn krk_k_selective_scan(x: *mut c_void, x_st: i64, dt: *mut c_void, dt_st: i64, z: *mut c_void, z_st: i64,
                                 b: *mut c_void, b_st: i64, b_sg: i64, c: *mut c_void, c_st: i64, c_sg: i64,
                                 out: *mut c_void, o_st: i64, dtype: c_int, a: *const c_float, d: *const c_float,
                                 dt_bias: *const c_float, state: *mut c_float, state_stride: i64, num_slots: c_int,
                                 slots: *const i32, init: *const i32, cu: *const i32, rows: c_int, requests: c_int,
-                                channels: c_int, states: c_int, groups: c_int, stream: *mut c_void) -> c_int;
+                                channels: c_int, states: c_int, groups: c_int, max_len: c_int, work: *mut c_float,
+                                work_floats: usize, stream: *mut c_void) -> c_int;
     pub fn krk_k_selective_step(x: *mut c_void, x_st: i64, dt: *mut c_void, dt_st: i64, z: *mut c_void, z_st: i64,
                                 b: *mut c_void, b_st: i64, b_sg: i64, c: *mut c_void, c_st: i64, c_sg: i64,
                                 out: *mut c_void, o_st: i64, dtype: c_int, a: *const c_float, d: *const c_float,

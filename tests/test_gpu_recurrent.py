@@ -209,7 +209,9 @@ def scan64(x, dt, a, b, c, d, z, bias, h, e=0.0):
         decay_e = decay * (EX + rate.abs() * (width_e[t, :, None] + 4 * U)) + 2.0 ** -126
         put = (delta[t] * x[t])[:, None] * b[t]
         new = decay * h + put
-        e = decay * e + decay_e * (h.abs() + e) + put.abs() * (width_e[t, :, None] + 3 * U) + U * new.abs()
+        # (the exponential unit gives 0 for what is below 2^-126: a delta of less may be lost, with what it puts)
+        lost = 2.0 ** -126 * (x[t].abs()[:, None] * b[t].abs())
+        e = decay * e + decay_e * (h.abs() + e) + put.abs() * (width_e[t, :, None] + 3 * U) + lost + U * new.abs()
         e = torch.where(torch.isfinite(new), e, 0.0)
         h = new
         ys[t] = (h * c[t]).sum(1) + d.to(F64) * x[t]
@@ -284,6 +286,41 @@ def test_scan_lengths(lens, init):
 def test_scan_long_prompts(ch, n):
     run_scan("f32", ch, n, 1, [2500, 600], 14)
     run_scan("f16", ch, n, 1, [4001], 14)
+
+
+@pytest.mark.parametrize("n", [3, 8, 16, 24, 64, 128, 130])
+@pytest.mark.parametrize("init", ["same", "none", "mixed"])
+def test_scan_long_prompts_among_others(n, init):
+    """Requests that are walked in pieces, of every rest, beside those that are not; states replaced where they are read."""
+    run_scan("f32", 10, n, 2, [449, 3, 0, 513, 448, 512, 64, 575, 0, 900], 19, init=init, pad=(3,), tail=5)
+
+
+def test_scan_is_repeatable_and_the_bound_only_sizes_it():
+    g = gen(28)
+    t = scan_inputs(g, "f32", 3000, 40, 16, 1)
+    cu = i32([0, 2000, 2000, 2100, 2999])
+    pool = type("P", (), {"slots": [0, 1, 2, 3], "begun": lambda self, s: torch.zeros(40, 16, device=DEV, dtype=F64)})()
+    want, bound, *_ = scan_want(t, [0, 2000, 2000, 2100, 2999], pool, 3000, 0.0)
+    for max_len in (0, 2000, 2001, 2999, 10 ** 6, 300):  # the last: too small, and not split
+        work = torch.full((K.selective_scan_work_floats(3000, 40, 16, 1, max_len) + 4,), math.nan, device=DEV)
+        out = K.selective_scan(**t, cu=cu, max_len=max_len, work=work)
+        assert torch.equal(out[:2999], K.selective_scan(**t, cu=cu, max_len=max_len)[:2999])
+        assert work[-4:].isnan().all()
+        close(out[:2999], want[:2999], bound[:2999])
+    with pytest.raises(_lib.KrikilError, match="work"):
+        K.selective_scan(**t, cu=cu, work=torch.empty(1000, device=DEV))
+    with pytest.raises(ValueError, match="work"):
+        K.selective_scan(**t, cu=cu, work=torch.empty(1 << 20, device=DEV, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("cu", [[0, 3000, 0, 3000, 0, 3000], [0, 3000, 10, 2999, 1, 2], [-7, 5000, -7, 5000]])
+def test_scan_of_long_requests_that_overlap_stays_in_bounds(cu):
+    """Offsets that do not ascend can name more pieces than there is scratch for."""
+    t = scan_inputs(gen(29), "f32", 3000, 40, 16, 1)
+    floats = K.selective_scan_work_floats(3000, 40, 16)
+    work = torch.full((floats + 100000,), 7.0, device=DEV)
+    out = K.selective_scan(**t, cu=i32(cu), work=work[:floats])
+    assert out.shape == (3000, 40) and (work[floats:] == 7).all()
 
 
 @pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 16, 17, 24, 32, 64, 100, 128, 256])

@@ -17,7 +17,8 @@ CONV = dict(x=P, x_st=64, weight=P, bias=P, out=FAR, o_st=64, type=0, **SLOT, cu
 CONV_STEP = dict(x=P, x_st=64, weight=P, bias=P, out=FAR, o_st=64, type=0, **SLOT, B=2, C=64, W=4, silu=1,
                  stream=None)
 SCAN = dict(x=P, x_st=64, dt=P, dt_st=64, z=P, z_st=64, b=P, b_st=16, b_sg=16, c=P, c_st=16, c_sg=16, out=FAR, o_st=64,
-            type=0, a=P, d=P, dt_bias=P, **SLOT, cu=P, T=5, S=2, D=64, N=16, G=1, stream=None)
+            type=0, a=P, d=P, dt_bias=P, **SLOT, cu=P, T=5, S=2, D=64, N=16, G=1, max_len=0, work=None, work_floats=0,
+            stream=None)
 STEP = dict(x=P, x_st=64, dt=P, dt_st=64, z=P, z_st=64, b=P, b_st=16, b_sg=16, c=P, c_st=16, c_sg=16, out=FAR, o_st=64,
             type=0, a=P, d=P, dt_bias=P, **SLOT, B=2, D=64, N=16, G=1, stream=None)
 LOGPROBS = dict(logits=P, ld=100, type=0, R=3, V=100, tokens=P, K=1, lp=P, entropy=P, top=5, ids=P, best=P, stream=None)
@@ -59,7 +60,9 @@ SCAN_FAULTS = POOL + [("type", 3, "type"), ("N", 0, "N must"), ("N", 257, "N mus
                           (n, P + 2, "aligned") for n in ("x", "dt", "b", "c", "out")]
 
 
-@pytest.mark.parametrize("what,value,word", SCAN_FAULTS + BARE + [("cu", None, "null"), ("T", -1, "rows"), ("S", -1, "rows")])
+@pytest.mark.parametrize("what,value,word", SCAN_FAULTS + BARE + [
+    ("cu", None, "null"), ("T", -1, "rows"), ("S", -1, "rows"), ("max_len", -1, "max_len"), ("T", 5000, "work must"),
+    (("T", "work", "work_floats"), (5000, P, 1000), "work must"), (("T", "work", "work_floats"), (5000, P + 4, 1 << 30), "work must")])
 def test_scan_refuses(what, value, word):
     refused(lib.krk_k_selective_scan, SCAN, what, value, word)
 
@@ -94,6 +97,16 @@ def test_sound_calls_reach_the_device():
                      (lib.krk_k_selective_step, STEP), (lib.krk_k_token_logprobs, LOGPROBS),
                      (lib.krk_k_token_logprobs, dict(LOGPROBS, entropy=None, top=0, ids=None, best=None))):
         assert fn(*args.values()) == _lib.CUDA, lib.krk_last_error()
+
+
+def test_scan_scratch():
+    """None for short requests; else room for every piece's states and step sums, whatever the requests' lengths."""
+    floats = lib.krk_selective_scan_work_floats
+    assert floats(448, 64, 16, 1, 0) == 0 and floats(449, 64, 16, 1, 0) > 0
+    assert floats(100000, 64, 16, 1, 1000) == 0 and floats(100000, 64, 16, 1, 100000) == floats(100000, 64, 16, 1, 0)
+    assert floats(16384, 5120, 16, 1, 8000) == 0  # as many channels as the device has room for: a request is not split
+    for args in ((0, 64, 16, 1, 0), (449, 64, 257, 1, 0), (449, 64, 16, 3, 0), (449, 64, 16, 1, -1), (449, 0, 16, 1, 0)):
+        assert floats(*args) == 0
 
 
 def test_wrappers_want_cuda_tensors():
