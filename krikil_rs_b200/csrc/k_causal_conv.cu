@@ -179,10 +179,6 @@ __global__ void __launch_bounds__(CONV_THREADS) conv_step_kernel(ConvArgs a, int
     }
 }
 
-bool fits(const void* p, int64_t stride, size_t bytes, size_t elem) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * elem % bytes == 0;
-}
-
 template <typename T, int W, int V>
 cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
     const int side = (a.C + CONV_THREADS * V - 1) / (CONV_THREADS * V);

@@ -6,9 +6,9 @@
 
 namespace krk {
 
-cudaError_t selective_scan_f32(const ScanArgs& a, float* work, int rows, cudaStream_t s);
-cudaError_t selective_scan_f16(const ScanArgs& a, float* work, int rows, cudaStream_t s);
-cudaError_t selective_scan_bf16(const ScanArgs& a, float* work, int rows, cudaStream_t s);
+cudaError_t selective_scan_f32(const ScanArgs& a, float* work, const ScanPlan& plan, cudaStream_t s);
+cudaError_t selective_scan_f16(const ScanArgs& a, float* work, const ScanPlan& plan, cudaStream_t s);
+cudaError_t selective_scan_bf16(const ScanArgs& a, float* work, const ScanPlan& plan, cudaStream_t s);
 
 namespace {
 
@@ -100,10 +100,6 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
     }
 }
 
-bool fits(const void* p, int64_t stride, size_t bytes, size_t elem) {
-    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * elem % bytes == 0;
-}
-
 template <typename T, bool WIDE, int Q, int R>
 cudaError_t launch_step(const ScanArgs& a, int lane_bits, cudaStream_t s) {
     const int64_t side = (((int64_t)a.D << lane_bits) + STEP_THREADS - 1) / STEP_THREADS;
@@ -137,9 +133,8 @@ cudaError_t step_type(const ScanArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-// A piece is the rows that leave the device one wave of blocks over all rows;
-// none when no request can be long enough to be split.
-int scan_piece_rows(int T, int D, int N, int G, int max_len) {
+// A piece is the rows that leave the device one wave of blocks over all rows.
+ScanPlan scan_plan(int T, int S, int D, int N, int G, int max_len) {
     int sms = paged_sm_count();
     if (sms <= 0) sms = 148;
     int lanes = 1;
@@ -150,17 +145,17 @@ int scan_piece_rows(int T, int D, int N, int G, int max_len) {
     int64_t rows = (T + pieces - 1) / pieces;
     rows = rows < SCAN_PIECE ? SCAN_PIECE : (rows + 3) / 4 * 4;
     const int bound = max_len > 0 && max_len < T ? max_len : T;
-    return bound > SCAN_ALONE * rows ? (int)rows : 0;
+    return {bound > SCAN_ALONE * rows ? (int)rows : 0, side * S <= sms};
 }
 size_t scan_work_floats(int T, int D, int N, int G, int max_len) {
-    const int rows = scan_piece_rows(T, D, N, G, max_len);
+    const int rows = scan_plan(T, 1, D, N, G, max_len).rows;
     return rows > 0 ? (size_t)scan_split_room(T, rows) * D * (N + 1) : 0;
 }
 
 cudaError_t selective_scan(const ScanArgs& a, int type, int max_len, float* work, cudaStream_t s) {
-    const int rows = scan_piece_rows(a.T, a.D, a.N, a.G, max_len);
-    return type == ELEM_F32 ? selective_scan_f32(a, work, rows, s)
-                            : type == ELEM_F16 ? selective_scan_f16(a, work, rows, s) : selective_scan_bf16(a, work, rows, s);
+    const ScanPlan plan = scan_plan(a.T, a.S, a.D, a.N, a.G, max_len);
+    return type == ELEM_F32 ? selective_scan_f32(a, work, plan, s)
+                            : type == ELEM_F16 ? selective_scan_f16(a, work, plan, s) : selective_scan_bf16(a, work, plan, s);
 }
 cudaError_t selective_step(const ScanArgs& a, int type, cudaStream_t s) {
     return type == ELEM_F32 ? step_type<float>(a, s)

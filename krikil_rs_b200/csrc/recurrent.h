@@ -48,9 +48,13 @@ struct ScanArgs {
     const int32_t* cu;                           // [S+1]; nullptr: one row a request
     int T, S, D, N, G;
 };
-// The scan's split of long requests: scratch of so many floats lets requests of
-// up to max_len rows be walked in pieces of scan_piece_rows rows (0: they are not).
-int scan_piece_rows(int T, int D, int N, int G, int max_len);
+// How the scan is launched: with scratch of scan_work_floats floats, requests of
+// more than SCAN_ALONE * rows rows are walked in pieces of that many (rows 0: none).
+struct ScanPlan {
+    int rows;
+    bool thin;  // lanes of few states
+};
+ScanPlan scan_plan(int T, int S, int D, int N, int G, int max_len);
 size_t scan_work_floats(int T, int D, int N, int G, int max_len);
 constexpr int64_t scan_split_room(int64_t T, int rows) { return T / rows * 8 / 7 + 2; }
 cudaError_t selective_scan(const ScanArgs& a, int type, int max_len, float* work, cudaStream_t s);
@@ -66,5 +70,10 @@ struct LogprobArgs {
     int32_t* top_ids; float* top_lp;             // [R][top]
 };
 cudaError_t token_logprobs(const LogprobArgs& a, int type, cudaStream_t s);
+
+// Whether a tensor whose rows are `stride` elements apart can be accessed so many bytes at a time.
+inline bool fits(const void* p, int64_t stride, size_t bytes, size_t elem) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * (int64_t)elem % (int64_t)bytes == 0;
+}
 
 }  // namespace krk

@@ -19,6 +19,10 @@
 // alone would take longer than twice what the whole call takes when it is shared
 // out evenly.
 #pragma once
+#include <limits.h>
+
+#include <type_traits>
+
 #include "kernels.h"
 #include "paged.h"
 #include "recurrent.cuh"
@@ -28,13 +32,14 @@ namespace {
 
 constexpr int SCAN_GROUP = 4;  // rows whose outputs are formed together
 
+// K lanes share a channel of N <= K * SPT states.
 template <int K, int SPT>
 struct ScanShape {
     static constexpr int CH = SCAN_THREADS / K, NP = K * SPT;
-    static constexpr int ROWS = NP <= 32 ? 32 : 1024 / NP;           // a tile of B and C
-    static constexpr int F = 2 * ROWS * NP / SCAN_THREADS;           // elements of them that a thread stages
-    static constexpr int OWN = K < SCAN_GROUP ? SCAN_GROUP / K : 1;  // rows of a group whose delta and output a lane forms
-    static constexpr int SHARE = K < SCAN_GROUP ? 1 : K / SCAN_GROUP;  // lanes that form the same one
+    static constexpr int ROWS = NP <= 32 ? 32 : 1024 / NP;             // a tile of B and C
+    static constexpr int F = 2 * ROWS * NP / SCAN_THREADS;             // elements of them that a thread stages
+    static constexpr int OWN = K < SCAN_GROUP ? SCAN_GROUP / K : 1;    // rows of a group whose inputs are a lane's work
+    static constexpr int SHARE = K < SCAN_GROUP ? 1 : K / SCAN_GROUP;  // lanes that have the same ones
 };
 
 // How a request is split.
@@ -46,6 +51,23 @@ struct ScanSplit {
 };
 KRK_DEV int scan_pieces(int n, int rows) { return rows > 0 && n > (int64_t)SCAN_ALONE * rows ? (n - 1) / rows + 1 : 1; }
 
+// The requests' order of turns: the longest first (of equal ones the first), so
+// that what is left when most blocks have ended is short; for more requests than
+// a block has threads, their own.  Returns whether `order` holds it.
+KRK_DEV bool longest_first(const int32_t* cu, int S, int T, int (&order)[SCAN_THREADS]) {
+    if (S < 2 || S > SCAN_THREADS) return false;
+    __shared__ int rows[SCAN_THREADS];
+    const int s = threadIdx.x;
+    const int mine = s < S ? clamp_row(cu[s + 1], T) - clamp_row(cu[s], T) : INT_MIN;
+    rows[s] = mine;
+    __syncthreads();
+    int place = 0;
+    for (int i = 0; i < S; ++i) place += rows[i] > mine || (rows[i] == mine && i < s);
+    if (s < S) order[place] = s;
+    __syncthreads();
+    return true;
+}
+
 // The piece-th piece of all requests' (or of the split ones' alone, or of those
 // each one's first): its request, its place there, and the place of the
 // request's first one among the split ones'.  request < 0: there are not so many.
@@ -56,14 +78,17 @@ enum ScanCount { COUNT_ALL, COUNT_SPLIT, COUNT_FIRST };
 KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piece, ScanCount count) {
     __shared__ int warp_sum[2][SCAN_THREADS / 32];
     __shared__ ScanPiece found;
+    __shared__ int order[SCAN_THREADS];
+    const bool ordered = longest_first(cu, S, T, order);
+    if (rows == 0) return {ordered ? order[piece] : piece, 0, 0};  // a piece a request
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int before = 0, before_split = 0;
     if (tid == 0) found.request = -1;
     __syncthreads();
     for (int s0 = 0; s0 < S; s0 += SCAN_THREADS) {
-        const int s = s0 + tid;
-        int n = 0, m = 0;
+        int s = s0 + tid, n = 0, m = 0;
         if (s < S) {
+            if (ordered) s = order[s];
             const int begin = clamp_row(cu[s], T), end = clamp_row(cu[s + 1], T);
             n = scan_pieces(end - begin, rows);
             m = n > 1 ? n : 0;
@@ -96,7 +121,7 @@ KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piec
 
 // Sums each of v's rows over K lanes.  While a lane holds several rows it keeps
 // half of them and gives the others away: with K < R lane i ends with rows
-// i * R/K .. of the R, else lanes i * K/R .. with row i.
+// i * R / K .. of the R, else lanes i * K / R .. with row i.
 template <int R, int K>
 KRK_DEV void sum_rows(float (&v)[R], int lane) {
     int n = R / 2;
@@ -125,12 +150,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     constexpr int CH = Sh::CH, NP = Sh::NP, ROWS = Sh::ROWS, F = Sh::F, OWN = Sh::OWN, U = SCAN_GROUP;
     __shared__ __align__(16) float s_bc[2][ROWS][2][NP];
 
-    const int tid = threadIdx.x, lane = tid % K, ch = tid / K, per = a.D / a.G;
+    const int tid = threadIdx.x, lane = tid % K, per = a.D / a.G;
     const int block = blockIdx.x / side, cb = blockIdx.x - block * side, sides = side / a.G;
-    const int g = cb / sides, ch0 = (cb - g * sides) * CH;  // within the group
-    const bool open = ch < per - ch0;
-    const int d = g * per + (open ? ch0 + ch : 0);
-    const ScanPiece piece = split.rows > 0 ? find_piece(a.cu, a.S, a.T, split.rows, block, CARRY ? COUNT_SPLIT : COUNT_ALL) : ScanPiece{block, 0, 0};
+    const int g = cb / sides, ch = (cb - g * sides) * CH + tid / K;  // within the group
+    const bool open = ch < per;
+    const int d = g * per + (open ? ch : 0);
+    const ScanPiece piece = find_piece(a.cu, a.S, a.T, split.rows, block, CARRY ? COUNT_SPLIT : COUNT_ALL);
     if (piece.request < 0) return;
     const Span span = request_rows(a.cu, piece.request, a.T);
     int to, from;
@@ -153,31 +178,34 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
             const int n = state_of(j);
             const bool in = open && (!PADDED || n < a.N);
             const int64_t at = (int64_t)d * a.N + n;
-            const float r = in ? scan_rate(a.a[at]) : 0.0f;
-            const float v = in && old ? old[at] : 0.0f;
+            const float r = in ? scan_rate(a.a[at]) : 0.0f, v = in && old ? old[at] : 0.0f;
             (j % 2 ? rate[j / 2].y : rate[j / 2].x) = r;
             (j % 2 ? h[j / 2].y : h[j / 2].x) = v;
         }
     }
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = !CARRY && a.d ? a.d[d] : 0.0f;
-    const T* xp = (const T*)a.x + d;
-    const T* dtp = (const T*)a.dt + d;
-    const T* zp = (const T*)a.z + d;
     const T* bp = (const T*)a.b + g * a.b_sg;
     const T* cp = (const T*)a.c + g * a.c_sg;
     const T zero = from_f32<T>(0.0f);
+    const bool gated = !CARRY && a.z;
 
-    // A thread's rows of a group, on their way while the group before is computed.
+    // A lane's rows of a group, on their way while the group before is computed; WHOLE: all four rows are there.
     const int own = lane / Sh::SHARE * OWN;
+    const T* xp = (const T*)a.x + (begin + own) * a.x_st + d;
+    const T* dtp = (const T*)a.dt + (begin + own) * a.dt_st + d;
+    const T* zp = (const T*)a.z + (begin + own) * a.z_st + d;
+    T* outp = (T*)a.out + (begin + own) * a.o_st + d;
     T xr[OWN], dtr[OWN], zr[OWN];
-    const auto fetch = [&](int t0) {
+    const auto fetch = [&](int t, auto whole) {
 #pragma unroll
         for (int o = 0; o < OWN; ++o) {
-            const int t = t0 + own + o;
-            const bool in = open && t < end;
-            xr[o] = in ? xp[t * a.x_st] : zero;
-            dtr[o] = in ? dtp[t * a.dt_st] : zero;
-            if (!CARRY) zr[o] = in && a.z ? zp[t * a.z_st] : zero;
+            const bool in = decltype(whole)::value || t + own + o < end;
+            xr[o] = in ? *xp : zero;
+            dtr[o] = in ? *dtp : zero;
+            if (gated) zr[o] = in ? *zp : zero;
+            xp += o + 1 < OWN ? a.x_st : (U - OWN + 1) * a.x_st;
+            dtp += o + 1 < OWN ? a.dt_st : (U - OWN + 1) * a.dt_st;
+            zp += o + 1 < OWN ? a.z_st : (U - OWN + 1) * a.z_st;
         }
     };
     // And its elements of the next tile of B and C.
@@ -197,83 +225,80 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     };
 
     float total = 0.0f;
+    int buffer = 0;
+    // Rows t .. t + 3, in rows r0 .. of the tile; WHOLE: they and the four behind them are there.
+    const auto group = [&](int t, int r0, auto whole) {
+        float mine[OWN], mine_put[OWN], gate[OWN], skipped[OWN], step[U], put[U];
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const float x = to_f32(xr[o]);
+            // rows behind the last one step by nothing: the states stay
+            mine[o] = decltype(whole)::value || t + own + o < end ? step_width(to_f32(dtr[o]) + bias) : 0.0f;
+            mine_put[o] = mine[o] * x;
+            skipped[o] = skip * x;
+            gate[o] = gated ? fast_silu(to_f32(zr[o])) : 1.0f;
+        }
+        fetch(t + U, whole);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            step[u] = K == 1 ? mine[u % OWN] : __shfl_sync(0xffffffffu, mine[u % OWN], u / OWN * Sh::SHARE, K);
+            put[u] = K == 1 ? mine_put[u % OWN] : __shfl_sync(0xffffffffu, mine_put[u % OWN], u / OWN * Sh::SHARE, K);
+        }
+        float y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float4* b = reinterpret_cast<const float4*>(s_bc[buffer][r0 + u][0]) + lane;
+            const float4* c = reinterpret_cast<const float4*>(s_bc[buffer][r0 + u][1]) + lane;
+            const float2 st = make_float2(step[u], step[u]), pt = make_float2(put[u], put[u]);
+            float2 acc = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int q = 0; q < SPT / 4; ++q) {
+                const float4 b4 = b[q * K];
+                const float4 c4 = CARRY ? b4 : c[q * K];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int j = 2 * q + i;
+                    const float2 e = __fmul2_rn(st, rate[j]);
+                    const float2 decay = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+                    h[j] = __ffma2_rn(decay, h[j], __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y)));
+                    if (CARRY) continue;
+                    float2 there = h[j];
+                    if (PADDED) {  // an infinite x makes no NaN of states that are not there
+                        if (state_of(2 * j) >= a.N) there.x = 0.0f;
+                        if (state_of(2 * j + 1) >= a.N) there.y = 0.0f;
+                    }
+                    const float2 ci = i ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y);
+                    acc = j == 0 ? __fmul2_rn(there, ci) : __ffma2_rn(there, ci, acc);
+                }
+            }
+            y[u] = acc.x + acc.y;
+            total += step[u];
+        }
+        if (CARRY) return;
+        sum_rows<U, K>(y, lane);
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            if (open && lane % Sh::SHARE == 0 && (decltype(whole)::value || t + own + o < end))
+                *outp = from_f32<T>((y[o] + skipped[o]) * gate[o]);
+            outp += o + 1 < OWN ? a.o_st : (U - OWN + 1) * a.o_st;
+        }
+    };
+
     if (begin < end) {
-        fetch(begin);
+        fetch(begin, std::false_type());
         fetch_bc(begin);
         stage_bc(0);
     }
     __syncthreads();
-    int buffer = 0;
     for (int t0 = begin; t0 < end; t0 += ROWS, buffer ^= 1) {
         const bool more = t0 + ROWS < end;
         if (more) fetch_bc(t0 + ROWS);
         const int rows = min(ROWS, end - t0);
         for (int r0 = 0; r0 < rows; r0 += U) {
-            float step[U], put[U], gate[OWN], skipped[OWN];
-#pragma unroll
-            for (int o = 0; o < OWN; ++o) {
-                const float x = to_f32(xr[o]);
-                // rows behind the last one step by nothing: the states stay
-                const float delta = t0 + r0 + own + o < end ? step_width(to_f32(dtr[o]) + bias) : 0.0f;
-                step[o] = delta;
-                put[o] = delta * x;
-                if (!CARRY) {
-                    skipped[o] = skip * x;
-                    gate[o] = a.z ? fast_silu(to_f32(zr[o])) : 1.0f;
-                }
-            }
-            fetch(t0 + r0 + U);
-            if (K > 1) {
-                float mine[OWN], mine_put[OWN];
-#pragma unroll
-                for (int o = 0; o < OWN; ++o) mine[o] = step[o], mine_put[o] = put[o];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    step[u] = __shfl_sync(0xffffffffu, mine[u % OWN], u / OWN * Sh::SHARE, K);
-                    put[u] = __shfl_sync(0xffffffffu, mine_put[u % OWN], u / OWN * Sh::SHARE, K);
-                }
-            }
-            float y[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float4* b = reinterpret_cast<const float4*>(s_bc[buffer][r0 + u][0]) + lane;
-                const float4* c = reinterpret_cast<const float4*>(s_bc[buffer][r0 + u][1]) + lane;
-                const float2 st = make_float2(step[u], step[u]), pt = make_float2(put[u], put[u]);
-                float2 acc = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int q = 0; q < SPT / 4; ++q) {
-                    const float4 b4 = b[q * K];
-                    const float4 c4 = CARRY ? b4 : c[q * K];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int j = 2 * q + i;
-                        const float2 e = __fmul2_rn(st, rate[j]);
-                        const float2 decay = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-                        h[j] = __ffma2_rn(decay, h[j], __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y)));
-                        if (!CARRY) {
-                            float2 live = h[j];
-                            if (PADDED) {  // an infinite x makes no NaN of states that are not there
-                                if (state_of(2 * j) >= a.N) live.x = 0.0f;
-                                if (state_of(2 * j + 1) >= a.N) live.y = 0.0f;
-                            }
-                            acc = __ffma2_rn(live, i ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y), acc);
-                        }
-                    }
-                }
-                if (CARRY)
-                    total += step[u];
-                else
-                    y[u] = acc.x + acc.y;
-            }
-            if (!CARRY) {
-                sum_rows<U, K>(y, lane);
-#pragma unroll
-                for (int o = 0; o < OWN; ++o) {
-                    const int t = t0 + r0 + own + o;
-                    if (open && t < end && lane % Sh::SHARE == 0)
-                        ((T*)a.out)[t * a.o_st + d] = from_f32<T>((y[o] + skipped[o]) * gate[o]);
-                }
-            }
+            if (end - (t0 + r0) >= 2 * U)
+                group(t0 + r0, r0, std::true_type());
+            else
+                group(t0 + r0, r0, std::false_type());
         }
         if (more) stage_bc(buffer ^ 1);
         __syncthreads();
@@ -314,13 +339,13 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanArgs a, Sc
 }
 
 // ---------------------------------------------------------------- the launches
-template <typename T, int K, int SPT, bool PADDED>
+template <typename T, int K, int SPT, bool PADDED, bool SPLIT>
 cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStream_t s) {
     using Sh = ScanShape<K, SPT>;
     const int64_t side = (int64_t)((a.D / a.G + Sh::CH - 1) / Sh::CH) * a.G;
     ScanSplit split{0, nullptr, nullptr, 0};
     int64_t pieces = a.S;
-    if (piece_rows > 0) {
+    if constexpr (SPLIT) {
         const int64_t room = scan_split_room(a.T, piece_rows), states = (int64_t)a.D * a.N;
         split = {piece_rows, work, work + room * states, (int)room};
         pieces = a.S + a.T / piece_rows;
@@ -341,20 +366,39 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
     return cudaGetLastError();
 }
 
-template <typename T, int K, int SPT>
+template <typename T, int K, int SPT, bool SPLIT>
 cudaError_t scan_padded(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
-    return a.N == K * SPT ? launch_scan<T, K, SPT, false>(a, work, rows, s) : launch_scan<T, K, SPT, true>(a, work, rows, s);
+    return a.N == K * SPT ? launch_scan<T, K, SPT, false, SPLIT>(a, work, rows, s)
+                          : launch_scan<T, K, SPT, true, SPLIT>(a, work, rows, s);
 }
 
+// Lanes of SCAN_LANE states; of four when the blocks of those would leave
+// multiprocessors without one.
 template <typename T>
-cudaError_t scan_type(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
-    if (a.N <= 4) return scan_padded<T, 1, 4>(a, work, rows, s);
-    if (a.N <= 8) return scan_padded<T, 1, 8>(a, work, rows, s);
-    if (a.N <= 16) return scan_padded<T, 1, 16>(a, work, rows, s);
-    if (a.N <= 32) return scan_padded<T, 2, 16>(a, work, rows, s);
-    if (a.N <= 64) return scan_padded<T, 4, 16>(a, work, rows, s);
-    if (a.N <= 128) return scan_padded<T, 8, 16>(a, work, rows, s);
-    return scan_padded<T, 16, 16>(a, work, rows, s);
+cudaError_t scan_type(const ScanArgs& a, float* work, const ScanPlan& plan, cudaStream_t s) {
+    if (plan.rows > 0) {
+        if (a.N <= 4) return scan_padded<T, 1, 4, true>(a, work, plan.rows, s);
+        if (a.N <= 8) return scan_padded<T, 1, 8, true>(a, work, plan.rows, s);
+        if (a.N <= 16) return scan_padded<T, 1, SCAN_LANE, true>(a, work, plan.rows, s);
+        if (a.N <= 32) return scan_padded<T, 2, SCAN_LANE, true>(a, work, plan.rows, s);
+        if (a.N <= 64) return scan_padded<T, 4, SCAN_LANE, true>(a, work, plan.rows, s);
+        if (a.N <= 128) return scan_padded<T, 8, SCAN_LANE, true>(a, work, plan.rows, s);
+        return scan_padded<T, 16, SCAN_LANE, true>(a, work, plan.rows, s);
+    }
+    if (a.N <= 4) return scan_padded<T, 1, 4, false>(a, work, 0, s);
+    if (plan.thin) {
+        if (a.N <= 8) return scan_padded<T, 2, 4, false>(a, work, 0, s);
+        if (a.N <= 16) return scan_padded<T, 4, 4, false>(a, work, 0, s);
+        if (a.N <= 32) return scan_padded<T, 8, 4, false>(a, work, 0, s);
+        if (a.N <= 64) return scan_padded<T, 16, 4, false>(a, work, 0, s);
+        if (a.N <= 128) return scan_padded<T, 32, 4, false>(a, work, 0, s);
+    }
+    if (a.N <= 8) return scan_padded<T, 1, 8, false>(a, work, 0, s);
+    if (a.N <= 16) return scan_padded<T, 1, SCAN_LANE, false>(a, work, 0, s);
+    if (a.N <= 32) return scan_padded<T, 2, SCAN_LANE, false>(a, work, 0, s);
+    if (a.N <= 64) return scan_padded<T, 4, SCAN_LANE, false>(a, work, 0, s);
+    if (a.N <= 128) return scan_padded<T, 8, SCAN_LANE, false>(a, work, 0, s);
+    return scan_padded<T, 16, SCAN_LANE, false>(a, work, 0, s);
 }
 
 }  // namespace
