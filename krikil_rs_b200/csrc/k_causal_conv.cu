@@ -11,19 +11,27 @@ namespace krk {
 namespace {
 
 constexpr int CONV_THREADS = 128;
-constexpr int CONV_GROUP = 4;  // rows whose loads are on their way together
+constexpr int CONV_GROUP = 4;  // rows that are computed together
+constexpr int CONV_AHEAD = 8;   // rows on their way to a thread
 
-// One thread: V channels; their taps, bias, and the window of W-1 rows.
+// A thread's copy of V elements into its place in shared memory; none for those of two bytes, which are loaded.
+template <int BYTES>
+KRK_DEV void copy_ahead(void* smem, const void* gmem) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_addr(smem)), "l"(gmem), "n"(BYTES) : "memory");
+}
+
+// One thread: V channels, their taps and bias; in pairs, a lone channel in the first half.
 template <typename T, int W, int V>
 struct ConvColumn {
+    static constexpr int P = pairs_of<V>;
     const ConvArgs& a;
     int c;
-    float w[W][V], bias[V];
+    float2 w[W][P], bias[P];
 
     KRK_DEV ConvColumn(const ConvArgs& args, int channel) : a(args), c(channel) {
         __align__(16) float flat[V * W];
         const float* from = a.w + (int64_t)c * W;
-        if (V % 4 == 0 && a.aligned) {
+        if (V * W % 4 == 0 && a.aligned) {
 #pragma unroll
             for (int i = 0; i < V * W / 4; ++i) reinterpret_cast<float4*>(flat)[i] = reinterpret_cast<const float4*>(from)[i];
         } else {
@@ -31,10 +39,11 @@ struct ConvColumn {
             for (int i = 0; i < V * W; ++i) flat[i] = from[i];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+        for (int i = 0; i < P; ++i) {
+            constexpr int next = V > 1;
 #pragma unroll
-            for (int j = 0; j < W; ++j) w[j][i] = flat[i * W + j];
-            bias[i] = a.bias ? a.bias[c + i] : 0.0f;
+            for (int j = 0; j < W; ++j) w[j][i] = make_float2(flat[2 * i * W + j], flat[(2 * i + next) * W + j]);
+            bias[i] = a.bias ? make_float2(a.bias[c + 2 * i], a.bias[c + 2 * i + next]) : make_float2(0.0f, 0.0f);
         }
     }
     KRK_DEV const T* row(int t) const { return (const T*)a.x + t * a.x_st + c; }
@@ -48,44 +57,64 @@ struct ConvColumn {
         for (int i = 0; i < V; ++i) zero.v[i] = from_f32<T>(0.0f);
         return zero;
     }
-    KRK_DEV void put(int t, const float (&win)[W - 1][V], const float (&x)[V]) const {
-        Pack<T, V> y;
+    // One row's output, from the rows before it (the latest last) and itself.
+    KRK_DEV Pack<T, V> convolve(const float2 (&win)[W - 1][P], const float2 (&x)[P]) const {
+        float2 y[P];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float s = bias[i];
+        for (int i = 0; i < P; ++i) {
+            y[i] = bias[i];
 #pragma unroll
-            for (int j = 0; j < W - 1; ++j) s = fmaf(w[j][i], win[j][i], s);
-            s = fmaf(w[W - 1][i], x[i], s);
-            y.v[i] = from_f32<T>(a.silu ? fast_silu(s) : s);
+            for (int j = 0; j < W - 1; ++j) y[i] = __ffma2_rn(w[j][i], win[j][i], y[i]);
+            y[i] = __ffma2_rn(w[W - 1][i], x[i], y[i]);
+            if (a.silu) y[i] = fast_silu(y[i]);
         }
-        store_pack<T, V>((T*)a.out + t * a.o_st + c, y);
+        return pack<T, V>(y);
     }
-    // Rows [i, j) of a request that begins at `begin`.
-    KRK_DEV void run(int i, int j, int begin, int from) const {
+    // Rows [i, j) of a request that begins at `begin`, CONV_AHEAD rows on their way to the thread's own places of `ring`
+    // (so many, of all threads, keep the memory busy; in registers there is room for a quarter of them).
+    KRK_DEV void run(int i, int j, int begin, int from, Pack<T, V> (*ring)[CONV_THREADS]) const {
         if (i >= j) return;
-        float win[W - 1][V];
+        constexpr int BYTES = V * sizeof(T);
+        const T* in = row(i);
+        T* out = (T*)a.out + i * a.o_st + c;
+        const int left = j - i;
+        const auto fetch = [&](int u) {
+            if (u < left) {
+                Pack<T, V>* place = &ring[u % CONV_AHEAD][threadIdx.x];
+                if constexpr (BYTES >= 4)
+                    copy_ahead<BYTES>(place, in);
+                else
+                    *place = load_pack<T, V>(in);
+            }
+            in += a.x_st;
+        };
+        for (int u = 0; u < CONV_AHEAD; u += CONV_GROUP) {
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-            const Pack<T, V> p = tap(i - (W - 1) + k, begin, from);
-#pragma unroll
-            for (int v = 0; v < V; ++v) win[k][v] = to_f32(p.v[v]);
+            for (int k = 0; k < CONV_GROUP; ++k) fetch(u + k);
+            cp_async_commit();
         }
-        for (int t = i; t < j; t += CONV_GROUP) {
-            Pack<T, V> p[CONV_GROUP];
+        float2 win[W - 1][P];
 #pragma unroll
-            for (int u = 0; u < CONV_GROUP; ++u)
-                if (t + u < j) p[u] = load_pack<T, V>(row(t + u));
+        for (int k = 0; k < W - 1; ++k) unpack(tap(i - (W - 1) + k, begin, from), win[k]);
+        for (int u = 0; u < left; u += CONV_GROUP) {
+            cp_async_wait<CONV_AHEAD / CONV_GROUP - 1>();
+            Pack<T, V> now[CONV_GROUP];
 #pragma unroll
-            for (int u = 0; u < CONV_GROUP; ++u) {
-                if (t + u >= j) break;
-                float x[V];
+            for (int k = 0; k < CONV_GROUP; ++k) now[k] = ring[(u + k) % CONV_AHEAD][threadIdx.x];
 #pragma unroll
-                for (int v = 0; v < V; ++v) x[v] = to_f32(p[u].v[v]);
-                put(t + u, win, x);
+            for (int k = 0; k < CONV_GROUP; ++k) fetch(u + CONV_AHEAD + k);
+            cp_async_commit();
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
+            for (int k = 0; k < CONV_GROUP; ++k) {
+                float2 x[P];
+                unpack(now[k], x);
+                const Pack<T, V> y = convolve(win, x);
+                if (u + k < left) store_pack<T, V>(out, y);
+                out += a.o_st;
 #pragma unroll
-                    for (int k = 0; k + 1 < W - 1; ++k) win[k][v] = win[k + 1][v];
+                for (int v = 0; v < P; ++v) {
+#pragma unroll
+                    for (int q = 0; q + 1 < W - 1; ++q) win[q][v] = win[q + 1][v];
                     win[W - 2][v] = x[v];
                 }
             }
@@ -124,6 +153,7 @@ KRK_DEV int requests_before(const int32_t* cu, int S, int r) {
 // the thread that writes the new one.
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(CONV_THREADS) conv_kernel(ConvArgs a, int rows, int side) {
+    __shared__ Pack<T, V> ring[CONV_AHEAD][CONV_THREADS];
     const int chunk = blockIdx.x / side, c = ((blockIdx.x - chunk * side) * CONV_THREADS + threadIdx.x) * V;
     const int r0 = chunk * rows;
     const bool last = r0 >= a.T - rows;
@@ -135,13 +165,13 @@ __global__ void __launch_bounds__(CONV_THREADS) conv_kernel(ConvArgs a, int rows
     if (s > 0) {
         const Span span = request_rows(a.cu, s - 1, a.T);
         if (span.end > r0 && request_slots(a.slot, s - 1, to, from))
-            col.run(max(r0, min(span.begin + W - 1, span.end)), min(span.end, r1), span.begin, from);
+            col.run(max(r0, min(span.begin + W - 1, span.end)), min(span.end, r1), span.begin, from, ring);
     }
     for (; s < a.S; ++s) {
         const Span span = request_rows(a.cu, s, a.T);
         if (!last && span.begin >= r1) break;
         if (!request_slots(a.slot, s, to, from)) continue;
-        col.run(span.begin, min(span.end, max(r1, span.begin + W - 1)), span.begin, from);
+        col.run(span.begin, min(span.end, max(r1, span.begin + W - 1)), span.begin, from, ring);
         col.keep(span, to, from);
     }
 }
@@ -166,14 +196,11 @@ __global__ void __launch_bounds__(CONV_THREADS) conv_step_kernel(ConvArgs a, int
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         if (!live[r]) continue;
-        float win[W - 1][V], x[V];
+        float2 win[W - 1][pairs_of<V>], x[pairs_of<V>];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-#pragma unroll
-            for (int k = 0; k < W - 1; ++k) win[k][v] = to_f32(rows[r][k].v[v]);
-            x[v] = to_f32(rows[r][W - 1].v[v]);
-        }
-        col.put(t0 + r, win, x);
+        for (int k = 0; k < W - 1; ++k) unpack(rows[r][k], win[k]);
+        unpack(rows[r][W - 1], x);
+        store_pack<T, V>((T*)a.out + (t0 + r) * a.o_st + c, col.convolve(win, x));
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) store_pack<T, V>(col.kept(to[r], k), rows[r][k + 1]);
     }
@@ -203,14 +230,24 @@ cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+// Whether rows are accessed V channels at a time.
+template <typename T>
+bool conv_fits(const ConvArgs& a, int V) {
+    const size_t bytes = V * sizeof(T);
+    return a.C % V == 0 && fits(a.x, a.T > 1 ? a.x_st : 0, bytes, sizeof(T)) &&
+           fits(a.out, a.T > 1 ? a.o_st : 0, bytes, sizeof(T)) &&
+           fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, bytes, sizeof(T));
+}
+
+// Eight bytes a thread: with sixteen its taps and window leave too few threads a multiprocessor (98 and 121 us for
+// 16,352 rows of 8192 bfloat16 channels).
 template <typename T, int W>
 cudaError_t conv_width(ConvArgs a, cudaStream_t s) {
     a.aligned = fits(a.w, 0, 16, 4);
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = a.C % V == 0 && fits(a.x, a.T > 1 ? a.x_st : 0, 16, sizeof(T)) &&
-                      fits(a.out, a.T > 1 ? a.o_st : 0, 16, sizeof(T)) &&
-                      fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, 16, sizeof(T));
-    return wide ? launch_conv<T, W, V>(a, s) : launch_conv<T, W, 1>(a, s);
+    constexpr int V = 8 / sizeof(T);
+    if (conv_fits<T>(a, V)) return launch_conv<T, W, V>(a, s);
+    if (V > 2 && conv_fits<T>(a, 2)) return launch_conv<T, W, 2>(a, s);
+    return launch_conv<T, W, 1>(a, s);
 }
 
 template <typename T>
