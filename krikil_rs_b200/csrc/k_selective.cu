@@ -16,86 +16,110 @@ namespace {
 // Bound by memory: a request's states are read and written once.  A lane has Q
 // times four of a channel's states, and a thread R requests' of them at once,
 // for which it reads the channel's decays once.
-constexpr int STEP_THREADS = 256;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr int STEP_THREADS = 128;
 
-KRK_DEV float4 load_four(const float* p, int n, int N, bool wide) {
-    if (wide) return *reinterpret_cast<const float4*>(p + n);
-    return make_float4(n < N ? p[n] : 0.0f, n + 1 < N ? p[n + 1] : 0.0f, n + 2 < N ? p[n + 2] : 0.0f,
-                       n + 3 < N ? p[n + 3] : 0.0f);
-}
-template <typename T>
-KRK_DEV float4 load_four(const T* p, int n, int N, bool wide) {
-    if (wide) return load4(p + n);
-    return make_float4(n < N ? to_f32(p[n]) : 0.0f, n + 1 < N ? to_f32(p[n + 1]) : 0.0f,
-                       n + 2 < N ? to_f32(p[n + 2]) : 0.0f, n + 3 < N ? to_f32(p[n + 3]) : 0.0f);
+template <bool WIDE, typename T>
+KRK_DEV float4 load_four(const T* p, int n, int N) {
+    if (WIDE) return load4(p + n);
+    return make_float4(to_f32(p[n]), n + 1 < N ? to_f32(p[n + 1]) : 0.0f, n + 2 < N ? to_f32(p[n + 2]) : 0.0f,
+                       n + 3 < N ? to_f32(p[n + 3]) : 0.0f);
 }
 
-// WIDE: whole groups of four states, aligned (states and decays; wide_bc: B and C).
+// WIDE: as many states as the lanes hold, aligned in groups of four, as are
+// decays, B and C.  Everything that the rows need is loaded before the first of
+// them is computed, whether they need it or not: where branches meet, a thread
+// waits for the loads that were in them.
 template <typename T, bool WIDE, int Q, int R>
-__global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane_bits, int side, bool wide_bc) {
+__global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane_bits, int side) {
     const int t0 = blockIdx.x / side * R, i = (blockIdx.x - blockIdx.x / side * side) * STEP_THREADS + threadIdx.x;
     const int lanes = 1 << lane_bits, lane = i & (lanes - 1), d = min(i >> lane_bits, a.D - 1);
     const bool open = (i >> lane_bits) < a.D;
     const int64_t row = (int64_t)d * a.N;
+    const int g = a.G == 1 ? 0 : d / (a.D / a.G);
     int to[R], from[R];
-    bool live[R];
-    float4 h[R][Q];
+    load_slots(a.slot, t0, a.T, to, from);
+    const T* zp = a.z ? (const T*)a.z : (const T*)a.x;  // (unused when there is none)
+    const int64_t z_st = a.z ? a.z_st : a.x_st;
+    float4 h[R][Q], b[R][Q], c[R][Q], rate[Q];
+    T x[R], dt[R], z[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        live[r] = t0 + r < a.T && request_slots(a.slot, t0 + r, to[r], from[r]) && open;
-        const float* old = (const float*)a.slot.state + from[r] * a.slot.stride + row;
+        const int t = min(t0 + r, a.T - 1);
+        const T* bt = (const T*)a.b + t * a.b_st + g * a.b_sg;
+        const T* ct = (const T*)a.c + t * a.c_st + g * a.c_sg;
+        x[r] = ((const T*)a.x)[t * a.x_st + d];
+        dt[r] = ((const T*)a.dt)[t * a.dt_st + d];
+        z[r] = zp[t * z_st + d];
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
             const int n = 4 * (q * lanes + lane);
-            h[r][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (live[r] && from[r] >= 0 && n < a.N) h[r][q] = load_four(old, n, a.N, WIDE);
+            b[r][q] = c[r][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (!WIDE && n >= a.N) continue;
+            b[r][q] = load_four<WIDE>(bt, n, a.N);
+            c[r][q] = load_four<WIDE>(ct, n, a.N);
         }
     }
-    float4 rate[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int n = 4 * (q * lanes + lane);
-        const float4 v = n < a.N ? load_four(a.a + row, n, a.N, WIDE) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        rate[q] = make_float4(scan_rate(v.x), scan_rate(v.y), scan_rate(v.z), scan_rate(v.w));
+        rate[q] = WIDE || n < a.N ? load_four<WIDE>(a.a + row, n, a.N) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = a.d ? a.d[d] : 0.0f;
-    const int g = a.G == 1 ? 0 : d / (a.D / a.G);
+    bool live[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int t = t0 + r;
-        float sum = 0.0f, x = 0.0f;
-        if (live[r]) {
-            x = to_f32(((const T*)a.x)[t * a.x_st + d]);
-            const float delta = step_width(to_f32(((const T*)a.dt)[t * a.dt_st + d]) + bias), put = delta * x;
-            const T* b = (const T*)a.b + t * a.b_st + g * a.b_sg;
-            const T* c = (const T*)a.c + t * a.c_st + g * a.c_sg;
-            float* kept = (float*)a.slot.state + to[r] * a.slot.stride + row;
+        live[r] = t0 + r < a.T && valid_slots(a.slot, to[r], from[r]);
+        const bool begun = live[r] && from[r] >= 0;
+        const float* old = (const float*)a.slot.state + (begun ? from[r] * a.slot.stride : 0) + row;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                const int n = 4 * (q * lanes + lane);
-                if (n >= a.N) continue;
-                const float4 b4 = load_four(b, n, a.N, WIDE && wide_bc), c4 = load_four(c, n, a.N, WIDE && wide_bc);
-                float4 v = h[r][q];
-                v.x = fmaf(fast_exp2(delta * rate[q].x), v.x, put * b4.x);
-                v.y = fmaf(fast_exp2(delta * rate[q].y), v.y, put * b4.y);
-                v.z = fmaf(fast_exp2(delta * rate[q].z), v.z, put * b4.z);
-                v.w = fmaf(fast_exp2(delta * rate[q].w), v.w, put * b4.w);
-                if (WIDE) {
-                    *reinterpret_cast<float4*>(kept + n) = v;
-                    sum = fmaf(v.x, c4.x, fmaf(v.y, c4.y, fmaf(v.z, c4.z, fmaf(v.w, c4.w, sum))));
-                } else {
-                    kept[n] = v.x;
-                    sum = fmaf(v.x, c4.x, sum);
-                    if (n + 1 < a.N) kept[n + 1] = v.y, sum = fmaf(v.y, c4.y, sum);
-                    if (n + 2 < a.N) kept[n + 2] = v.z, sum = fmaf(v.z, c4.z, sum);
-                    if (n + 3 < a.N) kept[n + 3] = v.w, sum = fmaf(v.w, c4.w, sum);
-                }
+        for (int q = 0; q < Q; ++q) {
+            const int n = 4 * (q * lanes + lane);
+            h[r][q] = WIDE || n < a.N ? load_four<WIDE>(old, n, a.N) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (!begun) h[r][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = a.d ? a.d[d] : 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float xv = to_f32(x[r]), delta = step_width(to_f32(dt[r]) + bias), put = delta * xv;
+        const float2 step2 = make_float2(delta * kLog2e, delta * kLog2e), put2 = make_float2(put, put);
+        float* kept = (float*)a.slot.state + (live[r] ? to[r] * a.slot.stride : 0) + row;
+        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int n = 4 * (q * lanes + lane);
+            float2 lo = make_float2(h[r][q].x, h[r][q].y), hi = make_float2(h[r][q].z, h[r][q].w);
+            const float2 e = __fmul2_rn(step2, make_float2(rate[q].x, rate[q].y));
+            const float2 f = __fmul2_rn(step2, make_float2(rate[q].z, rate[q].w));
+            lo = __ffma2_rn(make_float2(fast_exp2(e.x), fast_exp2(e.y)), lo,
+                            __fmul2_rn(put2, make_float2(b[r][q].x, b[r][q].y)));
+            hi = __ffma2_rn(make_float2(fast_exp2(f.x), fast_exp2(f.y)), hi,
+                            __fmul2_rn(put2, make_float2(b[r][q].z, b[r][q].w)));
+            if (!WIDE && n >= a.N) continue;
+            if (WIDE) {
+                sum = __ffma2_rn(lo, make_float2(c[r][q].x, c[r][q].y), sum);
+                sum = __ffma2_rn(hi, make_float2(c[r][q].z, c[r][q].w), sum);
+            } else {  // an infinite x makes no NaN of states that are not there
+                sum.x = fmaf(lo.x, c[r][q].x, sum.x);
+                if (n + 1 < a.N) sum.y = fmaf(lo.y, c[r][q].y, sum.y);
+                if (n + 2 < a.N) sum.x = fmaf(hi.x, c[r][q].z, sum.x);
+                if (n + 3 < a.N) sum.y = fmaf(hi.y, c[r][q].w, sum.y);
+            }
+            if (!live[r] || !open) continue;
+            if (WIDE) {
+                *reinterpret_cast<float4*>(kept + n) = make_float4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+                kept[n] = lo.x;
+                if (n + 1 < a.N) kept[n + 1] = lo.y;
+                if (n + 2 < a.N) kept[n + 2] = hi.x;
+                if (n + 3 < a.N) kept[n + 3] = hi.y;
             }
         }
-        for (int o = lanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (live[r] && lane == 0) {
-            const float gate = a.z ? fast_silu(to_f32(((const T*)a.z)[t * a.z_st + d])) : 1.0f;
-            ((T*)a.out)[t * a.o_st + d] = from_f32<T>(fmaf(skip, x, sum) * gate);
+        float y = sum.x + sum.y;
+        for (int o = lanes / 2; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
+        if (live[r] && open && lane == 0) {
+            const float gate = a.z ? fast_silu(to_f32(z[r])) : 1.0f;
+            ((T*)a.out)[(t0 + r) * a.o_st + d] = from_f32<T>(fmaf(skip, xv, y) * gate);
         }
     }
 }
@@ -105,10 +129,7 @@ cudaError_t launch_step(const ScanArgs& a, int lane_bits, cudaStream_t s) {
     const int64_t side = (((int64_t)a.D << lane_bits) + STEP_THREADS - 1) / STEP_THREADS;
     const int64_t blocks = side * ((a.T + (int64_t)R - 1) / R);
     if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    const int64_t rows = a.T > 1, groups = a.G > 1;
-    const bool wide_bc = fits(a.b, rows * a.b_st, 4 * sizeof(T), sizeof(T)) && fits(a.c, rows * a.c_st, 4 * sizeof(T), sizeof(T)) &&
-                         groups * a.b_sg % 4 == 0 && groups * a.c_sg % 4 == 0;
-    step_kernel<T, WIDE, Q, R><<<(unsigned)blocks, STEP_THREADS, 0, s>>>(a, lane_bits, (int)side, wide_bc);
+    step_kernel<T, WIDE, Q, R><<<(unsigned)blocks, STEP_THREADS, 0, s>>>(a, lane_bits, (int)side);
     add_launches(1);
     return cudaGetLastError();
 }
@@ -117,18 +138,21 @@ template <typename T, bool WIDE, int Q>
 cudaError_t step_rows(const ScanArgs& a, int lane_bits, cudaStream_t s) {
     const int sms = paged_sm_count();
     if (sms <= 0) return cudaErrorInvalidDevice;
-    // several requests a thread once that leaves every multiprocessor a full set of threads
-    const bool many = ((int64_t)a.D << lane_bits) * a.T >= (int64_t)sms * 2048 * 4;
-    return many ? launch_step<T, WIDE, Q, 4>(a, lane_bits, s) : launch_step<T, WIDE, Q, 1>(a, lane_bits, s);
+    // two requests a thread once that leaves every multiprocessor a full set of threads
+    const bool many = ((int64_t)a.D << lane_bits) * a.T >= (int64_t)sms * 2048 * 2;
+    return many ? launch_step<T, WIDE, Q, 2>(a, lane_bits, s) : launch_step<T, WIDE, Q, 1>(a, lane_bits, s);
 }
 
 template <typename T>
 cudaError_t step_type(const ScanArgs& a, cudaStream_t s) {
-    int bits = 0;
-    while (bits < 5 && 4 << bits < a.N) ++bits;
-    const bool wide = a.N % 4 == 0 && fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, 16, 4) && fits(a.a, 0, 16, 4);
-    if (a.N > 128) return wide ? step_rows<T, true, 2>(a, bits, s) : step_rows<T, false, 2>(a, bits, s);
-    return wide ? step_rows<T, true, 1>(a, bits, s) : step_rows<T, false, 1>(a, bits, s);
+    int bits = 0;  // lanes of eight states
+    while (bits < 5 && 8 << bits < a.N) ++bits;
+    const int64_t rows = a.T > 1, groups = a.G > 1;
+    const bool wide = a.N == (a.N <= 4 ? 4 : 8 << bits) && fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, 16, 4) && fits(a.a, 0, 16, 4) &&
+                      fits(a.b, rows * a.b_st, 4 * sizeof(T), sizeof(T)) && fits(a.c, rows * a.c_st, 4 * sizeof(T), sizeof(T)) &&
+                      groups * a.b_sg % 4 == 0 && groups * a.c_sg % 4 == 0;
+    if (a.N <= 4) return wide ? step_rows<T, true, 1>(a, 0, s) : step_rows<T, false, 1>(a, 0, s);
+    return wide ? step_rows<T, true, 2>(a, bits, s) : step_rows<T, false, 2>(a, bits, s);
 }
 
 }  // namespace
