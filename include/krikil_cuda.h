@@ -604,7 +604,7 @@ KRK_API int krk_k_sample(const float* logits, int64_t ld, int vocab, int B, uint
 
 /* Log probabilities under softmax of each row of logits [R][V] (of `type`, row r
  * at logits + r*ld; computed in 32 bits): logprobs[r*K + k] of token tokens[r*K +
- * k], entropy[r] (may be NULL; natural logarithm), and the `top` (at most 64)
+ * k], entropy[r] (may be NULL; natural logarithm), and the `top` (at most 32)
  * largest logits' ids and log probabilities, the largest first and of equal ones
  * the lower id.  A negative token asks for nothing and gets 0; one of at least V
  * gets -inf (reported by checked builds).  A logit of -inf is a masked token.  A

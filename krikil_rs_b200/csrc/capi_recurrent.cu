@@ -155,7 +155,7 @@ int krk_k_token_logprobs(void* logits, int64_t ld, int type, int R, int V, const
     const int es = elem_size(type);
     if (!es) return invalid(who, "unknown element type");
     if (R < 0 || V < 1 || K < 0) return invalid(who, "R and K must not be negative, V positive");
-    if (top < 0 || top > krk::LOGPROBS_MAX_TOP || top > V) return invalid(who, "top must be 0 to 64 and at most V");
+    if (top < 0 || top > krk::LOGPROBS_MAX_TOP || top > V) return invalid(who, "top must be 0 to 32 and at most V");
     if (R == 0) return KRK_OK;
     if (!logits || !aligned(logits, es)) return invalid(who, "logits must be set and aligned to their elements");
     if ((K > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_ids || !top_logprobs))) return invalid(who, "null pointer");

@@ -1,90 +1,371 @@
 // Log probabilities of given tokens, the entropy and the best alternatives of
 // each row of logits: with m the row's maximum and s = sum e^(x - m),
 //   lp(i) = (x_i - m) - log s,   H = log s - sum e^(x - m) (x - m) / s.
+//
+// One pass over the row, 16 bytes an access: each thread keeps the running
+// maximum of its own logits with the two sums relative to it, and where that
+// maximum is.  Bound by memory for 32 bits; for 16 bits the exponential unit (one
+// a logit, 16 a clock and multiprocessor) is close behind.
+//
+// The alternatives cost the pass nothing: of the threads' maxima the top-th
+// largest is a bound that no alternative lies below, and only the threads whose
+// maximum reaches it can hold one, as many as there are alternatives.  Their
+// logits are read again, and of the few that reach the bound each one's rank is
+// its place.  Few rows are shared by the blocks of a cluster, whose sums and
+// lists its first block joins.
+#include <cooperative_groups.h>
+
 #include "kernels.h"
+#include "paged.h"
 #include "recurrent.cuh"
 
 namespace krk {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_LIST = 32;     // entries of a sorted list, LOGPROBS_MAX_TOP of them used
+constexpr int LP_ROOM = 1024;   // logits that reach the bound; for more (the best ones all in few threads' ways) see below
+constexpr int LP_AHEAD = 4;     // accesses on their way
 constexpr float kLog2e = 1.44269504088896341f, kLowest = -3.402823466e38f;
+using Key = unsigned long long;
 
 // The order of the alternatives as whole numbers: larger logits first, of equal
-// ones the lower index; NaN counts as -inf and -0 as 0.
-KRK_DEV unsigned long long order_key(float x, int i) {
+// ones the lower index; NaN counts as -inf and -0 as 0.  Never 0.
+KRK_DEV Key order_key(float x, int i) {
     x = x == x ? x + 0.0f : -INFINITY;
     const unsigned u = __float_as_uint(x);
-    return (unsigned long long)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - (unsigned)i);
+    return (Key)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - (unsigned)i);
 }
+KRK_DEV int key_index(Key k) { return (int)(0xffffffffu - (unsigned)k); }
+KRK_DEV Key later(Key a, Key b) { return a < b ? a : b; }
+KRK_DEV Key sooner(Key a, Key b) { return a > b ? a : b; }
 
-template <typename V, typename F>
-KRK_DEV V block_fold(V x, V* part, F fold) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x = fold(x, __shfl_xor_sync(0xffffffffu, x, o));
-    __syncthreads();  // part may still be read
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = part[0];
-#pragma unroll
-    for (int w = 1; w < LP_WARPS; ++w) x = fold(x, part[w]);
-    return x;
+// sum e^(x - ref) and sum e^(x - ref) (x - ref) over some logits with maximum m; ref = max(m, lowest).
+struct Sums {
+    float m, s, e;
+};
+KRK_DEV float ref_of(float m) { return fmaxf(m, kLowest); }
+KRK_DEV Sums join(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m), r = ref_of(m);
+    // (what lies 1000 below adds nothing)
+    const float da = fmaxf(ref_of(a.m) - r, -1000.0f), db = fmaxf(ref_of(b.m) - r, -1000.0f);
+    const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
+    return {m, fmaf(a.s, fa, b.s * fb), fmaf(fa, fmaf(a.s, da, a.e), fb * fmaf(b.s, db, b.e))};
 }
-
+KRK_DEV Sums shuffle(const Sums& a, int o) {
+    return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.e, o)};
+}
 // (x - m) - log s; a row that its mask leaves empty gives every token -inf.
-KRK_DEV float log_prob(float x, float m, float s) { return s == 0.0f ? -INFINITY : (x - m) - logf(s); }
+KRK_DEV float log_prob(float x, const Sums& a) { return a.s == 0.0f ? -INFINITY : (x - ref_of(a.m)) - logf(a.s); }
+
+// Sorts a warp's keys, one a lane, the first the largest.
+KRK_DEV Key sort_step(Key k, int lane, int size, int o) {
+    const Key other = __shfl_xor_sync(0xffffffffu, k, o);
+    const bool first = ((lane & o) == 0) == ((lane & size) == 0);
+    return first ? sooner(k, other) : later(k, other);
+}
+KRK_DEV Key warp_sort(Key k, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int o = size / 2; o > 0; o /= 2) k = sort_step(k, lane, size, o);
+    return k;
+}
+// The 32 largest of two sorted lists, sorted.
+KRK_DEV Key warp_merge(const Key* a, const Key* b, int lane) {
+    Key k = sooner(a[lane], b[31 - lane]);
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) k = sort_step(k, lane, 32, o);
+    return k;
+}
+// Merges n (a power of two) sorted lists into the first.  All threads take part.
+template <typename L>
+KRK_DEV void merge_lists(L lists, int n) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int half = n / 2; half > 0; half /= 2) {
+        for (int i = warp; i < half; i += LP_WARPS) {
+            const Key k = warp_merge(lists(i), lists(i + half), lane);
+            __syncwarp();
+            lists(i)[lane] = k;
+        }
+        __syncthreads();
+    }
+}
 
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a) {
-    __shared__ float part[LP_WARPS];
-    __shared__ unsigned long long keys[LP_WARPS];
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const T* x = (const T*)a.logits + row * a.ld;
-    float m = kLowest;
-    for (int i = tid; i < a.V; i += LP_THREADS) m = fmaxf(m, to_f32(x[i]));
-    m = block_fold(m, part, [](float p, float q) { return fmaxf(p, q); });
-    float s = 0.0f, e = 0.0f;
-    for (int i = tid; i < a.V; i += LP_THREADS) {
-        const float u = to_f32(x[i]) - m, p = fast_exp2(u * kLog2e);
-        s += p;
-        e = fmaf(p, fmaxf(u, -1000.0f), e);  // 0 times -inf is 0 here
+struct Row {
+    static constexpr int VEC = 16 / sizeof(T);
+    using Vec = Pack<T, VEC>;
+    const T* x;      // logits [0, V)
+    int V, lead;     // vector k holds logits k * VEC - lead ..
+    KRK_DEV Row(const LogprobArgs& a, int row) : x((const T*)a.logits + row * a.ld), V(a.V) {
+        lead = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
     }
-    const auto add = [](float p, float q) { return p + q; };
-    s = block_fold(s, part, add);
-    e = block_fold(e, part, add);
-    if (a.entropy && tid == 0) a.entropy[row] = s == 0.0f ? 0.0f : logf(s) - e / s;
-    for (int k = tid; k < a.K; k += LP_THREADS) {
-        const int id = a.tokens[(int64_t)row * a.K + k];
+    KRK_DEV int vectors() const { return (int)(((int64_t)lead + V + VEC - 1) / VEC); }
+    KRK_DEV int first(int k) const { return k * VEC - lead; }
+    KRK_DEV bool whole(int k) const { return first(k) >= 0 && first(k) <= V - VEC; }
+    KRK_DEV Vec load(int k) const { return load_pack<T, VEC>(x + first(k)); }
+    // Any vector; NaN-free -inf where there is no logit.
+    KRK_DEV void floats(int k, float (&v)[VEC]) const {
+        if (whole(k)) {
+            const Vec p = load(k);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = to_f32(p.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int i = first(k) + j;
+                v[j] = i >= 0 && i < V ? to_f32(x[i]) : -INFINITY;
+            }
+        }
+    }
+    KRK_DEV bool has(int k, int j) const { return first(k) + j >= 0 && first(k) + j < V; }
+};
+
+// A thread's sums over its vectors, in two halves, and the first vector that holds its maximum (-1: none yet).
+template <int VEC>
+struct Running {
+    float m = -INFINITY;
+    float2 s = {0.0f, 0.0f}, e = {0.0f, 0.0f};
+    int best = -1;
+    KRK_DEV void add(const float (&x)[VEC], int k) {
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) top = fmaxf(top, x[j]);
+        if (top > m || best < 0) {
+            top = top == top ? top : -INFINITY;
+            const float d = fmaxf(ref_of(m) - ref_of(top), -1000.0f), f = fast_exp2(d * kLog2e);
+            e = make_float2(f * fmaf(s.x, d, e.x), f * fmaf(s.y, d, e.y));
+            s = make_float2(s.x * f, s.y * f);
+            m = top;
+            best = k;
+        }
+        const float r = ref_of(m);
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const float2 u = __fadd2_rn(make_float2(x[j], x[j + 1]), make_float2(-r, -r));
+            const float2 t = __fmul2_rn(u, make_float2(kLog2e, kLog2e));
+            const float2 p = make_float2(fast_exp2(t.x), fast_exp2(t.y));
+            s = __fadd2_rn(s, p);
+            e = __ffma2_rn(p, make_float2(fmaxf(u.x, -1000.0f), fmaxf(u.y, -1000.0f)), e);  // 0 times -inf is 0 here
+        }
+    }
+};
+
+struct Shared {
+    Sums part[LP_WARPS], all;
+    Key list[LP_WARPS][LP_LIST];   // sorted lists; in the end the first is the block's
+    Key near[LP_ROOM];             // logits that reach the bound
+    Key gathered[16][LP_LIST];     // a cluster's lists
+    int count;
+};
+
+// The block's `top` first keys into sh.list[0], sorted, 0 behind them.  `best`: the thread's first key.
+template <typename T>
+KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Shared& sh) {
+    constexpr int VEC = Row<T>::VEC;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    sh.list[warp][lane] = warp_sort(best, lane);
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    merge_lists([&](int i) { return sh.list[i]; }, LP_WARPS);
+    if (top == 1) return;
+    // The top-th thread's first key (0: there are not so many threads with logits) is one that `top` keys reach, so
+    // that those that do are the first ones; they are in the ways of the threads that the list names.
+    const Key bound = sh.list[0][top - 1];
+    const int ways = (k1 - k0 + LP_THREADS - 1) / LP_THREADS;
+    for (int i = warp; i < top; i += LP_WARPS) {
+        const Key first = sh.list[0][i];
+        if (first == 0) break;
+        const int way = ((key_index(first) + row.lead) / VEC - k0) % LP_THREADS;
+        for (int j = lane; j < ways; j += 32) {
+            const int k = k0 + way + j * LP_THREADS;
+            if (k >= k1) break;
+            float v[VEC];
+            row.floats(k, v);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) {
+                const Key key = order_key(v[q], row.first(k) + q);
+                if (key >= bound && row.has(k, q)) {
+                    const int at = atomicAdd(&sh.count, 1);  // (in any order: ranks tell)
+                    if (at < LP_ROOM) sh.near[at] = key;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int n = sh.count;
+    if (tid < LP_LIST) sh.list[0][tid] = 0;
+    __syncthreads();
+    if (n <= LP_ROOM) {
+        for (int i = tid; i < n; i += LP_THREADS) {
+            const Key key = sh.near[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += sh.near[j] > key;
+            if (rank < top) sh.list[0][rank] = key;
+        }
+        __syncthreads();
+        return;
+    }
+    // More than there is room for: one after the other, a pass each.
+    Key before = ~0ull;
+    for (int i = 0; i < top; ++i) {
+        Key next = 0;
+        for (int k = k0 + tid; k < k1; k += LP_THREADS) {
+            float v[VEC];
+            row.floats(k, v);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) {
+                const Key key = order_key(v[q], row.first(k) + q);
+                if (key < before && row.has(k, q)) next = sooner(next, key);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) next = sooner(next, __shfl_xor_sync(0xffffffffu, next, o));
+        if (lane == 0) sh.near[warp] = next;
+        __syncthreads();
+        next = sh.near[0];
+        for (int w = 1; w < LP_WARPS; ++w) next = sooner(next, sh.near[w]);
+        __syncthreads();
+        if (tid == 0) sh.list[0][i] = next;
+        if (next == 0) break;
+        before = next;
+    }
+    __syncthreads();
+}
+
+// One block a row, or the `parts` blocks of a cluster.
+template <typename T>
+__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a, int parts) {
+    constexpr int VEC = Row<T>::VEC;
+    __shared__ Shared sh;
+    const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Row<T> row(a, r);
+    const int n = row.vectors(), k0 = (int)((int64_t)n * part / parts), k1 = (int)((int64_t)n * (part + 1) / parts);
+
+    Running<VEC> run;
+    // (a thread's vectors are LP_THREADS apart, the row's ends among them, which may not be whole)
+    const int w0 = row.whole(k0) ? k0 : k0 + 1, w1 = k1 > w0 && !row.whole(k1 - 1) ? k1 - 1 : k1;
+    int k = k0 + tid;
+    if (k < w0) {
+        float v[VEC];
+        row.floats(k, v);
+        run.add(v, k);
+        k += LP_THREADS;
+    }
+    for (; k < w1; k += LP_AHEAD * LP_THREADS) {
+        typename Row<T>::Vec p[LP_AHEAD];
+#pragma unroll
+        for (int i = 0; i < LP_AHEAD; ++i)
+            if (k + i * LP_THREADS < w1) p[i] = row.load(k + i * LP_THREADS);
+#pragma unroll
+        for (int i = 0; i < LP_AHEAD; ++i) {
+            if (k + i * LP_THREADS >= w1) break;
+            float v[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = to_f32(p[i].v[j]);
+            run.add(v, k + i * LP_THREADS);
+        }
+    }
+    if (w1 < k1 && (w1 - k0) % LP_THREADS == tid) {
+        float v[VEC];
+        row.floats(w1, v);
+        run.add(v, w1);
+    }
+
+    Sums sums{run.m, run.s.x + run.s.y, run.e.x + run.e.y};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sums = join(sums, shuffle(sums, o));
+    if (lane == 0) sh.part[warp] = sums;
+    if (a.top > 0) {
+        Key best = 0;
+        if (run.best >= 0) {
+            float v[VEC];
+            row.floats(run.best, v);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (row.has(run.best, j)) best = sooner(best, order_key(v[j], row.first(run.best) + j));
+        }
+        best_keys(row, k0, k1, a.top, best, sh);
+    } else {
+        __syncthreads();
+    }
+    if (warp == 0) {
+        sums = sh.part[lane % LP_WARPS];
+#pragma unroll
+        for (int o = LP_WARPS / 2; o > 0; o >>= 1) sums = join(sums, shuffle(sums, o));
+        if (lane == 0) sh.all = sums;
+    }
+    if (parts > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        if (part == 0) {
+            if (a.top > 0) {
+                for (int i = warp; i < parts; i += LP_WARPS)
+                    sh.gathered[i][lane] = cluster.map_shared_rank(&sh, i)->list[0][lane];
+                __syncthreads();
+                merge_lists([&](int i) { return sh.gathered[i]; }, parts);
+                if (warp == 0) sh.list[0][lane] = sh.gathered[0][lane];
+            }
+            if (warp == 0) {
+                sums = lane < parts ? cluster.map_shared_rank(&sh, lane)->all : Sums{-INFINITY, 0.0f, 0.0f};
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) sums = join(sums, shuffle(sums, o));
+            }
+        }
+        cluster.sync();  // the others' memory is theirs until here
+        if (part > 0) return;
+        if (warp == 0 && lane == 0) sh.all = sums;
+    }
+    __syncthreads();
+    sums = sh.all;
+    if (a.entropy && tid == 0) a.entropy[r] = sums.s == 0.0f ? 0.0f : logf(sums.s) - sums.e / sums.s;
+    for (int i = tid; i < a.K; i += LP_THREADS) {
+        const int id = a.tokens[(int64_t)r * a.K + i];
         if (id >= a.V) check_fail(CHK_TOKEN);
-        a.lp[(int64_t)row * a.K + k] = id < 0 ? 0.0f : id >= a.V ? -INFINITY : log_prob(to_f32(x[id]), m, s);
+        a.lp[(int64_t)r * a.K + i] = id < 0 ? 0.0f : id >= a.V ? -INFINITY : log_prob(to_f32(row.x[id]), sums);
     }
-    unsigned long long before = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-        unsigned long long best = 0;
-        for (int i = tid; i < a.V; i += LP_THREADS) {
-            const unsigned long long key = order_key(to_f32(x[i]), i);
-            if (key < before && key > best) best = key;
-        }
-        before = block_fold(best, keys, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; });
-        if (tid == 0) {
-            const int id = (int)(0xffffffffu - (unsigned)before);
-            a.top_ids[(int64_t)row * a.top + k] = id;
-            a.top_lp[(int64_t)row * a.top + k] = log_prob(to_f32(x[id]), m, s);
-        }
+    if (tid < a.top) {
+        const int id = key_index(sh.list[0][tid]);
+        a.top_ids[(int64_t)r * a.top + tid] = id;
+        a.top_lp[(int64_t)r * a.top + tid] = log_prob(to_f32(row.x[id]), sums);
     }
+}
+
+template <typename T>
+cudaError_t launch(const LogprobArgs& a, cudaStream_t s) {
+    const int sms = paged_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    // a cluster for each of few rows, while its blocks have two accesses a thread
+    int parts = 1;
+    const int64_t vectors = (int64_t)a.V * sizeof(T) / 16;
+    while (parts < 16 && (int64_t)a.R * parts * 2 <= sms && vectors >= (int64_t)parts * 2 * LP_THREADS * 2) parts *= 2;
+    if ((int64_t)a.R * parts > INT32_MAX) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.R * parts));
+    cfg.blockDim = dim3(LP_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = parts > 1 ? &attr : nullptr;
+    cfg.numAttrs = parts > 1;
+    if (parts > 8) {
+        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, parts);
+    if (e == cudaSuccess) add_launches(1);
+    return e;
 }
 
 }  // namespace
 
 cudaError_t token_logprobs(const LogprobArgs& a, int type, cudaStream_t s) {
-    if (type == 0)
-        logprobs_kernel<float><<<a.R, LP_THREADS, 0, s>>>(a);
-    else if (type == 1)
-        logprobs_kernel<__half><<<a.R, LP_THREADS, 0, s>>>(a);
-    else
-        logprobs_kernel<__nv_bfloat16><<<a.R, LP_THREADS, 0, s>>>(a);
-    add_launches(1);
-    return cudaGetLastError();
+    return type == ELEM_F32 ? launch<float>(a, s) : type == ELEM_F16 ? launch<__half>(a, s) : launch<__nv_bfloat16>(a, s);
 }
 
 }  // namespace krk

@@ -60,7 +60,7 @@ constexpr int64_t scan_split_room(int64_t T, int rows) { return T / rows * 8 / 7
 cudaError_t selective_scan(const ScanArgs& a, int type, int max_len, float* work, cudaStream_t s);
 cudaError_t selective_step(const ScanArgs& a, int type, cudaStream_t s);
 
-constexpr int LOGPROBS_MAX_TOP = 64;
+constexpr int LOGPROBS_MAX_TOP = 32;
 struct LogprobArgs {
     const void* logits; int64_t ld; int R, V;    // (r, v) at r*ld + v
     const int32_t* tokens; int K;                // [R][K]

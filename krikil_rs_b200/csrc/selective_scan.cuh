@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     const int own = lane / Sh::SHARE * OWN;
     const T* xp = (const T*)a.x + (begin + own) * a.x_st + d;
     const T* dtp = (const T*)a.dt + (begin + own) * a.dt_st + d;
-    const T* zp = (const T*)a.z + (begin + own) * a.z_st + d;
+    const int64_t z_st = gated ? a.z_st : a.x_st;  // (x in place of a gate that there is none of)
+    const T* zp = (gated ? (const T*)a.z : (const T*)a.x) + (begin + own) * z_st + d;
     T* outp = (T*)a.out + (begin + own) * a.o_st + d;
     T xr[OWN], dtr[OWN], zr[OWN];
     const auto fetch = [&](int t, auto whole) {
@@ -202,10 +203,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
             const bool in = decltype(whole)::value || t + own + o < end;
             xr[o] = in ? *xp : zero;
             dtr[o] = in ? *dtp : zero;
-            if (gated) zr[o] = in ? *zp : zero;
+            if (!CARRY) zr[o] = in ? *zp : zero;
             xp += o + 1 < OWN ? a.x_st : (U - OWN + 1) * a.x_st;
             dtp += o + 1 < OWN ? a.dt_st : (U - OWN + 1) * a.dt_st;
-            zp += o + 1 < OWN ? a.z_st : (U - OWN + 1) * a.z_st;
+            zp += o + 1 < OWN ? z_st : (U - OWN + 1) * z_st;
         }
     };
     // And its elements of the next tile of B and C.
@@ -236,7 +237,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
             mine[o] = decltype(whole)::value || t + own + o < end ? step_width(to_f32(dtr[o]) + bias) : 0.0f;
             mine_put[o] = mine[o] * x;
             skipped[o] = skip * x;
-            gate[o] = gated ? fast_silu(to_f32(zr[o])) : 1.0f;
+            const float silu = fast_silu(to_f32(zr[o]));
+            gate[o] = gated ? silu : 1.0f;
         }
         fetch(t + U, whole);
 #pragma unroll

@@ -614,7 +614,7 @@ def selective_step(x, dt, a, b, c, state, slots=None, d=None, z=None, dt_bias=No
 def token_logprobs(logits, tokens=None, top: int = 0):
     """Log probabilities under softmax of each row of logits [R, V]: of tokens
     (int32 [R] or [R, K]; negative: none asked, 0), the entropy [R], and the ids
-    and log probabilities [R, top] of the largest logits (at most 64), the lower
+    and log probabilities [R, top] of the largest logits (at most 32), the lower
     id first among equal ones.  Returns (logprobs like tokens, or None; entropy;
     top_ids; top_logprobs), float32 and int32."""
     dev = _cuda_device(logits)
