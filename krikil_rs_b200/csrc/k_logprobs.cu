@@ -24,7 +24,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
+constexpr int LP_SHORT = 1024;  // accesses of a row that a small block takes in any case
 constexpr int LP_LIST = 32;     // entries of a sorted list, LOGPROBS_MAX_TOP of them used
 constexpr int LP_ROOM = 1024;   // logits that reach the bound; for more (the best ones all in few threads' ways) see below
 constexpr int LP_AHEAD = 4;     // accesses on their way
@@ -47,15 +47,11 @@ struct Sums {
     float m, s, e;
 };
 KRK_DEV float ref_of(float m) { return fmaxf(m, kLowest); }
-KRK_DEV Sums join(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m), r = ref_of(m);
+// Of a warp's, relative to their common maximum.
+KRK_DEV Sums warp_join(const Sums& a) {
+    const float m = warp_max(a.m), d = fmaxf(ref_of(a.m) - ref_of(m), -1000.0f), f = fast_exp2(d * kLog2e);
     // (what lies 1000 below adds nothing)
-    const float da = fmaxf(ref_of(a.m) - r, -1000.0f), db = fmaxf(ref_of(b.m) - r, -1000.0f);
-    const float fa = fast_exp2(da * kLog2e), fb = fast_exp2(db * kLog2e);
-    return {m, fmaf(a.s, fa, b.s * fb), fmaf(fa, fmaf(a.s, da, a.e), fb * fmaf(b.s, db, b.e))};
-}
-KRK_DEV Sums shuffle(const Sums& a, int o) {
-    return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.e, o)};
+    return {m, warp_sum(a.s * f), warp_sum(f * fmaf(a.s, d, a.e))};
 }
 // (x - m) - log s; a row that its mask leaves empty gives every token -inf.
 KRK_DEV float log_prob(float x, const Sums& a) { return a.s == 0.0f ? -INFINITY : (x - ref_of(a.m)) - logf(a.s); }
@@ -80,12 +76,12 @@ KRK_DEV Key warp_merge(const Key* a, const Key* b, int lane) {
     for (int o = 16; o > 0; o /= 2) k = sort_step(k, lane, 32, o);
     return k;
 }
-// Merges n (a power of two) sorted lists into the first.  All threads take part.
-template <typename L>
+// Merges n (a power of two) sorted lists into the first.  All WARPS warps take part.
+template <int WARPS, typename L>
 KRK_DEV void merge_lists(L lists, int n) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int half = n / 2; half > 0; half /= 2) {
-        for (int i = warp; i < half; i += LP_WARPS) {
+        for (int i = warp; i < half; i += WARPS) {
             const Key k = warp_merge(lists(i), lists(i + half), lane);
             __syncwarp();
             lists(i)[lane] = k;
@@ -154,39 +150,64 @@ struct Running {
     }
 };
 
+template <int WARPS>
 struct Shared {
-    Sums part[LP_WARPS], all;
-    Key list[LP_WARPS][LP_LIST];   // sorted lists; in the end the first is the block's
+    Sums part[WARPS], all;
+    Key list[WARPS][LP_LIST];   // sorted lists; in the end the first is the block's
     Key near[LP_ROOM];             // logits that reach the bound
     Key gathered[16][LP_LIST];     // a cluster's lists
     int count;
 };
 
+// The largest of a warp's keys: of their high halves, then of the low ones that go with it.
+KRK_DEV Key warp_first(Key k) {
+    const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(k >> 32));
+    const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(k >> 32) == high ? (unsigned)k : 0u);
+    return (Key)high << 32 | low;
+}
+
 // The block's `top` first keys into sh.list[0], sorted, 0 behind them.  `best`: the thread's first key.
-template <typename T>
-KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Shared& sh) {
-    constexpr int VEC = Row<T>::VEC;
+template <typename T, int WARPS>
+KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Shared<WARPS>& sh) {
+    constexpr int VEC = Row<T>::VEC, THREADS = 32 * WARPS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (top == 1) {
+        best = warp_first(best);
+        sh.list[warp][lane] = lane == 0 ? best : 0;
+        __syncthreads();
+        if (warp == 0) {
+            best = warp_first(lane < WARPS ? sh.list[lane][0] : 0);
+            if (lane == 0) sh.list[0][0] = best;
+        }
+        __syncthreads();
+        return;
+    }
     sh.list[warp][lane] = warp_sort(best, lane);
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    merge_lists([&](int i) { return sh.list[i]; }, LP_WARPS);
-    if (top == 1) return;
+    merge_lists<WARPS>([&](int i) { return sh.list[i]; }, WARPS);
     // The top-th thread's first key (0: there are not so many threads with logits) is one that `top` keys reach, so
     // that those that do are the first ones; they are in the ways of the threads that the list names.
     const Key bound = sh.list[0][top - 1];
-    const int ways = (k1 - k0 + LP_THREADS - 1) / LP_THREADS;
-    for (int i = warp; i < top; i += LP_WARPS) {
+    const unsigned high = (unsigned)(bound >> 32);
+    const float bound_value = bound == 0 ? -INFINITY : __uint_as_float(high & 0x80000000u ? high & 0x7fffffffu : ~high);
+    const int ways = (k1 - k0 + THREADS - 1) / THREADS;
+    for (int i = warp; i < top; i += WARPS) {
         const Key first = sh.list[0][i];
         if (first == 0) break;
-        const int way = ((key_index(first) + row.lead) / VEC - k0) % LP_THREADS;
+        const int way = ((key_index(first) + row.lead) / VEC - k0) % THREADS;
         for (int j = lane; j < ways; j += 32) {
-            const int k = k0 + way + j * LP_THREADS;
+            const int k = k0 + way + j * THREADS;
             if (k >= k1) break;
             float v[VEC];
             row.floats(k, v);
+            float near = v[0];
+#pragma unroll
+            for (int q = 1; q < VEC; ++q) near = fmaxf(near, v[q]);
+            if (near < bound_value) continue;  // (NaN counts as -inf, and only that bound takes it)
 #pragma unroll
             for (int q = 0; q < VEC; ++q) {
+                if (v[q] < bound_value) continue;
                 const Key key = order_key(v[q], row.first(k) + q);
                 if (key >= bound && row.has(k, q)) {
                     const int at = atomicAdd(&sh.count, 1);  // (in any order: ranks tell)
@@ -200,7 +221,7 @@ KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Sha
     if (tid < LP_LIST) sh.list[0][tid] = 0;
     __syncthreads();
     if (n <= LP_ROOM) {
-        for (int i = tid; i < n; i += LP_THREADS) {
+        for (int i = tid; i < n; i += THREADS) {
             const Key key = sh.near[i];
             int rank = 0;
             for (int j = 0; j < n; ++j) rank += sh.near[j] > key;
@@ -213,7 +234,7 @@ KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Sha
     Key before = ~0ull;
     for (int i = 0; i < top; ++i) {
         Key next = 0;
-        for (int k = k0 + tid; k < k1; k += LP_THREADS) {
+        for (int k = k0 + tid; k < k1; k += THREADS) {
             float v[VEC];
             row.floats(k, v);
 #pragma unroll
@@ -222,12 +243,11 @@ KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Sha
                 if (key < before && row.has(k, q)) next = sooner(next, key);
             }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) next = sooner(next, __shfl_xor_sync(0xffffffffu, next, o));
+        next = warp_first(next);
         if (lane == 0) sh.near[warp] = next;
         __syncthreads();
         next = sh.near[0];
-        for (int w = 1; w < LP_WARPS; ++w) next = sooner(next, sh.near[w]);
+        for (int w = 1; w < WARPS; ++w) next = sooner(next, sh.near[w]);
         __syncthreads();
         if (tid == 0) sh.list[0][i] = next;
         if (next == 0) break;
@@ -237,65 +257,71 @@ KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Sha
 }
 
 // One block a row, or the `parts` blocks of a cluster.
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a, int parts) {
-    constexpr int VEC = Row<T>::VEC;
-    __shared__ Shared sh;
-    const int r = blockIdx.x / parts, part = blockIdx.x - r * parts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(LogprobArgs a, int part_bits) {
+    constexpr int VEC = Row<T>::VEC, THREADS = 32 * WARPS;
+    __shared__ Shared<WARPS> sh;
+    const int parts = 1 << part_bits, r = blockIdx.x >> part_bits, part = blockIdx.x & (parts - 1);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Row<T> row(a, r);
-    const int n = row.vectors(), k0 = (int)((int64_t)n * part / parts), k1 = (int)((int64_t)n * (part + 1) / parts);
+    const int64_t n = row.vectors();
+    const int k0 = (int)(n * part >> part_bits), k1 = (int)(n * (part + 1) >> part_bits);
 
     Running<VEC> run;
-    // (a thread's vectors are LP_THREADS apart, the row's ends among them, which may not be whole)
+    // (a thread's vectors are THREADS apart, the row's ends among them, which may not be whole)
     const int w0 = row.whole(k0) ? k0 : k0 + 1, w1 = k1 > w0 && !row.whole(k1 - 1) ? k1 - 1 : k1;
     int k = k0 + tid;
     if (k < w0) {
         float v[VEC];
         row.floats(k, v);
         run.add(v, k);
-        k += LP_THREADS;
+        k += THREADS;
     }
-    for (; k < w1; k += LP_AHEAD * LP_THREADS) {
-        typename Row<T>::Vec p[LP_AHEAD];
+    const auto take = [&](const typename Row<T>::Vec& p, int at) {
+        float v[VEC];
 #pragma unroll
-        for (int i = 0; i < LP_AHEAD; ++i)
-            if (k + i * LP_THREADS < w1) p[i] = row.load(k + i * LP_THREADS);
+        for (int j = 0; j < VEC; ++j) v[j] = to_f32(p.v[j]);
+        run.add(v, at);
+    };
+    typename Row<T>::Vec p[LP_AHEAD];
+    for (; k + (LP_AHEAD - 1) * THREADS < w1; k += LP_AHEAD * THREADS) {
 #pragma unroll
-        for (int i = 0; i < LP_AHEAD; ++i) {
-            if (k + i * LP_THREADS >= w1) break;
-            float v[VEC];
+        for (int i = 0; i < LP_AHEAD; ++i) p[i] = row.load(k + i * THREADS);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = to_f32(p[i].v[j]);
-            run.add(v, k + i * LP_THREADS);
-        }
+        for (int i = 0; i < LP_AHEAD; ++i) take(p[i], k + i * THREADS);
     }
-    if (w1 < k1 && (w1 - k0) % LP_THREADS == tid) {
+    if (w0 < w1) {  // (the last one again where there are no more: in a branch each load would be waited for)
+#pragma unroll
+        for (int i = 0; i < LP_AHEAD - 1; ++i) p[i] = row.load(min(k + i * THREADS, w1 - 1));
+#pragma unroll
+        for (int i = 0; i < LP_AHEAD - 1; ++i)
+            if (k + i * THREADS < w1) take(p[i], k + i * THREADS);
+    }
+    if (w1 < k1 && (w1 - k0) % THREADS == tid) {
         float v[VEC];
         row.floats(w1, v);
         run.add(v, w1);
     }
 
-    Sums sums{run.m, run.s.x + run.s.y, run.e.x + run.e.y};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sums = join(sums, shuffle(sums, o));
+    Sums sums = warp_join({run.m, run.s.x + run.s.y, run.e.x + run.e.y});
     if (lane == 0) sh.part[warp] = sums;
     if (a.top > 0) {
         Key best = 0;
-        if (run.best >= 0) {
+        if (run.best >= 0) {  // the first of the vector's logits that is the maximum
             float v[VEC];
             row.floats(run.best, v);
+            int at = VEC;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (row.has(run.best, j)) best = sooner(best, order_key(v[j], row.first(run.best) + j));
+            for (int j = VEC - 1; j >= 0; --j)
+                if ((v[j] == run.m || run.m == -INFINITY) && row.has(run.best, j)) at = j;
+            best = order_key(run.m, row.first(run.best) + at);
         }
-        best_keys(row, k0, k1, a.top, best, sh);
+        best_keys<T, WARPS>(row, k0, k1, a.top, best, sh);
     } else {
         __syncthreads();
     }
     if (warp == 0) {
-        sums = sh.part[lane % LP_WARPS];
-#pragma unroll
-        for (int o = LP_WARPS / 2; o > 0; o >>= 1) sums = join(sums, shuffle(sums, o));
+        sums = warp_join(lane < WARPS ? sh.part[lane] : Sums{-INFINITY, 0.0f, 0.0f});
         if (lane == 0) sh.all = sums;
     }
     if (parts > 1) {
@@ -303,16 +329,14 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a, int
         cluster.sync();
         if (part == 0) {
             if (a.top > 0) {
-                for (int i = warp; i < parts; i += LP_WARPS)
+                for (int i = warp; i < parts; i += WARPS)
                     sh.gathered[i][lane] = cluster.map_shared_rank(&sh, i)->list[0][lane];
                 __syncthreads();
-                merge_lists([&](int i) { return sh.gathered[i]; }, parts);
+                merge_lists<WARPS>([&](int i) { return sh.gathered[i]; }, parts);
                 if (warp == 0) sh.list[0][lane] = sh.gathered[0][lane];
             }
             if (warp == 0) {
-                sums = lane < parts ? cluster.map_shared_rank(&sh, lane)->all : Sums{-INFINITY, 0.0f, 0.0f};
-#pragma unroll
-                for (int o = 8; o > 0; o >>= 1) sums = join(sums, shuffle(sums, o));
+                sums = warp_join(lane < parts ? cluster.map_shared_rank(&sh, lane)->all : Sums{-INFINITY, 0.0f, 0.0f});
             }
         }
         cluster.sync();  // the others' memory is theirs until here
@@ -322,7 +346,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a, int
     __syncthreads();
     sums = sh.all;
     if (a.entropy && tid == 0) a.entropy[r] = sums.s == 0.0f ? 0.0f : logf(sums.s) - sums.e / sums.s;
-    for (int i = tid; i < a.K; i += LP_THREADS) {
+    for (int i = tid; i < a.K; i += THREADS) {
         const int id = a.tokens[(int64_t)r * a.K + i];
         if (id >= a.V) check_fail(CHK_TOKEN);
         a.lp[(int64_t)r * a.K + i] = id < 0 ? 0.0f : id >= a.V ? -INFINITY : log_prob(to_f32(row.x[id]), sums);
@@ -334,38 +358,50 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(LogprobArgs a, int
     }
 }
 
-template <typename T>
-cudaError_t launch(const LogprobArgs& a, cudaStream_t s) {
-    const int sms = paged_sm_count();
-    if (sms <= 0) return cudaErrorInvalidDevice;
-    // a cluster for each of few rows, while its blocks have two accesses a thread
-    int parts = 1;
-    const int64_t vectors = (int64_t)a.V * sizeof(T) / 16;
-    while (parts < 16 && (int64_t)a.R * parts * 2 <= sms && vectors >= (int64_t)parts * 2 * LP_THREADS * 2) parts *= 2;
+template <typename T, int WARPS>
+cudaError_t launch(const LogprobArgs& a, int part_bits, cudaStream_t s) {
+    const int parts = 1 << part_bits;
     if ((int64_t)a.R * parts > INT32_MAX) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.R * parts));
-    cfg.blockDim = dim3(LP_THREADS);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.stream = s;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = parts;
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = parts > 1 ? &attr : nullptr;
+    cfg.attrs = &attr;
     cfg.numAttrs = parts > 1;
     if (parts > 8) {
-        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        const cudaError_t e = cudaFuncSetAttribute(logprobs_kernel<T, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
     }
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, parts);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_kernel<T, WARPS>, a, part_bits);
     if (e == cudaSuccess) add_launches(1);
     return e;
+}
+
+template <typename T>
+cudaError_t logprobs_type(const LogprobArgs& a, cudaStream_t s) {
+    const int sms = paged_sm_count();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    const int64_t vectors = (int64_t)a.V * sizeof(T) / 16;
+    // A row's end costs each warp about 500 instructions, as much as ten accesses: small blocks for short rows, and for
+    // 16 bits, where instructions are short, when there are rows for all multiprocessors (bfloat16, 4096 x 32768 with
+    // 20 alternatives: 84 us with four warps, 90 with eight, 153 with two; float32, 1024 x 50001: 47, 36 and 51).
+    if (vectors <= LP_SHORT) return launch<T, 2>(a, 0, s);
+    if (sizeof(T) == 2 && a.R >= 4 * sms) return launch<T, 4>(a, 0, s);
+    // a cluster for each of few rows, while its blocks have two accesses a thread
+    int bits = 0;
+    while (bits < 4 && (int64_t)a.R << (bits + 1) <= sms && vectors >= (int64_t)(2 * 8 * 32) << (bits + 1)) ++bits;
+    return launch<T, 8>(a, bits, s);
 }
 
 }  // namespace
 
 cudaError_t token_logprobs(const LogprobArgs& a, int type, cudaStream_t s) {
-    return type == ELEM_F32 ? launch<float>(a, s) : type == ELEM_F16 ? launch<__half>(a, s) : launch<__nv_bfloat16>(a, s);
+    return type == ELEM_F32 ? logprobs_type<float>(a, s)
+                            : type == ELEM_F16 ? logprobs_type<__half>(a, s) : logprobs_type<__nv_bfloat16>(a, s);
 }
 
 }  // namespace krk
