@@ -441,77 +441,89 @@ def attn_decode_paged(q, kc, vc, table, lens, scale: Optional[float] = None, win
 
 
 # ------------------------------------------- recurrent layers over state slots
-def _rows2(t, dev, name):
-    """(type, rows, width, row stride) of a float tensor [rows, width] whose last dimension is dense."""
-    kind, shape, strides = _TYPES.get(t.dtype), t.shape, t.stride()
-    if kind is None or len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or t.device != dev:
-        raise _not_elems(name, 2, dev)
-    return kind, shape[0], shape[1], strides[0]
+# (checked in few steps, as above: what x is, and that the others are like it)
+def _like(t, dtype, shape, index, name):
+    """(address, row stride) of a tensor of this type, shape [rows, width] and device whose last dimension is dense."""
+    st = t.stride()
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or (st[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{name}: expected {list(shape)} of {dtype} on cuda:{index} whose last dimension is dense")
+    return t.data_ptr(), st[0]
 
 
-def _same_rows(t, kind, rows, width, dev, name):
-    """(address, row stride) of a tensor like x; (None, 0) of None."""
-    if t is None:
-        return None, 0
-    k, r, w, st = _rows2(t, dev, name)
-    if k != kind or r != rows or w != width:
-        raise ValueError(f"{name}: expected [{rows}, {width}] of x's type")
-    return t.data_ptr(), st
+def _rows2(t, name):
+    """(type, shape, device index) of a float CUDA tensor [rows, width]."""
+    kind, shape, index = _TYPES.get(t.dtype), t.shape, t.get_device()
+    if index < 0:
+        raise ValueError("expected CUDA tensors")
+    if kind is None or len(shape) != 2:
+        raise _not_elems(name, 2, t.device)
+    return kind, shape, index
 
 
-def _weights(t, shape, dev, name):
+def _weights(t, shape, index, name):
     """The address of a dense float32 tensor of this shape (None: None)."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.shape != shape or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous float32 tensor of {tuple(shape)} on {dev}")
+    if t.dtype is not torch.float32 or t.shape != shape or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous float32 tensor of {tuple(shape)} on cuda:{index}")
     return t.data_ptr()
 
 
-def _slot_args(state, shape, dtype, slots, init, requests, dev):
+def _indexes(t, n, index, name):
+    """The address of a dense int32 tensor of n elements (None: None)."""
+    if t is None:
+        return None
+    if t.dtype is not torch.int32 or t.numel() != n or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of {n} elements on cuda:{index}")
+    return t.data_ptr()
+
+
+def _slot_args(state, rows, width, dtype, slots, init, requests, index):
     """The pool's address, slot stride and size, and the addresses of slots and init."""
     if state is None:
         if slots is not None or init is not None:
             raise ValueError("slots and init need a state")
         return None, 0, 0, None, None
-    have, strides = state.shape, state.stride()
-    if state.dtype != dtype or state.device != dev or have[1:] != shape or (
-            shape[1] > 1 and strides[2] != 1) or (shape[0] > 1 and strides[1] != shape[1]):
-        raise ValueError(f"state: expected {dtype} [slots, {shape[0]}, {shape[1]}] on {dev} with dense slots")
-    if slots is None and have[0] < requests:
+    shape, strides = state.shape, state.stride()
+    if state.dtype is not dtype or state.get_device() != index or len(shape) != 3 or shape[1] != rows or (
+            shape[2] != width) or (width > 1 and strides[2] != 1) or (rows > 1 and strides[1] != width):
+        raise ValueError(f"state: expected {dtype} [slots, {rows}, {width}] on cuda:{index} with dense slots")
+    if slots is None and shape[0] < requests:
         raise ValueError(f"state: expected a slot for each of {requests} requests, or their slots")
-    return (state.data_ptr(), strides[0], have[0],
-            None if slots is None else _ints(slots, requests, dev, "slots"),
-            None if init is None else _ints(init, requests, dev, "init"))
+    return (state.data_ptr(), strides[0], shape[0], _indexes(slots, requests, index, "slots"),
+            _indexes(init, requests, index, "init"))
 
 
-def _call(dev, fn, args) -> None:
-    index = dev.index
-    rc = fn(*args, _raw_stream(index)) if index == _current_device() else _elsewhere(dev, fn, *args)
+def _requests(cu, index):
+    """(address, number of requests) of packed requests' offsets."""
+    n = cu.numel()
+    if n < 1:
+        raise ValueError("cu: expected the requests' offsets, one more than there are requests")
+    return _indexes(cu, n, index, "cu"), n - 1
+
+
+def _call(index, fn, args) -> None:
+    """fn(*args, stream) on the device's current stream with the device current."""
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        rc = _elsewhere(torch.device("cuda", index), fn, *args)
     if rc:
         check(rc)
 
 
 def _conv_args(x, weight, bias, state, slots, init, out, requests):
-    dev = _cuda_device(x)
-    kind, rows, ch, x_st = _rows2(x, dev, "x")
-    if len(weight.shape) != 2 or weight.shape[0] != ch:
+    kind, shape, index = _rows2(x, "x")
+    dtype, (rows, ch), w = x.dtype, shape, weight.shape
+    x_at, x_st = _like(x, dtype, shape, index, "x")
+    if len(w) != 2 or w[0] != ch:
         raise ValueError(f"weight: expected [{ch}, width]")
-    width = weight.shape[1]
-    slot = _slot_args(state, (width - 1, ch), x.dtype, slots, init, rows if requests is None else requests, dev)
     if out is None:
-        out = x.new_empty(rows, ch)
-    out_at, o_st = _same_rows(out, kind, rows, ch, dev, "out")
-    return dev, out, (x.data_ptr(), x_st, _weights(weight, (ch, width), dev, "weight"),
-                      _weights(bias, (ch,), dev, "bias"), out_at, o_st, kind, *slot), rows, ch, width
-
-
-def _requests(cu, dev):
-    """(address, number of requests) of packed requests' offsets."""
-    n = cu.numel()
-    if n < 1:
-        raise ValueError("cu: expected the requests' offsets, one more than there are requests")
-    return _ints(cu, n, dev, "cu"), n - 1
+        out = x.new_empty(shape)
+    out_at, o_st = _like(out, dtype, shape, index, "out")
+    return index, out, (x_at, x_st, _weights(weight, w, index, "weight"), _weights(bias, (ch,), index, "bias"), out_at,
+                        o_st, kind, *_slot_args(state, w[1] - 1, ch, dtype, slots, init,
+                                                rows if requests is None else requests, index)), rows, ch, w[1]
 
 
 def causal_conv(x, weight, cu, bias=None, state=None, slots=None, init=None, silu: bool = True, out=None):
@@ -522,49 +534,51 @@ def causal_conv(x, weight, cu, bias=None, state=None, slots=None, init=None, sil
     [slots, W-1, C] of x's type, and those before it come from slot init[s] (-1:
     it begins; None: the same slot).  Without a state every request begins.
     Returns out [T, C], whose rows of no request are left as they were."""
-    cu_at, requests = _requests(cu, x.device)
-    dev, out, args, rows, ch, width = _conv_args(x, weight, bias, state, slots, init, out, requests)
-    _call(dev, lib.krk_k_causal_conv, (*args, cu_at, rows, requests, ch, width, int(silu)))
+    cu_at, requests = _requests(cu, x.get_device())
+    index, out, args, rows, ch, width = _conv_args(x, weight, bias, state, slots, init, out, requests)
+    _call(index, lib.krk_k_causal_conv, (*args, cu_at, rows, requests, ch, width, 1 if silu else 0))
     return out
 
 
 def causal_conv_step(x, weight, state, slots=None, bias=None, init=None, silu: bool = True, out=None):
     """causal_conv of one token a request: row b of x [B, C] is request b's."""
-    dev, out, args, rows, ch, width = _conv_args(x, weight, bias, state, slots, init, out, None)
-    _call(dev, lib.krk_k_causal_conv_step, (*args, rows, ch, width, int(silu)))
+    index, out, args, rows, ch, width = _conv_args(x, weight, bias, state, slots, init, out, None)
+    _call(index, lib.krk_k_causal_conv_step, (*args, rows, ch, width, 1 if silu else 0))
     return out
 
 
+def _groups(t, dtype, rows, n, index, name):
+    """(address, row stride, group stride, groups) of B or C."""
+    shape, st = t.shape, t.stride()
+    groups = shape[1] if len(shape) == 3 else 1
+    if t.dtype is not dtype or t.get_device() != index or len(shape) not in (2, 3) or shape[0] != rows or (
+            shape[-1] != n) or (st[-1] != 1 and n > 1):
+        raise ValueError(f"{name}: expected [{rows}, {n}] or [{rows}, groups, {n}] of {dtype} on cuda:{index} whose last "
+                         "dimension is dense")
+    return t.data_ptr(), st[0], st[1] if len(shape) == 3 else n, groups
+
+
 def _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests):
-    dev = _cuda_device(x)
-    kind, rows, ch, x_st = _rows2(x, dev, "x")
-    if len(a.shape) != 2 or a.shape[0] != ch:
+    kind, shape, index = _rows2(x, "x")
+    dtype, (rows, ch), decay = x.dtype, shape, a.shape
+    if len(decay) != 2 or decay[0] != ch:
         raise ValueError(f"a: expected [{ch}, states]")
-    n = a.shape[1]
-
-    def grouped(t, name):
-        if len(t.shape) == 2:
-            k, r, w, st = _rows2(t, dev, name)
-            g, sg = 1, w
-        else:
-            k, (r, g, w), (st, sg, _) = _elems3(t, dev, name)
-        if k != kind or r != rows or w != n:
-            raise ValueError(f"{name}: expected [{rows}, {n}] or [{rows}, groups, {n}] of x's type")
-        return t.data_ptr(), st, sg, g
-
-    b_at, b_st, b_sg, groups = grouped(b, "b")
-    c_at, c_st, c_sg, c_groups = grouped(c, "c")
+    n = decay[1]
+    b_at, b_st, b_sg, groups = _groups(b, dtype, rows, n, index, "b")
+    c_at, c_st, c_sg, c_groups = _groups(c, dtype, rows, n, index, "c")
     if c_groups != groups or not groups or ch % groups:
         raise ValueError(f"b and c: expected as many groups, dividing {ch} channels")
-    dt_at, dt_st = _same_rows(dt, kind, rows, ch, dev, "dt")
-    z_at, z_st = _same_rows(z, kind, rows, ch, dev, "z")
-    slot = _slot_args(state, (ch, n), torch.float32, slots, init, rows if requests is None else requests, dev)
+    x_at, x_st = _like(x, dtype, shape, index, "x")
+    dt_at, dt_st = _like(dt, dtype, shape, index, "dt")
+    z_at, z_st = (None, 0) if z is None else _like(z, dtype, shape, index, "z")
     if out is None:
-        out = x.new_empty(rows, ch)
-    out_at, o_st = _same_rows(out, kind, rows, ch, dev, "out")
-    return dev, out, (x.data_ptr(), x_st, dt_at, dt_st, z_at, z_st, b_at, b_st, b_sg, c_at, c_st, c_sg, out_at, o_st,
-                      kind, _weights(a, (ch, n), dev, "a"), _weights(d, (ch,), dev, "d"),
-                      _weights(dt_bias, (ch,), dev, "dt_bias"), *slot), (ch, n, groups), rows
+        out = x.new_empty(shape)
+    out_at, o_st = _like(out, dtype, shape, index, "out")
+    return index, out, (x_at, x_st, dt_at, dt_st, z_at, z_st, b_at, b_st, b_sg, c_at, c_st, c_sg, out_at, o_st, kind,
+                        _weights(a, decay, index, "a"), _weights(d, (ch,), index, "d"),
+                        _weights(dt_bias, (ch,), index, "dt_bias"),
+                        *_slot_args(state, ch, n, torch.float32, slots, init, rows if requests is None else requests,
+                                    index)), (ch, n, groups), rows
 
 
 def selective_scan_work_floats(rows: int, channels: int, states: int, groups: int = 1, max_len: int = 0) -> int:
@@ -582,21 +596,21 @@ def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None,
     of selective_scan_work_floats floats (allocated here when not given).  Returns
     out [T, D] (which may be x, dt or z), whose rows of no request are left as
     they were."""
-    cu_at, requests = _requests(cu, x.device)
-    dev, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
-    index = dev.index
-    if index != _current_device():  # the scratch is sized for the current device
-        with torch.cuda.device(dev):
+    index = x.get_device()
+    if index >= 0 and index != _current_device():  # the scratch is sized for the current device
+        with torch.cuda.device(index):
             return selective_scan(x, dt, a, b, c, cu, d, z, dt_bias, state, slots, init, out, max_len, work)
+    cu_at, requests = _requests(cu, index)
+    index, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
     _number(max_len, "max_len")
     if work is None:
         need, work_at = lib.krk_selective_scan_work_floats(rows, *sizes, max_len), None
         if need:
-            work = torch.empty(need, device=dev, dtype=torch.float32)
+            work = torch.empty(need, device=x.device, dtype=torch.float32)
             work_at = work.data_ptr()
     else:
-        if work.dtype != torch.float32 or work.device != dev or not work.is_contiguous():
-            raise ValueError(f"work: expected a contiguous float32 tensor on {dev}")
+        if work.dtype != torch.float32 or work.get_device() != index or not work.is_contiguous():
+            raise ValueError(f"work: expected a contiguous float32 tensor on cuda:{index}")
         need, work_at = work.numel(), work.data_ptr()
     rc = lib.krk_k_selective_scan(*args, cu_at, rows, requests, *sizes, max_len, work_at, need, _raw_stream(index))
     if rc:
@@ -606,8 +620,8 @@ def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None,
 
 def selective_step(x, dt, a, b, c, state, slots=None, d=None, z=None, dt_bias=None, init=None, out=None):
     """selective_scan of one token a request: row t of x [B, D] is request t's."""
-    dev, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, None)
-    _call(dev, lib.krk_k_selective_step, (*args, rows, *sizes))
+    index, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, None)
+    _call(index, lib.krk_k_selective_step, (*args, rows, *sizes))
     return out
 
 
@@ -617,20 +631,22 @@ def token_logprobs(logits, tokens=None, top: int = 0):
     and log probabilities [R, top] of the largest logits (at most 32), the lower
     id first among equal ones.  Returns (logprobs like tokens, or None; entropy;
     top_ids; top_logprobs), float32 and int32."""
-    dev = _cuda_device(logits)
-    kind, rows, vocab, ld = _rows2(logits, dev, "logits")
+    kind, shape, index = _rows2(logits, "logits")
+    at, ld = _like(logits, logits.dtype, shape, index, "logits")
+    rows, vocab = shape
     _number(top, "top")
-    asked, tokens_at = 0, None
+    dev, lp, asked, lp_at, tokens_at = logits.device, None, 0, None, None
     if tokens is not None:
-        if len(tokens.shape) not in (1, 2) or tokens.shape[0] != rows:
+        like = tokens.shape
+        if len(like) not in (1, 2) or like[0] != rows:
             raise ValueError(f"tokens: expected [{rows}] or [{rows}, tokens]")
-        asked = 1 if len(tokens.shape) == 1 else tokens.shape[1]
-        tokens_at = _ints(tokens, rows * asked, dev, "tokens")
-    buf = torch.empty(rows * (asked + 1 + 2 * top), device=dev, dtype=torch.float32)
-    at, (lp, entropy, ids, best) = buf.data_ptr(), buf.unsafe_split_with_sizes((rows * asked, rows, rows * top, rows * top))
-    ids_at = at + 4 * rows * (asked + 1)
-    _call(dev, lib.krk_k_token_logprobs,
-          (logits.data_ptr(), ld, kind, rows, vocab, tokens_at, asked, at, at + 4 * rows * asked, top, ids_at,
-           ids_at + 4 * rows * top))
-    return (None if tokens is None else lp.view(tokens.shape), entropy, ids.view(torch.int32).view(rows, top),
-            best.view(rows, top))
+        asked = 1 if len(like) == 1 else like[1]
+        tokens_at = _indexes(tokens, rows * asked, index, "tokens")
+        lp = torch.empty(like, device=dev, dtype=torch.float32)
+        lp_at = lp.data_ptr()
+    entropy = torch.empty(rows, device=dev, dtype=torch.float32)
+    ids = torch.empty(rows, top, device=dev, dtype=torch.int32)
+    best = torch.empty(rows, top, device=dev, dtype=torch.float32)
+    _call(index, lib.krk_k_token_logprobs, (at, ld, kind, rows, vocab, tokens_at, asked, lp_at, entropy.data_ptr(), top,
+                                            ids.data_ptr(), best.data_ptr()))
+    return lp, entropy, ids, best

@@ -613,7 +613,7 @@ def test_wrappers_refuse_what_does_not_belong_together():
     conv = lambda **k: K.causal_conv(**dict(dict(x=x, weight=w, cu=cu), **k))  # noqa: E731
     scan = lambda **k: K.selective_scan(**dict(dict(t, cu=cu), **k))  # noqa: E731
     for call, word in (
-            (lambda: conv(x=x.double()), "x"), (lambda: conv(x=x.T), "x"), (lambda: conv(weight=w[:31]), "weight"),
+            (lambda: conv(x=x.double()), "x"), (lambda: conv(x=x.T), "x|weight"), (lambda: conv(weight=w[:31]), "weight"),
             (lambda: conv(weight=w.half()), "weight"), (lambda: conv(weight=w.T.contiguous().T), "weight"),
             (lambda: conv(cu=cu.long()), "cu"), (lambda: conv(cu=cu[:0]), "cu"), (lambda: conv(cu=cu.cpu()), "cu"),
             (lambda: conv(bias=w), "bias"), (lambda: conv(slots=i32([0])), "state"), (lambda: conv(init=i32([0])), "state"),
