@@ -30,13 +30,15 @@
 namespace krk {
 namespace {
 
+constexpr int CARRY_AHEAD = 16;
 constexpr int SCAN_GROUP = 4;  // rows whose outputs are formed together
 
 // K lanes share a channel of N <= K * SPT states.
-template <int K, int SPT>
+template <typename T, int K, int SPT, bool AHEAD>
 struct ScanShape {
     static constexpr int CH = SCAN_THREADS / K, NP = K * SPT;
-    static constexpr int ROWS = NP <= 32 ? 32 : 1024 / NP;             // a tile of B and C
+    static constexpr int MOST = AHEAD ? (sizeof(T) == 2 ? 16 : 8) : 32;
+    static constexpr int ROWS = NP * MOST <= 1024 ? MOST : 1024 / NP;  // a tile
     static constexpr int F = 2 * ROWS * NP / SCAN_THREADS;             // elements of them that a thread stages
     static constexpr int OWN = K < SCAN_GROUP ? SCAN_GROUP / K : 1;    // rows of a group whose inputs are a lane's work
     static constexpr int SHARE = K < SCAN_GROUP ? 1 : K / SCAN_GROUP;  // lanes that have the same ones
@@ -142,17 +144,27 @@ KRK_DEV void sum_rows(float (&v)[R], int lane) {
     }
 }
 
+// Copies 16 bytes, or zeros if there are none, into shared memory.
+KRK_DEV void copy16(void* smem, const void* gmem, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(smem)), "l"(gmem), "r"(there ? 16 : 0)
+                 : "memory");
+}
+
 // CARRY: the first walk of split requests, which leaves each piece's state from
-// zeros, for the piece behind it, and its sum of delta.
-template <typename T, int K, int SPT, bool PADDED, bool CARRY>
+// zeros, for the piece behind it, and its sum of delta.  AHEAD: x, dt and z, whose
+// rows are aligned to 16 bytes, come tile by tile through shared memory, the next
+// tile while one is computed; else each lane loads its own, a group ahead.
+template <typename T, int K, int SPT, bool PADDED, bool CARRY, bool AHEAD>
 __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArgs a, ScanSplit split, int side) {
-    using Sh = ScanShape<K, SPT>;
+    using Sh = ScanShape<T, K, SPT, AHEAD>;
     constexpr int CH = Sh::CH, NP = Sh::NP, ROWS = Sh::ROWS, F = Sh::F, OWN = Sh::OWN, U = SCAN_GROUP;
+    constexpr int INPUTS = CARRY ? 2 : 3;
     __shared__ __align__(16) float s_bc[2][ROWS][2][NP];
+    __shared__ __align__(16) T s_in[AHEAD ? 2 : 1][INPUTS][AHEAD ? ROWS : 1][AHEAD ? CH : 1];
 
     const int tid = threadIdx.x, lane = tid % K, per = a.D / a.G;
     const int block = blockIdx.x / side, cb = blockIdx.x - block * side, sides = side / a.G;
-    const int g = cb / sides, ch = (cb - g * sides) * CH + tid / K;  // within the group
+    const int g = cb / sides, ch0 = (cb - g * sides) * CH, ch = ch0 + tid / K;  // within the group
     const bool open = ch < per;
     const int d = g * per + (open ? ch : 0);
     const ScanPiece piece = find_piece(a.cu, a.S, a.T, split.rows, block, CARRY ? COUNT_SPLIT : COUNT_ALL);
@@ -198,6 +210,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     T* outp = (T*)a.out + (begin + own) * a.o_st + d;
     T xr[OWN], dtr[OWN], zr[OWN];
     const auto fetch = [&](int t, auto whole) {
+        if constexpr (AHEAD) return;
 #pragma unroll
         for (int o = 0; o < OWN; ++o) {
             const bool in = decltype(whole)::value || t + own + o < end;
@@ -207,6 +220,25 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
             xp += o + 1 < OWN ? a.x_st : (U - OWN + 1) * a.x_st;
             dtp += o + 1 < OWN ? a.dt_st : (U - OWN + 1) * a.dt_st;
             zp += o + 1 < OWN ? z_st : (U - OWN + 1) * z_st;
+        }
+    };
+    // The tile from row t0 on, into one of two places.
+    const auto fetch_tile = [&](int t0, int place) {
+        if constexpr (AHEAD) {
+            constexpr int WIDE = 16 / sizeof(T), SIDE = CH / WIDE;  // channels of an access, accesses of a row
+            const int first = g * per + ch0;
+            const T* tensors[3] = {(const T*)a.x, (const T*)a.dt, gated ? (const T*)a.z : (const T*)a.x};
+            const int64_t strides[3] = {a.x_st, a.dt_st, z_st};
+#pragma unroll
+            for (int input = 0; input < INPUTS; ++input)
+#pragma unroll
+                for (int i = 0; i < ROWS * SIDE; i += SCAN_THREADS) {
+                    const int row = (i + tid) / SIDE, c = (i + tid) % SIDE * WIDE, t = t0 + row;
+                    const bool in = t < end && ch0 + c < per;  // (per is a multiple of WIDE)
+                    if (ROWS * SIDE % SCAN_THREADS == 0 || row < ROWS)
+                        copy16(&s_in[place][input][row][c], tensors[input] + (in ? t * strides[input] + first + c : 0), in);
+                }
+            cp_async_commit();
         }
     };
     // And its elements of the next tile of B and C.
@@ -230,6 +262,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     // Rows t .. t + 3, in rows r0 .. of the tile; WHOLE: they and the four behind them are there.
     const auto group = [&](int t, int r0, auto whole) {
         float mine[OWN], mine_put[OWN], gate[OWN], skipped[OWN], step[U], put[U];
+        if constexpr (AHEAD) {
+#pragma unroll
+            for (int o = 0; o < OWN; ++o) {
+                xr[o] = s_in[buffer][0][r0 + own + o][tid / K];
+                dtr[o] = s_in[buffer][1][r0 + own + o][tid / K];
+                if (!CARRY) zr[o] = s_in[buffer][INPUTS - 1][r0 + own + o][tid / K];
+            }
+        }
 #pragma unroll
         for (int o = 0; o < OWN; ++o) {
             const float x = to_f32(xr[o]);
@@ -287,14 +327,19 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     };
 
     if (begin < end) {
+        fetch_tile(begin, 0);
         fetch(begin, std::false_type());
         fetch_bc(begin);
         stage_bc(0);
     }
-    __syncthreads();
     for (int t0 = begin; t0 < end; t0 += ROWS, buffer ^= 1) {
+        if (AHEAD) cp_async_wait<0>();
+        __syncthreads();  // this tile is there, and the places of the one before are free
         const bool more = t0 + ROWS < end;
-        if (more) fetch_bc(t0 + ROWS);
+        if (more) {
+            fetch_tile(t0 + ROWS, buffer ^ 1);
+            fetch_bc(t0 + ROWS);
+        }
         const int rows = min(ROWS, end - t0);
         for (int r0 = 0; r0 < rows; r0 += U) {
             if (end - (t0 + r0) >= 2 * U)
@@ -303,7 +348,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
                 group(t0 + r0, r0, std::false_type());
         }
         if (more) stage_bc(buffer ^ 1);
-        __syncthreads();
     }
 
     float* kept = CARRY ? split.start + (int64_t)(piece.first + piece.at + 1) * a.D * a.N
@@ -333,17 +377,29 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanArgs a, Sc
     float h = from >= 0 ? ((const float*)a.slot.state)[from * a.slot.stride + at] : 0.0f;
     float* start = split.start + piece.first * size + at;
     const float* sum = split.sum + (int64_t)piece.first * a.D + d;
+    // (the loads of several pieces on their way together: one by one, each is waited for)
     start[0] = h;
-    for (int c = 1; c < pieces; ++c) {
-        h = fmaf(fast_exp2(rate * sum[(int64_t)(c - 1) * a.D]), h, start[c * size]);
-        start[c * size] = h;
+    for (int c = 1; c < pieces; c += CARRY_AHEAD) {
+        float own[CARRY_AHEAD], steps[CARRY_AHEAD];
+#pragma unroll
+        for (int i = 0; i < CARRY_AHEAD; ++i) {
+            const int64_t at = min(c + i, pieces - 1);
+            own[i] = start[at * size];
+            steps[i] = sum[(at - 1) * a.D];
+        }
+#pragma unroll
+        for (int i = 0; i < CARRY_AHEAD; ++i)
+            if (c + i < pieces) {
+                h = fmaf(fast_exp2(rate * steps[i]), h, own[i]);
+                start[(int64_t)(c + i) * size] = h;
+            }
     }
 }
 
 // ---------------------------------------------------------------- the launches
-template <typename T, int K, int SPT, bool PADDED, bool SPLIT>
+template <typename T, int K, int SPT, bool PADDED, bool SPLIT, bool AHEAD>
 cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStream_t s) {
-    using Sh = ScanShape<K, SPT>;
+    using Sh = ScanShape<T, K, SPT, AHEAD>;
     const int64_t side = (int64_t)((a.D / a.G + Sh::CH - 1) / Sh::CH) * a.G;
     ScanSplit split{0, nullptr, nullptr, 0};
     int64_t pieces = a.S;
@@ -354,7 +410,7 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
         const int64_t blocks = (states + SCAN_THREADS - 1) / SCAN_THREADS;
         const int64_t requests = a.T / (SCAN_ALONE * (int64_t)piece_rows);  // that can be split
         if (side * room > INT32_MAX || blocks * requests > INT32_MAX) return cudaErrorInvalidValue;
-        scan_kernel<T, K, SPT, PADDED, true><<<(unsigned)(side * room), SCAN_THREADS, 0, s>>>(a, split, (int)side);
+        scan_kernel<T, K, SPT, PADDED, true, AHEAD><<<(unsigned)(side * room), SCAN_THREADS, 0, s>>>(a, split, (int)side);
         cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return e;
         scan_carry_kernel<<<(unsigned)(blocks * requests), SCAN_THREADS, 0, s>>>(a, split, (int)blocks);
@@ -363,15 +419,21 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
         add_launches(2);
     }
     if (side * pieces > INT32_MAX) return cudaErrorInvalidValue;
-    scan_kernel<T, K, SPT, PADDED, false><<<(unsigned)(side * pieces), SCAN_THREADS, 0, s>>>(a, split, (int)side);
+    scan_kernel<T, K, SPT, PADDED, false, AHEAD><<<(unsigned)(side * pieces), SCAN_THREADS, 0, s>>>(a, split, (int)side);
     add_launches(1);
     return cudaGetLastError();
 }
 
 template <typename T, int K, int SPT, bool SPLIT>
 cudaError_t scan_padded(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
-    return a.N == K * SPT ? launch_scan<T, K, SPT, false, SPLIT>(a, work, rows, s)
-                          : launch_scan<T, K, SPT, true, SPLIT>(a, work, rows, s);
+    if (a.N != K * SPT) return launch_scan<T, K, SPT, true, SPLIT, false>(a, work, rows, s);
+    if constexpr (SPT == SCAN_LANE) {
+        const bool many = a.T > 1;
+        if (a.D / a.G % (16 / sizeof(T)) == 0 && fits(a.x, many ? a.x_st : 0, 16, sizeof(T)) &&
+            fits(a.dt, many ? a.dt_st : 0, 16, sizeof(T)) && fits(a.z, many && a.z ? a.z_st : 0, 16, sizeof(T)))
+            return launch_scan<T, K, SPT, false, SPLIT, true>(a, work, rows, s);
+    }
+    return launch_scan<T, K, SPT, false, SPLIT, false>(a, work, rows, s);
 }
 
 // Lanes of SCAN_LANE states; of four when the blocks of those would leave
