@@ -154,7 +154,7 @@ int krk_k_token_logprobs(void* logits, int64_t ld, int type, int R, int V, const
     const char* who = "token_logprobs";
     const int es = elem_size(type);
     if (!es) return invalid(who, "unknown element type");
-    if (R < 0 || V < 1 || K < 0) return invalid(who, "R and K must not be negative, V positive");
+    if (R < 0 || V < 1 || V > (1 << 30) || K < 0) return invalid(who, "R and K must not be negative, V 1 to 2^30");
     if (top < 0 || top > krk::LOGPROBS_MAX_TOP || top > V) return invalid(who, "top must be 0 to 32 and at most V");
     if (R == 0) return KRK_OK;
     if (!logits || !aligned(logits, es)) return invalid(who, "logits must be set and aligned to their elements");

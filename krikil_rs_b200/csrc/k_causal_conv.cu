@@ -150,29 +150,49 @@ KRK_DEV int requests_before(const int32_t* cu, int S, int r) {
 // A block takes `rows` packed rows of CONV_THREADS * V channels, and the
 // requests that begin there: it keeps their states, and computes their first
 // W-1 rows even past its own, so that whatever reads a request's old state is
-// the thread that writes the new one.
+// the thread that writes the new one.  Requests without rows, of which there may
+// be any number in one place, are left to blocks of their own, 32 for each.
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(CONV_THREADS) conv_kernel(ConvArgs a, int rows, int side) {
+__global__ void __launch_bounds__(CONV_THREADS) conv_kernel(ConvArgs a, int rows, int chunks, int side) {
     __shared__ Pack<T, V> ring[CONV_AHEAD][CONV_THREADS];
     const int chunk = blockIdx.x / side, c = ((blockIdx.x - chunk * side) * CONV_THREADS + threadIdx.x) * V;
+    const bool open = c < a.C;
+    const ConvColumn<T, W, V> col(a, open ? c : 0);
+    int to, from;
+    if (chunk >= chunks) {
+        const int s0 = (chunk - chunks) * 32, s = s0 + (threadIdx.x & 31);
+        bool idle = false;
+        if (s < a.S) {
+            const Span span = request_rows(a.cu, s, a.T);
+            idle = span.begin == span.end && request_slots(a.slot, s, to, from) && to >= 0 && to != from;
+        }
+        for (unsigned left = __ballot_sync(0xffffffffu, idle); left; left &= left - 1) {
+            const int i = s0 + __ffs(left) - 1;
+            if (open && request_slots(a.slot, i, to, from)) col.keep({0, 0}, to, from);
+        }
+        return;
+    }
     const int r0 = chunk * rows;
-    const bool last = r0 >= a.T - rows;
+    const bool last = chunk == chunks - 1;
     const int r1 = last ? a.T : r0 + rows;
     int s = chunk == 0 ? 0 : requests_before(a.cu, a.S, r0);
-    if (c >= a.C) return;
-    const ConvColumn<T, W, V> col(a, c);
-    int to, from;
     if (s > 0) {
         const Span span = request_rows(a.cu, s - 1, a.T);
-        if (span.end > r0 && request_slots(a.slot, s - 1, to, from))
+        if (open && span.end > r0 && request_slots(a.slot, s - 1, to, from))
             col.run(max(r0, min(span.begin + W - 1, span.end)), min(span.end, r1), span.begin, from, ring);
     }
-    for (; s < a.S; ++s) {
+    while (s < a.S) {
         const Span span = request_rows(a.cu, s, a.T);
         if (!last && span.begin >= r1) break;
-        if (!request_slots(a.slot, s, to, from)) continue;
-        col.run(span.begin, min(span.end, max(r1, span.begin + W - 1)), span.begin, from, ring);
-        col.keep(span, to, from);
+        if (span.begin == span.end) {  // on to the one that has this place's row
+            s = max(s + 1, requests_before(a.cu + 1, a.S, span.begin + 1));
+            continue;
+        }
+        if (open && request_slots(a.slot, s, to, from)) {
+            col.run(span.begin, min(span.end, max(r1, span.begin + W - 1)), span.begin, from, ring);
+            col.keep(span, to, from);
+        }
+        ++s;
     }
 }
 
@@ -222,9 +242,10 @@ cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
     } else {
         const int64_t share = (int64_t)a.T * side / (sms * 16);
         const int rows = share < 8 ? 8 : share > 64 ? 64 : (int)share;
-        const int64_t blocks = (int64_t)(a.T > 0 ? (a.T + (int64_t)rows - 1) / rows : 1) * side;
+        const int64_t chunks = a.T > 0 ? (a.T + (int64_t)rows - 1) / rows : 1;
+        const int64_t blocks = (chunks + (a.slot.state ? (a.S + 31LL) / 32 : 0)) * side;
         if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-        conv_kernel<T, W, V><<<(unsigned)blocks, CONV_THREADS, 0, s>>>(a, rows, side);
+        conv_kernel<T, W, V><<<(unsigned)blocks, CONV_THREADS, 0, s>>>(a, rows, (int)chunks, side);
     }
     add_launches(1);
     return cudaGetLastError();

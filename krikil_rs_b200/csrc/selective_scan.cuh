@@ -53,49 +53,45 @@ struct ScanSplit {
 };
 KRK_DEV int scan_pieces(int n, int rows) { return rows > 0 && n > (int64_t)SCAN_ALONE * rows ? (n - 1) / rows + 1 : 1; }
 
-// The requests' order of turns: the longest first (of equal ones the first), so
-// that what is left when most blocks have ended is short; for more requests than
-// a block has threads, their own.  Returns whether `order` holds it.
-KRK_DEV bool longest_first(const int32_t* cu, int S, int T, int (&order)[SCAN_THREADS]) {
-    if (S < 2 || S > SCAN_THREADS) return false;
-    __shared__ int rows[SCAN_THREADS];
+// A request's turn among all: the longest first (of equal ones the first), so
+// that what is left when most blocks have ended is short; of more requests than a
+// block has threads, their own.
+KRK_DEV int request_of_turn(const int32_t* cu, int S, int T, int turn) {
+    if (S < 2 || S > SCAN_THREADS) return turn;
+    __shared__ int rows[SCAN_THREADS], found;
     const int s = threadIdx.x;
     const int mine = s < S ? clamp_row(cu[s + 1], T) - clamp_row(cu[s], T) : INT_MIN;
     rows[s] = mine;
     __syncthreads();
     int place = 0;
     for (int i = 0; i < S; ++i) place += rows[i] > mine || (rows[i] == mine && i < s);
-    if (s < S) order[place] = s;
+    if (s < S && place == turn) found = s;
     __syncthreads();
-    return true;
+    return found;
 }
 
-// The piece-th piece of all requests' (or of the split ones' alone, or of those
-// each one's first): its request, its place there, and the place of the
-// request's first one among the split ones'.  request < 0: there are not so many.
+// The piece-th piece of the requests that are split: its request, its place
+// there, and the place of the request's first one among all; FIRST: the piece-th
+// such request's first piece.  request < 0: there are not so many.
 struct ScanPiece {
     int request, at, first;
 };
-enum ScanCount { COUNT_ALL, COUNT_SPLIT, COUNT_FIRST };
-KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piece, ScanCount count) {
+template <bool FIRST>
+KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piece) {
     __shared__ int warp_sum[2][SCAN_THREADS / 32];
     __shared__ ScanPiece found;
-    __shared__ int order[SCAN_THREADS];
-    const bool ordered = longest_first(cu, S, T, order);
-    if (rows == 0) return {ordered ? order[piece] : piece, 0, 0};  // a piece a request
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int before = 0, before_split = 0;
+    int before = 0, places = 0;  // of the requests so far: what is counted, and their pieces
     if (tid == 0) found.request = -1;
     __syncthreads();
     for (int s0 = 0; s0 < S; s0 += SCAN_THREADS) {
-        int s = s0 + tid, n = 0, m = 0;
+        const int s = s0 + tid;
+        int m = 0;
         if (s < S) {
-            if (ordered) s = order[s];
-            const int begin = clamp_row(cu[s], T), end = clamp_row(cu[s + 1], T);
-            n = scan_pieces(end - begin, rows);
-            m = n > 1 ? n : 0;
-            if (count != COUNT_ALL) n = count == COUNT_SPLIT ? m : m > 0;
+            m = scan_pieces(clamp_row(cu[s + 1], T) - clamp_row(cu[s], T), rows);
+            if (m == 1) m = 0;
         }
+        const int n = FIRST ? m > 0 : m;
         int x = n, y = m;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -104,17 +100,17 @@ KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piec
         }
         if (lane == 31) warp_sum[0][warp] = x, warp_sum[1][warp] = y;
         __syncthreads();
-        int all = 0, all_split = 0;
+        int all = 0, all_places = 0;
 #pragma unroll
         for (int w = 0; w < SCAN_THREADS / 32; ++w) {
-            if (w == warp) x += all, y += all_split;
+            if (w == warp) x += all, y += all_places;
             all += warp_sum[0][w];
-            all_split += warp_sum[1][w];
+            all_places += warp_sum[1][w];
         }
         const int at = piece - before - (x - n);
-        if (at >= 0 && at < n) found = {s, at, before_split + y - m};
+        if (at >= 0 && at < n) found = {s, at, places + y - m};
         before += all;
-        before_split += all_split;
+        places += all_places;
         __syncthreads();
         if (found.request >= 0) break;
     }
@@ -167,14 +163,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     const int g = cb / sides, ch0 = (cb - g * sides) * CH, ch = ch0 + tid / K;  // within the group
     const bool open = ch < per;
     const int d = g * per + (open ? ch : 0);
-    const ScanPiece piece = find_piece(a.cu, a.S, a.T, split.rows, block, CARRY ? COUNT_SPLIT : COUNT_ALL);
+    // (blocks for the pieces that there is room for come before those for a request each)
+    const ScanPiece piece = block < split.room ? find_piece<false>(a.cu, a.S, a.T, split.rows, block)
+                                               : ScanPiece{request_of_turn(a.cu, a.S, a.T, block - split.room), 0, 0};
     if (piece.request < 0) return;
     const Span span = request_rows(a.cu, piece.request, a.T);
     int to, from;
     if (!request_slots(a.slot, piece.request, to, from)) return;
     const int pieces = scan_pieces(span.end - span.begin, split.rows);
     const bool last = piece.at == pieces - 1;
-    if (pieces > 1 && (piece.first < 0 || piece.first > split.room - pieces)) return;
+    if (block >= split.room && pieces > 1) return;
+    if (block < split.room && (piece.first < 0 || piece.first > split.room - pieces)) return;
     if (CARRY && last) return;
     const int begin = span.begin + piece.at * split.rows, end = last ? span.end : begin + split.rows;
 
@@ -366,7 +365,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
 __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanArgs a, ScanSplit split, int blocks) {
     const int place = blockIdx.x / blocks;
     const int64_t at = (int64_t)(blockIdx.x - place * blocks) * SCAN_THREADS + threadIdx.x, size = (int64_t)a.D * a.N;
-    const ScanPiece piece = find_piece(a.cu, a.S, a.T, split.rows, place, COUNT_FIRST);
+    const ScanPiece piece = find_piece<true>(a.cu, a.S, a.T, split.rows, place);
     if (piece.request < 0) return;
     const Span span = request_rows(a.cu, piece.request, a.T);
     int to, from;
@@ -406,7 +405,7 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
     if constexpr (SPLIT) {
         const int64_t room = scan_split_room(a.T, piece_rows), states = (int64_t)a.D * a.N;
         split = {piece_rows, work, work + room * states, (int)room};
-        pieces = a.S + a.T / piece_rows;
+        pieces = a.S + room;
         const int64_t blocks = (states + SCAN_THREADS - 1) / SCAN_THREADS;
         const int64_t requests = a.T / (SCAN_ALONE * (int64_t)piece_rows);  // that can be split
         if (side * room > INT32_MAX || blocks * requests > INT32_MAX) return cudaErrorInvalidValue;

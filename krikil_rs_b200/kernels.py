@@ -635,18 +635,19 @@ def token_logprobs(logits, tokens=None, top: int = 0):
     at, ld = _like(logits, logits.dtype, shape, index, "logits")
     rows, vocab = shape
     _number(top, "top")
-    dev, lp, asked, lp_at, tokens_at = logits.device, None, 0, None, None
+    lp, asked, lp_at, tokens_at = None, 0, None, None
     if tokens is not None:
         like = tokens.shape
         if len(like) not in (1, 2) or like[0] != rows:
             raise ValueError(f"tokens: expected [{rows}] or [{rows}, tokens]")
         asked = 1 if len(like) == 1 else like[1]
         tokens_at = _indexes(tokens, rows * asked, index, "tokens")
-        lp = torch.empty(like, device=dev, dtype=torch.float32)
+    entropy = torch.empty(rows, device=logits.device, dtype=torch.float32)
+    if tokens is not None:
+        lp = entropy.new_empty(like)
         lp_at = lp.data_ptr()
-    entropy = torch.empty(rows, device=dev, dtype=torch.float32)
-    ids = torch.empty(rows, top, device=dev, dtype=torch.int32)
-    best = torch.empty(rows, top, device=dev, dtype=torch.float32)
+    best = entropy.new_empty(rows, top)
+    ids = torch.empty(rows, top, device=logits.device, dtype=torch.int32) if tokens is None else tokens.new_empty(rows, top)
     _call(index, lib.krk_k_token_logprobs, (at, ld, kind, rows, vocab, tokens_at, asked, lp_at, entropy.data_ptr(), top,
                                             ids.data_ptr(), best.data_ptr()))
     return lp, entropy, ids, best

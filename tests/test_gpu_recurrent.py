@@ -190,6 +190,13 @@ def test_conv_without_activation_bias_or_slots():
     assert torch.equal(state[2].to(F64), before[2])
 
 
+@pytest.mark.parametrize("lens", [[0] * 300 + [5], [5] + [0] * 300 + [70] + [0] * 33, [0] * 31 + [1] + [0] * 64 + [9] + [0],
+                                  [3, 0, 0, 0, 200] + [0] * 40])
+@pytest.mark.parametrize("init", ["same", "none", "mixed"])
+def test_conv_many_requests_without_rows(lens, init):
+    run_conv("f16", 4, 36, lens, 10, init=init, pad=(2, 3, len(lens) - 1), tail=1)
+
+
 # ------------------------------------------------------------------ the scan
 def scan64(x, dt, a, b, c, d, z, bias, h, e=0.0):
     """One request, row after row, from the state h (known within e): outputs, the last state, and bounds of what float32
@@ -293,6 +300,11 @@ def test_scan_long_prompts(ch, n):
 def test_scan_long_prompts_among_others(n, init):
     """Requests that are walked in pieces, of every rest, beside those that are not; states replaced where they are read."""
     run_scan("f32", 10, n, 2, [449, 3, 0, 513, 448, 512, 64, 575, 0, 900], 19, init=init, pad=(3,), tail=5)
+
+
+def test_scan_of_long_prompts_among_very_many():
+    """More requests than a block has threads, some of them walked in pieces."""
+    run_scan("bf16", 6, 4, 1, [(i * 7) % 4 for i in range(700)] + [1000, 3, 0, 1111] + [1] * 300, 41, init="mixed", pad=(5, 702))
 
 
 def test_scan_is_repeatable_and_the_bound_only_sizes_it():
@@ -745,6 +757,26 @@ def test_logprobs_of_large_logits(act):
     x[1] = x[1].abs() / 2 + big / 2
     x[2] = -x[1]
     check_logprobs(x, i32([0, 1, 2, 776]), 5)
+
+
+@pytest.mark.parametrize("act", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(1, 131072), (5, 70001), (300, 40000)])
+def test_logprobs_replayed_from_a_graph(act, rows, vocab):
+    """Rows shared by the blocks of clusters and rows of one block each, over new logits."""
+    g, x, tokens = gen(36), torch.zeros(rows, vocab, device=DEV, dtype=TYPES[act]), i32([0] * rows)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            captured = K.token_logprobs(x, tokens, 9)
+    torch.cuda.current_stream().wait_stream(stream)
+    for _ in range(2):
+        x.copy_((2 * normal(g, rows, vocab)).to(x.dtype))
+        tokens.copy_(torch.randint(0, vocab, (rows,), generator=g, device=DEV, dtype=torch.int32))
+        graph.replay()
+        for p, q in zip(captured, K.token_logprobs(x, tokens, 9)):
+            assert torch.equal(p, q)
 
 
 def test_logprobs_of_tokens_outside_the_vocabulary():

@@ -73,7 +73,7 @@ def test_step_refuses(what, value, word):
 
 
 @pytest.mark.parametrize("what,value,word", [
-    ("type", 3, "type"), ("R", -1, "R and K"), ("K", -1, "R and K"), ("V", 0, "V positive"), ("top", -1, "top"),
+    ("type", 3, "type"), ("R", -1, "R and K"), ("K", -1, "R and K"), ("V", 0, "V 1"), ("V", (1 << 30) + 1, "V 1"), ("top", -1, "top"),
     ("top", 33, "top"), (("top", "V"), (5, 4), "top"), ("logits", None, "logits"), ("logits", P + 2, "aligned"),
     ("tokens", None, "null"), ("lp", None, "null"), ("ids", None, "null"), ("best", None, "null")])
 def test_logprobs_refuses(what, value, word):
