@@ -28,6 +28,10 @@ constexpr int LP_SHORT = 1024;  // accesses of a row that a small block takes in
 constexpr int LP_LIST = 32;     // entries of a sorted list, LOGPROBS_MAX_TOP of them used
 constexpr int LP_ROOM = 1024;   // logits that reach the bound; for more (the best ones all in few threads' ways) see below
 constexpr int LP_AHEAD = 4;     // accesses on their way
+// Threads a multiprocessor: all of them in 32 bits, and 40 registers each in 16 (81 us for 4096 x 50001; 87 with 56
+// registers, 136 with 32, which spill).
+template <typename T>
+constexpr int LP_RESIDENT = sizeof(T) == 4 ? 2048 : 1536;
 constexpr float kLog2e = 1.44269504088896341f, kLowest = -3.402823466e38f;
 using Key = unsigned long long;
 
@@ -126,18 +130,21 @@ struct Running {
     float m = -INFINITY;
     float2 s = {0.0f, 0.0f}, e = {0.0f, 0.0f};
     int best = -1;
+    // A larger maximum, or the first one; NaN counts as -inf.
+    KRK_DEV void raise(float top, int k) {
+        top = top == top ? top : -INFINITY;
+        if (top <= m && best >= 0) return;
+        const float d = fmaxf(ref_of(m) - ref_of(top), -1000.0f), f = fast_exp2(d * kLog2e);
+        e = make_float2(f * fmaf(s.x, d, e.x), f * fmaf(s.y, d, e.y));
+        s = make_float2(s.x * f, s.y * f);
+        m = top;
+        best = k;
+    }
     KRK_DEV void add(const float (&x)[VEC], int k) {
         float top = x[0];
 #pragma unroll
         for (int j = 1; j < VEC; ++j) top = fmaxf(top, x[j]);
-        if (top > m || best < 0) {
-            top = top == top ? top : -INFINITY;
-            const float d = fmaxf(ref_of(m) - ref_of(top), -1000.0f), f = fast_exp2(d * kLog2e);
-            e = make_float2(f * fmaf(s.x, d, e.x), f * fmaf(s.y, d, e.y));
-            s = make_float2(s.x * f, s.y * f);
-            m = top;
-            best = k;
-        }
+        if (!(top <= m) || best < 0) raise(top, k);
         const float r = ref_of(m);
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
@@ -258,7 +265,7 @@ KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Sha
 
 // One block a row, or the `parts` blocks of a cluster.
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) logprobs_kernel(LogprobArgs a, int part_bits) {
+__global__ void __launch_bounds__(32 * WARPS, LP_RESIDENT<T> / (32 * WARPS)) logprobs_kernel(LogprobArgs a, int part_bits) {
     constexpr int VEC = Row<T>::VEC, THREADS = 32 * WARPS;
     __shared__ Shared<WARPS> sh;
     const int parts = 1 << part_bits, r = blockIdx.x >> part_bits, part = blockIdx.x & (parts - 1);
