@@ -209,16 +209,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     T* outp = (T*)a.out + (begin + own) * a.o_st + d;
     T xr[OWN], dtr[OWN], zr[OWN];
     const auto fetch = [&](int t, auto whole) {
-        if constexpr (AHEAD) return;
+        if constexpr (!AHEAD) {
 #pragma unroll
-        for (int o = 0; o < OWN; ++o) {
-            const bool in = decltype(whole)::value || t + own + o < end;
-            xr[o] = in ? *xp : zero;
-            dtr[o] = in ? *dtp : zero;
-            if (!CARRY) zr[o] = in ? *zp : zero;
-            xp += o + 1 < OWN ? a.x_st : (U - OWN + 1) * a.x_st;
-            dtp += o + 1 < OWN ? a.dt_st : (U - OWN + 1) * a.dt_st;
-            zp += o + 1 < OWN ? z_st : (U - OWN + 1) * z_st;
+            for (int o = 0; o < OWN; ++o) {
+                const bool in = decltype(whole)::value || t + own + o < end;
+                xr[o] = in ? *xp : zero;
+                dtr[o] = in ? *dtp : zero;
+                if (!CARRY) zr[o] = in ? *zp : zero;
+                xp += o + 1 < OWN ? a.x_st : (U - OWN + 1) * a.x_st;
+                dtp += o + 1 < OWN ? a.dt_st : (U - OWN + 1) * a.dt_st;
+                zp += o + 1 < OWN ? z_st : (U - OWN + 1) * z_st;
+            }
         }
     };
     // The tile from row t0 on, into one of two places.
@@ -315,13 +316,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
             y[u] = acc.x + acc.y;
             total += step[u];
         }
-        if (CARRY) return;
-        sum_rows<U, K>(y, lane);
+        if constexpr (!CARRY) {
+            sum_rows<U, K>(y, lane);
 #pragma unroll
-        for (int o = 0; o < OWN; ++o) {
-            if (open && lane % Sh::SHARE == 0 && (decltype(whole)::value || t + own + o < end))
-                *outp = from_f32<T>((y[o] + skipped[o]) * gate[o]);
-            outp += o + 1 < OWN ? a.o_st : (U - OWN + 1) * a.o_st;
+            for (int o = 0; o < OWN; ++o) {
+                if (open && lane % Sh::SHARE == 0 && (decltype(whole)::value || t + own + o < end))
+                    *outp = from_f32<T>((y[o] + skipped[o]) * gate[o]);
+                outp += o + 1 < OWN ? a.o_st : (U - OWN + 1) * a.o_st;
+            }
         }
     };
 

@@ -598,7 +598,7 @@ def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None,
     they were."""
     index = x.get_device()
     if index >= 0 and index != _current_device():  # the scratch is sized for the current device
-        with torch.cuda.device(index):
+        with torch.cuda.device(torch.device("cuda", index)):
             return selective_scan(x, dt, a, b, c, cu, d, z, dt_bias, state, slots, init, out, max_len, work)
     cu_at, requests = _requests(cu, index)
     index, out, args, sizes, rows = _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)

@@ -138,7 +138,7 @@ def run_conv(act, width, ch, lens, seed, init="mixed", pad=(), tail=0, silu=True
 
 @pytest.mark.parametrize("width", [2, 3, 4])
 @pytest.mark.parametrize("act", list(TYPES))
-@pytest.mark.parametrize("ch,strided", [(1, 0), (33, 3), (64, 8), (1472, 0), (520, 1)])
+@pytest.mark.parametrize("ch,strided", [(1, 0), (33, 3), (64, 8), (34, 2), (1472, 0), (520, 1)])
 def test_conv_types_widths_and_channels(act, width, ch, strided):
     run_conv(act, width, ch, [5, 0, 1, 2, 17, 3, 40, 0], 3, strided=strided, tail=2)
 
@@ -230,12 +230,12 @@ def scan64(x, dt, a, b, c, d, z, bias, h, e=0.0):
     return ys, es, h, e
 
 
-def scan_inputs(g, act, rows, ch, n, groups, gate=True, wide=False):
+def scan_inputs(g, act, rows, ch, n, groups, gate=True, wide=False, lead=3):
     dtype = TYPES[act]
-    bc = normal(g, rows, 3 + 2 * groups * n, dtype=dtype)
+    bc = normal(g, rows, lead + 2 * groups * n, dtype=dtype)
     x = normal(g, rows, ch + 5, dtype=dtype)[:, 5:] if wide else normal(g, rows, ch, dtype=dtype)
     return dict(x=x, dt=normal(g, rows, ch, dtype=dtype), a=-torch.exp(normal(g, ch, n)) * 3,
-                b=bc[:, 3:3 + groups * n].unflatten(1, (groups, n)), c=bc[:, 3 + groups * n:].unflatten(1, (groups, n)),
+                b=bc[:, lead:lead + groups * n].unflatten(1, (groups, n)), c=bc[:, lead + groups * n:].unflatten(1, (groups, n)),
                 d=normal(g, ch), z=normal(g, rows, 2 * ch, dtype=dtype)[:, ch:] if gate else None,
                 dt_bias=normal(g, ch) - 3)
 
@@ -253,10 +253,10 @@ def scan_want(t, cu, pool, rows, fill):
     return want, bound, kept, kept_e
 
 
-def run_scan(act, ch, n, groups, lens, seed, init="mixed", pad=(), tail=0, step=False, gate=True, wide=False):
+def run_scan(act, ch, n, groups, lens, seed, init="mixed", pad=(), tail=0, step=False, gate=True, wide=False, lead=3):
     g = gen(seed)
     rows = sum(lens) + tail
-    t = scan_inputs(g, act, rows, ch, n, groups, gate, wide)
+    t = scan_inputs(g, act, rows, ch, n, groups, gate, wide, lead)
     pool = Pool(g, (ch, n), torch.float32, len(lens), init, pad)
     out = torch.full((rows, ch), 7.0, device=DEV, dtype=TYPES[act])
     cu = list(itertools.accumulate(lens, initial=0))
@@ -274,6 +274,15 @@ def run_scan(act, ch, n, groups, lens, seed, init="mixed", pad=(), tail=0, step=
 @pytest.mark.parametrize("act", list(TYPES))
 def test_scan_types_and_states(act, n):
     run_scan(act, 70, n, 1, [5, 0, 1, 33, 64, 2], 11, tail=2)
+
+
+@pytest.mark.parametrize("n", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("act", list(TYPES))
+@pytest.mark.parametrize("ch,groups,lens,gate", [(8, 1, [1, 17, 0, 16, 40], True), (72, 1, [33, 15, 2], False),
+                                                 (400, 2, [9, 8, 7], True), (16, 2, [700, 5, 0, 461], True)])
+def test_scan_of_aligned_inputs(act, n, ch, groups, lens, gate):
+    """Rows of whole accesses, which come tile by tile: their ends, channels that end inside a block, requests in pieces."""
+    run_scan(act, ch, n, groups, lens, 42, gate=gate, lead=8, tail=3)
 
 
 @pytest.mark.parametrize("ch,groups,wide", [(1, 1, False), (6, 3, True), (130, 2, True), (1216, 1, False), (512, 4, True)])
@@ -339,6 +348,14 @@ def test_scan_of_long_requests_that_overlap_stays_in_bounds(cu):
 @pytest.mark.parametrize("act", list(TYPES))
 def test_step_types_and_states(act, n):
     run_scan(act, 70, n, 2, [1] * 9, 15, pad=(2, 8), step=True)
+
+
+@pytest.mark.parametrize("n", [4, 8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("act", list(TYPES))
+@pytest.mark.parametrize("rows,ch,groups", [(1, 24, 1), (9, 70, 2), (1800, 96, 1)])
+def test_step_of_aligned_inputs(act, n, rows, ch, groups):
+    """States, B and C in whole groups of four, by one and by two requests a thread."""
+    run_scan(act, ch, n, groups, [1] * (rows if n <= 32 else min(rows, 9)), 43, pad=(2, 8), step=True, lead=8, gate=n != 64)
 
 
 @pytest.mark.parametrize("rows,ch,groups,init", [(1, 1216, 1, "same"), (300, 24, 1, "mixed"), (3, 5120, 4, "none"),
@@ -584,6 +601,78 @@ def test_offsets_past_32_bits():
     p = K.selective_scan(**t, cu=i32([0, 1, 1, 3]), state=state, slots=i32([2, 0, 1]), init=i32([1, 2, -1]))
     q = K.selective_scan(**t, cu=i32([0, 1, 1, 3]), state=small, slots=i32([2, 0, 1]), init=i32([1, 2, -1]))
     assert torch.equal(p, q)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams that continue from the same slots, each with its own slots, scratch and outputs."""
+    g = gen(44)
+    t = scan_inputs(g, "bf16", 1500, 64, 16, 1, lead=8)
+    w, x = normal(g, 64, 4), normal(g, 1500, 64, dtype=torch.bfloat16)
+    cs, hs = normal(g, 9, 3, 64, dtype=torch.bfloat16), normal(g, 9, 64, 16)
+    cu, init, logits = i32([0, 900, 1500]), i32([8, 7]), normal(g, 2, 140000)
+    slots = [i32([0, 1]), i32([2, 3])]
+
+    def calls(i):
+        return (K.causal_conv(x, w, cu, state=cs, slots=slots[i], init=init),
+                K.selective_scan(**t, cu=cu, state=hs, slots=slots[i], init=init), *K.token_logprobs(logits, None, 5)[1:])
+
+    want = calls(0)
+    states = cs[:2].clone(), hs[:2].clone()
+    streams = [torch.cuda.Stream() for _ in slots]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for call in got[i]:
+            assert all(torch.equal(p, q) for p, q in zip(call, want))
+        assert torch.equal(cs[slots[i].long()], states[0]) and torch.equal(hs[slots[i].long()], states[1])
+
+
+def test_calls_run_with_their_tensors_device_current(monkeypatch):
+    """With another device current, every library call -- the size of the scratch, too -- is made with the tensors'
+    device current, and the other device is current again behind it.  (The other device is pretended: what the wrappers
+    ask and set is stood in for.)"""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, dev):
+            self.index = dev.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append((name, current[0]))
+                return getattr(lib, name)(*args)
+            return call
+
+    lib = K.lib
+    g = gen(45)
+    t = scan_inputs(g, "f32", 600, 32, 16, 1)
+    w, cs, hs = normal(g, 32, 4), normal(g, 600, 3, 32), normal(g, 600, 32, 16)
+
+    def calls():
+        return [K.causal_conv(t["x"], w, i32([0, 600])), K.causal_conv_step(t["x"], w, cs.clone()),
+                K.selective_scan(**t, cu=i32([0, 600])), K.selective_step(**t, state=hs.clone()),
+                *K.token_logprobs(t["x"], i32([3] * 600), 4)]
+
+    here = calls()
+    monkeypatch.setattr(K, "lib", Lib())
+    monkeypatch.setattr(K, "_current_device", lambda: current[0])
+    monkeypatch.setattr(K.torch.cuda, "device", Device)
+    current[0] = 1
+    there = calls()
+    assert all(torch.equal(p, q) for p, q in zip(here, there))
+    assert len(seen) == 6 and all(dev == 0 for _, dev in seen) and current[0] == 1, seen
 
 
 def test_every_call_launches_its_own_kernels():
