@@ -33,7 +33,7 @@ constexpr int SCAN_MAX_STATES = 256;
 constexpr int SCAN_THREADS = 128;
 constexpr int SCAN_BLOCKS = 4;  // blocks a multiprocessor, by registers
 constexpr int SCAN_LANE = 16;   // states a lane holds, if there are as many
-constexpr int SCAN_ALONE = 7;   // a request of up to so many pieces is not split
+constexpr int SCAN_ALONE = 5;   // a request of up to so many pieces is not split
 constexpr int SCAN_PIECE = 64;  // fewest rows of one
 struct ScanArgs {
     const void* x; int64_t x_st;                 // (t, d) at t*x_st + d
@@ -56,7 +56,7 @@ struct ScanPlan {
 };
 ScanPlan scan_plan(int T, int S, int D, int N, int G, int max_len);
 size_t scan_work_floats(int T, int D, int N, int G, int max_len);
-constexpr int64_t scan_split_room(int64_t T, int rows) { return T / rows * 8 / 7 + 2; }
+constexpr int64_t scan_split_room(int64_t T, int rows) { return T / rows * (SCAN_ALONE + 1) / SCAN_ALONE + 2; }
 cudaError_t selective_scan(const ScanArgs& a, int type, int max_len, float* work, cudaStream_t s);
 cudaError_t selective_step(const ScanArgs& a, int type, cudaStream_t s);
 

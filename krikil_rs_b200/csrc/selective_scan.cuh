@@ -12,12 +12,20 @@
 // converts them once for its 128 / K channels.  The multiply-adds are packed in
 // pairs of states.
 //
-// A request is walked row by row; walking requests in pieces at once costs about
-// twice the work (a first walk finds each piece's own state and sum of delta, a
-// short kernel carries the states from piece to piece, and the last walk starts
-// from them), so that only a request of more than its share is split: one that
-// alone would take longer than twice what the whole call takes when it is shared
-// out evenly.
+// A request is walked row by row; walking requests in pieces at once costs twice
+// the work (a first walk finds each piece's own state and sum of delta, a short
+// kernel carries the states from piece to piece, and the last walk starts from
+// them), so that only a request of more than its share is split: a piece has the
+// rows that give the device one wave of blocks, and a request of up to five of
+// them is walked alone (one prompt of 4000 rows, bfloat16, in pieces and alone:
+// 5120 channels, 14 pieces, 247 and 720 us; 12,000, six, 548 and 725; 16,384, four,
+// 809 and 770).
+//
+// Measured (N = 16): 64 prompts of 0 to 511 rows x 5120 bfloat16 channels 470 us --
+// 20 exponentials a row and channel would be 372 us, and a walk of the same
+// instructions without its inputs takes 168 cycles for 32 channels, 387 us -- and
+// 8192 rows x 1536 half channels in 49 pieces 153 us.  A polynomial in place of an
+// eighth of the exponentials takes as long (167 cycles), of a quarter longer (177).
 #pragma once
 #include <limits.h>
 
@@ -52,23 +60,6 @@ struct ScanSplit {
     int room;       // pieces of split requests that there is room for: more come from offsets that do not ascend
 };
 KRK_DEV int scan_pieces(int n, int rows) { return rows > 0 && n > (int64_t)SCAN_ALONE * rows ? (n - 1) / rows + 1 : 1; }
-
-// A request's turn among all: the longest first (of equal ones the first), so
-// that what is left when most blocks have ended is short; of more requests than a
-// block has threads, their own.
-KRK_DEV int request_of_turn(const int32_t* cu, int S, int T, int turn) {
-    if (S < 2 || S > SCAN_THREADS) return turn;
-    __shared__ int rows[SCAN_THREADS], found;
-    const int s = threadIdx.x;
-    const int mine = s < S ? clamp_row(cu[s + 1], T) - clamp_row(cu[s], T) : INT_MIN;
-    rows[s] = mine;
-    __syncthreads();
-    int place = 0;
-    for (int i = 0; i < S; ++i) place += rows[i] > mine || (rows[i] == mine && i < s);
-    if (s < S && place == turn) found = s;
-    __syncthreads();
-    return found;
-}
 
 // The piece-th piece of the requests that are split: its request, its place
 // there, and the place of the request's first one among all; FIRST: the piece-th
@@ -114,6 +105,36 @@ KRK_DEV ScanPiece find_piece(const int32_t* cu, int S, int T, int rows, int piec
         __syncthreads();
         if (found.request >= 0) break;
     }
+    return found;
+}
+
+// The turn-th unit of work of the last walk -- a request, or a piece of one that
+// is split -- of up to S + room.  The longest ones come first, so that what is
+// left when most blocks have ended is short; of more requests than a block has
+// threads, the pieces come first, then the requests in their order.
+KRK_DEV ScanPiece find_unit(const int32_t* cu, int S, int T, const ScanSplit& split, int turn) {
+    if (S > SCAN_THREADS) {
+        if (turn < split.room) return find_piece<false>(cu, S, T, split.rows, turn);
+        const int s = turn - split.room, n = clamp_row(cu[s + 1], T) - clamp_row(cu[s], T);
+        return {scan_pieces(n, split.rows) > 1 ? -1 : s, 0, 0};
+    }
+    __shared__ int rows[SCAN_THREADS], pieces[SCAN_THREADS];
+    __shared__ ScanPiece found;
+    const int s = threadIdx.x;
+    const int n = s < S ? clamp_row(cu[s + 1], T) - clamp_row(cu[s], T) : INT_MIN, p = s < S ? scan_pieces(n, split.rows) : 0;
+    rows[s] = p > 1 ? split.rows : n;
+    pieces[s] = p;
+    if (s == 0) found.request = -1;
+    __syncthreads();
+    // the units before this request's, and the pieces of split requests with a lower number
+    int before = 0, first = 0;
+    for (int i = 0; i < S; ++i) {
+        const bool sooner = rows[i] > rows[s] || (rows[i] == rows[s] && i < s);
+        before += sooner ? pieces[i] : 0;
+        first += i < s && pieces[i] > 1 ? pieces[i] : 0;
+    }
+    if (turn >= before && turn < before + p) found = {s, turn - before, first};
+    __syncthreads();
     return found;
 }
 
@@ -163,17 +184,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     const int g = cb / sides, ch0 = (cb - g * sides) * CH, ch = ch0 + tid / K;  // within the group
     const bool open = ch < per;
     const int d = g * per + (open ? ch : 0);
-    // (blocks for the pieces that there is room for come before those for a request each)
-    const ScanPiece piece = block < split.room ? find_piece<false>(a.cu, a.S, a.T, split.rows, block)
-                                               : ScanPiece{request_of_turn(a.cu, a.S, a.T, block - split.room), 0, 0};
+    const ScanPiece piece = CARRY ? find_piece<false>(a.cu, a.S, a.T, split.rows, block)
+                                  : find_unit(a.cu, a.S, a.T, split, block);
     if (piece.request < 0) return;
     const Span span = request_rows(a.cu, piece.request, a.T);
     int to, from;
     if (!request_slots(a.slot, piece.request, to, from)) return;
     const int pieces = scan_pieces(span.end - span.begin, split.rows);
     const bool last = piece.at == pieces - 1;
-    if (block >= split.room && pieces > 1) return;
-    if (block < split.room && (piece.first < 0 || piece.first > split.room - pieces)) return;
+    if (pieces > 1 && (piece.first < 0 || piece.first > split.room - pieces)) return;
     if (CARRY && last) return;
     const int begin = span.begin + piece.at * split.rows, end = last ? span.end : begin + split.rows;
 

@@ -102,10 +102,10 @@ def test_sound_calls_reach_the_device():
 def test_scan_scratch():
     """None for short requests; else room for every piece's states and step sums, whatever the requests' lengths."""
     floats = lib.krk_selective_scan_work_floats
-    assert floats(448, 64, 16, 1, 0) == 0 and floats(449, 64, 16, 1, 0) > 0
-    assert floats(100000, 64, 16, 1, 1000) == 0 and floats(100000, 64, 16, 1, 100000) == floats(100000, 64, 16, 1, 0)
-    assert floats(16384, 5120, 16, 1, 8000) == 0  # as many channels as the device has room for: a request is not split
-    for args in ((0, 64, 16, 1, 0), (449, 64, 257, 1, 0), (449, 64, 16, 3, 0), (449, 64, 16, 1, -1), (449, 0, 16, 1, 0)):
+    assert floats(320, 64, 16, 1, 0) == 0 and floats(321, 64, 16, 1, 0) > 0
+    assert floats(100000, 64, 16, 1, 800) == 0 and floats(100000, 64, 16, 1, 100000) == floats(100000, 64, 16, 1, 0)
+    assert floats(16384, 5120, 16, 1, 5000) == 0  # as many channels as the device has room for: a request is not split
+    for args in ((0, 64, 16, 1, 0), (321, 64, 257, 1, 0), (321, 64, 16, 3, 0), (321, 64, 16, 1, -1), (321, 0, 16, 1, 0)):
         assert floats(*args) == 0
 
 
