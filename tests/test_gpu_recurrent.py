@@ -171,6 +171,12 @@ def test_conv_step(act, rows, ch, width, pad, init):
     run_conv(act, width, ch, [1] * rows, 8, init=init, pad=pad, step=True)
 
 
+@pytest.mark.parametrize("act,rows,ch", [("bf16", 2501, 64), ("f32", 5003, 30), ("f16", 2400, 33)])
+def test_conv_step_of_very_many_requests(act, rows, ch):
+    """Blocks that take several turns, the last of them not whole."""
+    run_conv(act, 4, ch, [1] * rows, 11, pad=(0, 7, rows - 1), step=True)
+
+
 def test_conv_without_activation_bias_or_slots():
     run_conv("f16", 4, 48, [9, 4], 9, silu=False, bias=False)
     g = gen(1)
@@ -356,6 +362,12 @@ def test_step_types_and_states(act, n):
 def test_step_of_aligned_inputs(act, n, rows, ch, groups):
     """States, B and C in whole groups of four, by one and by two requests a thread."""
     run_scan(act, ch, n, groups, [1] * (rows if n <= 32 else min(rows, 9)), 43, pad=(2, 8), step=True, lead=8, gate=n != 64)
+
+
+@pytest.mark.parametrize("act,rows,ch,n,lead", [("bf16", 4003, 96, 32, 8), ("f32", 3001, 70, 48, 3)])
+def test_step_of_very_many_requests(act, rows, ch, n, lead):
+    """Blocks that take several turns, the last of them not whole."""
+    run_scan(act, ch, n, 1, [1] * rows, 46, pad=(0, 7, rows - 1), step=True, lead=lead)
 
 
 @pytest.mark.parametrize("rows,ch,groups,init", [(1, 1216, 1, "same"), (300, 24, 1, "mixed"), (3, 5120, 4, "none"),
