@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanArgs a, Sc
 #pragma unroll
         for (int i = 0; i < CARRY_AHEAD; ++i)
             if (c + i < pieces) {
-                h = fmaf(fast_exp2(rate * steps[i]), h, own[i]);
+                // (a decay that no float holds leaves an infinite state infinite, as its steps one by one do)
+                h = fmaf(fmaxf(fast_exp2(rate * steps[i]), 1.17549435e-38f), h, own[i]);
                 start[(int64_t)(c + i) * size] = h;
             }
     }

@@ -395,18 +395,18 @@ def test_scan_steps_of_any_width(step):
     pool.check(kept, kept_e)
 
 
-@pytest.mark.parametrize("n", [16, 20])
-def test_scan_infinite_inputs_stay_in_their_channels(n):
+@pytest.mark.parametrize("n,rows", [(16, 40), (20, 40), (16, 900)])
+def test_scan_infinite_inputs_stay_in_their_channels(n, rows):
     """An infinite x makes its channel infinite from its row on, and no other value."""
     g = gen(18)
-    t = scan_inputs(g, "f32", 40, 24, n, 1, gate=False)
+    t = scan_inputs(g, "f32", rows, 24, n, 1, gate=False)
     t["b"], t["c"] = t["b"].abs() + 0.1, t["c"].abs() + 0.1
     t["a"] = -torch.exp(normal(g, 24, n)) * 0.01
     t["d"] = t["d"].abs() + 0.1
     t["x"][20, 5] = math.inf
-    out = K.selective_scan(**t, cu=i32([0, 40]))
-    want, bound, *_ = scan_want(t, [0, 40], type("P", (), {"slots": [0], "begun": lambda self, s: torch.zeros(
-        24, n, device=DEV, dtype=F64)})(), 40, 0.0)
+    out = K.selective_scan(**t, cu=i32([0, rows]))
+    want, bound, *_ = scan_want(t, [0, rows], type("P", (), {"slots": [0], "begun": lambda self, s: torch.zeros(
+        24, n, device=DEV, dtype=F64)})(), rows, 0.0)
     assert (out[20:, 5] == math.inf).all()
     keep = torch.ones_like(out, dtype=torch.bool)
     keep[20:, 5] = False
@@ -584,6 +584,49 @@ def test_calls_replayed_from_a_graph_on_another_stream():
             else:
                 assert torch.equal(p, q)
         assert torch.equal(after[0], conv) and torch.equal(after[1], hidden)
+
+
+@pytest.mark.parametrize("act", list(TYPES))
+def test_views_off_the_grid(act):
+    """Weights, decays, states and inputs that begin one element beside an aligned place give what their copies give: the
+    same operations in the same order, bit for bit."""
+    g, dtype = gen(47), TYPES[act]
+
+    def beside(t):  # a copy one element into its memory, rows as far apart as a row and three
+        wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 3, device=DEV, dtype=t.dtype)
+        view = wide[..., 1:1 + t.shape[-1]]
+        view.copy_(t)
+        return view
+
+    def shifted(t):  # dense, one element beside
+        flat = torch.zeros(t.numel() + 1, device=DEV, dtype=t.dtype)
+        flat[1:] = t.flatten()
+        return flat[1:].view(t.shape)
+
+    def pool(t):  # slots dense, apart, beside
+        wide = torch.zeros(t.shape[0], t[0].numel() + 3, device=DEV, dtype=t.dtype)
+        view = wide[:, 1:1 + t[0].numel()].unflatten(1, t.shape[1:])
+        view.copy_(t)
+        return view
+
+    ch, rows, cu = 64, 70, i32([0, 33, 33, 70])
+    x = normal(g, rows, ch, dtype=dtype)
+    for width in (2, 3, 4):
+        w, bias, state = normal(g, ch, width), normal(g, ch), normal(g, rows, width - 1, ch, dtype=dtype)
+        for step in (False, True):
+            s, p = state.clone(), pool(state)
+            call = (lambda x, w, bias, s: K.causal_conv_step(x, w, s, bias=bias)) if step else (
+                lambda x, w, bias, s: K.causal_conv(x, w, cu, bias=bias, state=s))
+            assert torch.equal(call(x, w, bias, s), call(beside(x), shifted(w), shifted(bias), p)) and torch.equal(s, p)
+            assert torch.equal(call(x, shifted(w), bias, state.clone()), call(x, w, bias, state.clone()))
+    for n in (4, 16, 32):
+        t = {k: v.contiguous() for k, v in scan_inputs(g, act, rows, ch, n, 1).items()}
+        state = normal(g, rows, ch, n)
+        off = {k: shifted(v) if k in ("a", "d", "dt_bias") else beside(v) for k, v in t.items()}
+        for step in (False, True):
+            s, p = state.clone(), pool(state)
+            call = (lambda t, s: K.selective_step(**t, state=s)) if step else (lambda t, s: K.selective_scan(**t, cu=cu, state=s))
+            assert torch.equal(call(t, s), call(off, p)) and torch.equal(s, p)
 
 
 def test_offsets_past_32_bits():
