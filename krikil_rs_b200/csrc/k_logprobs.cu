@@ -199,27 +199,24 @@ KRK_DEV void best_keys(const Row<T>& row, int k0, int k1, int top, Key best, Sha
     const unsigned high = (unsigned)(bound >> 32);
     const float bound_value = bound == 0 ? -INFINITY : __uint_as_float(high & 0x80000000u ? high & 0x7fffffffu : ~high);
     const int ways = (k1 - k0 + THREADS - 1) / THREADS;
-    for (int i = warp; i < top; i += WARPS) {
-        const Key first = sh.list[0][i];
-        if (first == 0) break;
-        const int way = ((key_index(first) + row.lead) / VEC - k0) % THREADS;
-        for (int j = lane; j < ways; j += 32) {
-            const int k = k0 + way + j * THREADS;
-            if (k >= k1) break;
-            float v[VEC];
-            row.floats(k, v);
-            float near = v[0];
+    for (int i = tid; i < top * ways; i += THREADS) {
+        const int which = i / ways;
+        const Key first = sh.list[0][which];
+        const int k = k0 + ((key_index(first) + row.lead) / VEC - k0) % THREADS + (i - which * ways) * THREADS;
+        if (first == 0 || k >= k1) continue;
+        float v[VEC];
+        row.floats(k, v);
+        float near = v[0];
 #pragma unroll
-            for (int q = 1; q < VEC; ++q) near = fmaxf(near, v[q]);
-            if (near < bound_value) continue;  // (NaN counts as -inf, and only that bound takes it)
+        for (int q = 1; q < VEC; ++q) near = fmaxf(near, v[q]);
+        if (near < bound_value) continue;  // (NaN counts as -inf, and only that bound takes it)
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) {
-                if (v[q] < bound_value) continue;
-                const Key key = order_key(v[q], row.first(k) + q);
-                if (key >= bound && row.has(k, q)) {
-                    const int at = atomicAdd(&sh.count, 1);  // (in any order: ranks tell)
-                    if (at < LP_ROOM) sh.near[at] = key;
-                }
+        for (int q = 0; q < VEC; ++q) {
+            if (v[q] < bound_value) continue;
+            const Key key = order_key(v[q], row.first(k) + q);
+            if (key >= bound && row.has(k, q)) {
+                const int at = atomicAdd(&sh.count, 1);  // (in any order: ranks tell)
+                if (at < LP_ROOM) sh.near[at] = key;
             }
         }
     }

@@ -22,19 +22,24 @@ namespace {
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int STEP_THREADS = 128;
 
+// States n .. n + 3 (some there): WIDE, all of them and aligned.
 template <bool WIDE, typename T>
 KRK_DEV float4 load_four(const T* p, int n, int N) {
     if (WIDE) return load4(p + n);
-    return make_float4(to_f32(p[n]), n + 1 < N ? to_f32(p[n + 1]) : 0.0f, n + 2 < N ? to_f32(p[n + 2]) : 0.0f,
-                       n + 3 < N ? to_f32(p[n + 3]) : 0.0f);
+    return make_float4(to_f32(p[n]), to_f32(p[min(n + 1, N - 1)]), to_f32(p[min(n + 2, N - 1)]), to_f32(p[min(n + 3, N - 1)]));
 }
 
-// WIDE: as many states as the lanes hold, aligned in groups of four, as are
-// decays, B and C.  Everything that the rows need is loaded before the first of
-// them is computed, whether they need it or not: where branches meet, a thread
-// waits for the loads that were in them.
-template <typename T, bool WIDE, int Q, int R>
+// The form of a call: states and decays in whole and aligned groups of four, B and
+// C, too, and as many states as the lanes hold.
+enum StepForm { STEP_ANY, STEP_WIDE, STEP_WIDE_BC, STEP_WHOLE };
+
+// Everything that the rows need is loaded before the first of them is
+// computed, whether they need it or not -- the last states again in the place of
+// those that are not there: where branches meet, a thread waits for the loads
+// that were in them.
+template <typename T, StepForm FORM, int Q, int R>
 __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane_bits, int turns, int side) {
+    constexpr bool WIDE = FORM != STEP_ANY, WIDE_BC = FORM >= STEP_WIDE_BC;
     const int group = blockIdx.x / side, i = (blockIdx.x - group * side) * STEP_THREADS + threadIdx.x;
     const int lanes = 1 << lane_bits, lane = i & (lanes - 1), d = min(i >> lane_bits, a.D - 1);
     const bool open = (i >> lane_bits) < a.D;
@@ -42,11 +47,15 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
     const int g = a.G == 1 ? 0 : d / (a.D / a.G);
     const T* zp = a.z ? (const T*)a.z : (const T*)a.x;  // (unused when there is none)
     const int64_t z_st = a.z ? a.z_st : a.x_st;
+    int at[Q];    // the first of a group's states, or of the last group's
+    bool there[Q];
     float4 rate[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int n = 4 * (q * lanes + lane);
-        rate[q] = WIDE || n < a.N ? load_four<WIDE>(a.a + row, n, a.N) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        there[q] = FORM == STEP_WHOLE || n < a.N;
+        at[q] = there[q] ? n : (a.N - 1) / 4 * 4;
+        rate[q] = load_four<WIDE>(a.a + row, at[q], a.N);
     }
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, skip = a.d ? a.d[d] : 0.0f;
     const int64_t share = (int64_t)turns * R;
@@ -66,11 +75,8 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
             z[r] = zp[t * z_st + d];
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                const int n = 4 * (q * lanes + lane);
-                b[r][q] = c[r][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (!WIDE && n >= a.N) continue;
-                b[r][q] = load_four<WIDE>(bt, n, a.N);
-                c[r][q] = load_four<WIDE>(ct, n, a.N);
+                b[r][q] = load_four<WIDE_BC>(bt, at[q], a.N);
+                c[r][q] = load_four<WIDE_BC>(ct, at[q], a.N);
             }
         }
         bool live[R];
@@ -81,8 +87,7 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
             const float* old = (const float*)a.slot.state + (begun ? from[r] * a.slot.stride : 0) + row;
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                const int n = 4 * (q * lanes + lane);
-                h[r][q] = WIDE || n < a.N ? load_four<WIDE>(old, n, a.N) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                h[r][q] = load_four<WIDE>(old, at[q], a.N);
                 if (!begun) h[r][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
         }
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
             float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
-                const int n = 4 * (q * lanes + lane);
+                const int n = at[q];
                 float2 lo = make_float2(h[r][q].x, h[r][q].y), hi = make_float2(h[r][q].z, h[r][q].w);
                 const float2 e = __fmul2_rn(step2, make_float2(rate[q].x, rate[q].y));
                 const float2 f = __fmul2_rn(step2, make_float2(rate[q].z, rate[q].w));
@@ -102,16 +107,17 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
                                 __fmul2_rn(put2, make_float2(b[r][q].x, b[r][q].y)));
                 hi = __ffma2_rn(make_float2(fast_exp2(f.x), fast_exp2(f.y)), hi,
                                 __fmul2_rn(put2, make_float2(b[r][q].z, b[r][q].w)));
-                if (!WIDE && n >= a.N) continue;
+                float2 part;
                 if (WIDE) {
-                    sum = __ffma2_rn(lo, make_float2(c[r][q].x, c[r][q].y), sum);
-                    sum = __ffma2_rn(hi, make_float2(c[r][q].z, c[r][q].w), sum);
+                    part = __fmul2_rn(lo, make_float2(c[r][q].x, c[r][q].y));
+                    part = __ffma2_rn(hi, make_float2(c[r][q].z, c[r][q].w), part);
                 } else {  // an infinite x makes no NaN of states that are not there
-                    sum.x = fmaf(lo.x, c[r][q].x, sum.x);
-                    if (n + 1 < a.N) sum.y = fmaf(lo.y, c[r][q].y, sum.y);
-                    if (n + 2 < a.N) sum.x = fmaf(hi.x, c[r][q].z, sum.x);
-                    if (n + 3 < a.N) sum.y = fmaf(hi.y, c[r][q].w, sum.y);
+                    part = make_float2(lo.x * c[r][q].x, n + 1 < a.N ? lo.y * c[r][q].y : 0.0f);
+                    if (n + 2 < a.N) part.x = fmaf(hi.x, c[r][q].z, part.x);
+                    if (n + 3 < a.N) part.y = fmaf(hi.y, c[r][q].w, part.y);
                 }
+                if (!there[q]) continue;
+                sum = __fadd2_rn(sum, part);
                 if (!live[r] || !open) continue;
                 if (WIDE) {
                     *reinterpret_cast<float4*>(kept + n) = make_float4(lo.x, lo.y, hi.x, hi.y);
@@ -132,38 +138,44 @@ __global__ void __launch_bounds__(STEP_THREADS) step_kernel(ScanArgs a, int lane
     }
 }
 
-template <typename T, bool WIDE, int Q, int R>
+template <typename T, StepForm FORM, int Q, int R>
 cudaError_t launch_step(const ScanArgs& a, int lane_bits, int64_t side, int turns, cudaStream_t s) {
     const int64_t blocks = side * ((a.T + (int64_t)R * turns - 1) / ((int64_t)R * turns));
     if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    step_kernel<T, WIDE, Q, R><<<(unsigned)blocks, STEP_THREADS, 0, s>>>(a, lane_bits, turns, (int)side);
+    step_kernel<T, FORM, Q, R><<<(unsigned)blocks, STEP_THREADS, 0, s>>>(a, lane_bits, turns, (int)side);
     add_launches(1);
     return cudaGetLastError();
 }
 
-template <typename T, bool WIDE, int Q>
+template <typename T, StepForm FORM, int Q>
 cudaError_t step_rows(const ScanArgs& a, int lane_bits, cudaStream_t s) {
     const int sms = paged_sm_count();
     if (sms <= 0) return cudaErrorInvalidDevice;
     const int64_t side = (((int64_t)a.D << lane_bits) + STEP_THREADS - 1) / STEP_THREADS, units = side * a.T;
     // two requests a thread at once when that leaves every multiprocessor a full set of threads
-    if (units < (int64_t)sms * 2048 * 2 / STEP_THREADS) return launch_step<T, WIDE, Q, 1>(a, lane_bits, side, 1, s);
+    if (units < (int64_t)sms * 2048 * 2 / STEP_THREADS) return launch_step<T, FORM, Q, 1>(a, lane_bits, side, 1, s);
     // and up to four times, with the channels' decays loaded once, while there are two waves of blocks (six a
     // multiprocessor, by registers): 253 requests x 5120 channels, 36.1 us by four times, 38.5 by one, 41.8 by eight
     const int64_t turns = units / 2 / (12LL * sms);
-    return launch_step<T, WIDE, Q, 2>(a, lane_bits, side, turns < 1 ? 1 : turns > 4 ? 4 : (int)turns, s);
+    return launch_step<T, FORM, Q, 2>(a, lane_bits, side, turns < 1 ? 1 : turns > 4 ? 4 : (int)turns, s);
+}
+
+template <typename T, int Q>
+cudaError_t step_wide(const ScanArgs& a, int lane_bits, cudaStream_t s) {
+    const int64_t rows = a.T > 1, groups = a.G > 1;
+    const bool wide = a.N % 4 == 0 && fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, 16, 4) && fits(a.a, 0, 16, 4);
+    const bool wide_bc = fits(a.b, rows * a.b_st, 4 * sizeof(T), sizeof(T)) && fits(a.c, rows * a.c_st, 4 * sizeof(T), sizeof(T)) &&
+                         groups * a.b_sg % 4 == 0 && groups * a.c_sg % 4 == 0;
+    if (!wide) return step_rows<T, STEP_ANY, Q>(a, lane_bits, s);
+    if (!wide_bc) return step_rows<T, STEP_WIDE, Q>(a, lane_bits, s);
+    return a.N == 4 * Q << lane_bits ? step_rows<T, STEP_WHOLE, Q>(a, lane_bits, s) : step_rows<T, STEP_WIDE_BC, Q>(a, lane_bits, s);
 }
 
 template <typename T>
 cudaError_t step_type(const ScanArgs& a, cudaStream_t s) {
     int bits = 0;  // lanes of eight states
     while (bits < 5 && 8 << bits < a.N) ++bits;
-    const int64_t rows = a.T > 1, groups = a.G > 1;
-    const bool wide = a.N == (a.N <= 4 ? 4 : 8 << bits) && fits(a.slot.state, a.slot.num_slots > 1 ? a.slot.stride : 0, 16, 4) && fits(a.a, 0, 16, 4) &&
-                      fits(a.b, rows * a.b_st, 4 * sizeof(T), sizeof(T)) && fits(a.c, rows * a.c_st, 4 * sizeof(T), sizeof(T)) &&
-                      groups * a.b_sg % 4 == 0 && groups * a.c_sg % 4 == 0;
-    if (a.N <= 4) return wide ? step_rows<T, true, 1>(a, 0, s) : step_rows<T, false, 1>(a, 0, s);
-    return wide ? step_rows<T, true, 2>(a, bits, s) : step_rows<T, false, 2>(a, bits, s);
+    return a.N <= 4 ? step_wide<T, 1>(a, 0, s) : step_wide<T, 2>(a, bits, s);
 }
 
 }  // namespace

@@ -198,6 +198,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
 
     // States 4 (q K + lane) .. + 3 of the channel for q < SPT / 4: lanes read B and C side by side.
     const auto state_of = [&](int j) { return 4 * (j / 4 * K + lane) + j % 4; };
+    // (a lane's groups of four that are there; states beside them in the last one stay 0)
+    const int fours = PADDED ? max(0, (a.N + 3) / 4 - lane + K - 1) / K : SPT / 4;
     float2 h[SPT / 2], rate[SPT / 2];
     {
         const float* old = CARRY ? nullptr
@@ -314,6 +316,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
             float2 acc = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int q = 0; q < SPT / 4; ++q) {
+                if (PADDED && q >= fours) continue;
                 const float4 b4 = b[q * K];
                 const float4 c4 = CARRY ? b4 : c[q * K];
 #pragma unroll
@@ -323,13 +326,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
                     const float2 decay = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                     h[j] = __ffma2_rn(decay, h[j], __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y)));
                     if (CARRY) continue;
-                    float2 there = h[j];
-                    if (PADDED) {  // an infinite x makes no NaN of states that are not there
-                        if (state_of(2 * j) >= a.N) there.x = 0.0f;
-                        if (state_of(2 * j + 1) >= a.N) there.y = 0.0f;
-                    }
                     const float2 ci = i ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y);
-                    acc = j == 0 ? __fmul2_rn(there, ci) : __ffma2_rn(there, ci, acc);
+                    acc = __ffma2_rn(h[j], ci, acc);
                 }
             }
             y[u] = acc.x + acc.y;
