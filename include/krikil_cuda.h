@@ -545,8 +545,8 @@ KRK_API int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int typ
  * x, dt, z, b, c and out are of `type` (KRK_TYPE_*), weights and scan states
  * float32; everything is computed in 32 bits and rounded once when written.
  * Element (t, i) of a [T][.] tensor is p[t*p_st + i]; pointers are aligned to
- * their elements, and 16-byte aligned rows are read and written 16 bytes at a
- * time.  The calls run on the current device, to which `stream` and all pointers
+ * their elements (rows that are aligned to 16 bytes, states, B and C to four
+ * elements are faster).  The calls run on the current device, to which `stream` and all pointers
  * belong, and can be captured into a CUDA graph. */
 
 /* Causal depthwise convolution of width W (2, 3 or 4) over C channels:
