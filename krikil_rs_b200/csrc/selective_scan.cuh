@@ -47,7 +47,8 @@ struct ScanShape {
     static constexpr int CH = SCAN_THREADS / K, NP = K * SPT;
     static constexpr int MOST = AHEAD ? (sizeof(T) == 2 ? 16 : 8) : 32;
     static constexpr int ROWS = NP * MOST <= 1024 ? MOST : 1024 / NP;  // a tile
-    static constexpr int F = 2 * ROWS * NP / SCAN_THREADS;             // elements of them that a thread stages
+    static constexpr int BC = 2 * ROWS * NP;                           // elements of B and C in it
+    static constexpr int F = (BC + SCAN_THREADS - 1) / SCAN_THREADS;   // and those that a thread stages
     static constexpr int OWN = K < SCAN_GROUP ? SCAN_GROUP / K : 1;    // rows of a group whose inputs are a lane's work
     static constexpr int SHARE = K < SCAN_GROUP ? 1 : K / SCAN_GROUP;  // lanes that have the same ones
 };
@@ -174,7 +175,8 @@ KRK_DEV void copy16(void* smem, const void* gmem, bool there) {
 template <typename T, int K, int SPT, bool PADDED, bool CARRY, bool AHEAD>
 __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArgs a, ScanSplit split, int side) {
     using Sh = ScanShape<T, K, SPT, AHEAD>;
-    constexpr int CH = Sh::CH, NP = Sh::NP, ROWS = Sh::ROWS, F = Sh::F, OWN = Sh::OWN, U = SCAN_GROUP;
+    constexpr int CH = Sh::CH, NP = Sh::NP, ROWS = Sh::ROWS, BC = Sh::BC, F = Sh::F, OWN = Sh::OWN,
+                  U = SCAN_GROUP;
     constexpr int INPUTS = CARRY ? 2 : 3;
     __shared__ __align__(16) float s_bc[2][ROWS][2][NP];
     __shared__ __align__(16) T s_in[AHEAD ? 2 : 1][INPUTS][AHEAD ? ROWS : 1][AHEAD ? CH : 1];
@@ -269,13 +271,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
         for (int f = 0; f < F; ++f) {
             const int i = f * SCAN_THREADS + tid, t = t0 + i / (2 * NP), n = i % NP;
             const bool is_c = i / NP % 2;
-            const bool in = t < end && (!PADDED || n < a.N) && !(CARRY && is_c);
+            const bool in = i < BC && t < end && (!PADDED || n < a.N) && !(CARRY && is_c);
             bcr[f] = in ? (is_c ? cp + t * a.c_st : bp + t * a.b_st)[n] : zero;
         }
     };
     const auto stage_bc = [&](int buffer) {
 #pragma unroll
-        for (int f = 0; f < F; ++f) (&s_bc[buffer][0][0][0])[f * SCAN_THREADS + tid] = to_f32(bcr[f]);
+        for (int f = 0; f < F; ++f)
+            if (f * SCAN_THREADS + tid < BC) (&s_bc[buffer][0][0][0])[f * SCAN_THREADS + tid] = to_f32(bcr[f]);
     };
 
     float total = 0.0f;
@@ -446,7 +449,7 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
 template <typename T, int K, int SPT, bool SPLIT>
 cudaError_t scan_padded(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
     if (a.N != K * SPT) return launch_scan<T, K, SPT, true, SPLIT, false>(a, work, rows, s);
-    if constexpr (SPT == SCAN_LANE) {
+    if constexpr (SPT == SCAN_LANE || K == 1) {
         const bool many = a.T > 1;
         if (a.D / a.G % (16 / sizeof(T)) == 0 && fits(a.x, many ? a.x_st : 0, 16, sizeof(T)) &&
             fits(a.dt, many ? a.dt_st : 0, 16, sizeof(T)) && fits(a.z, many && a.z ? a.z_st : 0, 16, sizeof(T)))

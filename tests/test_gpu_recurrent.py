@@ -282,7 +282,7 @@ def test_scan_types_and_states(act, n):
     run_scan(act, 70, n, 1, [5, 0, 1, 33, 64, 2], 11, tail=2)
 
 
-@pytest.mark.parametrize("n", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("n", [4, 8, 16, 32, 64, 128, 256])
 @pytest.mark.parametrize("act", list(TYPES))
 @pytest.mark.parametrize("ch,groups,lens,gate", [(8, 1, [1, 17, 0, 16, 40], True), (72, 1, [33, 15, 2], False),
                                                  (400, 2, [9, 8, 7], True), (16, 2, [700, 5, 0, 461], True)])
