@@ -13,6 +13,11 @@
 // logits are read again, and of the few that reach the bound each one's rank is
 // its place.  Few rows are shared by the blocks of a cluster, whose sums and
 // lists its first block joins.
+//
+// Measured: float32, 1024 x 50001, 36 us (5.6 TB/s, 85% of the copy rate);
+// bfloat16, 4096 x 50001, 82 us (5.0 TB/s; issue slots 75% busy, the exponential
+// unit 62%); float32, one row of 131,072 with 20 alternatives, 8.5 us in 16 blocks;
+// bfloat16, 4096 x 32768 with 20 alternatives, 80 us, half of it the rows' ends.
 #include <cooperative_groups.h>
 
 #include "kernels.h"
