@@ -200,8 +200,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
 
     // States 4 (q K + lane) .. + 3 of the channel for q < SPT / 4: lanes read B and C side by side.
     const auto state_of = [&](int j) { return 4 * (j / 4 * K + lane) + j % 4; };
-    // (a lane's groups of four that are there; states beside them in the last one stay 0)
+    // a lane's groups of four that are there, and the one of them, if any, that holds the last states and others
     const int fours = PADDED ? max(0, (a.N + 3) / 4 - lane + K - 1) / K : SPT / 4;
+    const int edge = PADDED && a.N % 4 && a.N / 4 % K == lane ? a.N / 4 / K : -1;
     float2 h[SPT / 2], rate[SPT / 2];
     {
         const float* old = CARRY ? nullptr
@@ -327,7 +328,12 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
                     const int j = 2 * q + i;
                     const float2 e = __fmul2_rn(st, rate[j]);
                     const float2 decay = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-                    h[j] = __ffma2_rn(decay, h[j], __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y)));
+                    float2 in = __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
+                    if (PADDED && q == edge) {  // states that are not there stay 0, also when x is infinite
+                        if (2 * i >= a.N % 4) in.x = 0.0f;
+                        if (2 * i + 1 >= a.N % 4) in.y = 0.0f;
+                    }
+                    h[j] = __ffma2_rn(decay, h[j], in);
                     if (CARRY) continue;
                     const float2 ci = i ? make_float2(c4.z, c4.w) : make_float2(c4.x, c4.y);
                     acc = __ffma2_rn(h[j], ci, acc);

@@ -395,7 +395,7 @@ def test_scan_steps_of_any_width(step):
     pool.check(kept, kept_e)
 
 
-@pytest.mark.parametrize("n,rows", [(16, 40), (20, 40), (16, 900)])
+@pytest.mark.parametrize("n,rows", [(16, 40), (20, 40), (3, 40), (5, 40), (17, 40), (50, 40), (16, 900), (23, 900)])
 def test_scan_infinite_inputs_stay_in_their_channels(n, rows):
     """An infinite x makes its channel infinite from its row on, and no other value."""
     g = gen(18)
