@@ -168,11 +168,14 @@ KRK_DEV void copy16(void* smem, const void* gmem, bool there) {
                  : "memory");
 }
 
+// What a lane holds besides states: nothing, whole groups of four, or parts of them.
+enum ScanPadding { PAD_NONE, PAD_FOURS, PAD_STATES };
+
 // CARRY: the first walk of split requests, which leaves each piece's state from
 // zeros, for the piece behind it, and its sum of delta.  AHEAD: x, dt and z, whose
 // rows are aligned to 16 bytes, come tile by tile through shared memory, the next
 // tile while one is computed; else each lane loads its own, a group ahead.
-template <typename T, int K, int SPT, bool PADDED, bool CARRY, bool AHEAD>
+template <typename T, int K, int SPT, ScanPadding PADDED, bool CARRY, bool AHEAD>
 __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArgs a, ScanSplit split, int side) {
     using Sh = ScanShape<T, K, SPT, AHEAD>;
     constexpr int CH = Sh::CH, NP = Sh::NP, ROWS = Sh::ROWS, BC = Sh::BC, F = Sh::F, OWN = Sh::OWN,
@@ -202,7 +205,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
     const auto state_of = [&](int j) { return 4 * (j / 4 * K + lane) + j % 4; };
     // a lane's groups of four that are there, and the one of them, if any, that holds the last states and others
     const int fours = PADDED ? max(0, (a.N + 3) / 4 - lane + K - 1) / K : SPT / 4;
-    const int edge = PADDED && a.N % 4 && a.N / 4 % K == lane ? a.N / 4 / K : -1;
+    const int edge = PADDED == PAD_STATES && a.N / 4 % K == lane ? a.N / 4 / K : -1;
     float2 h[SPT / 2], rate[SPT / 2];
     {
         const float* old = CARRY ? nullptr
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, SCAN_BLOCKS) scan_kernel(ScanArg
                     const float2 e = __fmul2_rn(st, rate[j]);
                     const float2 decay = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                     float2 in = __fmul2_rn(pt, i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
-                    if (PADDED && q == edge) {  // states that are not there stay 0, also when x is infinite
+                    if (PADDED == PAD_STATES && q == edge) {  // states that are not there stay 0, also when x is infinite
                         if (2 * i >= a.N % 4) in.x = 0.0f;
                         if (2 * i + 1 >= a.N % 4) in.y = 0.0f;
                     }
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(SCAN_THREADS) scan_carry_kernel(ScanArgs a, Sc
 }
 
 // ---------------------------------------------------------------- the launches
-template <typename T, int K, int SPT, bool PADDED, bool SPLIT, bool AHEAD>
+template <typename T, int K, int SPT, ScanPadding PADDED, bool SPLIT, bool AHEAD>
 cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStream_t s) {
     using Sh = ScanShape<T, K, SPT, AHEAD>;
     const int64_t side = (int64_t)((a.D / a.G + Sh::CH - 1) / Sh::CH) * a.G;
@@ -454,14 +457,15 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
 
 template <typename T, int K, int SPT, bool SPLIT>
 cudaError_t scan_padded(const ScanArgs& a, float* work, int rows, cudaStream_t s) {
-    if (a.N != K * SPT) return launch_scan<T, K, SPT, true, SPLIT, false>(a, work, rows, s);
+    if (a.N % 4) return launch_scan<T, K, SPT, PAD_STATES, SPLIT, false>(a, work, rows, s);
+    if (a.N != K * SPT) return launch_scan<T, K, SPT, PAD_FOURS, SPLIT, false>(a, work, rows, s);
     if constexpr (SPT == SCAN_LANE || K == 1) {
         const bool many = a.T > 1;
         if (a.D / a.G % (16 / sizeof(T)) == 0 && fits(a.x, many ? a.x_st : 0, 16, sizeof(T)) &&
             fits(a.dt, many ? a.dt_st : 0, 16, sizeof(T)) && fits(a.z, many && a.z ? a.z_st : 0, 16, sizeof(T)))
-            return launch_scan<T, K, SPT, false, SPLIT, true>(a, work, rows, s);
+            return launch_scan<T, K, SPT, PAD_NONE, SPLIT, true>(a, work, rows, s);
     }
-    return launch_scan<T, K, SPT, false, SPLIT, false>(a, work, rows, s);
+    return launch_scan<T, K, SPT, PAD_NONE, SPLIT, false>(a, work, rows, s);
 }
 
 // Lanes of SCAN_LANE states; of four when the blocks of those would leave
