@@ -530,7 +530,10 @@ KRK_API int krk_k_attn_decode_paged(void* q, int64_t q_sb, int64_t q_sh, int typ
  *
  * Packed: request s (of S) owns rows cu[s] .. cu[s+1]-1 of T; rows of no request
  * are left alone.  cu is not trusted: its values are cut to [0, T], and a request
- * that ends before it begins is empty.  Single tokens: request b owns row b.
+ * that ends before it begins is empty.  Offsets that do not ascend, which name
+ * rows of several requests, cost the results of the call's requests (their rows
+ * and slots hold something of the call's inputs or what they held before) and
+ * nothing else.  Single tokens: request b owns row b.
  * Slots: request s continues from slot init[s] -- below 0: it begins, from zeros
  * -- and leaves its state in slot slots[s].  slots NULL: slot s; init NULL: the
  * slot it goes to.  A request of no rows leaves there what it continues from.  A

@@ -58,7 +58,8 @@ struct ScanSplit {
     int rows;       // a piece's
     float* start;   // [pieces of split requests][D][N]: the states that pieces start from
     float* sum;     // [pieces of split requests][D]: their sums of delta
-    int room;       // pieces of split requests that there is room for: more come from offsets that do not ascend
+    int room;       // pieces of split requests that there is room for: more come from offsets that do not ascend,
+                    // and the requests that have none are left alone
 };
 KRK_DEV int scan_pieces(int n, int rows) { return rows > 0 && n > (int64_t)SCAN_ALONE * rows ? (n - 1) / rows + 1 : 1; }
 
@@ -439,7 +440,8 @@ cudaError_t launch_scan(const ScanArgs& a, float* work, int piece_rows, cudaStre
         split = {piece_rows, work, work + room * states, (int)room};
         pieces = a.S + room;
         const int64_t blocks = (states + SCAN_THREADS - 1) / SCAN_THREADS;
-        const int64_t requests = a.T / (SCAN_ALONE * (int64_t)piece_rows);  // that can be split
+        // that can be split and have room, whatever the offsets: each has more than SCAN_ALONE pieces
+        const int64_t requests = room / (SCAN_ALONE + 1);
         if (side * room > INT32_MAX || blocks * requests > INT32_MAX) return cudaErrorInvalidValue;
         scan_kernel<T, K, SPT, PADDED, true, AHEAD><<<(unsigned)(side * room), SCAN_THREADS, 0, s>>>(a, split, (int)side);
         cudaError_t e = cudaGetLastError();

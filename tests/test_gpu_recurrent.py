@@ -350,6 +350,28 @@ def test_scan_of_long_requests_that_overlap_stays_in_bounds(cu):
     assert out.shape == (3000, 40) and (work[floats:] == 7).all()
 
 
+@pytest.mark.parametrize("cu", [[0, 360, 10, 370], [0, 576, 0, 576], [0, 330, 100, 430, 200, 530, 576]])
+@pytest.mark.parametrize("requests", [0, 200])
+@pytest.mark.parametrize("init", ["same", "mixed"])
+def test_scan_of_long_requests_that_overlap_takes_nothing_from_scratch(cu, requests, init):
+    """Offsets that step back can name more requests in pieces than ascending ones: a slot holds its request's own state
+    or what it held, and scratch of NaN reaches neither slots nor outputs."""
+    g, rows, ch, n = gen(48), 576, 64, 16
+    cu = cu + [cu[-1]] * (requests - len(cu))  # (the rest have no rows)
+    t, pool = scan_inputs(g, "f32", rows, ch, n, 1), Pool(g, (ch, n), torch.float32, len(cu) - 1, init)
+    out = torch.full((rows, ch), 7.0, device=DEV)
+    work = torch.full((K.selective_scan_work_floats(rows, ch, n),), math.nan, device=DEV)
+    assert work.numel() > 0
+    K.selective_scan(**t, cu=i32(cu), out=out, work=work, **pool.args())
+    assert not out.isnan().any()
+    _, _, kept, kept_e = scan_want(t, cu, pool, rows, 7.0)
+    for slot in list(kept):
+        if torch.equal(pool.all[slot], pool.before[slot]):
+            del kept[slot], kept_e[slot]
+    assert pool.slots[0] in kept
+    pool.check(kept, kept_e)
+
+
 @pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 16, 17, 24, 32, 64, 100, 128, 256])
 @pytest.mark.parametrize("act", list(TYPES))
 def test_step_types_and_states(act, n):
