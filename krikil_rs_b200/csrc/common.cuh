@@ -84,14 +84,15 @@ KRK_DEV float warp_max(float v) {
     return v;
 }
 
-// 16-byte global->shared asynchronous copy (bypasses L1).
+// 16-byte global->shared asynchronous copy (bypasses L1).  The three state that they touch memory: else the compiler may
+// move a load of what was copied to before the wait, where no barrier stands behind it.
 KRK_DEV void cp_async16(void* smem, const void* gmem) {
     unsigned s = static_cast<unsigned>(__cvta_generic_to_shared(smem));
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(s), "l"(gmem));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(s), "l"(gmem) : "memory");
 }
-KRK_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+KRK_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
-KRK_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+KRK_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 // ---- bulk (TMA engine) copies completing on a shared-memory mbarrier -------
 KRK_DEV uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
