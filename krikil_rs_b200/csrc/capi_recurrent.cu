@@ -35,18 +35,34 @@ bool writable(const void* p, int64_t stride, int64_t rows, int64_t width, int es
     return p && aligned(p, es) && (rows <= 1 || stride >= width);
 }
 
-// Whether two tensors [rows, width] share memory.
-bool overlap(const void* p, int64_t p_st, const void* q, int64_t q_st, int64_t rows, int64_t width, int es) {
+// Whether two tensors [rows, p_w] and [rows, q_w] share memory.
+bool overlap(const void* p, int64_t p_st, int64_t p_w, const void* q, int64_t q_st, int64_t q_w, int64_t rows, int es) {
     if (rows <= 0) return false;
-    const int64_t a = (int64_t)(uintptr_t)p, b = (int64_t)(uintptr_t)q, pr = p_st * es, qr = q_st * es, w = width * es;
+    const int64_t a = (int64_t)(uintptr_t)p, b = (int64_t)(uintptr_t)q, pr = p_st * es, qr = q_st * es;
     const auto low = [&](int64_t at, int64_t row) { return row < 0 ? at + (rows - 1) * row : at; };
-    const auto high = [&](int64_t at, int64_t row) { return (row > 0 ? at + (rows - 1) * row : at) + w; };
-    if (high(a, pr) <= low(b, qr) || high(b, qr) <= low(a, pr)) return false;
-    if (rows > 1 && pr == qr && pr > 0) {  // columns of one matrix are apart if they begin `width` apart
+    const auto high = [&](int64_t at, int64_t row, int64_t w) { return (row > 0 ? at + (rows - 1) * row : at) + w * es; };
+    if (high(a, pr, p_w) <= low(b, qr) || high(b, qr, q_w) <= low(a, pr)) return false;
+    if (rows > 1 && pr == qr && pr > 0) {  // columns of one matrix are apart if each begins behind the other's end
         const int64_t off = ((a - b) % pr + pr) % pr;
-        return off < w || pr - off < w;
+        return off < q_w * es || pr - off < p_w * es;
     }
     return true;
+}
+
+// Whether the scan's output shares memory with an input [T][D] that it is not.
+bool over_input(const krk::ScanArgs& a, const void* p, int64_t st, int es) {
+    const bool same = p == a.out && (a.T <= 1 || st == a.o_st);
+    return p && !same && overlap(a.out, a.o_st, a.D, p, st, a.D, a.T, es);
+}
+// And with B or C [T][G][N]: with what they span, then, if it does, with one of their groups.
+bool over_groups(const krk::ScanArgs& a, const void* p, int64_t st, int64_t sg, int es) {
+    const int64_t reach = (a.G - 1) * sg;
+    const char* first = (const char*)p;
+    if (!overlap(a.out, a.o_st, a.D, first + (reach < 0 ? reach * es : 0), st, a.N + (reach < 0 ? -reach : reach), a.T, es))
+        return false;
+    for (int g = 0; g < a.G; ++g)
+        if (overlap(a.out, a.o_st, a.D, first + g * sg * es, st, a.N, a.T, es)) return true;
+    return false;
 }
 
 const char* slots_fault(const krk::SlotArgs& a, int64_t size, int es) {
@@ -72,7 +88,7 @@ static int conv_call(const char* who, const krk::ConvArgs& a, int W, int type, c
     if (!a.w || !aligned(a.w, 4) || !aligned(a.bias, 4)) return invalid(who, "weight and bias must be set (bias may be null) and aligned");
     if (a.T > 0 && (!readable(a.x, es) || !writable(a.out, a.o_st, a.T, a.C, es)))
         return invalid(who, "x and out must be set and aligned to their elements, rows of out must not overlap");
-    if (overlap(a.x, a.x_st, a.out, a.o_st, a.T, a.C, es)) return invalid(who, "out must not overlap x");
+    if (overlap(a.x, a.x_st, a.C, a.out, a.o_st, a.C, a.T, es)) return invalid(who, "out must not overlap x");
     return done(who, krk::causal_conv(a, W, type, stream));
 }
 
@@ -110,6 +126,9 @@ static int scan_call(const char* who, const krk::ScanArgs& a, int type, int max_
     if (a.T > 0 && (!readable(a.x, es) || !readable(a.dt, es) || !readable(a.b, es) || !readable(a.c, es) ||
                     (a.z && !readable(a.z, es)) || !writable(a.out, a.o_st, a.T, a.D, es)))
         return invalid(who, "x, dt, b, c and out must be set and aligned to their elements, rows of out must not overlap");
+    if (over_input(a, a.x, a.x_st, es) || over_input(a, a.dt, a.dt_st, es) || over_input(a, a.z, a.z_st, es) ||
+        over_groups(a, a.b, a.b_st, a.b_sg, es) || over_groups(a, a.c, a.c_st, a.c_sg, es))
+        return invalid(who, "out must be x, dt or z with their strides, or not overlap them, and not overlap b and c");
     if (!a.cu) return done(who, krk::selective_step(a, type, stream));
     if (max_len < 0) return invalid(who, "max_len must not be negative");
     const size_t need = krk::scan_work_floats(a.T, a.D, a.N, a.G, max_len);

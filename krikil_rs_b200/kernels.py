@@ -594,8 +594,8 @@ def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None,
     and slots as for causal_conv; state is float32 [slots, D, N].  max_len, a
     bound of the requests' rows (0: T), only sizes the launch; `work` is scratch
     of selective_scan_work_floats floats (allocated here when not given).  Returns
-    out [T, D] (which may be x, dt or z), whose rows of no request are left as
-    they were."""
+    out [T, D], which may be x, dt or z and shares no other memory with the
+    inputs, and whose rows of no request are left as they were."""
     index = x.get_device()
     if index >= 0 and index != _current_device():  # the scratch is sized for the current device
         with torch.cuda.device(torch.device("cuda", index)):

@@ -117,3 +117,39 @@ def test_wrappers_want_cuda_tensors():
                  lambda: K.token_logprobs(x)):
         with pytest.raises(ValueError, match="CUDA|cuda"):
             call()
+
+
+# tensors far from one another, rows as long as they need be
+APART = dict(x=FAR, dt=2 * FAR, z=3 * FAR, b=4 * FAR, c=5 * FAR, out=6 * FAR)
+# out over others: a row or a part of one further, with other strides, over B or C or the second of their groups
+OVER = [dict(out=FAR + 4 * 64), dict(out=FAR + 4 * 63), dict(out=FAR - 4), dict(x_st=65, out=FAR), dict(out=2 * FAR, dt_st=0),
+        dict(out=3 * FAR + 4 * 63), dict(out=4 * FAR), dict(out=4 * FAR - 4 * 63), dict(out=5 * FAR + 4 * 15, c_st=64),
+        dict(G=2, b_st=200, b_sg=100, o_st=200, out=4 * FAR + 4 * 90), dict(G=2, b_st=200, b_sg=100, o_st=200, out=4 * FAR + 4 * 37),
+        dict(G=2, b_st=16, b_sg=-1000, out=4 * FAR - 4 * 1000), dict(z=FAR + 4 * 32, z_st=100, x_st=100, o_st=100, out=FAR)]
+# and beside them: in place, columns of one matrix, the gap between two groups, other rows
+BESIDE = [dict(out=FAR), dict(out=2 * FAR), dict(out=3 * FAR), dict(b=FAR + 4 * 64, c=FAR + 4 * 80, x_st=96, b_st=96, c_st=96, o_st=96, out=FAR),
+          dict(G=2, b_st=200, b_sg=100, o_st=200, out=4 * FAR + 4 * 16), dict(G=2, b_st=200, b_sg=100, o_st=200, out=4 * FAR + 4 * 36),
+          dict(G=2, b_st=200, b_sg=100, o_st=200, out=4 * FAR + 4 * 216),
+          dict(x_st=128, o_st=128, out=FAR + 4 * 64), dict(z=None, z_st=0, out=3 * FAR), dict(x=FAR, dt=FAR, z=FAR, out=FAR)]
+
+
+@pytest.mark.parametrize("name,rows", [("scan", "T"), ("step", "B")])
+@pytest.mark.parametrize("how", OVER)
+def test_scan_and_step_refuse_an_out_over_what_others_read(name, rows, how):
+    fn, base = (lib.krk_k_selective_scan, SCAN) if name == "scan" else (lib.krk_k_selective_step, STEP)
+    args = dict(base, **{rows: 5}, **APART)
+    args.update(how)
+    assert fn(*args.values()) == _lib.INVALID, lib.krk_last_error()
+    assert "overlap" in lib.krk_last_error().decode()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would read the placeholder addresses")
+@pytest.mark.parametrize("name,rows", [("scan", "T"), ("step", "B")])
+@pytest.mark.parametrize("how", BESIDE)
+def test_scan_and_step_take_an_out_in_place_or_beside(name, rows, how):
+    fn, base = (lib.krk_k_selective_scan, SCAN) if name == "scan" else (lib.krk_k_selective_step, STEP)
+    args = dict(base, **{rows: 5}, **APART)
+    args.update(how)
+    assert fn(*args.values()) == _lib.CUDA, lib.krk_last_error()
+    one = dict(args, **{rows: 1}, x_st=7, dt_st=9, z_st=11)  # the stride of a single row does not matter
+    assert fn(*one.values()) == _lib.CUDA, lib.krk_last_error()
