@@ -488,6 +488,7 @@ def _slot_args(state, rows, width, dtype, slots, init, requests, index):
     if state.dtype is not dtype or state.get_device() != index or len(shape) != 3 or shape[1] != rows or (
             shape[2] != width) or (width > 1 and strides[2] != 1) or (rows > 1 and strides[1] != width):
         raise ValueError(f"state: expected {dtype} [slots, {rows}, {width}] on cuda:{index} with dense slots")
+    _number(shape[0], "the number of slots")
     if slots is None and shape[0] < requests:
         raise ValueError(f"state: expected a slot for each of {requests} requests, or their slots")
     return (state.data_ptr(), strides[0], shape[0], _indexes(slots, requests, index, "slots"),
@@ -499,6 +500,7 @@ def _requests(cu, index):
     n = cu.numel()
     if n < 1:
         raise ValueError("cu: expected the requests' offsets, one more than there are requests")
+    _number(n - 1, "the number of requests")
     return _indexes(cu, n, index, "cu"), n - 1
 
 
@@ -518,6 +520,7 @@ def _conv_args(x, weight, bias, state, slots, init, out, requests):
     x_at, x_st = _like(x, dtype, shape, index, "x")
     if len(w) != 2 or w[0] != ch:
         raise ValueError(f"weight: expected [{ch}, width]")
+    _number(rows | ch | w[1], "the sizes of x and weight")
     if out is None:
         out = x.new_empty(shape)
     out_at, o_st = _like(out, dtype, shape, index, "out")
@@ -568,6 +571,7 @@ def _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
     c_at, c_st, c_sg, c_groups = _groups(c, dtype, rows, n, index, "c")
     if c_groups != groups or not groups or ch % groups:
         raise ValueError(f"b and c: expected as many groups, dividing {ch} channels")
+    _number(rows | ch | n, "the sizes of x and a")
     x_at, x_st = _like(x, dtype, shape, index, "x")
     dt_at, dt_st = _like(dt, dtype, shape, index, "dt")
     z_at, z_st = (None, 0) if z is None else _like(z, dtype, shape, index, "z")
@@ -582,7 +586,10 @@ def _scan_args(x, dt, a, b, c, d, z, dt_bias, state, slots, init, out, requests)
 
 
 def selective_scan_work_floats(rows: int, channels: int, states: int, groups: int = 1, max_len: int = 0) -> int:
-    return int(lib.krk_selective_scan_work_floats(rows, channels, states, groups, max_len))
+    sizes = rows, channels, states, groups, max_len
+    if max(sizes) >> 31 > 0 or min(sizes) >> 31 < -1:  # (no scratch for negative ones)
+        raise ValueError("sizes must lie below 2^31")
+    return int(lib.krk_selective_scan_work_floats(*sizes))
 
 
 def selective_scan(x, dt, a, b, c, cu, d=None, z=None, dt_bias=None, state=None, slots=None, init=None, out=None,
@@ -635,12 +642,14 @@ def token_logprobs(logits, tokens=None, top: int = 0):
     at, ld = _like(logits, logits.dtype, shape, index, "logits")
     rows, vocab = shape
     _number(top, "top")
+    _number(rows | vocab, "the sizes of logits")
     lp, asked, lp_at, tokens_at = None, 0, None, None
     if tokens is not None:
         like = tokens.shape
         if len(like) not in (1, 2) or like[0] != rows:
             raise ValueError(f"tokens: expected [{rows}] or [{rows}, tokens]")
         asked = 1 if len(like) == 1 else like[1]
+        _number(asked, "the tokens of a row")
         tokens_at = _indexes(tokens, rows * asked, index, "tokens")
     entropy = torch.empty(rows, device=logits.device, dtype=torch.float32)
     if tokens is not None:

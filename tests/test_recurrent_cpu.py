@@ -1,6 +1,8 @@
 """Refusals of the entry points of recurrent layers over state slots and of the log probabilities.  Arguments are
 checked before a device is touched, so these run without a GPU: a refused call answers INVALID and names the fault, a
 sound one gets as far as the missing device."""
+import math
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -153,3 +155,66 @@ def test_scan_and_step_take_an_out_in_place_or_beside(name, rows, how):
     assert fn(*args.values()) == _lib.CUDA, lib.krk_last_error()
     one = dict(args, **{rows: 1}, x_st=7, dt_st=9, z_st=11)  # the stride of a single row does not matter
     assert fn(*one.values()) == _lib.CUDA, lib.krk_last_error()
+
+
+class Tensor:
+    """What the wrappers look at of a CUDA tensor, of any size."""
+
+    def __init__(self, *shape, dtype=torch.float32, zeros=()):
+        self.shape, self.dtype, self.device = torch.Size(shape), dtype, torch.device("cuda", 0)
+        self.steps = [0 if i in zeros else math.prod(shape[i + 1:]) for i in range(len(shape))]
+
+    def stride(self):
+        return tuple(self.steps)
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return P
+
+    def new_empty(self, *shape):
+        return Tensor(*(shape[0] if isinstance(shape[0], (tuple, torch.Size)) else shape), dtype=self.dtype)
+
+
+LONG = (1 << 32) + 2  # two of the low 32 bits
+
+
+@pytest.mark.parametrize("what", ["conv rows", "conv channels", "conv width", "conv requests", "conv slots", "conv step rows", "scan rows",
+                                  "scan requests", "scan slots", "scan states", "scan groups", "step rows", "step slots",
+                                  "logprobs rows", "logprobs vocab", "logprobs asked", "scratch rows"])
+def test_wrappers_refuse_sizes_past_31_bits(what, monkeypatch):
+    """A size that the library's 32-bit arguments do not hold is not cut to its low bits."""
+
+    class Lib:
+        def __getattr__(self, name):
+            if name == "krk_selective_scan_work_floats":
+                return lambda *sizes: 0
+            return lambda *args: pytest.fail(f"{name} was called")
+
+    monkeypatch.setattr(K, "lib", Lib())
+    monkeypatch.setattr(K, "_current_device", lambda: 0)
+    monkeypatch.setattr(K, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(K.torch, "empty", lambda *shape, device=None, dtype=None: Tensor(*shape, dtype=dtype))
+    n = {k: LONG if k == what.split()[-1] else v for k, v in dict(
+        rows=2, channels=2, width=4, requests=1, slots=2, states=4, groups=1, vocab=9, asked=1).items()}
+    ints = lambda *shape: Tensor(*shape, dtype=torch.int32)  # noqa: E731
+    rows, ch = n["rows"], 2 * n["groups"] if n["groups"] > 1 else n["channels"]
+    x, cu = Tensor(rows, ch), ints(n["requests"] + 1)
+    bc, a = Tensor(rows, n["groups"], n["states"]), Tensor(ch, n["states"])
+    conv = dict(weight=Tensor(ch, n["width"]), state=Tensor(n["slots"], n["width"] - 1, ch))
+    state = Tensor(n["slots"], ch, n["states"])
+    calls = {"conv": lambda: K.causal_conv(x, cu=cu, slots=ints(n["requests"]), **conv),
+             "conv step": lambda: K.causal_conv_step(x, slots=ints(rows), **conv),
+             "scan": lambda: K.selective_scan(x, x, a, bc, bc, cu, state=state, slots=ints(n["requests"])),
+             "step": lambda: K.selective_step(x, x, a, bc, bc, state, slots=ints(rows)),
+             "logprobs": lambda: K.token_logprobs(Tensor(rows, n["vocab"]), ints(rows, n["asked"])),
+             "scratch": lambda: K.selective_scan_work_floats(rows, 2, 4)}
+    with pytest.raises(ValueError, match="2\\^31|31 bits"):
+        calls[what.rsplit(" ", 1)[0]]()
