@@ -350,6 +350,44 @@ def test_scan_of_long_requests_that_overlap_stays_in_bounds(cu):
     assert out.shape == (3000, 40) and (work[floats:] == 7).all()
 
 
+def scan_want_of_many(t, lens, pool, rows, fill):
+    """scan_want of many short requests: those of one length are walked as one request of all their channels."""
+    ch, groups = t["x"].shape[1], t["b"].shape[1]
+    want, bound = torch.full((rows, ch), fill, device=DEV, dtype=F64), torch.zeros(rows, ch, device=DEV, dtype=F64)
+    kept, kept_e, starts = {}, {}, list(itertools.accumulate(lens, initial=0))
+    for length in sorted(set(lens)):
+        same = [s for s, k in enumerate(lens) if k == length and pool.slots[s] >= 0]
+        at = torch.tensor([[starts[s] + i for s in same] for i in range(length)], device=DEV).long().view(length, len(same))
+        flat = lambda v: v[at].flatten(1)  # noqa: E731
+        group = lambda v: v[at].flatten(1, 2)  # noqa: E731
+        often = lambda v: v.repeat(len(same), *[1] * (v.dim() - 1))  # noqa: E731
+        y, e, h, he = scan64(flat(t["x"]), flat(t["dt"]), often(t["a"]), group(t["b"]), group(t["c"]), often(t["d"]),
+                             flat(t["z"]), often(t["dt_bias"]), torch.cat([pool.begun(s) for s in same]))
+        want[at], bound[at] = y.view(length, len(same), ch), e.view(length, len(same), ch)
+        for i, s in enumerate(same):
+            kept[pool.slots[s]], kept_e[pool.slots[s]] = h[i * ch:(i + 1) * ch], he[i * ch:(i + 1) * ch]
+    return want, bound, kept, kept_e
+
+
+@pytest.mark.parametrize("n", [4, 5, 8, 12, 16, 17, 24, 32, 50, 64, 100, 128, 200, 256])
+@pytest.mark.parametrize("act", list(TYPES))
+@pytest.mark.parametrize("requests,ch,groups,wide,lead", [(200, 40, 1, True, 3), (161, 48, 1, False, 8), (90, 80, 2, False, 8)])
+def test_scan_of_many_short_requests(act, n, requests, ch, groups, wide, lead):
+    """More blocks than multiprocessors and no request that may be split, as a server's prompts are: whole lanes of states,
+    and the requests' order with and without a place for each in a block."""
+    assert requests * groups > torch.cuda.get_device_properties(DEV).multi_processor_count
+    assert K.selective_scan_work_floats(5 * requests, ch, n, groups, 9) == 0
+    g, lens = gen(49), [(i * 7) % 10 for i in range(requests)]
+    rows = sum(lens) + 2
+    t = scan_inputs(g, act, rows, ch, n, groups, wide=wide, lead=lead)
+    pool = Pool(g, (ch, n), torch.float32, requests, "mixed", (3, 77, requests - 1))
+    out = torch.full((rows, ch), 7.0, device=DEV, dtype=TYPES[act])
+    K.selective_scan(**t, cu=i32(list(itertools.accumulate(lens, initial=0))), out=out, max_len=9, **pool.args())
+    want, bound, kept, kept_e = scan_want_of_many(t, lens, pool, rows, 7.0)
+    close(out, want, bound, "out")
+    pool.check(kept, kept_e)
+
+
 @pytest.mark.parametrize("cu", [[0, 360, 10, 370], [0, 576, 0, 576], [0, 330, 100, 430, 200, 530, 576]])
 @pytest.mark.parametrize("requests", [0, 200])
 @pytest.mark.parametrize("init", ["same", "mixed"])
