@@ -248,8 +248,9 @@ cudaError_t launch_conv(const ConvArgs& a, cudaStream_t s) {
     if (sms <= 0) return cudaErrorInvalidDevice;
     if (!a.cu) {
         // two requests a thread at once when that leaves every multiprocessor a full set of threads, then so many times
-        // that the blocks (seven a multiprocessor, by registers) are one wave, which load the taps once (509 requests x
-        // 8192 bfloat16 channels: 15.8 us by four times, 18.6 by one)
+        // that there are seven blocks a multiprocessor, which load the taps once (509 requests x 8192 bfloat16 channels:
+        // 16 us by four times, 18.6 by one; that form's 62 registers leave room for eight blocks, those of fewer taps or
+        // channels a thread for more, which no measurement has set apart)
         const int64_t units = (int64_t)a.T * side;
         if (units > INT32_MAX) return cudaErrorInvalidValue;
         if (units >= (int64_t)sms * 2048 / CONV_THREADS) {

@@ -17,7 +17,8 @@
 // Measured: float32, 1024 x 50001, 36 us (5.6 TB/s, 85% of the copy rate);
 // bfloat16, 4096 x 50001, 82 us (5.0 TB/s; issue slots 75% busy, the exponential
 // unit 62%); float32, one row of 131,072 with 20 alternatives, 8.5 us in 16 blocks;
-// bfloat16, 4096 x 32768 with 20 alternatives, 80 us, half of it the rows' ends.
+// bfloat16, 4096 x 32768 with 20 alternatives, 80 us, 54 without them; 8192 x 2048
+// with five, 32 us, 15 without them.
 #include <cooperative_groups.h>
 
 #include "kernels.h"
@@ -33,8 +34,9 @@ constexpr int LP_SHORT = 1024;  // accesses of a row that a small block takes in
 constexpr int LP_LIST = 32;     // entries of a sorted list, LOGPROBS_MAX_TOP of them used
 constexpr int LP_ROOM = 1024;   // logits that reach the bound; for more (the best ones all in few threads' ways) see below
 constexpr int LP_AHEAD = 4;     // accesses on their way
-// Threads a multiprocessor: all of them in 32 bits, and 40 registers each in 16 (81 us for 4096 x 50001; 87 with 56
-// registers, 136 with 32, which spill).
+// Threads a multiprocessor that registers are left for: all of them in 32 bits, and 40 registers each in 16 (82 us for
+// 4096 x 50001; 87 with 56 registers, 136 with 32, which spill).  Blocks of two warps reach 1024, by their shared memory
+// (12.8 KB, so that 16 of them fit).
 template <typename T>
 constexpr int LP_RESIDENT = sizeof(T) == 4 ? 2048 : 1536;
 constexpr float kLog2e = 1.44269504088896341f, kLowest = -3.402823466e38f;

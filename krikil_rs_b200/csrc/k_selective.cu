@@ -154,8 +154,9 @@ cudaError_t step_rows(const ScanArgs& a, int lane_bits, cudaStream_t s) {
     const int64_t side = (((int64_t)a.D << lane_bits) + STEP_THREADS - 1) / STEP_THREADS, units = side * a.T;
     // two requests a thread at once when that leaves every multiprocessor a full set of threads
     if (units < (int64_t)sms * 2048 * 2 / STEP_THREADS) return launch_step<T, FORM, Q, 1>(a, lane_bits, side, 1, s);
-    // and up to four times, with the channels' decays loaded once, while there are two waves of blocks (six a
-    // multiprocessor, by registers): 253 requests x 5120 channels, 36.1 us by four times, 38.5 by one, 41.8 by eight
+    // and up to four times, with the channels' decays loaded once, while there are two waves of blocks, six a
+    // multiprocessor: 253 requests x 5120 channels, 36.1 us by four times, 38.5 by one, 41.8 by eight (six are what the
+    // registers of whole groups of eight states leave room for, 80 a thread; of other forms three to nine)
     const int64_t turns = units / 2 / (12LL * sms);
     return launch_step<T, FORM, Q, 2>(a, lane_bits, side, turns < 1 ? 1 : turns > 4 ? 4 : (int)turns, s);
 }

@@ -21,11 +21,13 @@
 // 5120 channels, 14 pieces, 247 and 720 us; 12,000, six, 548 and 725; 16,384, four,
 // 809 and 770).
 //
-// Measured (N = 16): 64 prompts of 0 to 511 rows x 5120 bfloat16 channels 470 us --
+// Measured (N = 16): 64 prompts of 0 to 511 rows x 5120 bfloat16 channels 480 us --
 // 20 exponentials a row and channel would be 372 us, and a walk of the same
 // instructions without its inputs takes 168 cycles for 32 channels, 387 us -- and
-// 8192 rows x 1536 half channels in 49 pieces 153 us.  A polynomial in place of an
-// eighth of the exponentials takes as long (167 cycles), of a quarter longer (177).
+// 8192 rows x 1536 half channels in 49 pieces 157 us (apart and cold: the first walk
+// 76, the carry 10, the last walk 84; their exponentials 50 and 55).  A polynomial in
+// place of an eighth of the exponentials takes as long (167 cycles), of a quarter
+// longer (177).
 #pragma once
 #include <limits.h>
 
